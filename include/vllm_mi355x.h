@@ -552,6 +552,107 @@ int moe_split_align(const int32_t* topk_ids, int64_t numel, int64_t num_experts,
                     int32_t* eids32, int32_t* eids16, const int64_t* eids_numel, int32_t* ntpp,
                     void* stream);
 
+/* ---- MXFP4: microscaled 4-bit floating point ----------------------------------
+ *
+ * A block is 32 consecutive elements of a row: 32 E2M1 codes (0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6 and their negatives), two a byte with the even element in the low
+ * nibble, under one E8M0 scale byte b, the factor 2^(b - 127) (255: NaN).  A
+ * row of k elements (k a multiple of 32) is k / 2 code bytes and k / 32 scale
+ * bytes; matrices are row-major and contiguous, codes 16-byte aligned.  None
+ * of these entry points has a counterpart in the reference.
+ */
+
+/*
+ * codes, scales = the MXFP4 form of x [rows][k] (row stride x_stride elements;
+ * VQ_BF16, VQ_FP16 or VQ_FP32).  Per block with the largest magnitude m: scale
+ * 2^s, s = max(floor(log2 m) - 2, -127) (-127 for m = 0); each code the nearest
+ * to x 2^-s, ties to the even code, saturating at 6, signs kept.  A block
+ * with a NaN or an infinity gets scale byte 255 over zero codes.
+ */
+int mxfp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_stride,
+                   uint8_t* codes, uint8_t* scales, void* stream);
+
+/* out [rows][k] = the values of codes under their scales, rounded once to
+ * out_dtype (exact in FP32 and BF16 but below 2^-126; FP16 may overflow). */
+int mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k,
+                     void* out, int out_dtype, void* stream);
+
+/*
+ * out [rows][n] = RN_out(sum_k a[r][k] w[n][k]) of MXFP4 a [rows][k] and w
+ * [n][k], products exact and summed in FP32 on the matrix cores.  The order
+ * of the sums, and so the last bits, depend on rows, k and n alone.
+ * workspace: mxfp4_matmul_workspace_size(rows, k, n) bytes, 16-byte aligned
+ * (null where that is 0), used by one call at a time.
+ */
+int64_t mxfp4_matmul_workspace_size(int64_t rows, int64_t k, int64_t n);
+int mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, int64_t rows, int64_t k,
+                 const uint8_t* w, const uint8_t* w_scales, int64_t n, void* out, int out_dtype,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * mxfp4_matmul of x as mxfp4_quantize quantizes it (x [rows][k] of VQ_BF16,
+ * VQ_FP16 or VQ_FP32, row stride x_stride): the same codes, products and
+ * tolerance.  workspace: mxfp4_linear_workspace_size bytes, as above.
+ */
+int64_t mxfp4_linear_workspace_size(int64_t rows, int64_t k, int64_t n);
+int mxfp4_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_stride,
+                 const uint8_t* w, const uint8_t* w_scales, int64_t n, void* out, int out_dtype,
+                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Routed experts with MXFP4 weights: out[t] = RN(sum over t's slots, in slot
+ * order, of topk_w[slot] * y[slot]) in FP32, with x the MXFP4 form of x[t],
+ *   g | u = x W13_e^T,  h = SiLU(min(g, L)) clamp(u, -L, L) in FP32, quantized
+ *   to MXFP4,  y = h W2_e^T.
+ * x / out [tokens][hidden] of act_dtype (VQ_BF16 or VQ_FP16; x rows of x_stride
+ * elements, out contiguous); w13 [experts][2 inter][hidden] (gate rows, then
+ * up rows), w2 [experts][hidden][inter]; topk_ids int32 [tokens][top_k];
+ * expert_map int32 [map_size] global id -> local expert (map_size 0: none).
+ * Slots outside [0, experts) add nothing.  limit L > 0 (infinity: no clamp).
+ * hidden and inter multiples of 32, at most 1024 experts.  workspace:
+ * mxfp4_moe_workspace_size bytes, 16-byte aligned; calls that share one must
+ * be on one stream.
+ */
+int64_t mxfp4_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int64_t inter,
+                                 int64_t experts);
+int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, const uint8_t* w13,
+              const uint8_t* s13, const uint8_t* w2, const uint8_t* s2, int64_t experts,
+              const int32_t* topk_ids, const float* topk_w, int64_t top_k,
+              const int32_t* expert_map, int64_t map_size, int64_t hidden, int64_t inter,
+              float limit, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- a router's load -----------------------------------------------------------
+ * Up to 1024 experts; rows with is_padding[t] != 0 (optional uint8 [rows]) are
+ * left out.  No counterparts in the reference.  workspace:
+ * moe_balance_workspace_size bytes, 8-byte aligned, used by one call at a time.
+ */
+int64_t moe_balance_workspace_size(int64_t rows, int64_t experts);
+
+/* counts[e] = the slots of topk_ids (int32 [rows][top_k]) that chose e; add != 0:
+ * counts[e] += that.  Ids outside [0, experts) are not counted. */
+int moe_expert_counts(const int32_t* topk_ids, const uint8_t* is_padding, int64_t rows,
+                      int64_t top_k, int64_t experts, int add, int64_t* counts, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/*
+ * loss = sum_e f_e P_e over the n counted rows: f_e = counts_e experts / (n
+ * top_k), P_e the mean of p_te, p_t = softmax (scoring 0) of the row's logits or
+ * their sigmoids divided by the sum of these (scoring 1).  A row whose logits
+ * leave nothing (all -infinity) has p = 0; no counted row: loss 0.  Even load
+ * gives 1.  logits [rows][experts] of dtype, row stride `stride`.  stats
+ * [experts + 1]: f_e, then 1 / n (0 for n = 0), for moe_balance_grad.
+ */
+int moe_balance_loss(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,
+                     const int32_t* topk_ids, int64_t top_k, const uint8_t* is_padding,
+                     int scoring, float* loss, int64_t* counts, float* stats, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/* grad [rows][experts] (contiguous, of the logits' dtype) = upstream[0] *
+ * dloss/dlogits with the counts constant, zeros in padding rows. */
+int moe_balance_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,
+                     const uint8_t* is_padding, int scoring, const float* stats,
+                     const float* upstream, void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,7 +32,8 @@ SOURCES = [("exl3_gemv_part.hip", f"exl3_gemv_part{p}", [f"-DVQ_GEMV_PART={p}"])
           [("exl3_tile_part.hip", f"exl3_tile_part{p}", [f"-DVQ_TILE_PART={p}"]) for p in range(TILE_PARTS)] + \
           [("marlin_moe.hip", "marlin_moe", []), ("exl3_gemm.hip", "exl3_gemm", []),
            ("exl3_linear.hip", "exl3_linear", []), ("exl3_moe.hip", "exl3_moe", []),
-           ("exl3_ple.hip", "exl3_ple", []),
+           ("exl3_ple.hip", "exl3_ple", []), ("mxfp4.hip", "mxfp4", []),
+           ("mxfp4_moe.hip", "mxfp4_moe", []), ("moe_balance.hip", "moe_balance", []),
            ("common.cpp", "common", [])]
 
 ARCH = "gfx950"
@@ -92,20 +93,22 @@ def _check_undefined(library: str) -> None:
         return
     res = subprocess.run([nm, "-u", "-C", library], capture_output=True, text=True)
     bad = [line.strip() for line in res.stdout.splitlines()
-           if "__device_stub__" in line or any(ns in line for ns in ("exl3::", "marlin::", "vq::"))]
+           if "__device_stub__" in line or any(ns in line for ns in ("exl3::", "marlin::", "vq::", "mx::", "moe::",
+                                                                    "balance::"))]
     if bad:
         os.remove(library)
         raise RuntimeError("linked library has undefined project symbols:\n  " + "\n  ".join(bad[:10]))
 
 
 TORCH_LIBRARY_PATH = os.path.join(PACKAGE, "libvllm_mi355x_torch.so")
+TORCH_SOURCES = ["torch_classes", "torch_ops", "torch_mxfp4", "torch_balance"]
 
 
 def build_torch_classes(verbose: bool = False) -> str:
-    """libvllm_mi355x_torch.so: the linear and MoE operators' implementations
-    (csrc/torch_ops.cpp) and the torch custom classes the reference's loader
-    requires (csrc/torch_classes.cpp): host-only, built with g++ against the
-    installed torch."""
+    """libvllm_mi355x_torch.so: the operators' host side (csrc/torch_ops.cpp,
+    torch_mxfp4.cpp, torch_balance.cpp) and the torch custom classes the
+    reference's loader requires (csrc/torch_classes.cpp): host-only, built with
+    g++ against the installed torch, one process a source."""
     import torch
     from torch.utils import cpp_extension
 
@@ -113,18 +116,28 @@ def build_torch_classes(verbose: bool = False) -> str:
     if not cxx:
         raise RuntimeError("g++ not found (needed for libvllm_mi355x_torch.so)")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [cxx, "-O2", "-fPIC", "-shared", "-std=c++17", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={abi}"]
     # (the HIP headers' platform, for torch's stream type)
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    cmd += ["-D__HIP_PLATFORM_AMD__=1", f"-I{os.path.join(rocm, 'include')}"]
-    cmd += [f"-I{p}" for p in cpp_extension.include_paths()]
-    cmd += [os.path.join(CSRC, src) for src in ("torch_classes.cpp", "torch_ops.cpp")]
-    cmd += ["-o", TORCH_LIBRARY_PATH + ".tmp"]
-    cmd += [f"-L{p}" for p in cpp_extension.library_paths()]
-    cmd += ["-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"building libvllm_mi355x_torch.so failed:\n{res.stdout}\n{res.stderr}")
+    flags = ["-O2", "-fPIC", "-std=c++17", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+             "-D__HIP_PLATFORM_AMD__=1", f"-I{os.path.join(rocm, 'include')}"]
+    flags += [f"-I{p}" for p in cpp_extension.include_paths()]
+
+    def run(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"building libvllm_mi355x_torch.so failed:\n{res.stdout}\n{res.stderr}")
+
+    def compile_one(name):
+        obj = os.path.join(OBJDIR, name + ".o")
+        run([cxx, *flags, "-c", os.path.join(CSRC, name + ".cpp"), "-o", obj])
+        return obj
+
+    os.makedirs(OBJDIR, exist_ok=True)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(TORCH_SOURCES)) as pool:
+        objs = list(pool.map(compile_one, TORCH_SOURCES))
+    run([cxx, "-shared", *objs, "-o", TORCH_LIBRARY_PATH + ".tmp",
+         *[f"-L{p}" for p in cpp_extension.library_paths()],
+         "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch"])
     os.replace(TORCH_LIBRARY_PATH + ".tmp", TORCH_LIBRARY_PATH)
     if verbose:
         print(f"built {TORCH_LIBRARY_PATH}")

@@ -1,0 +1,152 @@
+// The router's load operators (kernels/moe/balance.py), in host-only C++: the
+// expert counts, and the balance loss with its gradient as an autograd node.
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
+#include <dlfcn.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <optional>
+#include <tuple>
+
+#include "../../include/vllm_mi355x.h"
+#include "torch_common.h"
+
+namespace {
+
+using vq_torch::check_status;
+using vq_torch::dtype_code;
+using vq_torch::stream_of;
+
+decltype(&moe_expert_counts) native_counts = nullptr;
+decltype(&moe_balance_loss) native_loss = nullptr;
+decltype(&moe_balance_grad) native_grad = nullptr;
+decltype(&moe_balance_workspace_size) native_workspace = nullptr;
+decltype(&vllm_mi355x_last_error) native_error = nullptr;
+
+at::Tensor scratch(int64_t rows, int64_t experts, const at::Tensor& on) {
+  const int64_t bytes = native_workspace(rows, experts);
+  if (bytes < 0) TORCH_CHECK(false, native_error());
+  return at::empty({bytes}, on.options().dtype(at::kByte));
+}
+
+void check_routing(const at::Tensor& ids, const std::optional<at::Tensor>& padding, const at::Tensor& on, const char* what) {
+  TORCH_CHECK(ids.is_cuda() && ids.device() == on.device(), what, ": topk_ids must be on the logits' GPU");
+  TORCH_CHECK(ids.scalar_type() == at::kInt && ids.dim() == 2 && ids.is_contiguous() && ids.size(1) > 0, what,
+              ": topk_ids must be a contiguous int32 [rows, topk]");
+  TORCH_CHECK(!padding || (padding->device() == on.device() && (padding->scalar_type() == at::kBool || padding->scalar_type() == at::kByte) &&
+                           padding->dim() == 1 && padding->size(0) == ids.size(0) && padding->is_contiguous()),
+              what, ": is_padding must be a contiguous bool or uint8 [rows] on the same GPU");
+}
+
+const uint8_t* bytes_of(const std::optional<at::Tensor>& t) { return t ? static_cast<const uint8_t*>(t->const_data_ptr()) : nullptr; }
+
+void expert_counts(const at::Tensor& ids, const std::optional<at::Tensor>& padding, const at::Tensor& out, bool add) {
+  constexpr const char* what = "moe_expert_counts";
+  TORCH_CHECK(ids.is_cuda(), what, ": topk_ids must be on a GPU");
+  check_routing(ids, padding, ids, what);
+  TORCH_CHECK(out.device() == ids.device() && out.scalar_type() == at::kLong && out.dim() == 1 && out.is_contiguous(), what,
+              ": out must be a contiguous int64 [num_experts] on the ids' GPU");
+  const c10::DeviceGuard guard(ids.device());
+  at::Tensor ws = scratch(ids.size(0), out.size(0), ids);
+  check_status(native_counts(static_cast<const int32_t*>(ids.const_data_ptr()), bytes_of(padding), ids.size(0), ids.size(1),
+                             out.size(0), add, static_cast<int64_t*>(out.mutable_data_ptr()), ws.mutable_data_ptr(), ws.numel(),
+                             stream_of(ids)));
+}
+
+// (loss, counts, stats): stats is what the gradient needs beside the logits.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> forward(const at::Tensor& logits, const at::Tensor& ids,
+                                                       const std::optional<at::Tensor>& padding, int64_t scoring) {
+  constexpr const char* what = "moe_balance_loss";
+  TORCH_CHECK(logits.is_cuda(), what, ": logits must be on a GPU");
+  TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf || logits.scalar_type() == at::kFloat, what,
+              ": logits must be BF16, FP16 or FP32");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0 && (logits.numel() == 0 || logits.size(1) == 1 || logits.stride(1) == 1), what,
+              ": logits must be [rows, experts] with unit inner stride");
+  check_routing(ids, padding, logits, what);
+  const int64_t rows = logits.size(0), experts = logits.size(1);
+  TORCH_CHECK(ids.size(0) == rows, what, ": topk_ids must have a row for each row of the logits");
+  const c10::DeviceGuard guard(logits.device());
+  at::Tensor ws = scratch(rows, experts, logits);
+  at::Tensor loss = at::empty({}, logits.options().dtype(at::kFloat));
+  at::Tensor counts = at::empty({experts}, logits.options().dtype(at::kLong));
+  at::Tensor stats = at::empty({experts + 1}, logits.options().dtype(at::kFloat));
+  check_status(native_loss(logits.const_data_ptr(), dtype_code(logits.scalar_type()), rows, experts, rows > 1 ? logits.stride(0) : experts,
+                           static_cast<const int32_t*>(ids.const_data_ptr()), ids.size(1), bytes_of(padding), int(scoring),
+                           static_cast<float*>(loss.mutable_data_ptr()), static_cast<int64_t*>(counts.mutable_data_ptr()),
+                           static_cast<float*>(stats.mutable_data_ptr()), ws.mutable_data_ptr(), ws.numel(), stream_of(logits)));
+  return {loss, counts, stats};
+}
+
+std::tuple<at::Tensor, at::Tensor> loss_no_grad(const at::Tensor& logits, const at::Tensor& ids, const std::optional<at::Tensor>& padding,
+                                                int64_t scoring) {
+  auto [loss, counts, stats] = forward(logits, ids, padding, scoring);
+  return {loss, counts};
+}
+
+struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids,
+                                                const std::optional<at::Tensor>& padding, int64_t scoring) {
+    auto [loss, counts, stats] = ::forward(logits, ids, padding, scoring);
+    ctx->save_for_backward({logits, stats, padding.value_or(at::Tensor())});
+    ctx->saved_data["scoring"] = scoring;
+    ctx->mark_non_differentiable({counts});
+    return {loss, counts};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    TORCH_CHECK(!c10::GradMode::is_enabled(), "moe_balance_loss: its gradient has no gradient (create_graph)");
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &logits = saved[0], &stats = saved[1], &padding = saved[2];
+    const int64_t rows = logits.size(0), experts = logits.size(1);
+    const c10::DeviceGuard guard(logits.device());
+    at::Tensor grad = at::empty({rows, experts}, logits.options());
+    const at::Tensor upstream = grads[0].to(logits.device(), at::kFloat).contiguous();
+    check_status(native_grad(logits.const_data_ptr(), dtype_code(logits.scalar_type()), rows, experts,
+                             rows > 1 ? logits.stride(0) : experts,
+                             padding.defined() ? static_cast<const uint8_t*>(padding.const_data_ptr()) : nullptr,
+                             int(ctx->saved_data["scoring"].toInt()), static_cast<const float*>(stats.const_data_ptr()),
+                             static_cast<const float*>(upstream.const_data_ptr()), grad.mutable_data_ptr(), stream_of(logits)));
+    return {grad, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> loss_autograd(const at::Tensor& logits, const at::Tensor& ids, const std::optional<at::Tensor>& padding,
+                                                 int64_t scoring) {
+  if (!c10::GradMode::is_enabled() || !logits.requires_grad()) return loss_no_grad(logits, ids, padding, scoring);
+  const torch::autograd::variable_list out = BalanceLoss::apply(logits, ids, padding, scoring);
+  return {out[0], out[1]};
+}
+
+std::tuple<at::Tensor, at::Tensor> loss_meta(const at::Tensor& logits, const at::Tensor&, const std::optional<at::Tensor>&, int64_t) {
+  return {at::empty({}, logits.options().dtype(at::kFloat)), at::empty({logits.size(1)}, logits.options().dtype(at::kLong))};
+}
+
+template <typename F>
+bool find(void* library, const char* name, F& f) {
+  f = reinterpret_cast<F>(dlsym(library, name));
+  return f != nullptr;
+}
+
+}  // namespace
+
+bool vq_torch::bind_balance(void* library) {
+  return find(library, "moe_expert_counts", native_counts) && find(library, "moe_balance_loss", native_loss) &&
+         find(library, "moe_balance_grad", native_grad) && find(library, "moe_balance_workspace_size", native_workspace) &&
+         find(library, "vllm_mi355x_last_error", native_error);
+}
+
+TORCH_LIBRARY_FRAGMENT(_vllm_mi355x, m) {
+  m.def("moe_expert_counts(Tensor topk_ids, Tensor? is_padding, Tensor(a!) out, bool add) -> ()");
+  m.def("moe_balance_loss(Tensor logits, Tensor topk_ids, Tensor? is_padding, int scoring) -> (Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(_vllm_mi355x, CUDA, m) {
+  m.impl("moe_expert_counts", &expert_counts);
+  m.impl("moe_balance_loss", &loss_no_grad);
+}
+TORCH_LIBRARY_IMPL(_vllm_mi355x, Meta, m) { m.impl("moe_balance_loss", &loss_meta); }
+TORCH_LIBRARY_IMPL(_vllm_mi355x, Autograd, m) { m.impl("moe_expert_counts", torch::CppFunction::makeFallthrough()); }
+TORCH_LIBRARY_IMPL(_vllm_mi355x, AutogradCUDA, m) { m.impl("moe_balance_loss", &loss_autograd); }

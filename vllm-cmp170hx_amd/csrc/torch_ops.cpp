@@ -5,6 +5,7 @@
 //    torch's current stream (schemas: vllm_mi355x/kernels/exl3/_C.py);
 //  * _vllm_mi355x::marlin_moe, the launches of one fused Marlin MoE call on the
 //    path and buffers that kernels/marlin_moe/fused.py chose.
+// (The MXFP4 operators and the router's load: torch_mxfp4.cpp, torch_balance.cpp.)
 // From Python the same checks and calls took longer than the kernels of a small
 // call: a 5120 x 512 linear of one row 21.6 us a call (6 on the GPU), 10.2
 // with its operator here; the fused MoE of 48 tokens 85 us of host work for four
@@ -26,8 +27,13 @@
 #include <optional>
 
 #include "../../include/vllm_mi355x.h"
+#include "torch_common.h"
 
 namespace {
+
+using vq_torch::check_status;
+using vq_torch::dtype_code;
+using vq_torch::stream_of;
 
 decltype(&exl3_linear_out) native_linear_out = nullptr;
 decltype(&exl3_moe_out) native_moe_out = nullptr;
@@ -40,10 +46,6 @@ decltype(&marlin_moe_w2_sum) native_w2_sum = nullptr;
 decltype(&marlin_moe_rows) native_rows = nullptr;
 decltype(&moe_sum) native_sum = nullptr;
 decltype(&vllm_mi355x_last_error) native_last_error = nullptr;
-
-int dtype_code(at::ScalarType t) {
-  return t == at::kBFloat16 ? VQ_BF16 : (t == at::kHalf ? VQ_FP16 : VQ_FP32);
-}
 
 void check_tensor(const at::Tensor& t, const at::Tensor& x, std::initializer_list<at::ScalarType> dtypes,
                   const char* name) {
@@ -58,10 +60,6 @@ void check_integer(const at::Tensor& t, const at::Tensor& x, const char* name) {
   TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must have int32 or int64 dtype");
   check_tensor(t, x, {t.scalar_type()}, name);
 }
-
-void* stream_of(const at::Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
-
-void check_status(int status) { TORCH_CHECK(status == 0, native_last_error()); }
 
 void linear_out(const at::Tensor& x, const at::Tensor& trellis, const at::Tensor& suh, const at::Tensor& svh,
                 int64_t bits_x2, int64_t codebook, int64_t logical_in, int64_t logical_out,
@@ -284,6 +282,14 @@ bool find(void* library, const char* name, F& f) {
 
 }  // namespace
 
+int vq_torch::dtype_code(at::ScalarType t) {
+  return t == at::kBFloat16 ? VQ_BF16 : (t == at::kHalf ? VQ_FP16 : VQ_FP32);
+}
+
+void* vq_torch::stream_of(const at::Tensor& x) { return c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
+
+void vq_torch::check_status(int status) { TORCH_CHECK(status == 0, native_last_error()); }
+
 // The entry points of the loaded library (its dlopen handle); 0, or 1 when one
 // is missing.
 extern "C" int vllm_mi355x_torch_bind(void* library) {
@@ -294,7 +300,8 @@ extern "C" int vllm_mi355x_torch_bind(void* library) {
                    find(library, "marlin_moe_gemm_direct", native_gemm_direct) &&
                    find(library, "marlin_moe_w13_act", native_w13_act) &&
                    find(library, "marlin_moe_w2_sum", native_w2_sum) && find(library, "marlin_moe_rows", native_rows) &&
-                   find(library, "moe_sum", native_sum) && find(library, "vllm_mi355x_last_error", native_last_error);
+                   find(library, "moe_sum", native_sum) && find(library, "vllm_mi355x_last_error", native_last_error) &&
+                   vq_torch::bind_mxfp4(library) && vq_torch::bind_balance(library);
   return all ? 0 : 1;
 }
 

@@ -13,7 +13,8 @@ import threading
 
 LIBRARY_NAME = "libvllm_mi355x.so"
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIBRARY_NAME)
-# The host-only operator implementations (csrc/torch_ops.cpp) and the torch
+# The host-only operator implementations (csrc/torch_ops.cpp, torch_mxfp4.cpp,
+# torch_balance.cpp) and the torch
 # custom classes the reference's loader requires (csrc/torch_classes.cpp).
 TORCH_CLASSES_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                   "libvllm_mi355x_torch.so")
@@ -138,6 +139,42 @@ SIGNATURES = {
         c_vp, c_vp, c_vp, c_vp,                  # is_padding, logits, topk_weights, topk_ids
         c_vp, c_i64, c_vp, c_i64, c_vp,          # sorted, numel, expert_ids, numel, ntpp
         c_vp,                                    # stream
+    ]),
+    "mxfp4_quantize": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "mxfp4_dequantize": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_int, c_vp]),
+    "mxfp4_matmul_workspace_size": (c_i64, [c_i64, c_i64, c_i64]),
+    "mxfp4_matmul": (c_int, [
+        c_vp, c_vp, c_i64, c_i64,                # a, a_scales, rows, k
+        c_vp, c_vp, c_i64, c_vp, c_int,          # w, w_scales, n, out, out_dtype
+        c_vp, c_i64, c_vp,                       # workspace, bytes, stream
+    ]),
+    "mxfp4_linear_workspace_size": (c_i64, [c_i64, c_i64, c_i64]),
+    "mxfp4_linear": (c_int, [
+        c_vp, c_int, c_i64, c_i64, c_i64,        # x, x_dtype, rows, k, x_stride
+        c_vp, c_vp, c_i64, c_vp, c_int,          # w, w_scales, n, out, out_dtype
+        c_vp, c_i64, c_vp,                       # workspace, bytes, stream
+    ]),
+    "mxfp4_moe_workspace_size": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "mxfp4_moe": (c_int, [
+        c_vp, c_int, c_i64, c_i64,               # x, act_dtype, tokens, x_stride
+        c_vp, c_vp, c_vp, c_vp, c_i64,           # w13, s13, w2, s2, experts
+        c_vp, c_vp, c_i64, c_vp, c_i64,          # topk_ids, topk_w, top_k, expert_map, map_size
+        c_i64, c_i64, ctypes.c_float,            # hidden, inter, limit
+        c_vp, c_vp, c_i64, c_vp,                 # out, workspace, bytes, stream
+    ]),
+    "moe_balance_workspace_size": (c_i64, [c_i64, c_i64]),
+    "moe_expert_counts": (c_int, [
+        c_vp, c_vp, c_i64, c_i64, c_i64,         # topk_ids, is_padding, rows, top_k, experts
+        c_int, c_vp, c_vp, c_i64, c_vp,          # add, counts, workspace, bytes, stream
+    ]),
+    "moe_balance_loss": (c_int, [
+        c_vp, c_int, c_i64, c_i64, c_i64,        # logits, dtype, rows, experts, stride
+        c_vp, c_i64, c_vp, c_int,                # topk_ids, top_k, is_padding, scoring
+        c_vp, c_vp, c_vp, c_vp, c_i64, c_vp,     # loss, counts, stats, workspace, bytes, stream
+    ]),
+    "moe_balance_grad": (c_int, [
+        c_vp, c_int, c_i64, c_i64, c_i64,        # logits, dtype, rows, experts, stride
+        c_vp, c_int, c_vp, c_vp, c_vp, c_vp,     # is_padding, scoring, stats, upstream, grad, stream
     ]),
     "moe_split_align": (c_int, [
         c_vp, c_i64, c_i64, c_vp, c_vp, c_i64,  # topk_ids, numel, num_experts, expert_map, cover, rows
