@@ -146,6 +146,20 @@ def test_linear_matches_the_oracle(mx, device, rows, k, n, dtype):
         assert_product(y, a, wv, y.dtype, k)
 
 
+@pytest.mark.parametrize("rows,k,n,out", [
+    (1500, 288, 2200, torch.bfloat16), (1500, 320, 2205, torch.float32), (3600, 288, 3730, torch.bfloat16),
+    (3585, 512, 3704, torch.float32), (3600, 544, 3704, torch.float16), (1290, 800, 2304, torch.float16)])
+def test_many_tiles(mx, device, rows, k, n, out):
+    """Enough tiles of every size, ragged on each side, ends of k inside a stage."""
+    print(f"tiles {rows}x{k}x{n} {out}", flush=True)
+    rng = np.random.default_rng(rows + k)
+    a, sa, av = random_packed(rng, device, rows, k, spread=2)
+    w, ws, wv = random_packed(rng, device, n, k, spread=2)
+    if out is torch.float16:
+        sa, av = sa - 6, av / 64  # keeps the sums inside FP16
+    assert_product(mx.mxfp4_matmul(a, sa, w, ws, out), av, wv, out, k)
+
+
 @pytest.mark.parametrize("rows,k,n", SIZES)
 def test_matmul_matches_the_oracle_and_the_linear(mx, device, rows, k, n):
     print(f"matmul {rows}x{k}x{n}", flush=True)

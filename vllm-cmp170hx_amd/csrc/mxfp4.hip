@@ -7,6 +7,7 @@
 
 #include "../../include/vllm_mi355x.h"
 #include "mxfp4.h"
+#include "mxfp4_tile.h"
 
 namespace mx {
 namespace {
@@ -86,7 +87,43 @@ __global__ __launch_bounds__(64) void matmul_kernel(MatmulArgs g) {
   }
 }
 
+#ifdef MX_TUNE
+int g_force = 0;
+#endif
+
+template <int kN, int kM>
+int launch_tile(const MatmulArgs& g, hipStream_t s) {
+  TileArgs t{};
+  t.a = g.a;
+  t.as = g.as;
+  t.w = g.w;
+  t.ws = g.ws;
+  t.rows = g.rows;
+  t.n = g.n;
+  t.blocks = g.blocks;
+  t.out = g.out;
+  t.out_dtype = g.out_dtype;
+  t.wide = g.n % 8 == 0 && aligned(g.out, 16);
+  t.tiles_n = int((g.n + 64 * kN - 1) / (64 * kN));
+  t.tiles_m = int((g.rows + 64 * kM - 1) / (64 * kM));
+  const int64_t total = int64_t(t.tiles_n) * t.tiles_m;
+  hipLaunchKernelGGL((tile_kernel<kN, kM, kDense>), dim3(unsigned((total + 7) / 8 * 8)), dim3(kTileThreads), 0, s, t);
+  return vq::check_launch("mxfp4 tile");
+}
+
+int64_t tiles_of(const MatmulArgs& g, int cols, int rows) { return ((g.n + cols - 1) / cols) * ((g.rows + rows - 1) / rows); }
+
 int launch_matmul(const MatmulArgs& g, hipStream_t s) {
+  // the tile kernel: whole stages of blocks, tiles below 2 GiB, a grid in 32 bits
+  if (g.rows > 32 && g.blocks >= kStageBlocks && int64_t(g.blocks) * kBlockBytes * 256 <= INT_MAX && tiles_of(g, 64, 64) <= INT_MAX / 8) {
+    int force = 0;
+#ifdef MX_TUNE
+    force = g_force;
+#endif
+    if (force == 44 || (!force && tiles_of(g, 256, 256) >= 200)) return launch_tile<4, 4>(g, s);
+    if (force == 22 || (!force && tiles_of(g, 128, 128) >= 200)) return launch_tile<2, 2>(g, s);
+    if (force == 11 || !force) return launch_tile<1, 1>(g, s);
+  }
   const int64_t tiles_n = (g.n + 15) / 16, tiles_m = (g.rows + 15) / 16;
   if (tiles_n > INT_MAX || tiles_m > 65535) return vq::fail("mxfp4: too many rows or columns");
   hipLaunchKernelGGL(matmul_kernel, dim3(unsigned(tiles_n), unsigned(tiles_m)), dim3(64), 0, s, g);
@@ -242,3 +279,7 @@ extern "C" int mxfp4_linear(const void* x, int x_dtype, int64_t rows, int64_t k,
   if (int rc = launch_quantize(x, x_dtype, rows, k, x_stride, codes, scales, s)) return rc;
   return launch_matmul({codes, scales, w, w_scales, rows, n, int(k / kBlock), out, out_dtype}, s);
 }
+
+#ifdef MX_TUNE
+extern "C" void mx_force(int f) { mx::g_force = f; }
+#endif

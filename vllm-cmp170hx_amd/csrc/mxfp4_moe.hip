@@ -11,12 +11,17 @@
 #include "../../include/vllm_mi355x.h"
 #include "moe_rows.h"
 #include "mxfp4.h"
+#include "mxfp4_tile.h"
 
 namespace mx {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTaskRows = 16;
+constexpr int kTileRows = 128;  // rows of a task on the tile kernel
+#ifdef MX_TUNE
+int g_moe_force = 0;
+#endif
 
 // The local expert of a slot: through the map where the call brings one, -1
 // outside [0, experts).
@@ -94,13 +99,6 @@ __device__ __forceinline__ f32x4_t row_tile(const GemmArgs& g, int64_t arow, int
     acc = mfma16(wv, sw, av, sa, acc);
   }
   return acc;
-}
-
-// SiLU(min(g, L)) clamp(u, -L, L); a NaN stays one (comparisons, not fminf).
-__device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  g = g > limit ? limit : g;
-  u = u > limit ? limit : (u < -limit ? -limit : u);
-  return g / (1.0f + __expf(-g)) * u;
 }
 
 // One wavefront: a task's rows (at most 16) by 32 columns of h.
@@ -244,6 +242,11 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   if (groups > INT_MAX || sums > INT_MAX || lay.max_tasks > 65535) return vq::fail("mxfp4 moe: too many rows");
   const bool wide = aligned(x, 16) && x_stride % 8 == 0;
   const size_t lds = size_t(experts) * sizeof(int);
+  bool tiles = slots >= 24 * std::min(experts, slots) && hb >= kStageBlocks && ib >= kStageBlocks && hidden * inter < (int64_t(1) << 31) &&
+               tokens * hidden / 2 < (int64_t(1) << 31);
+#ifdef MX_TUNE
+  if (g_moe_force) tiles = g_moe_force == 2;
+#endif
   uint32_t* xq = reinterpret_cast<uint32_t*>(base + ws.xq);
   if (act_dtype == vq::kBF16) {
     hipLaunchKernelGGL(count_quantize_kernel<vq::kBF16>, dim3(unsigned(groups)), dim3(moe::kRowsPartThreads), lds, st, of, lay, table,
@@ -253,8 +256,42 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
                        x, tokens, int(hb), x_stride, wide, xq, base + ws.xs);
   }
   if (int rc = vq::check_launch("mxfp4 moe count")) return rc;
-  hipLaunchKernelGGL(fill_kernel, dim3(unsigned(lay.parts())), dim3(moe::kRowsPartThreads), lds, st, lay, table, kTaskRows);
+  hipLaunchKernelGGL(fill_kernel, dim3(unsigned(lay.parts())), dim3(moe::kRowsPartThreads), lds, st, lay, table, tiles ? kTileRows : kTaskRows);
   if (int rc = vq::check_launch("mxfp4 moe fill")) return rc;
+  if (tiles) {
+    TileArgs t{};
+    t.a = base + ws.xq;
+    t.as = base + ws.xs;
+    t.a_rows = tokens;
+    t.w = w13;
+    t.ws = s13;
+    t.n = 2 * inter;
+    t.blocks = int(hb);
+    t.tiles_n = int((inter + 63) / 64);
+    t.table = table;
+    t.tasks = lay.tasks();
+    t.sorted = lay.sorted();
+    t.topk_w = topk_w;
+    t.top_k = int(top_k);
+    t.limit = limit;
+    t.h = base + ws.hq;
+    t.hs = base + ws.hs;
+    const int64_t bound = (slots / kTileRows + std::min(experts, slots) + 7) / 8 * 8;
+    hipLaunchKernelGGL((tile_kernel<2, 2, kGateUp>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
+    if (int rc = vq::check_launch("mxfp4 moe gate_up")) return rc;
+    t.a = base + ws.hq;
+    t.as = base + ws.hs;
+    t.w = w2;
+    t.ws = s2;
+    t.n = hidden;
+    t.blocks = int(ib);
+    t.tiles_n = int((hidden + 127) / 128);
+    t.out = base + ws.c3;
+    hipLaunchKernelGGL((tile_kernel<2, 2, kDown>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
+    if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
+    hipLaunchKernelGGL(slot_sum_kernel, dim3(unsigned(sums)), dim3(kThreads), 0, st, static_cast<const float*>(t.out), of, tokens, int(top_k), int(hidden), out, act_dtype);
+    return vq::check_launch("mxfp4 moe sum");
+  }
   GemmArgs g{};
   g.a = base + ws.xq;
   g.as = base + ws.xs;
@@ -284,3 +321,7 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   hipLaunchKernelGGL(slot_sum_kernel, dim3(unsigned(sums)), dim3(kThreads), 0, st, g.out, of, tokens, int(top_k), int(hidden), out, act_dtype);
   return vq::check_launch("mxfp4 moe sum");
 }
+
+#ifdef MX_TUNE
+extern "C" void mx_moe_force(int f) { mx::g_moe_force = f; }
+#endif

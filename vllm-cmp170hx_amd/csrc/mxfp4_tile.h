@@ -1,0 +1,408 @@
+// The many-row product of MXFP4 activations with MXFP4 weights, dense and for
+// the routed experts' tasks.
+//
+// One workgroup of four wavefronts (2 x 2) computes 64 kN columns by 64 kM
+// rows, each wavefront 32 kN x 32 kM of v_mfma_scale_f32_32x32x64 tiles (its
+// rate is twice the 16x16x128 form's: 8.9 against 4.6 PFLOP/s in a loop of
+// nothing else).  A stage is 256 k: the 128 code bytes and 8 scale bytes of
+// every row and column.
+//  * Codes come to LDS by DMA, one 128-byte line of a row in eight lanes, the
+//    next stage's while this one is multiplied (two buffers, one barrier a
+//    stage).  A row's eight 16-byte blocks lie in LDS in the order kb ^ (row / 2
+//    & 7), so that the 16 rows that a ds_read_b128 reads at once, all at one kb,
+//    lie on 16 different 16-byte columns of the 64 banks.
+//  * A lane of the 32x32x64 form holds one block: row lane & 31, block 2 sub +
+//    (lane >> 5) of the stage's 64-k sub-step `sub`.  Scales come through
+//    registers, a row's even blocks' bytes in one dword and the odd blocks' in
+//    another: a lane reads one dword a row and stage, and the MFMA's byte
+//    selector is `sub`.
+//  * Weights are the A operand, rows the B operand, so that a lane's sums are
+//    of one row: 16 of a 32-column block, the other 16 in lane ^ 32.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mxfp4.h"
+
+namespace mx {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+constexpr int kTileThreads = 256;
+constexpr int kStageBlocks = 8;                          // 256 k
+constexpr int kStageBytes = kStageBlocks * kBlockBytes;  // of codes, a row
+
+enum TileMode : int { kDense = 0, kGateUp = 1, kDown = 2 };
+
+struct TileArgs {
+  const uint8_t *a, *as;  // activations: rows of `blocks` blocks
+  int64_t a_rows;         // kGateUp: tokens
+  const uint8_t *w, *ws;  // kDense [n], kGateUp [experts][n = 2 inter], kDown [experts][n]
+  int64_t rows, n;
+  int blocks;
+  void* out;              // kDense: [rows][n] of out_dtype; kDown: FP32 [slots][n]
+  int out_dtype;
+  int wide;               // kDense: n a multiple of eight, out 16-byte aligned
+  int tiles_n, tiles_m;   // kDense: workgroups; else tiles_n alone
+  // the routed forms
+  const int32_t* table;
+  int64_t tasks, sorted;  // offsets in the table
+  const float* topk_w;
+  int top_k;
+  float limit;
+  uint8_t *h, *hs;        // kGateUp: rows of n / 2
+};
+
+// SiLU(min(g, L)) clamp(u, -L, L); a NaN stays one (comparisons, not fminf).
+__device__ __forceinline__ float swiglu(float g, float u, float limit) {
+  g = g > limit ? limit : g;
+  u = u > limit ? limit : (u < -limit ? -limit : u);
+  return g / (1.0f + __expf(-g)) * u;
+}
+
+// Two values rounded to nearest even, the first one in the low half.
+template <int kDtype>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (kDtype == vq::kBF16) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, bf16x2_t{__bf16(a), __bf16(b)});  // v_cvt_pk_bf16_f32
+  } else {
+    return uint32_t(__builtin_bit_cast(uint16_t, _Float16(a))) | (uint32_t(__builtin_bit_cast(uint16_t, _Float16(b))) << 16);
+  }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, int(bytes), 0x00020000);
+}
+
+// An offset past any buffer: such loads give zeros.
+constexpr uint32_t kPastEnd = 0x80000000u;
+
+// Eight scale bytes of a row of at least eight blocks, from block b0 on (the
+// last eight, where fewer are left), as they come from memory,
+__device__ __forceinline__ uint64_t load_scales(const uint8_t* row, int b0, int blocks) {
+  uint64_t v;
+  __builtin_memcpy(&v, row + min(b0, blocks - kStageBlocks), 8);
+  return v;
+}
+// and block b0's first, 127 past the row, as the even blocks' dword and the odd
+// blocks'.
+__device__ __forceinline__ uint2 order_scales(uint64_t v, int b0, int blocks) {
+  const int past = max(b0 - (blocks - kStageBlocks), 0) * 8;  // bits, less than 64
+  if (past) v = (v >> past) | (0x7f7f7f7f7f7f7f7full << (64 - past));
+  const uint32_t lo = uint32_t(v), hi = uint32_t(v >> 32);
+  return make_uint2(__builtin_amdgcn_perm(hi, lo, 0x06040200u), __builtin_amdgcn_perm(hi, lo, 0x07050301u));
+}
+
+template <int kSub>
+__device__ __forceinline__ void mfma32(f32x16_t& acc, const u32x4_t& a, uint32_t sa, const u32x4_t& b, uint32_t sb) {
+  const i32x8_t av{int(a[0]), int(a[1]), int(a[2]), int(a[3]), 0, 0, 0, 0};
+  const i32x8_t bv{int(b[0]), int(b[1]), int(b[2]), int(b[3]), 0, 0, 0, 0};
+  acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc, 4, 4, kSub, int(sa), kSub, int(sb));
+}
+
+// 32 rows of 32 kN columns from LDS to the output, eight columns a lane (n a
+// multiple of eight, rows 16-byte aligned).  sorted: the rows' slots, whose
+// router weights multiply them.
+template <int kN, int kDtype>
+__device__ __forceinline__ void store_rows(const float* part, int stride, int lane, int mt, int nrows, int ct, const TileArgs& g,
+                                           int64_t m0, const int32_t* sorted) {
+  constexpr int kChunks = 4 * kN;  // of eight columns, a row
+  const int ch = lane % kChunks, r0 = lane / kChunks;
+  const int c = ct + 8 * ch;
+#pragma unroll
+  for (int k = 0; k < kChunks / 2; ++k) {
+    const int mr = r0 + k * (64 / kChunks);
+    const int m = mt + mr;
+    const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(part + mr * stride + 8 * ch);
+    const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(part + mr * stride + 8 * ch + 4);
+    if (m >= nrows || c >= g.n) continue;
+    int64_t row = m0 + m;
+    float weight = 1;
+    if (sorted) {
+      row = sorted[m];
+      weight = g.topk_w[row];
+    }
+    const int64_t at = row * g.n + c;
+    if constexpr (kDtype == vq::kFP32) {
+      float* out = static_cast<float*>(g.out) + at;
+      *reinterpret_cast<f32x4_t*>(out) = lo * weight;
+      *reinterpret_cast<f32x4_t*>(out + 4) = hi * weight;
+    } else {
+      u32x4_t w;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = pack16<kDtype>((q < 2 ? lo : hi)[2 * (q & 1)], (q < 2 ? lo : hi)[2 * (q & 1) + 1]);
+      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(g.out) + at) = w;
+    }
+  }
+}
+
+template <int kN, int kM, int kMode>
+__global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel(TileArgs g) {
+  constexpr int kCols = 64 * kN, kRows = 64 * kM, kLines = kCols + kRows;
+  constexpr int kLoadsW = kCols / 32, kLoadsA = kRows / 32;  // 1 KB DMA loads a wavefront and stage
+  constexpr int kLoads = kLoadsW + kLoadsA;
+  constexpr int kScaleRows = (kLines + kTileThreads - 1) / kTileThreads;
+  __shared__ __attribute__((aligned(1024))) uint8_t buf0[kLines * kStageBytes], buf1[kLines * kStageBytes];
+  __shared__ __attribute__((aligned(16))) uint2 scale0[kLines], scale1[kLines];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = vq::uniform(tid >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  const int wn = wave & 1, wm = wave >> 1;
+
+  // ---- which columns and rows
+  int64_t wbase = 0;   // first weight row of the matrix
+  int c0, nrows;       // first column (kGateUp: of h); rows of this tile
+  int64_t m0 = 0;      // kDense: first row; else the task's first sorted row
+  const int32_t* sorted = nullptr;
+  const int inter = int(g.n / 2);
+  if constexpr (kMode == kDense) {
+    // XCD x (workgroups x, x + 8, ...) takes a run of tiles, rows first: it
+    // fetches few weight columns and its L2 keeps them for all the rows
+    const int total = g.tiles_n * g.tiles_m, per = (total + 7) / 8;
+    const int t = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
+    if (int(blockIdx.x >> 3) >= per || t >= total) return;
+    c0 = t / g.tiles_m * kCols;
+    m0 = int64_t(t % g.tiles_m) * kRows;
+    nrows = int(min(int64_t(kRows), g.rows - m0));
+  } else {
+    // XCD x takes tasks x, x + 8, ..., a task's columns one after another
+    const int local = int(blockIdx.x >> 3);
+    const int task = local / g.tiles_n * 8 + int(blockIdx.x & 7);
+    if (task >= g.table[0]) return;
+    const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[task];
+    wbase = int64_t(vq::uniform(tk.x)) * g.n;
+    m0 = vq::uniform(tk.y);
+    nrows = vq::uniform(tk.z);
+    sorted = g.table + g.sorted + m0;
+    c0 = local % g.tiles_n * (kMode == kGateUp ? kCols / 2 : kCols);
+  }
+  // the weight row of the tile's line i (< kCols): kGateUp has, per wavefront
+  // column, kN / 2 gate blocks and then their up blocks
+  const auto weight_row = [&](int i) -> int64_t {
+    if constexpr (kMode == kGateUp) {
+      const int half = i / (32 * kN), j = i % (32 * kN) / 32;
+      const bool up = j >= kN / 2;
+      const int c = c0 + 16 * kN * half + 32 * (up ? j - kN / 2 : j) + (i & 31);
+      return min(c, inter - 1) + (up ? inter : 0);
+    } else {
+      return min(int64_t(c0 + i), g.n - 1);
+    }
+  };
+  const auto act_row = [&](int i) -> int64_t {  // relative to the activations' base
+    const int t = min(i, nrows - 1);
+    if constexpr (kMode == kGateUp) return sorted[t] / g.top_k;
+    return t;
+  };
+  const int64_t act0 = kMode == kGateUp ? 0 : m0;
+  const int64_t line = int64_t(g.blocks) * kBlockBytes;
+  // this tile's weight rows from the first one's address on
+  const int64_t w0 = kMode == kGateUp ? 0 : c0;
+  const int w_rows = kMode == kGateUp ? int(g.n) : int(min(int64_t(kCols), g.n - c0));
+  const __amdgpu_buffer_rsrc_t wbuf = buffer(g.w + (wbase + w0) * line, uint32_t(w_rows) * uint32_t(line));
+  const __amdgpu_buffer_rsrc_t abuf =
+      buffer(g.a + act0 * line, uint32_t(kMode == kGateUp ? g.a_rows : int64_t(nrows)) * uint32_t(line));
+
+  // ---- loads: 1 KB each, 8 lines; a wavefront's first kLoadsW bring weights.
+  // Rows that follow each other: the first one's offset is scalar (a row of the
+  // buffer also where the eight lie past its end: their sums are not stored; the
+  // rest of eight that begin inside it are zeros), and the lane's part has two
+  // values, by the parity of the line's eight.  Scattered rows (kGateUp's
+  // tokens): an offset a lane and load.
+  const uint32_t rline = uint32_t(line);
+  const int sub_row = lane >> 3;
+  const auto first_line = [&](int i) { return i < kLoadsW ? 8 * (kLoadsW * wave + i) : kCols + 8 * (kLoadsA * wave + i - kLoadsW); };
+  const auto block_of = [&](int parity) { return (lane & 7) ^ ((4 * parity + (sub_row >> 1)) & 7); };
+  const int kb[2] = {block_of(0), block_of(1)};
+  const uint32_t lane_off[2] = {sub_row * rline + kb[0] * kBlockBytes, sub_row * rline + kb[1] * kBlockBytes};
+  uint32_t token_off[kMode == kGateUp ? kLoadsA : 1];
+  if constexpr (kMode == kGateUp) {
+#pragma unroll
+    for (int i = 0; i < kLoadsA; ++i) {
+      token_off[i] = uint32_t(act_row(first_line(kLoadsW + i) - kCols + sub_row)) * rline + kb[(kLoadsA * wave + i) & 1] * kBlockBytes;
+    }
+  }
+  // the scalar first row of load i
+  const auto first_row = [&](int i) -> int {
+    if (i >= kLoadsW) return first_line(i) - kCols < nrows ? first_line(i) - kCols : 0;
+    if constexpr (kMode == kGateUp) {
+      const int l = first_line(i), half = l / (32 * kN), j = l % (32 * kN) / 32;
+      const bool up = j >= kN / 2;
+      const int c = c0 + 16 * kN * half + 32 * (up ? j - kN / 2 : j) + (l & 31);
+      return (c < inter ? c : 0) + (up ? inter : 0);  // inter: whole eights
+    }
+    return first_line(i) < w_rows ? first_line(i) : 0;
+  };
+  const uint8_t* srow[kScaleRows];
+#pragma unroll
+  for (int i = 0; i < kScaleRows; ++i) {
+    const int l = min(tid + i * kTileThreads, kLines - 1);
+    srow[i] = l < kCols ? g.ws + (wbase + weight_row(l)) * g.blocks : g.as + (act0 + act_row(l - kCols)) * g.blocks;
+  }
+  const int stages = (g.blocks + kStageBlocks - 1) / kStageBlocks;
+  uint64_t sreg[kScaleRows];
+  const auto fetch = [&](int s, uint8_t* buf) {
+    const int left = g.blocks - s * kStageBlocks;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int parity = (i < kLoadsW ? kLoadsW * wave + i : kLoadsA * wave + i - kLoadsW) & 1;
+      const bool scattered = kMode == kGateUp && i >= kLoadsW;
+      const uint32_t lane_part = scattered ? token_off[scattered ? i - kLoadsW : 0] : lane_off[parity];
+      const uint32_t o = left >= kStageBlocks || kb[parity] < left ? lane_part : kPastEnd;
+      const int row_part = scattered ? 0 : first_row(i) * int(rline);
+      // (the scalar offset stays below the buffer's size, or its bounds check would wrap)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? wbuf : abuf, (lds_ptr_t)(buf + first_line(i) * kStageBytes), 16,
+                                               int(o), row_part + (left > 0 ? s * kStageBytes : 0), 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i) sreg[i] = load_scales(srow[i], s * kStageBlocks, g.blocks);
+    __builtin_amdgcn_sched_barrier(0);  // issued here, not where their results are waited for
+  };
+
+  f32x16_t acc[kN][kM];
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+#pragma unroll
+    for (int j = 0; j < kM; ++j)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) acc[i][j][k] = 0;
+
+  const int wline = 32 * kN * wn + r, aline = kCols + 32 * kM * wm + r;
+  const int swizzle = (r >> 1) & 7;
+  const auto multiply = [&](const uint8_t* buf, const uint2* scales) {
+    uint32_t sw[kN], sa[kM];
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(scales);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) sw[i] = words[2 * (wline + 32 * i) + h];
+#pragma unroll
+    for (int j = 0; j < kM; ++j) sa[j] = words[2 * (aline + 32 * j) + h];
+    u32x4_t fw[2][kN], fa[2][kM];
+    const auto read = [&](int sub, u32x4_t (&w)[kN], u32x4_t (&a)[kM]) {
+      const int at = ((2 * sub + h) ^ swizzle) * kBlockBytes;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) w[i] = *reinterpret_cast<const u32x4_t*>(buf + (wline + 32 * i) * kStageBytes + at);
+#pragma unroll
+      for (int j = 0; j < kM; ++j) a[j] = *reinterpret_cast<const u32x4_t*>(buf + (aline + 32 * j) * kStageBytes + at);
+    };
+    read(0, fw[0], fa[0]);
+    const auto step = [&](auto sub_c) {
+      constexpr int sub = decltype(sub_c)::value;
+      // the next sub-step's operands are on their way while this one's are multiplied
+      if constexpr (sub < 3) read(sub + 1, fw[(sub + 1) & 1], fa[(sub + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+#pragma unroll
+        for (int j = 0; j < kM; ++j) mfma32<sub>(acc[i][j], fw[sub & 1][i], sw[i], fa[sub & 1][j], sa[j]);
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 3>{});
+  };
+  // a stage: its codes and scales have landed; every wavefront has read the
+  // other buffers (the barrier), which then take the next stage (zeros past the
+  // last one).  Stages in pairs, one buffer each by name: the compiler then sees
+  // that a stage's reads are not of the buffer that the DMA is filling.
+  const auto land = [&](int s, uint2* scales) {
+    vq::wait_vmcnt<0>();
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i) {
+      if (kLines % kTileThreads == 0 || tid + i * kTileThreads < kLines) {
+        scales[tid + i * kTileThreads] = order_scales(sreg[i], s * kStageBlocks, g.blocks);
+      }
+    }
+    __syncthreads();
+  };
+  fetch(0, buf0);
+  int s = 0;
+  for (; s + 1 < stages; s += 2) {
+    land(s, scale0);
+    fetch(s + 1, buf1);
+    multiply(buf0, scale0);
+    land(s + 1, scale1);
+    fetch(s + 2, buf0);
+    multiply(buf1, scale1);
+  }
+  land(min(s, stages - 1), scale0);
+  if (s < stages) multiply(buf0, scale0);
+
+  // ---- results
+  if constexpr (kMode == kGateUp) {
+    // block j of this wavefront: column cb .. cb + 31 of h, row m = lane & 31 of
+    // row tile i; this lane holds elements 8 p + 4 h + q (p, q < 4)
+#pragma unroll
+    for (int j = 0; j < kN / 2; ++j) {
+      const int cb = c0 + 16 * kN * wn + 32 * j;
+      if (cb >= inter) continue;
+#pragma unroll
+      for (int i = 0; i < kM; ++i) {
+        float v[16];
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          v[k] = swiglu(acc[j][i][k], acc[j + kN / 2][i][k], g.limit);
+          top = max(top, magnitude(v[k]));
+        }
+        top = max(top, uint32_t(__shfl_xor(int(top), 32)));
+        const uint32_t s = block_scale(top);
+        const uint32_t w0v = s == 255u ? 0u : codes8(v, s), w1v = s == 255u ? 0u : codes8(v + 8, s);
+        // halves 8 p + 4 h: even h low, odd h high in dword p
+        const uint32_t o0 = uint32_t(__shfl_xor(int(w0v), 32)), o1 = uint32_t(__shfl_xor(int(w1v), 32));
+        const int m = 32 * (kM * wm + i) + r;
+        if (h == 0 && m < nrows) {
+          u32x4_t block;
+          block[0] = (w0v & 0xffffu) | (o0 << 16);
+          block[1] = (w0v >> 16) | (o0 & 0xffff0000u);
+          block[2] = (w1v & 0xffffu) | (o1 << 16);
+          block[3] = (w1v >> 16) | (o1 & 0xffff0000u);
+          const int64_t row = m0 + m;
+          *reinterpret_cast<u32x4_t*>(g.h + row * (inter / 2) + cb / 2) = block;
+          g.hs[row * (inter / kBlock) + cb / kBlock] = uint8_t(s);
+        }
+      }
+    }
+  } else {
+    // each row tile through LDS (a wavefront's own part, rows 16 bytes apart
+    // from a bank's multiple), then whole rows of 32 kN columns
+    constexpr int kStride = 32 * kN + 4;
+    static_assert(2 * 32 * kStride * 4 <= int(sizeof(buf0)), "two wavefronts' exchange fits a stage buffer");
+    float* part = reinterpret_cast<float*>(wave < 2 ? buf0 : buf1) + (wave & 1) * 32 * kStride;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kM; ++i) {
+#pragma unroll
+      for (int j = 0; j < kN; ++j) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          f32x4_t v;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = acc[j][i][4 * p + q];
+          *reinterpret_cast<f32x4_t*>(part + r * kStride + 32 * j + 8 * p + 4 * h) = v;
+        }
+      }
+      const int mt = 32 * (kM * wm + i), ct = c0 + 32 * kN * wn;
+      if constexpr (kMode == kDense) {
+        if (g.wide) {
+          if (g.out_dtype == vq::kBF16) store_rows<kN, vq::kBF16>(part, kStride, lane, mt, nrows, ct, g, m0, nullptr);
+          else if (g.out_dtype == vq::kFP16) store_rows<kN, vq::kFP16>(part, kStride, lane, mt, nrows, ct, g, m0, nullptr);
+          else store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, m0, nullptr);
+        } else {
+          for (int at = lane; at < 32 * 32 * kN; at += 64) {
+            const int m = mt + at / (32 * kN), c = ct + at % (32 * kN);
+            if (m < nrows && c < g.n) {
+              vq::store_act(g.out, g.out_dtype, (m0 + m) * g.n + c, part[at / (32 * kN) * kStride + at % (32 * kN)]);
+            }
+          }
+        }
+      } else {
+        store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, m0, sorted);
+      }
+    }
+  }
+}
+
+}  // namespace mx
