@@ -34,6 +34,19 @@ constexpr int kTileThreads = 256;
 constexpr int kStageBlocks = 8;                          // 256 k
 constexpr int kStageBytes = kStageBlocks * kBlockBytes;  // of codes, a row
 
+// f(std::integral_constant<int, i>) for i = first .. last - 1.
+template <int first, int last, typename F>
+__device__ __forceinline__ void for_range(F&& f) {
+  if constexpr (first < last) {
+    f(std::integral_constant<int, first>{});
+    for_range<first + 1, last>(f);
+  }
+}
+template <int n, typename F>
+__device__ __forceinline__ void for_each(F&& f) {
+  for_range<0, n>(f);
+}
+
 enum TileMode : int { kDense = 0, kGateUp = 1, kDown = 2 };
 
 struct TileArgs {
@@ -243,23 +256,36 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
     srow[i] = l < kCols ? g.ws + (wbase + weight_row(l)) * g.blocks : g.as + (act0 + act_row(l - kCols)) * g.blocks;
   }
   const int stages = (g.blocks + kStageBlocks - 1) / kStageBlocks;
-  uint64_t sreg[kScaleRows];
-  const auto fetch = [&](int s, uint8_t* buf) {
+  // DMA load i of stage s (zeros past the last stage)
+  const auto fetch = [&](auto i_c, int s, uint8_t* buf) {
+    constexpr int i = decltype(i_c)::value;
     const int left = g.blocks - s * kStageBlocks;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int parity = (i < kLoadsW ? kLoadsW * wave + i : kLoadsA * wave + i - kLoadsW) & 1;
-      const bool scattered = kMode == kGateUp && i >= kLoadsW;
-      const uint32_t lane_part = scattered ? token_off[scattered ? i - kLoadsW : 0] : lane_off[parity];
-      const uint32_t o = left >= kStageBlocks || kb[parity] < left ? lane_part : kPastEnd;
-      const int row_part = scattered ? 0 : first_row(i) * int(rline);
-      // (the scalar offset stays below the buffer's size, or its bounds check would wrap)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? wbuf : abuf, (lds_ptr_t)(buf + first_line(i) * kStageBytes), 16,
-                                               int(o), row_part + (left > 0 ? s * kStageBytes : 0), 0, 0);
-    }
+    const int parity = (i < kLoadsW ? kLoadsW * wave + i : kLoadsA * wave + i - kLoadsW) & 1;
+    constexpr bool scattered = kMode == kGateUp && i >= kLoadsW;
+    const uint32_t lane_part = scattered ? token_off[scattered ? i - kLoadsW : 0] : lane_off[parity];
+    const uint32_t o = left >= kStageBlocks || kb[parity] < left ? lane_part : kPastEnd;
+    const int row_part = scattered ? 0 : first_row(i) * int(rline);
+    // (the scalar offset stays below the buffer's size, or its bounds check would wrap)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? wbuf : abuf, (lds_ptr_t)(buf + first_line(i) * kStageBytes), 16,
+                                             int(o), row_part + (left > 0 ? s * kStageBytes : 0), 0, 0);
+  };
+  uint64_t sreg[kScaleRows];
+  const auto fetch_scales = [&](int s) {
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i) sreg[i] = load_scales(srow[i], s * kStageBlocks, g.blocks);
-    __builtin_amdgcn_sched_barrier(0);  // issued here, not where their results are waited for
+  };
+  // stage s has landed (its loads of this wavefront, then everyone's), and no
+  // wavefront reads the buffer before it any more
+  const auto land = [&](int s, uint2* scales) {
+    vq::wait_vmcnt<0>();
+    const int b0 = min(s, stages - 1) * kStageBlocks;
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i) {
+      if (kLines % kTileThreads == 0 || tid + i * kTileThreads < kLines) {
+        scales[tid + i * kTileThreads] = order_scales(sreg[i], b0, g.blocks);
+      }
+    }
+    __syncthreads();
   };
 
   f32x16_t acc[kN][kM];
@@ -272,63 +298,71 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
 
   const int wline = 32 * kN * wn + r, aline = kCols + 32 * kM * wm + r;
   const int swizzle = (r >> 1) & 7;
-  const auto multiply = [&](const uint8_t* buf, const uint2* scales) {
-    uint32_t sw[kN], sa[kM];
+  uint32_t sw[2][kN], sa[2][kM];          // this stage's scales and the next one's
+  u32x4_t fw[2][kN], fa[2][kM];           // this sub-step's operands and the next one's
+  const auto read_scales = [&](const uint2* scales, uint32_t (&w)[kN], uint32_t (&a)[kM]) {
     const uint32_t* words = reinterpret_cast<const uint32_t*>(scales);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) sw[i] = words[2 * (wline + 32 * i) + h];
+    for (int i = 0; i < kN; ++i) w[i] = words[2 * (wline + 32 * i) + h];
 #pragma unroll
-    for (int j = 0; j < kM; ++j) sa[j] = words[2 * (aline + 32 * j) + h];
-    u32x4_t fw[2][kN], fa[2][kM];
-    const auto read = [&](int sub, u32x4_t (&w)[kN], u32x4_t (&a)[kM]) {
-      const int at = ((2 * sub + h) ^ swizzle) * kBlockBytes;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) w[i] = *reinterpret_cast<const u32x4_t*>(buf + (wline + 32 * i) * kStageBytes + at);
-#pragma unroll
-      for (int j = 0; j < kM; ++j) a[j] = *reinterpret_cast<const u32x4_t*>(buf + (aline + 32 * j) * kStageBytes + at);
-    };
-    read(0, fw[0], fa[0]);
-    const auto step = [&](auto sub_c) {
-      constexpr int sub = decltype(sub_c)::value;
-      // the next sub-step's operands are on their way while this one's are multiplied
-      if constexpr (sub < 3) read(sub + 1, fw[(sub + 1) & 1], fa[(sub + 1) & 1]);
+    for (int j = 0; j < kM; ++j) a[j] = words[2 * (aline + 32 * j) + h];
+  };
+  // operand i of a sub-step: kN of weights, then kM of rows
+  const auto read = [&](auto i_c, const uint8_t* buf, int sub, int set) {
+    constexpr int i = decltype(i_c)::value;
+    const int at = ((2 * sub + h) ^ swizzle) * kBlockBytes;
+    if constexpr (i < kN) fw[set][i] = *reinterpret_cast<const u32x4_t*>(buf + (wline + 32 * i) * kStageBytes + at);
+    else fa[set][i - kN] = *reinterpret_cast<const u32x4_t*>(buf + (aline + 32 * (i - kN)) * kStageBytes + at);
+  };
+  // Sub-step `sub` of a stage, in kN groups of kM MFMAs: beside them the next
+  // sub-step's operands are read (of `next`, at sub-step next_sub) and loads
+  // kFirst .. kLast - 1 of stage s issued into `into`.  A wavefront issues in
+  // order and alone on its SIMD, so loads in one burst would hold up its MFMAs
+  // (16 cycles a load and CU): spread out they cost nothing.
+  const auto step = [&](auto sub_c, auto first_c, auto last_c, int set, const uint8_t* next, int next_sub, int s, uint8_t* into) {
+    constexpr int sub = decltype(sub_c)::value, kFirst = decltype(first_c)::value, kLast = decltype(last_c)::value;
+    for_each<kN>([&](auto i_c) {
+      constexpr int i = decltype(i_c)::value;
+      constexpr int kReads = kN + kM;
+      for_range<i * kReads / kN, (i + 1) * kReads / kN>([&](auto k) { read(k, next, next_sub, (sub + 1) & 1); });
+      for_range<kFirst + i * (kLast - kFirst) / kN, kFirst + (i + 1) * (kLast - kFirst) / kN>([&](auto k) { fetch(k, s, into); });
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < kN; ++i)
-#pragma unroll
-        for (int j = 0; j < kM; ++j) mfma32<sub>(acc[i][j], fw[sub & 1][i], sw[i], fa[sub & 1][j], sa[j]);
-    };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
-    step(std::integral_constant<int, 2>{});
-    step(std::integral_constant<int, 3>{});
+      for (int j = 0; j < kM; ++j) mfma32<sub>(acc[i][j], fw[sub & 1][i], sw[set][i], fa[sub & 1][j], sa[set][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
-  // a stage: its codes and scales have landed; every wavefront has read the
-  // other buffers (the barrier), which then take the next stage (zeros past the
-  // last one).  Stages in pairs, one buffer each by name: the compiler then sees
-  // that a stage's reads are not of the buffer that the DMA is filling.
-  const auto land = [&](int s, uint2* scales) {
-    vq::wait_vmcnt<0>();
-#pragma unroll
-    for (int i = 0; i < kScaleRows; ++i) {
-      if (kLines % kTileThreads == 0 || tid + i * kTileThreads < kLines) {
-        scales[tid + i * kTileThreads] = order_scales(sreg[i], s * kStageBlocks, g.blocks);
-      }
-    }
-    __syncthreads();
+  // Stage s from cur.  The barrier comes before the last sub-step, whose
+  // operands are in registers by then: its MFMAs run while the next stage's
+  // first operands are read.
+  constexpr int kHalf = kLoads / 2, kMore = kHalf + kLoads / 4;
+  const auto stage = [&](int s, int set, uint8_t* cur, uint8_t* next, uint2* next_scales) {
+    using std::integral_constant;
+    constexpr integral_constant<int, 0> c0{};
+    step(c0, integral_constant<int, kHalf>{}, integral_constant<int, kMore>{}, set, cur, 1, s + 1, next);
+    step(integral_constant<int, 1>{}, integral_constant<int, kMore>{}, integral_constant<int, kLoads>{}, set, cur, 2, s + 1, next);
+    step(integral_constant<int, 2>{}, c0, c0, set, cur, 3, 0, cur);
+    land(s + 1, next_scales);
+    fetch_scales(s + 2);
+    read_scales(next_scales, sw[set ^ 1], sa[set ^ 1]);
+    step(integral_constant<int, 3>{}, c0, integral_constant<int, kHalf>{}, set, next, 0, s + 2, cur);
   };
-  fetch(0, buf0);
+  for_range<0, kLoads>([&](auto k) { fetch(k, 0, buf0); });
+  fetch_scales(0);
+  land(0, scale0);
+  fetch_scales(1);
+  for_range<0, kHalf>([&](auto k) { fetch(k, 1, buf1); });
+  read_scales(scale0, sw[0], sa[0]);
+  for_range<0, kN + kM>([&](auto k) { read(k, buf0, 0, 0); });
+  // stages in pairs, one buffer each by name: the compiler then sees that a
+  // stage's reads are not of the buffer that the DMA is filling
   int s = 0;
   for (; s + 1 < stages; s += 2) {
-    land(s, scale0);
-    fetch(s + 1, buf1);
-    multiply(buf0, scale0);
-    land(s + 1, scale1);
-    fetch(s + 2, buf0);
-    multiply(buf1, scale1);
+    stage(s, 0, buf0, buf1, scale1);
+    stage(s + 1, 1, buf1, buf0, scale0);
   }
-  land(min(s, stages - 1), scale0);
-  if (s < stages) multiply(buf0, scale0);
+  if (s < stages) stage(s, 0, buf0, buf1, scale1);
+  vq::wait_vmcnt<0>();  // the last loads (zeros) are in before their buffers are used again
 
   // ---- results
   if constexpr (kMode == kGateUp) {
