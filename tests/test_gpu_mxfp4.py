@@ -126,7 +126,10 @@ def test_refusals(mx, device):
 
 
 SIZES = [(1, 32, 1), (1, 4096, 256), (2, 96, 33), (5, 2592, 77), (8, 1024, 1000), (16, 4128, 130), (17, 736, 515),
-         (33, 256, 64), (64, 2048, 512), (100, 992, 300), (129, 512, 257), (257, 1184, 384), (300, 4096, 640), (513, 160, 1031)]
+         (33, 256, 64), (64, 2048, 512), (100, 992, 300), (129, 512, 257), (257, 1184, 384), (300, 4096, 640), (513, 160, 1031),
+         # K split over workgroups, ragged; few rows whose codes come from memory, or
+         # are quantized by wide workgroups; row groups of a column group
+         (70, 4096, 192), (130, 8224, 331), (16, 8192, 96), (11, 4128, 4100), (3, 2592, 12900), (40, 2080, 777)]
 
 
 @pytest.mark.parametrize("rows,k,n", SIZES)

@@ -52,51 +52,93 @@ __device__ __forceinline__ uint32_t codes8(const float* v, uint32_t b) {
 
 __device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
-// Eight consecutive elements p[0 .. 7] as FP32; `wide`: p is 16-byte aligned.
+// Eight consecutive elements as they lie in memory.
 template <int kDtype>
-__device__ __forceinline__ void load8(const void* p, int64_t i, bool wide, float (&v)[8]) {
-  if constexpr (kDtype == vq::kFP32) {
-    const float* f = static_cast<const float*>(p) + i;
-    if (wide) {
-      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(f), b = *reinterpret_cast<const f32x4_t*>(f + 4);
+struct Eight {
+  static constexpr int kWords = kDtype == vq::kFP32 ? 8 : 4;
+  uint32_t w[kWords];
+};
+
+// Elements i .. i + 7 of p; `wide`: their address is 16-byte aligned.
+template <int kDtype>
+__device__ __forceinline__ Eight<kDtype> load8(const void* p, int64_t i, bool wide) {
+  constexpr int kWords = Eight<kDtype>::kWords;
+  Eight<kDtype> v;
+  if (wide) {
+    const u32x4_t* q = reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(p) + i * (kWords / 2));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = a[j];
-        v[4 + j] = b[j];
-      }
-    } else {
+    for (int k = 0; k < kWords / 4; ++k) {
+      const u32x4_t a = q[k];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = f[j];
+      for (int j = 0; j < 4; ++j) v.w[4 * k + j] = a[j];
     }
+  } else if constexpr (kDtype == vq::kFP32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v.w[j] = static_cast<const uint32_t*>(p)[i + j];
   } else {
     const uint16_t* h = static_cast<const uint16_t*>(p) + i;
-    uint16_t u[8];
-    if (wide) {
-      const u32x4_t a = *reinterpret_cast<const u32x4_t*>(h);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u[2 * j] = uint16_t(a[j]);
-        u[2 * j + 1] = uint16_t(a[j] >> 16);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = h[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = kDtype == vq::kBF16 ? vq::bf16_to_f32(u[j]) : vq::f16_to_f32(u[j]);
+    for (int j = 0; j < 4; ++j) v.w[j] = uint32_t(h[2 * j]) | (uint32_t(h[2 * j + 1]) << 16);
   }
+  return v;
+}
+
+// The FP32 bits of the largest magnitude of eight elements.  (16-bit magnitudes
+// order as whole numbers do, two at a time.)
+template <int kDtype>
+__device__ __forceinline__ uint32_t top8(const Eight<kDtype>& v) {
+  if constexpr (kDtype == vq::kFP32) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, v.w[j] & 0x7fffffffu);
+    return top;
+  } else {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    u16x2_t m = __builtin_bit_cast(u16x2_t, v.w[0] & 0x7fff7fffu);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, v.w[j] & 0x7fff7fffu));
+    const uint16_t top = m[0] > m[1] ? m[0] : m[1];
+    return kDtype == vq::kBF16 ? uint32_t(top) << 16 : __builtin_bit_cast(uint32_t, vq::f16_to_f32(top));
+  }
+}
+
+// Their codes under the scale byte b, as codes8.
+template <int kDtype>
+__device__ __forceinline__ uint32_t codes_of(const Eight<kDtype>& v, uint32_t b) {
+  const float scale = __builtin_bit_cast(float, b << 23);
+  uint32_t w = 0;
+  if constexpr (kDtype == vq::kFP32) {
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = __builtin_bit_cast(float, v.w[j]);
+    w = codes8(f, b);
+  } else if constexpr (kDtype == vq::kBF16) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    const auto pair = [&](int j) { return __builtin_bit_cast(bf16x2_t, v.w[j]); };
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(0), scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(1), scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(2), scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(3), scale, 3);
+  } else {
+    typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+    const auto pair = [&](int j) { return __builtin_bit_cast(half2_t, v.w[j]); };
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, pair(0), scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, pair(1), scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, pair(2), scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, pair(3), scale, 3);
+  }
+  return w;
 }
 
 // A quarter of a block held by lane j of a quad (elements 8 j .. 8 j + 7): its
 // four code bytes, and the block's scale byte in every lane of the quad.
-__device__ __forceinline__ uint32_t quantize_quarter(const float (&v)[8], uint32_t& scale) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, magnitude(v[j]));
+template <int kDtype>
+__device__ __forceinline__ uint32_t quantize_quarter(const Eight<kDtype>& v, uint32_t& scale) {
+  uint32_t top = top8(v);
   top = max(top, uint32_t(__builtin_amdgcn_mov_dpp(int(top), 0xB1, 0xF, 0xF, false)));
   top = max(top, uint32_t(__builtin_amdgcn_mov_dpp(int(top), 0x4E, 0xF, 0xF, false)));
   scale = block_scale(top);
-  const uint32_t w = codes8(v, scale);
+  const uint32_t w = codes_of(v, scale);
   return scale == 255u ? 0u : w;
 }
 

@@ -7,6 +7,7 @@
 
 #include "../../include/vllm_mi355x.h"
 #include "mxfp4.h"
+#include "mxfp4_small.h"
 #include "mxfp4_tile.h"
 
 namespace mx {
@@ -26,10 +27,8 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const void* x, int64
   if (b >= rows * blocks) return;
   const int64_t r = b / blocks;
   const int c = int(b - r * blocks);
-  float v[8];
-  load8<kDtype>(x, r * stride + int64_t(c) * kBlock + 8 * j, wide, v);
   uint32_t s;
-  codes[quarter] = quantize_quarter(v, s);
+  codes[quarter] = quantize_quarter(load8<kDtype>(x, r * stride + int64_t(c) * kBlock + 8 * j, wide), s);
   if (j == 0) scales[b] = uint8_t(s);
 }
 
@@ -47,6 +46,20 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint32_t* co
 
 // ---- product -------------------------------------------------------------------
 
+struct SmallArgs {
+  const void* x;            // unquantized rows, or
+  int64_t stride;
+  bool wide;
+  const uint8_t *a, *as;    // their codes and scales
+  const uint8_t *w, *ws;
+  int64_t rows, n;
+  int blocks;  // k / 32
+  void* out;
+  int out_dtype;
+  int64_t groups_n;  // column groups
+  int groups_m;      // row groups
+};
+
 struct MatmulArgs {
   const uint8_t *a, *as, *w, *ws;
   int64_t rows, n;
@@ -55,44 +68,107 @@ struct MatmulArgs {
   int out_dtype;
 };
 
-// One wavefront: 16 rows x 16 columns, every operand from global memory.
-__global__ __launch_bounds__(64) void matmul_kernel(MatmulArgs g) {
-  const int lane = threadIdx.x;
+// Few rows: a workgroup of kCols x `parts` wavefronts has 16 kCols columns and 16
+// rows, chunk c of K multiplied by part c % parts; the parts' sums are added
+// through LDS in order.  kQuantize: x comes unquantized and is quantized into
+// LDS, while the first weights are on their way; else its codes come from memory
+// (L2, after the first workgroup).
+template <int kCols, bool kQuantize, int kDtype>
+__global__ __launch_bounds__(1024, 4) void small_kernel(SmallArgs g) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63;
+  const int wave = vq::uniform(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int64_t n0 = int64_t(blockIdx.x) * 16, m0 = int64_t(blockIdx.y) * 16;
-  const int64_t wrow = min(n0 + r, g.n - 1), arow = min(m0 + r, g.rows - 1);
-  const uint8_t* a = g.a + arow * g.blocks * kBlockBytes;
+  const int col = wave % kCols, part = wave / kCols, parts = threads / 64 / kCols;
+  const int chunks = (g.blocks + kChunk - 1) / kChunk;
+  // workgroups b, b + 8, ... run on one XCD: the row groups of a column group
+  // follow each other there, so that its L2 fetches the weights once
+  const int local = int(blockIdx.x >> 3);
+  const int64_t group = int64_t(local / g.groups_m) * 8 + (blockIdx.x & 7);
+  if (group >= g.groups_n) return;
+  const int64_t n0 = (group * kCols + col) * 16;
+  const int64_t m0 = int64_t(local % g.groups_m) * 16;
+  const int rows = int(min(int64_t(16), g.rows - m0));
+  const int64_t wrow = min(n0 + r, g.n - 1);
   const uint8_t* w = g.w + wrow * g.blocks * kBlockBytes;
-  const uint8_t* as = g.as + arow * g.blocks;
   const uint8_t* ws = g.ws + wrow * g.blocks;
+  const auto weights = [&](int c) {
+    ChunkOperand o{};
+    if (c < chunks) o = load_chunk(w, ws, c, g.blocks, q);
+    return o;
+  };
   f32x4_t acc{0, 0, 0, 0};
-  for (int b0 = 0; b0 < g.blocks; b0 += 4) {
-    // blocks past the last multiply zeros by zeros
-    const int b = b0 + q;
-    u32x4_t av{0, 0, 0, 0}, wv{0, 0, 0, 0};
-    uint32_t sa = 127, sw = 127;
-    if (b < g.blocks) {
-      av = *reinterpret_cast<const u32x4_t*>(a + int64_t(b) * kBlockBytes);
-      wv = *reinterpret_cast<const u32x4_t*>(w + int64_t(b) * kBlockBytes);
-      sa = as[b];
-      sw = ws[b];
+  if constexpr (kQuantize) {
+    ChunkOperand a = weights(part), b = weights(part + parts);
+    quantize_to_lds<kDtype>(g.x, [&](int m) { return (m0 + m) * g.stride; }, rows, g.blocks, chunks, g.wide, lds, tid, threads);
+    __syncthreads();
+    for (int c = part; c < chunks; c += parts) {
+      const ChunkOperand next = weights(c + 2 * parts);
+      multiply_lds(a, lds, c, rows, chunks, r, q, acc);
+      a = b;
+      b = next;
     }
-    acc = mfma16(wv, sw, av, sa, acc);
+  } else {
+    const int64_t row = m0 + min(r, rows - 1);
+    const uint8_t* x = g.a + row * g.blocks * kBlockBytes;
+    const uint8_t* xs = g.as + row * g.blocks;
+    const auto activations = [&](int c) {
+      ChunkOperand o{};
+      if (c < chunks) o = load_chunk(x, xs, c, g.blocks, q);
+      return o;
+    };
+    ChunkOperand a = weights(part), ax = activations(part);
+    for (int c = part; c < chunks; c += parts) {
+      const ChunkOperand next = weights(c + parts), nx = activations(c + parts);
+      multiply_loaded(a, ax, acc);
+      a = next;
+      ax = nx;
+    }
   }
-  if (m0 + r >= g.rows) return;
+  // the sums of parts 1, 2, ... through LDS, [part - 1][col][lane]
+  f32x4_t* sums = reinterpret_cast<f32x4_t*>(lds);
+  __syncthreads();
+  if (part > 0) sums[((part - 1) * kCols + col) * 64 + lane] = acc;
+  __syncthreads();
+  if (part > 0) return;
+  for (int p = 1; p < parts; ++p) acc += sums[((p - 1) * kCols + col) * 64 + lane];
+  if (r >= rows) return;
+  const int64_t at = (m0 + r) * g.n;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t n = n0 + 4 * q + i;
-    if (n < g.n) vq::store_act(g.out, g.out_dtype, (m0 + r) * g.n + n, acc[i]);
+    if (n < g.n) vq::store_act(g.out, g.out_dtype, at + n, acc[i]);
   }
 }
 
-#ifdef MX_TUNE
-int g_force = 0;
-#endif
+// out[i] = RN(part 0's i + part 1's i + ...), eight elements a thread.
+__global__ __launch_bounds__(kThreads) void combine_kernel(const float* part, int splits, int64_t numel, void* out, int dtype) {
+  const int64_t i = (int64_t(blockIdx.x) * kThreads + threadIdx.x) * 8;
+  if (i >= numel) return;
+  float v[8];
+  if (i + 8 <= numel && (numel & 3) == 0) {
+    f32x4_t a{0, 0, 0, 0}, b{0, 0, 0, 0};
+    for (int p = 0; p < splits; ++p) {
+      a += *reinterpret_cast<const f32x4_t*>(part + p * numel + i);
+      b += *reinterpret_cast<const f32x4_t*>(part + p * numel + i + 4);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = a[j];
+      v[4 + j] = b[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = 0;
+      for (int p = 0; p < splits && i + j < numel; ++p) v[j] += part[p * numel + i + j];
+    }
+  }
+  vq::store8_act(out, dtype, i, v, numel - i);
+}
 
 template <int kN, int kM>
-int launch_tile(const MatmulArgs& g, hipStream_t s) {
+int launch_tile(const MatmulArgs& g, int splits, float* part, hipStream_t s) {
   TileArgs t{};
   t.a = g.a;
   t.as = g.as;
@@ -101,33 +177,147 @@ int launch_tile(const MatmulArgs& g, hipStream_t s) {
   t.rows = g.rows;
   t.n = g.n;
   t.blocks = g.blocks;
-  t.out = g.out;
-  t.out_dtype = g.out_dtype;
-  t.wide = g.n % 8 == 0 && aligned(g.out, 16);
+  t.out = splits > 1 ? part : g.out;
+  t.out_dtype = splits > 1 ? int(vq::kFP32) : g.out_dtype;
+  t.wide = g.n % 8 == 0 && aligned(t.out, 16);
   t.tiles_n = int((g.n + 64 * kN - 1) / (64 * kN));
   t.tiles_m = int((g.rows + 64 * kM - 1) / (64 * kM));
+  const int stages = (g.blocks + kStageBlocks - 1) / kStageBlocks;
+  t.split_stages = (stages + splits - 1) / splits;
   const int64_t total = int64_t(t.tiles_n) * t.tiles_m;
-  hipLaunchKernelGGL((tile_kernel<kN, kM, kDense>), dim3(unsigned((total + 7) / 8 * 8)), dim3(kTileThreads), 0, s, t);
-  return vq::check_launch("mxfp4 tile");
+  hipLaunchKernelGGL((tile_kernel<kN, kM, kDense>), dim3(unsigned((total + 7) / 8 * 8), unsigned(splits)), dim3(kTileThreads), 0, s, t);
+  if (int rc = vq::check_launch("mxfp4 tile")) return rc;
+  if (splits == 1) return vq::kOk;
+  const int64_t numel = g.rows * g.n;
+  hipLaunchKernelGGL(combine_kernel, dim3(unsigned((numel + 8 * kThreads - 1) / (8 * kThreads))), dim3(kThreads), 0, s, part, splits,
+                     numel, g.out, g.out_dtype);
+  return vq::check_launch("mxfp4 combine");
 }
 
-int64_t tiles_of(const MatmulArgs& g, int cols, int rows) { return ((g.n + cols - 1) / cols) * ((g.rows + rows - 1) / rows); }
+// ---- which kernel ------------------------------------------------------------
 
-int launch_matmul(const MatmulArgs& g, hipStream_t s) {
-  // the tile kernel: whole stages of blocks, tiles below 2 GiB, a grid in 32 bits
-  if (g.rows > 32 && g.blocks >= kStageBlocks && int64_t(g.blocks) * kBlockBytes * 256 <= INT_MAX && tiles_of(g, 64, 64) <= INT_MAX / 8) {
-    int force = 0;
 #ifdef MX_TUNE
-    force = g_force;
+int g_tile = 0, g_splits = 0, g_parts = 0, g_cols = 0, g_fuse = -1;
 #endif
-    if (force == 44 || (!force && tiles_of(g, 256, 256) >= 200)) return launch_tile<4, 4>(g, s);
-    if (force == 22 || (!force && tiles_of(g, 128, 128) >= 200)) return launch_tile<2, 2>(g, s);
-    if (force == 11 || !force) return launch_tile<1, 1>(g, s);
+
+// How a product runs.  tile 0: the few-rows kernel, `cols` column tiles and
+// `parts` parts of K a workgroup, `fused`: it quantizes x itself; else the tile
+// kernel with 64 `tile` columns and rows, K in `splits`.
+struct Plan {
+  int tile, splits, cols, parts;
+  bool fused;
+};
+
+constexpr int kCUs = 256;
+
+// The tile kernel's time in us as its workgroups fill the chip: a stage costs
+// `alone` where a workgroup has a CU's loads and matrix cores for itself, and
+// `shared` per workgroup of a CU that is full; K splits write and read FP32 sums
+// at about 3 TB/s, in one more launch.  Fitted to the tile sizes and splits
+// measured at 24 to 4096 rows of 4096 x 14336, 14336 x 4096, 4096 x 4096 and
+// 2592 x 5003: it picks the fastest of them or one within 10%.
+double tile_cost(int size, int64_t rows, int64_t n, int64_t stages, int64_t splits) {
+  const double alone = size == 4 ? 1.48 : size == 2 ? 0.75 : 0.55, shared = size == 4 ? 2.3 : size == 2 ? 0.85 : 0.385;
+  const int64_t groups = ((n + 64 * size - 1) / (64 * size)) * ((rows + 64 * size - 1) / (64 * size)) * splits;
+  // whole rounds of the one workgroup of the largest tiles that a CU holds
+  const double load = size == 4 ? double((groups + kCUs - 1) / kCUs) : double(groups) / kCUs;
+  const double each = size == 4 && groups < kCUs / 2 ? alone : std::max(alone, shared * load);
+  const double sums = splits > 1 ? 3.0 + double(rows) * double(n) * 8.0 * double(splits) / 3e6 : 0.0;
+  return double((stages + splits - 1) / splits) * each + sums;
+}
+
+Plan plan_of(int64_t rows, int64_t k, int64_t n) {
+  Plan p{0, 1, 1, 1, false};
+  const int64_t blocks = k / kBlock, stages = (blocks + kStageBlocks - 1) / kStageBlocks;
+  // the tile kernel wants whole stages, buffers below 2 GiB and a 32-bit grid
+  const bool tiles = rows > 16 && blocks >= kStageBlocks && k <= (int64_t(1) << 22) &&
+                     ((n + 63) / 64) * ((rows + 63) / 64) <= INT_MAX / 8;
+  // A group of 16 rows reads the weights once more, from L2: 20 rows of 2592 x
+  // 5003 10.6 us (tiles 13.0), 64 rows 11.4 (13.9), but 20 rows of 4096 x 14336
+  // 20.9 (15.3).
+  if (tiles && (rows > 64 || (rows + 15) / 16 * double(n) * double(k) > 64e6)) {
+    double best = 0;
+    for (const int size : {1, 2, 4}) {
+      for (const int splits : {1, 2, 4, 8}) {
+        if (splits > 1 && stages < 4 * splits) continue;
+        const double cost = tile_cost(size, rows, n, stages, splits);
+        if (!p.tile || cost < best) {
+          best = cost;
+          p.tile = size;
+          p.splits = splits;
+        }
+      }
+    }
   }
-  const int64_t tiles_n = (g.n + 15) / 16, tiles_m = (g.rows + 15) / 16;
-  if (tiles_n > INT_MAX || tiles_m > 65535) return vq::fail("mxfp4: too many rows or columns");
-  hipLaunchKernelGGL(matmul_kernel, dim3(unsigned(tiles_n), unsigned(tiles_m)), dim3(64), 0, s, g);
-  return vq::check_launch("mxfp4 matmul");
+  if (!p.tile) {
+    // wide enough workgroups to share the activations, wavefronts enough to have
+    // all of a small matrix in flight: one row of 4096 x 14336 9.1 us with 4 column
+    // tiles and 4 parts (1 and 4: 9.8, 1 and 16: 13.6), of 14336 x 4096 9.2 with 1
+    // and 16 (4 and 4: 18.5)
+    const int64_t groups = (n + 15) / 16, chunks = (blocks + kChunk - 1) / kChunk;
+    p.cols = groups >= 800 ? 4 : groups >= 400 ? 2 : 1;
+    while (2 * p.parts * p.cols <= 16 && 2 * p.parts <= chunks && groups * p.parts < 3500) p.parts *= 2;
+    // every workgroup quantizes its rows itself, as long as that is less than a
+    // launch (per CU 28k elements 11.7 against 13.2 us, 57k 15.6 against 14.7 and
+    // 11.8 against 11.4)
+    const int64_t groups_cu = ((groups + p.cols - 1) / p.cols + kCUs - 1) / kCUs;
+    p.fused = rows <= 16 && groups_cu * rows * k <= 40960;
+  }
+#ifdef MX_TUNE
+  if (g_tile >= 0 && g_tile != 9) p.tile = tiles ? g_tile : 0;
+  if (g_splits) p.splits = g_splits;
+  if (g_cols) p.cols = g_cols;
+  if (g_parts) p.parts = g_parts;
+  if (g_fuse >= 0) p.fused = g_fuse;
+#endif
+  if (p.splits > 1) p.splits = int((stages + (stages + p.splits - 1) / p.splits - 1) / ((stages + p.splits - 1) / p.splits));
+  return p;
+}
+
+// Bytes of rows' codes and scales, in whole sixteens.
+int64_t packed_bytes(int64_t rows, int64_t k) { return rows * (k / 2) + (rows * (k / kBlock) + 15) / 16 * 16; }
+
+// Bytes of a plan's K splits.
+int64_t split_bytes(const Plan& p, int64_t rows, int64_t n) { return p.tile && p.splits > 1 ? p.splits * rows * n * 4 : 0; }
+
+template <int kCols, bool kQuantize, int kDtype>
+int launch_small_as(SmallArgs g, int parts, hipStream_t s) {
+  g.groups_n = (g.n + 16 * kCols - 1) / (16 * kCols);
+  g.groups_m = int((g.rows + 15) / 16);
+  const int64_t chunks = (g.blocks + kChunk - 1) / kChunk, rows = std::min<int64_t>(g.rows, 16);
+  const int64_t lds = std::max<int64_t>(kQuantize ? small_bytes(rows, chunks) : 0, int64_t(parts - 1) * kCols * 1024);
+  const int64_t grid = (g.groups_n + 7) / 8 * 8 * ((g.rows + 15) / 16);
+  if (grid > INT_MAX) return vq::fail("mxfp4: too many rows or columns");
+  hipLaunchKernelGGL((small_kernel<kCols, kQuantize, kDtype>), dim3(unsigned(grid)), dim3(64 * kCols * parts), size_t(lds), s, g);
+  return vq::check_launch("mxfp4 few rows");
+}
+
+template <bool kQuantize, int kDtype>
+int launch_small(const SmallArgs& g, const Plan& p, hipStream_t s) {
+  if (p.cols == 4) return launch_small_as<4, kQuantize, kDtype>(g, p.parts, s);
+  if (p.cols == 2) return launch_small_as<2, kQuantize, kDtype>(g, p.parts, s);
+  return launch_small_as<1, kQuantize, kDtype>(g, p.parts, s);
+}
+
+SmallArgs small_args(const MatmulArgs& g) {
+  SmallArgs m{};
+  m.a = g.a;
+  m.as = g.as;
+  m.w = g.w;
+  m.ws = g.ws;
+  m.rows = g.rows;
+  m.n = g.n;
+  m.blocks = g.blocks;
+  m.out = g.out;
+  m.out_dtype = g.out_dtype;
+  return m;
+}
+
+int launch_matmul(const MatmulArgs& g, const Plan& p, float* part, hipStream_t s) {
+  if (p.tile == 4) return launch_tile<4, 4>(g, p.splits, part, s);
+  if (p.tile == 2) return launch_tile<2, 2>(g, p.splits, part, s);
+  if (p.tile == 1) return launch_tile<1, 1>(g, p.splits, part, s);
+  return launch_small<false, vq::kBF16>(small_args(g), p, s);
 }
 
 int launch_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t stride, uint8_t* codes, uint8_t* scales,
@@ -232,9 +422,20 @@ extern "C" int mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, int64_t r
   if (vq::overlaps(out, out_bytes, a, rows * k / 2) || vq::overlaps(out, out_bytes, a_scales, rows * k / kBlock)) {
     return vq::fail("mxfp4: out must not overlap the activations");
   }
-  (void)workspace;
-  (void)workspace_bytes;
-  return launch_matmul({a, a_scales, w, w_scales, rows, n, int(k / kBlock), out, out_dtype}, static_cast<hipStream_t>(stream));
+  const Plan p = plan_of(rows, k, n);
+  const int64_t need = split_bytes(p, rows, n);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) {
+      return vq::fail("mxfp4: workspace too small or not 16-byte aligned");
+    }
+    if (vq::overlaps(workspace, need, a, rows * k / 2) || vq::overlaps(workspace, need, a_scales, rows * k / kBlock) ||
+        vq::overlaps(workspace, need, out, out_bytes) || vq::overlaps(workspace, need, w, n * k / 2) ||
+        vq::overlaps(workspace, need, w_scales, n * k / kBlock)) {
+      return vq::fail("mxfp4: the workspace must not overlap another argument");
+    }
+  }
+  return launch_matmul({a, a_scales, w, w_scales, rows, n, int(k / kBlock), out, out_dtype}, p, static_cast<float*>(workspace),
+                       static_cast<hipStream_t>(stream));
 }
 
 extern "C" int64_t mxfp4_matmul_workspace_size(int64_t rows, int64_t k, int64_t n) {
@@ -243,7 +444,7 @@ extern "C" int64_t mxfp4_matmul_workspace_size(int64_t rows, int64_t k, int64_t 
     vq::fail("mxfp4: k must be a positive multiple of 32, sizes not negative");
     return -1;
   }
-  return 0;
+  return split_bytes(plan_of(rows, k, n), rows, n);
 }
 
 extern "C" int64_t mxfp4_linear_workspace_size(int64_t rows, int64_t k, int64_t n) {
@@ -252,7 +453,8 @@ extern "C" int64_t mxfp4_linear_workspace_size(int64_t rows, int64_t k, int64_t 
     vq::fail("mxfp4: k must be a positive multiple of 32, sizes not negative");
     return -1;
   }
-  return rows * (k / 2) + (rows * (k / kBlock) + 15) / 16 * 16;
+  const Plan p = plan_of(rows, k, n);
+  return (p.fused ? 0 : packed_bytes(rows, k)) + split_bytes(p, rows, n);
 }
 
 extern "C" int mxfp4_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_stride, const uint8_t* w,
@@ -265,6 +467,18 @@ extern "C" int mxfp4_linear(const void* x, int x_dtype, int64_t rows, int64_t k,
   const int64_t x_bytes = ((rows - 1) * x_stride + k) * vq::dtype_bytes(x_dtype);
   const int64_t out_bytes = rows * n * vq::dtype_bytes(out_dtype);
   if (vq::overlaps(out, out_bytes, x, x_bytes)) return vq::fail("mxfp4: out must not overlap x");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const Plan p = plan_of(rows, k, n);
+  const MatmulArgs g{nullptr, nullptr, w, w_scales, rows, n, int(k / kBlock), out, out_dtype};
+  if (p.fused) {
+    SmallArgs m = small_args(g);
+    m.x = x;
+    m.stride = x_stride;
+    m.wide = aligned(x, 16) && x_stride * vq::dtype_bytes(x_dtype) % 16 == 0;
+    if (x_dtype == vq::kBF16) return launch_small<true, vq::kBF16>(m, p, s);
+    if (x_dtype == vq::kFP16) return launch_small<true, vq::kFP16>(m, p, s);
+    return launch_small<true, vq::kFP32>(m, p, s);
+  }
   const int64_t need = mxfp4_linear_workspace_size(rows, k, n);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) {
     return vq::fail("mxfp4: workspace too small or not 16-byte aligned");
@@ -273,13 +487,21 @@ extern "C" int mxfp4_linear(const void* x, int x_dtype, int64_t rows, int64_t k,
       vq::overlaps(workspace, need, w, n * k / 2) || vq::overlaps(workspace, need, w_scales, n * k / kBlock)) {
     return vq::fail("mxfp4: the workspace must not overlap another argument");
   }
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + rows * (k / 2);
   if (int rc = launch_quantize(x, x_dtype, rows, k, x_stride, codes, scales, s)) return rc;
-  return launch_matmul({codes, scales, w, w_scales, rows, n, int(k / kBlock), out, out_dtype}, s);
+  MatmulArgs packed = g;
+  packed.a = codes;
+  packed.as = scales;
+  return launch_matmul(packed, p, reinterpret_cast<float*>(codes + packed_bytes(rows, k)), s);
 }
 
 #ifdef MX_TUNE
-extern "C" void mx_force(int f) { mx::g_force = f; }
+extern "C" void mx_plan(int tile, int splits, int cols, int parts, int fuse) {
+  mx::g_tile = tile;
+  mx::g_splits = splits;
+  mx::g_cols = cols;
+  mx::g_parts = parts;
+  mx::g_fuse = fuse;
+}
 #endif

@@ -55,10 +55,8 @@ __global__ __launch_bounds__(moe::kRowsPartThreads) void count_quantize_kernel(E
   if (b >= tokens * blocks) return;
   const int64_t r = b / blocks;
   const int c = int(b - r * blocks);
-  float v[8];
-  load8<kDtype>(x, r * stride + int64_t(c) * kBlock + 8 * j, wide, v);
   uint32_t s;
-  codes[quarter] = quantize_quarter(v, s);
+  codes[quarter] = quantize_quarter(load8<kDtype>(x, r * stride + int64_t(c) * kBlock + 8 * j, wide), s);
   if (j == 0) scales[b] = uint8_t(s);
 }
 

@@ -59,6 +59,8 @@ struct TileArgs {
   int out_dtype;
   int wide;               // kDense: n a multiple of eight, out 16-byte aligned
   int tiles_n, tiles_m;   // kDense: workgroups; else tiles_n alone
+  int split_stages;       // kDense: stages of one split of K (gridDim.y splits, whose
+                          // sums go to FP32 [split][rows][n] at out)
   // the routed forms
   const int32_t* table;
   int64_t tasks, sorted;  // offsets in the table
@@ -255,11 +257,16 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
     const int l = min(tid + i * kTileThreads, kLines - 1);
     srow[i] = l < kCols ? g.ws + (wbase + weight_row(l)) * g.blocks : g.as + (act0 + act_row(l - kCols)) * g.blocks;
   }
-  const int stages = (g.blocks + kStageBlocks - 1) / kStageBlocks;
+  const int all_stages = (g.blocks + kStageBlocks - 1) / kStageBlocks;
+  int first = 0, stages = all_stages;  // this split's, up to `stages`
+  if constexpr (kMode == kDense) {
+    first = int(blockIdx.y) * g.split_stages;
+    stages = min(first + g.split_stages, all_stages);
+  }
   // DMA load i of stage s (zeros past the last stage)
   const auto fetch = [&](auto i_c, int s, uint8_t* buf) {
     constexpr int i = decltype(i_c)::value;
-    const int left = g.blocks - s * kStageBlocks;
+    const int left = s < stages ? g.blocks - s * kStageBlocks : 0;
     const int parity = (i < kLoadsW ? kLoadsW * wave + i : kLoadsA * wave + i - kLoadsW) & 1;
     constexpr bool scattered = kMode == kGateUp && i >= kLoadsW;
     const uint32_t lane_part = scattered ? token_off[scattered ? i - kLoadsW : 0] : lane_off[parity];
@@ -278,7 +285,7 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
   // wavefront reads the buffer before it any more
   const auto land = [&](int s, uint2* scales) {
     vq::wait_vmcnt<0>();
-    const int b0 = min(s, stages - 1) * kStageBlocks;
+    const int b0 = min(s, all_stages - 1) * kStageBlocks;
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i) {
       if (kLines % kTileThreads == 0 || tid + i * kTileThreads < kLines) {
@@ -347,16 +354,16 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
     read_scales(next_scales, sw[set ^ 1], sa[set ^ 1]);
     step(integral_constant<int, 3>{}, c0, integral_constant<int, kHalf>{}, set, next, 0, s + 2, cur);
   };
-  for_range<0, kLoads>([&](auto k) { fetch(k, 0, buf0); });
-  fetch_scales(0);
-  land(0, scale0);
-  fetch_scales(1);
-  for_range<0, kHalf>([&](auto k) { fetch(k, 1, buf1); });
+  for_range<0, kLoads>([&](auto k) { fetch(k, first, buf0); });
+  fetch_scales(first);
+  land(first, scale0);
+  fetch_scales(first + 1);
+  for_range<0, kHalf>([&](auto k) { fetch(k, first + 1, buf1); });
   read_scales(scale0, sw[0], sa[0]);
   for_range<0, kN + kM>([&](auto k) { read(k, buf0, 0, 0); });
   // stages in pairs, one buffer each by name: the compiler then sees that a
   // stage's reads are not of the buffer that the DMA is filling
-  int s = 0;
+  int s = first;
   for (; s + 1 < stages; s += 2) {
     stage(s, 0, buf0, buf1, scale1);
     stage(s + 1, 1, buf1, buf0, scale0);
@@ -419,21 +426,25 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
         }
       }
       const int mt = 32 * (kM * wm + i), ct = c0 + 32 * kN * wn;
+      const int64_t o0 = kMode == kDense ? m0 + int64_t(blockIdx.y) * g.rows : m0;  // first output row
       if constexpr (kMode == kDense) {
         if (g.wide) {
-          if (g.out_dtype == vq::kBF16) store_rows<kN, vq::kBF16>(part, kStride, lane, mt, nrows, ct, g, m0, nullptr);
-          else if (g.out_dtype == vq::kFP16) store_rows<kN, vq::kFP16>(part, kStride, lane, mt, nrows, ct, g, m0, nullptr);
-          else store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, m0, nullptr);
+          if (g.out_dtype == vq::kBF16) store_rows<kN, vq::kBF16>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
+          else if (g.out_dtype == vq::kFP16) store_rows<kN, vq::kFP16>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
+          else store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
         } else {
-          for (int at = lane; at < 32 * 32 * kN; at += 64) {
-            const int m = mt + at / (32 * kN), c = ct + at % (32 * kN);
-            if (m < nrows && c < g.n) {
-              vq::store_act(g.out, g.out_dtype, (m0 + m) * g.n + c, part[at / (32 * kN) * kStride + at % (32 * kN)]);
-            }
+          // rows of any alignment: 64 consecutive elements a store, or fewer
+          constexpr int kSpan = 32 * kN < 64 ? 32 * kN : 64;
+          const int c = lane % kSpan;
+#pragma unroll 8
+          for (int k = 0; k < 32 * 32 * kN / 64; ++k) {
+            const int mr = k * 64 / (32 * kN) + (kSpan < 64 ? lane / kSpan : 0), cc = k * 64 % (32 * kN) + c;
+            const float v = part[mr * kStride + cc];
+            if (mt + mr < nrows && ct + cc < g.n) vq::store_act(g.out, g.out_dtype, (o0 + mt + mr) * g.n + ct + cc, v);
           }
         }
       } else {
-        store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, m0, sorted);
+        store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, o0, sorted);
       }
     }
   }
