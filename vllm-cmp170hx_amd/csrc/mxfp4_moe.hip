@@ -11,6 +11,7 @@
 #include "../../include/vllm_mi355x.h"
 #include "moe_rows.h"
 #include "mxfp4.h"
+#include "mxfp4_small.h"
 #include "mxfp4_tile.h"
 
 namespace mx {
@@ -20,7 +21,7 @@ constexpr int kThreads = 256;
 constexpr int kTaskRows = 16;
 constexpr int kTileRows = 128;  // rows of a task on the tile kernel
 #ifdef MX_TUNE
-int g_moe_force = 0;
+int g_moe_force = -1, g_split = 1024, g_target = 1024;
 #endif
 
 // The local expert of a slot: through the map where the call brings one, -1
@@ -65,92 +66,349 @@ __global__ __launch_bounds__(moe::kRowsPartThreads) void fill_kernel(moe::RowsLa
   moe::rows_fill_part(lay, table, task_rows, int(blockIdx.x), first);
 }
 
-struct GemmArgs {
-  const uint8_t *a, *as;  // rows of k: tokens (gate | up), sorted rows (down)
-  const uint8_t *w, *ws;  // [experts][n][k]
+// ---- few rows an expert ---------------------------------------------------------
+
+constexpr int kScanSlots = 1024;  // slots that a workgroup looks through itself
+
+struct SmallMoeArgs {
+  ExpertOf of;
+  const void* x;            // kScan: unquantized rows, else
+  int64_t stride;
+  bool wide;
+  const uint8_t *a, *as;    // their codes and scales
+  const uint8_t *w, *ws;    // [experts][n][k]
+  int slots, top_k;
+  int by_slot;              // kScan: workgroups go by slot, the first of an expert's does the work
   const int32_t* table;
-  int64_t tasks, sorted;  // offsets in the table
+  int64_t tasks, sorted;    // offsets in the table
   const float* topk_w;
-  int top_k, n, blocks;   // k / 32
+  int n, blocks;            // k / 32
   float limit;
-  uint8_t *h, *hs;        // gate | up: rows of n / 2
-  float* out;             // down: [slots][n]
+  uint8_t *h, *hs;          // [slots][inter]
+  float* c3;                // [slots][n]
+  void* out;
+  int out_dtype;
 };
 
-// 16 x 16 sums of rows `arow` (one per lane & 15) with weight rows `wrow`.
-__device__ __forceinline__ f32x4_t row_tile(const GemmArgs& g, int64_t arow, int64_t wrow, int q) {
-  const uint8_t* a = g.a + arow * g.blocks * kBlockBytes;
-  const uint8_t* w = g.w + wrow * g.blocks * kBlockBytes;
-  const uint8_t* as = g.as + arow * g.blocks;
-  const uint8_t* ws = g.ws + wrow * g.blocks;
-  f32x4_t acc{0, 0, 0, 0};
-  for (int b0 = 0; b0 < g.blocks; b0 += 4) {
-    const int b = b0 + q;
-    u32x4_t av{0, 0, 0, 0}, wv{0, 0, 0, 0};
-    uint32_t sa = 127, sw = 127;
-    if (b < g.blocks) {
-      av = *reinterpret_cast<const u32x4_t*>(a + int64_t(b) * kBlockBytes);
-      wv = *reinterpret_cast<const u32x4_t*>(w + int64_t(b) * kBlockBytes);
-      sa = as[b];
-      sw = ws[b];
+// The expert and the slots of workgroup `index`, in slot order; count 0: no work.
+// kScan: from the ids themselves (list: LDS of kScanSlots entries); else a task of
+// the table.
+struct RowsOf {
+  int expert, count;
+  const int32_t* slots;
+};
+
+template <bool kScan>
+__device__ __forceinline__ RowsOf rows_of(const SmallMoeArgs& g, int index, int32_t* list, int* count) {
+  if constexpr (!kScan) {
+    (void)list;
+    (void)count;
+    if (index >= g.table[0]) return {0, 0, nullptr};
+    const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[index];
+    return {vq::uniform(tk.x), vq::uniform(tk.z), g.table + g.sorted + vq::uniform(tk.y)};
+  } else {
+    const int e = g.by_slot ? vq::uniform(g.of(index)) : index;
+    if (e < 0) return {0, 0, nullptr};
+    if (threadIdx.x < 64) {
+      const int lane = threadIdx.x;
+      int n = 0;
+      bool later = false;  // an earlier slot's workgroup has this expert
+      constexpr int kEach = 4;
+      for (int s0 = 0; s0 < g.slots; s0 += 64 * kEach) {
+        int id[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+          const int s = s0 + 64 * u + lane;
+          id[u] = s < g.slots ? g.of(s) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+          const bool mine = id[u] == e;
+          const uint64_t all = __ballot(mine);
+          if (mine) list[n + __popcll(all & ((uint64_t(1) << lane) - 1))] = s0 + 64 * u + lane;
+          n += __popcll(all);
+        }
+      }
+      if (g.by_slot) later = list[0] != index;
+      if (lane == 0) *count = later ? 0 : n;
     }
-    acc = mfma16(wv, sw, av, sa, acc);
+    __syncthreads();
+    return {e, vq::uniform(*count), list};
   }
-  return acc;
 }
 
-// One wavefront: a task's rows (at most 16) by 32 columns of h.
-__global__ __launch_bounds__(64) void gate_up_kernel(GemmArgs g) {
-  const int task = blockIdx.y;
-  if (task >= g.table[0]) return;
-  const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[task];
-  const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
-  const int inter = g.n / 2;
-  const int c0 = blockIdx.x * kBlock;
-  const int t = min(r, tk.z - 1);
-  const int64_t row = tk.y + t;
-  const int64_t token = g.table[g.sorted + row] / g.top_k;
-  const int64_t w0 = int64_t(tk.x) * g.n + c0 + r;
-  float v[8];
+// gate | up and the SwiGLU for the rows of one expert, 16 at a time, by one block
+// of 32 columns of h: wavefront (tile = wave % 4: gate 0, gate 1, up 0, up 1; part
+// = wave / 4 of K).  Its sums meet in LDS; one wavefront forms h, four lanes a row.
+// For calls of few blocks, whose time is one block's.
+template <int kDtype>
+__global__ __launch_bounds__(1024, 4) void gate_up_split_kernel(SmallMoeArgs g) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int32_t list[kScanSlots];
+  __shared__ int count;
+  constexpr int kRow = 20;  // floats of a row's 16 sums in LDS
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63;
+  const int wave = vq::uniform(tid >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int tile = wave & 3, part = wave >> 2, parts = threads >> 8;
+  const int inter = g.n / 2, groups = inter / kBlock;
+  const int c0 = int(blockIdx.x) % groups * kBlock;
+  const RowsOf rows = rows_of<true>(g, int(blockIdx.x) / groups, list, &count);
+  if (rows.count == 0) return;
+  const int chunks = (g.blocks + kChunk - 1) / kChunk;
+  const int64_t wrow = int64_t(rows.expert) * g.n + (tile & 2 ? inter : 0) + c0 + 16 * (tile & 1) + r;
+  const uint8_t* w = g.w + wrow * g.blocks * kBlockBytes;
+  const uint8_t* ws = g.ws + wrow * g.blocks;
+  const auto weights = [&](int c) {
+    ChunkOperand o{};
+    if (c < chunks) o = load_chunk(w, ws, c, g.blocks, q);
+    return o;
+  };
+  float* sums = reinterpret_cast<float*>(lds);
+  for (int m0 = 0; m0 < rows.count; m0 += 16) {
+    const int here = min(rows.count - m0, 16);
+    f32x4_t acc{0, 0, 0, 0};
+    ChunkOperand a = weights(part), b = weights(part + parts);
+    quantize_to_lds<kDtype>(g.x, [&](int m) { return int64_t(rows.slots[m0 + m] / g.top_k) * g.stride; }, here, g.blocks, chunks,
+                            g.wide, lds, tid, threads);
+    __syncthreads();
+    for (int c = part; c < chunks; c += parts) {
+      const ChunkOperand next = weights(c + 2 * parts);
+      multiply_lds(a, lds, c, here, chunks, r, q, acc);
+      a = b;
+      b = next;
+    }
+    __syncthreads();
+    *reinterpret_cast<f32x4_t*>(sums + ((part * 4 + tile) * 16 + r) * kRow + 4 * q) = acc;
+    __syncthreads();
+    if (wave == 0) {
+      const int m = lane >> 2, j = lane & 3;
+      // columns 8 j .. 8 j + 7 of the block: tile j / 2, 8 (j & 1) on
+      float gate[8], up[8];
+      const auto eight = [&](int t, float (&v)[8]) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const f32x4_t gate = row_tile(g, token, w0 + 16 * i, q);
-    const f32x4_t up = row_tile(g, token, w0 + inter + 16 * i, q);
+        for (int k = 0; k < 8; ++k) v[k] = 0;
+        for (int p = 0; p < parts; ++p) {
+          const float* at = sums + ((p * 4 + t) * 16 + m) * kRow + 8 * (j & 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[4 * i + j] = swiglu(gate[j], up[j], g.limit);
+          for (int k = 0; k < 8; ++k) v[k] += at[k];
+        }
+      };
+      eight(j >> 1, gate);
+      eight(2 + (j >> 1), up);
+      Eight<vq::kFP32> v;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v.w[k] = __builtin_bit_cast(uint32_t, swiglu(gate[k], up[k], g.limit));
+      uint32_t s;
+      const uint32_t code = quantize_quarter(v, s);
+      if (m < here) {
+        const int64_t slot = rows.slots[m0 + m];
+        *reinterpret_cast<uint32_t*>(g.h + slot * (inter / 2) + c0 / 2 + 4 * j) = code;
+        if (j == 0) g.hs[slot * groups + c0 / kBlock] = uint8_t(s);
+      }
+    }
+    __syncthreads();
   }
-  // the row's 32 columns lie in its four lanes (q): elements 4 q + j and 16 + 4 q + j
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) top = max(top, magnitude(v[j]));
-  top = max(top, uint32_t(__shfl_xor(int(top), 16)));
-  top = max(top, uint32_t(__shfl_xor(int(top), 32)));
-  const uint32_t s = block_scale(top);
-  const uint32_t w = s == 255u ? 0u : codes8(v, s);
-  if (r >= tk.z) return;
-  uint16_t* out = reinterpret_cast<uint16_t*>(g.h + row * (inter / 2) + c0 / 2);
-  out[q] = uint16_t(w);
-  out[4 + q] = uint16_t(w >> 16);
-  if (q == 0) g.hs[row * (inter / kBlock) + blockIdx.x] = uint8_t(s);
 }
 
-// One wavefront: a task's rows by 16 columns of the slot rows.
-__global__ __launch_bounds__(64) void down_kernel(GemmArgs g) {
-  const int task = blockIdx.y;
-  if (task >= g.table[0]) return;
-  const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[task];
-  const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int64_t row = tk.y + min(r, tk.z - 1);
-  const int slot = g.table[g.sorted + row];
-  const f32x4_t acc = row_tile(g, row, int64_t(tk.x) * g.n + min(n0 + r, g.n - 1), q);
-  if (r >= tk.z) return;
-  const float weight = g.topk_w[slot];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = n0 + 4 * q + i;
-    if (n < g.n) g.out[int64_t(slot) * g.n + n] = weight * acc[i];
+// A wavefront's way through weight tiles of 16 rows, chunk by chunk, its loads
+// kAhead chunks in front of what it multiplies: tile i of the run lies at
+// base(i), its chunks follow each other.
+constexpr int kAhead = 2;
+template <typename Base>
+struct WeightStream {
+  const Base& base;
+  int tiles, chunks, blocks, q;
+  int tile, chunk;  // the next chunk to load
+  ChunkOperand ring[kAhead];
+
+  __device__ __forceinline__ ChunkOperand load() {
+    ChunkOperand o{};
+    if (tile < tiles) {
+      const uint8_t *w, *ws;
+      base(tile, w, ws);
+      o = load_chunk(w, ws, chunk, blocks, q);
+      if (++chunk == chunks) {
+        chunk = 0;
+        ++tile;
+      }
+    }
+    return o;
   }
+  __device__ __forceinline__ void start() {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ring[i] = load();
+  }
+  __device__ __forceinline__ ChunkOperand next() {
+    const ChunkOperand o = ring[0];
+#pragma unroll
+    for (int i = 0; i + 1 < kAhead; ++i) ring[i] = ring[i + 1];
+    ring[kAhead - 1] = load();
+    return o;
+  }
+};
+
+// gate | up and the SwiGLU for the rows of one expert, 16 at a time: the rows in
+// LDS, a wavefront whole blocks of 32 columns of h (four weight tiles each), one
+// after another with no barrier between.  `wgs` workgroups an expert.
+template <bool kScan, int kDtype>
+__global__ __launch_bounds__(256, 4) void gate_up_kernel(SmallMoeArgs g, int wgs) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int32_t list[kScan ? kScanSlots : 1];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = vq::uniform(tid >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int inter = g.n / 2, groups = inter / kBlock;
+  const RowsOf rows = rows_of<kScan>(g, int(blockIdx.x) / wgs, list, &count);
+  if (rows.count == 0) return;
+  const int chunks = (g.blocks + kChunk - 1) / kChunk;
+  const int first = int(blockIdx.x) % wgs * 4 + wave, stride = 4 * wgs;
+  const int mine = first < groups ? (groups - first + stride - 1) / stride : 0;  // blocks of h
+  const int64_t line = int64_t(g.blocks) * kBlockBytes;
+  const uint8_t* w = g.w + (int64_t(rows.expert) * g.n + r) * line;
+  const uint8_t* ws = g.ws + (int64_t(rows.expert) * g.n + r) * g.blocks;
+  const auto base = [&](int i, const uint8_t*& wt, const uint8_t*& wst) {  // gate 0, gate 1, up 0, up 1
+    const int64_t row = int64_t(first + (i >> 2) * stride) * kBlock + 16 * (i & 1) + (i & 2 ? inter : 0);
+    wt = w + row * line;
+    wst = ws + row * g.blocks;
+  };
+  for (int m0 = 0; m0 < rows.count; m0 += 16) {
+    const int here = min(rows.count - m0, 16);
+    WeightStream<decltype(base)> stream{base, 4 * mine, chunks, g.blocks, q, 0, 0, {}};
+    stream.start();
+    if (m0) __syncthreads();
+    if constexpr (kScan) {
+      quantize_to_lds<kDtype>(g.x, [&](int m) { return int64_t(rows.slots[m0 + m] / g.top_k) * g.stride; }, here, g.blocks, chunks,
+                              g.wide, lds, tid, 256);
+    } else {
+      copy_to_lds(g.a, g.as, [&](int m) { return int64_t(rows.slots[m0 + m] / g.top_k); }, here, g.blocks, chunks, lds, tid, 256);
+    }
+    __syncthreads();
+    const int64_t slot = rows.slots[m0 + min(r, here - 1)];
+    for (int i = 0; i < mine; ++i) {
+      f32x4_t acc[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        acc[t] = f32x4_t{0, 0, 0, 0};
+        for (int c = 0; c < chunks; ++c) {
+          const ChunkOperand a = stream.next();
+          multiply_lds(a, lds, c, here, chunks, r, q, acc[t]);
+        }
+      }
+      // row r's block of h lies in its four lanes (q): elements 4 q + j and 16 + 4 q + j
+      float v[8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = swiglu(acc[0][j], acc[2][j], g.limit);
+        v[4 + j] = swiglu(acc[1][j], acc[3][j], g.limit);
+        top = max(top, max(magnitude(v[j]), magnitude(v[4 + j])));
+      }
+      top = max(top, uint32_t(__shfl_xor(int(top), 16)));
+      top = max(top, uint32_t(__shfl_xor(int(top), 32)));
+      const uint32_t s = block_scale(top);
+      const uint32_t code = s == 255u ? 0u : codes8(v, s);
+      if (r < here) {
+        const int block = first + i * stride;
+        uint16_t* out = reinterpret_cast<uint16_t*>(g.h + slot * (inter / 2) + block * kBlockBytes);
+        out[q] = uint16_t(code);
+        out[4 + q] = uint16_t(code >> 16);
+        if (q == 0) g.hs[slot * groups + block] = uint8_t(s);
+      }
+    }
+  }
+}
+
+// down for the rows of one expert: the rows of h in LDS, a wavefront 16 columns
+// after another; the weighted slot rows.
+template <bool kScan>
+__global__ __launch_bounds__(256, 4) void down_kernel(SmallMoeArgs g, int wgs) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int32_t list[kScan ? kScanSlots : 1];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = vq::uniform(tid >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const RowsOf rows = rows_of<kScan>(g, int(blockIdx.x) / wgs, list, &count);
+  if (rows.count == 0) return;
+  const int groups = g.n / 16, chunks = (g.blocks + kChunk - 1) / kChunk;  // n: whole sixteens
+  const int first = int(blockIdx.x) % wgs * 4 + wave, stride = 4 * wgs;
+  const int mine = first < groups ? (groups - first + stride - 1) / stride : 0;
+  const int64_t line = int64_t(g.blocks) * kBlockBytes;
+  const uint8_t* w = g.w + (int64_t(rows.expert) * g.n + r) * line;
+  const uint8_t* ws = g.ws + (int64_t(rows.expert) * g.n + r) * g.blocks;
+  const auto base = [&](int i, const uint8_t*& wt, const uint8_t*& wst) {
+    const int64_t row = int64_t(first + i * stride) * 16;
+    wt = w + row * line;
+    wst = ws + row * g.blocks;
+  };
+  for (int m0 = 0; m0 < rows.count; m0 += 16) {
+    const int here = min(rows.count - m0, 16);
+    WeightStream<decltype(base)> stream{base, mine, chunks, g.blocks, q, 0, 0, {}};
+    stream.start();
+    if (m0) __syncthreads();
+    copy_to_lds(g.h, g.hs, [&](int m) { return int64_t(rows.slots[m0 + m]); }, here, g.blocks, chunks, lds, tid, 256);
+    __syncthreads();
+    const int64_t slot = rows.slots[m0 + min(r, here - 1)];
+    const float weight = g.topk_w[slot];
+    float* out = g.c3 + slot * g.n + 4 * q;
+    for (int i = 0; i < mine; ++i) {
+      f32x4_t acc{0, 0, 0, 0};
+      for (int c = 0; c < chunks; ++c) {
+        const ChunkOperand a = stream.next();
+        multiply_lds(a, lds, c, here, chunks, r, q, acc);
+      }
+      if (r < here) *reinterpret_cast<f32x4_t*>(out + (first + i * stride) * 16) = acc * weight;
+    }
+  }
+}
+
+// down and the slot sum for one token by 16 columns, a wavefront a slot: where
+// tokens are few, their experts' weights are read a token at a time (those two
+// share come from L2) and the slot rows never leave the workgroup.
+template <int kDtype>
+__global__ __launch_bounds__(512, 4) void down_sum_kernel(SmallMoeArgs g) {
+  extern __shared__ float part[];  // [top_k][16]
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = vq::uniform(int(threadIdx.x) >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int groups = g.n / 16;
+  const int n0 = int(blockIdx.x) % groups * 16;
+  const int token = int(blockIdx.x) / groups;
+  const int chunks = (g.blocks + kChunk - 1) / kChunk;
+  for (int k = wave; k < g.top_k; k += waves) {
+    const int64_t slot = int64_t(token) * g.top_k + k;
+    const int e = vq::uniform(g.of(slot));
+    f32x4_t acc{0, 0, 0, 0};
+    if (e >= 0) {
+      const int64_t wrow = int64_t(e) * g.n + n0 + r;
+      const uint8_t* w = g.w + wrow * g.blocks * kBlockBytes;
+      const uint8_t* ws = g.ws + wrow * g.blocks;
+      const uint8_t* x = g.h + slot * g.blocks * kBlockBytes;
+      const uint8_t* xs = g.hs + slot * g.blocks;
+      ChunkOperand a = load_chunk(w, ws, 0, g.blocks, q), ax = load_chunk(x, xs, 0, g.blocks, q);
+      for (int c = 0; c < chunks; ++c) {
+        ChunkOperand next{}, nx{};
+        if (c + 1 < chunks) {
+          next = load_chunk(w, ws, c + 1, g.blocks, q);
+          nx = load_chunk(x, xs, c + 1, g.blocks, q);
+        }
+        multiply_loaded(a, ax, acc);
+        a = next;
+        ax = nx;
+      }
+      acc = acc * g.topk_w[slot];
+    }
+    if (r == 0) *reinterpret_cast<f32x4_t*>(part + k * 16 + 4 * q) = acc;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16) return;
+  float sum = 0;
+  for (int k = 0; k < g.top_k; ++k) {
+    if (g.of(int64_t(token) * g.top_k + k) >= 0) sum += part[k * 16 + threadIdx.x];
+  }
+  vq::store_act(g.out, kDtype, int64_t(token) * g.n + n0 + threadIdx.x, sum);
 }
 
 // out[t][c] = RN(sum over t's slots with a local expert, in slot order).
@@ -237,14 +495,92 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   const int64_t hb = hidden / kBlock, ib = inter / kBlock;
   const int64_t groups = lay.parts() + (tokens * hb * 4 + moe::kRowsPartThreads - 1) / moe::kRowsPartThreads;
   const int64_t sums = (tokens * hidden / 4 + kThreads - 1) / kThreads;
-  if (groups > INT_MAX || sums > INT_MAX || lay.max_tasks > 65535) return vq::fail("mxfp4 moe: too many rows");
+  if (groups > INT_MAX || sums > INT_MAX) return vq::fail("mxfp4 moe: too many rows");
   const bool wide = aligned(x, 16) && x_stride % 8 == 0;
   const size_t lds = size_t(experts) * sizeof(int);
-  bool tiles = slots >= 24 * std::min(experts, slots) && hb >= kStageBlocks && ib >= kStageBlocks && hidden * inter < (int64_t(1) << 31) &&
-               tokens * hidden / 2 < (int64_t(1) << 31);
+  // 0 few slots (each workgroup looks through them), 1 tasks of 16 rows, 2 tiles
+  const bool can_tile = hb >= kStageBlocks && ib >= kStageBlocks && hidden * inter < (int64_t(1) << 31) && tokens * hidden / 2 < (int64_t(1) << 31);
+  const int64_t small_rows = std::min<int64_t>(slots, 16), chunks = (hb + kChunk - 1) / kChunk;
+  const bool can_scan = slots <= kScanSlots && small_bytes(small_rows, chunks) <= 56 * 1024 &&
+                        small_bytes(small_rows, (ib + kChunk - 1) / kChunk) <= 56 * 1024;
+  // rows an expert held here may expect (a map says how many share the slots)
+  const double rows_each = double(slots) / double(std::max(experts, map_size));
+  int path = can_tile && rows_each >= 10 ? 2 : can_scan ? 0 : 1;
 #ifdef MX_TUNE
-  if (g_moe_force) tiles = g_moe_force == 2;
+  if (g_moe_force >= 0) path = g_moe_force;
 #endif
+  SmallMoeArgs m{};
+  m.of = of;
+  m.x = x;
+  m.stride = x_stride;
+  m.wide = wide;
+  m.a = base + ws.xq;
+  m.as = base + ws.xs;
+  m.w = w13;
+  m.ws = s13;
+  m.slots = int(slots);
+  m.top_k = int(top_k);
+  m.table = table;
+  m.tasks = lay.tasks();
+  m.sorted = lay.sorted();
+  m.topk_w = topk_w;
+  m.n = int(2 * inter);
+  m.blocks = int(hb);
+  m.limit = limit;
+  m.h = base + ws.hq;
+  m.hs = base + ws.hs;
+  m.c3 = reinterpret_cast<float*>(base + ws.c3);
+  m.out = out;
+  m.out_dtype = act_dtype;
+  const size_t rows2 = size_t(small_bytes(small_rows, (ib + kChunk - 1) / kChunk));
+  int64_t split_blocks = 1024, target = 1024;
+#ifdef MX_TUNE
+  split_blocks = g_split;
+  target = g_target;
+#endif
+  // workgroups an expert: about `target` in all
+  const auto wgs_of = [&](int64_t units, int64_t most) { return int(std::max<int64_t>(1, std::min(most, target / units))); };
+  const int parts = chunks >= 8 ? 4 : chunks >= 2 ? 2 : 1;
+  const size_t sums_lds = size_t(parts) * 4 * 16 * 20 * sizeof(float);
+  const auto second = [&](SmallMoeArgs& a) {
+    a.w = w2;
+    a.ws = s2;
+    a.n = int(hidden);
+    a.blocks = int(ib);
+  };
+  const auto sum = [&] {
+    hipLaunchKernelGGL(slot_sum_kernel, dim3(unsigned(sums)), dim3(kThreads), 0, st, m.c3, of, tokens, int(top_k), int(hidden), out, act_dtype);
+    return vq::check_launch("mxfp4 moe sum");
+  };
+  if (path == 0) {
+    m.by_slot = slots < experts;
+    const int64_t units = m.by_slot ? slots : experts;
+    const size_t rows13 = size_t(small_bytes(small_rows, chunks));
+    if (units * ib < split_blocks) {
+      const size_t need13 = std::max<size_t>(sums_lds, rows13);
+      const dim3 grid13(unsigned(units * ib)), block13(256 * parts);
+      if (act_dtype == vq::kBF16) hipLaunchKernelGGL(gate_up_split_kernel<vq::kBF16>, grid13, block13, need13, st, m);
+      else hipLaunchKernelGGL(gate_up_split_kernel<vq::kFP16>, grid13, block13, need13, st, m);
+    } else {
+      const int wgs = wgs_of(units, (ib + 3) / 4);
+      const dim3 grid13(unsigned(units * wgs)), block13(256);
+      if (act_dtype == vq::kBF16) hipLaunchKernelGGL((gate_up_kernel<true, vq::kBF16>), grid13, block13, rows13, st, m, wgs);
+      else hipLaunchKernelGGL((gate_up_kernel<true, vq::kFP16>), grid13, block13, rows13, st, m, wgs);
+    }
+    if (int rc = vq::check_launch("mxfp4 moe gate_up")) return rc;
+    second(m);
+    if (tokens <= 4 && top_k <= 64) {
+      const dim3 grid(unsigned(tokens * (hidden / 16))), block(unsigned(64 * std::min<int64_t>(top_k, 8)));
+      const size_t bytes = size_t(top_k) * 16 * sizeof(float);
+      if (act_dtype == vq::kBF16) hipLaunchKernelGGL(down_sum_kernel<vq::kBF16>, grid, block, bytes, st, m);
+      else hipLaunchKernelGGL(down_sum_kernel<vq::kFP16>, grid, block, bytes, st, m);
+      return vq::check_launch("mxfp4 moe down");
+    }
+    const int wgs = wgs_of(units, (hidden + 63) / 64);
+    hipLaunchKernelGGL(down_kernel<true>, dim3(unsigned(units * wgs)), dim3(256), rows2, st, m, wgs);
+    if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
+    return sum();
+  }
   uint32_t* xq = reinterpret_cast<uint32_t*>(base + ws.xq);
   if (act_dtype == vq::kBF16) {
     hipLaunchKernelGGL(count_quantize_kernel<vq::kBF16>, dim3(unsigned(groups)), dim3(moe::kRowsPartThreads), lds, st, of, lay, table,
@@ -254,72 +590,58 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
                        x, tokens, int(hb), x_stride, wide, xq, base + ws.xs);
   }
   if (int rc = vq::check_launch("mxfp4 moe count")) return rc;
-  hipLaunchKernelGGL(fill_kernel, dim3(unsigned(lay.parts())), dim3(moe::kRowsPartThreads), lds, st, lay, table, tiles ? kTileRows : kTaskRows);
+  hipLaunchKernelGGL(fill_kernel, dim3(unsigned(lay.parts())), dim3(moe::kRowsPartThreads), lds, st, lay, table,
+                     path == 2 ? kTileRows : kTaskRows);
   if (int rc = vq::check_launch("mxfp4 moe fill")) return rc;
-  if (tiles) {
-    TileArgs t{};
-    t.a = base + ws.xq;
-    t.as = base + ws.xs;
-    t.a_rows = tokens;
-    t.w = w13;
-    t.ws = s13;
-    t.n = 2 * inter;
-    t.blocks = int(hb);
-    t.tiles_n = int((inter + 63) / 64);
-    t.table = table;
-    t.tasks = lay.tasks();
-    t.sorted = lay.sorted();
-    t.topk_w = topk_w;
-    t.top_k = int(top_k);
-    t.limit = limit;
-    t.h = base + ws.hq;
-    t.hs = base + ws.hs;
-    const int64_t bound = (slots / kTileRows + std::min(experts, slots) + 7) / 8 * 8;
-    hipLaunchKernelGGL((tile_kernel<2, 2, kGateUp>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
+  if (path == 1) {
+    const int wgs13 = wgs_of(lay.max_tasks, (ib + 3) / 4), wgs2 = wgs_of(lay.max_tasks, (hidden + 63) / 64);
+    if (lay.max_tasks * std::max(wgs13, wgs2) > INT_MAX) return vq::fail("mxfp4 moe: too many rows");
+    hipLaunchKernelGGL((gate_up_kernel<false, vq::kBF16>), dim3(unsigned(lay.max_tasks * wgs13)), dim3(256),
+                       size_t(small_bytes(small_rows, chunks)), st, m, wgs13);
     if (int rc = vq::check_launch("mxfp4 moe gate_up")) return rc;
-    t.a = base + ws.hq;
-    t.as = base + ws.hs;
-    t.w = w2;
-    t.ws = s2;
-    t.n = hidden;
-    t.blocks = int(ib);
-    t.tiles_n = int((hidden + 127) / 128);
-    t.out = base + ws.c3;
-    hipLaunchKernelGGL((tile_kernel<2, 2, kDown>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
+    second(m);
+    hipLaunchKernelGGL(down_kernel<false>, dim3(unsigned(lay.max_tasks * wgs2)), dim3(256), rows2, st, m, wgs2);
     if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
-    hipLaunchKernelGGL(slot_sum_kernel, dim3(unsigned(sums)), dim3(kThreads), 0, st, static_cast<const float*>(t.out), of, tokens, int(top_k), int(hidden), out, act_dtype);
-    return vq::check_launch("mxfp4 moe sum");
+    return sum();
   }
-  GemmArgs g{};
-  g.a = base + ws.xq;
-  g.as = base + ws.xs;
-  g.w = w13;
-  g.ws = s13;
-  g.table = table;
-  g.tasks = lay.tasks();
-  g.sorted = lay.sorted();
-  g.topk_w = topk_w;
-  g.top_k = int(top_k);
-  g.n = int(2 * inter);
-  g.blocks = int(hb);
-  g.limit = limit;
-  g.h = base + ws.hq;
-  g.hs = base + ws.hs;
-  hipLaunchKernelGGL(gate_up_kernel, dim3(unsigned(ib), unsigned(lay.max_tasks)), dim3(64), 0, st, g);
+  TileArgs t{};
+  t.a = base + ws.xq;
+  t.as = base + ws.xs;
+  t.a_rows = tokens;
+  t.w = w13;
+  t.ws = s13;
+  t.n = 2 * inter;
+  t.blocks = int(hb);
+  t.tiles_n = int((inter + 63) / 64);
+  t.table = table;
+  t.tasks = lay.tasks();
+  t.sorted = lay.sorted();
+  t.topk_w = topk_w;
+  t.top_k = int(top_k);
+  t.limit = limit;
+  t.h = base + ws.hq;
+  t.hs = base + ws.hs;
+  const int64_t bound = (slots / kTileRows + std::min(experts, slots) + 7) / 8 * 8;
+  if (bound * std::max((inter + 63) / 64, (hidden + 127) / 128) > INT_MAX) return vq::fail("mxfp4 moe: too many rows");
+  hipLaunchKernelGGL((tile_kernel<2, 2, kGateUp>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
   if (int rc = vq::check_launch("mxfp4 moe gate_up")) return rc;
-  g.a = base + ws.hq;
-  g.as = base + ws.hs;
-  g.w = w2;
-  g.ws = s2;
-  g.n = int(hidden);
-  g.blocks = int(ib);
-  g.out = reinterpret_cast<float*>(base + ws.c3);
-  hipLaunchKernelGGL(down_kernel, dim3(unsigned((hidden + 15) / 16), unsigned(lay.max_tasks)), dim3(64), 0, st, g);
+  t.a = base + ws.hq;
+  t.as = base + ws.hs;
+  t.w = w2;
+  t.ws = s2;
+  t.n = hidden;
+  t.blocks = int(ib);
+  t.tiles_n = int((hidden + 127) / 128);
+  t.out = base + ws.c3;
+  hipLaunchKernelGGL((tile_kernel<2, 2, kDown>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
   if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
-  hipLaunchKernelGGL(slot_sum_kernel, dim3(unsigned(sums)), dim3(kThreads), 0, st, g.out, of, tokens, int(top_k), int(hidden), out, act_dtype);
-  return vq::check_launch("mxfp4 moe sum");
+  return sum();
 }
 
 #ifdef MX_TUNE
 extern "C" void mx_moe_force(int f) { mx::g_moe_force = f; }
+#endif
+
+#ifdef MX_TUNE
+extern "C" void mx_moe_tune(int s, int t) { mx::g_split = s; mx::g_target = t; }
 #endif

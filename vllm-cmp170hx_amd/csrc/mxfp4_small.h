@@ -87,6 +87,26 @@ __device__ __forceinline__ void quantize_to_lds(const void* x, const RowAt& row_
   }
 }
 
+// The same of rows that are codes and scales already (row_at: their numbers).
+template <typename RowAt>
+__device__ __forceinline__ void copy_to_lds(const uint8_t* codes, const uint8_t* scales, const RowAt& row_at, int rows, int blocks,
+                                            int chunks, uint8_t* lds, int tid, int threads) {
+  uint8_t* scale = lds + small_codes_bytes(rows, chunks);
+  for (int m = 0; m < rows; ++m) {
+    const int64_t row = row_at(m) * blocks;
+    for (int b = tid; b < chunks * kChunk; b += threads) {
+      u32x4_t w{0, 0, 0, 0};
+      uint8_t s = 127;
+      if (b < blocks) {
+        w = *reinterpret_cast<const u32x4_t*>(codes + (row + b) * kBlockBytes);
+        s = scales[row + b];
+      }
+      *reinterpret_cast<u32x4_t*>(lds + (b * rows + m) * kBlockBytes) = w;
+      scale[(((b >> 4) * 4 + (b & 3)) * rows + m) * 4 + ((b >> 2) & 3)] = s;
+    }
+  }
+}
+
 // acc += chunk c of the weights times row r of the LDS activations (lanes past
 // the rows repeat the last one).
 __device__ __forceinline__ void multiply_lds(const ChunkOperand& w, const uint8_t* lds, int c, int rows, int chunks, int r, int q,
