@@ -167,7 +167,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const float* part, in
   vq::store8_act(out, dtype, i, v, numel - i);
 }
 
-template <int kN, int kM>
+template <int kSize, int kBufs>
 int launch_tile(const MatmulArgs& g, int splits, float* part, hipStream_t s) {
   TileArgs t{};
   t.a = g.a;
@@ -180,12 +180,12 @@ int launch_tile(const MatmulArgs& g, int splits, float* part, hipStream_t s) {
   t.out = splits > 1 ? part : g.out;
   t.out_dtype = splits > 1 ? int(vq::kFP32) : g.out_dtype;
   t.wide = g.n % 8 == 0 && aligned(t.out, 16);
-  t.tiles_n = int((g.n + 64 * kN - 1) / (64 * kN));
-  t.tiles_m = int((g.rows + 64 * kM - 1) / (64 * kM));
+  t.tiles_n = int((g.n + 64 * kSize - 1) / (64 * kSize));
+  t.tiles_m = int((g.rows + 64 * kSize - 1) / (64 * kSize));
   const int stages = (g.blocks + kStageBlocks - 1) / kStageBlocks;
   t.split_stages = (stages + splits - 1) / splits;
   const int64_t total = int64_t(t.tiles_n) * t.tiles_m;
-  hipLaunchKernelGGL((tile_kernel<kN, kM, kDense>), dim3(unsigned((total + 7) / 8 * 8), unsigned(splits)), dim3(kTileThreads), 0, s, t);
+  hipLaunchKernelGGL((tile_kernel<kSize, kSize, kDense, kBufs>), dim3(unsigned((total + 7) / 8 * 8), unsigned(splits)), dim3(kTileThreads), 0, s, t);
   if (int rc = vq::check_launch("mxfp4 tile")) return rc;
   if (splits == 1) return vq::kOk;
   const int64_t numel = g.rows * g.n;
@@ -202,10 +202,11 @@ int g_tile = 0, g_splits = 0, g_parts = 0, g_cols = 0, g_fuse = -1;
 
 // How a product runs.  tile 0: the few-rows kernel, `cols` column tiles and
 // `parts` parts of K a workgroup, `fused`: it quantizes x itself; else the tile
-// kernel with 64 `tile` columns and rows, K in `splits`.
+// kernel with 64 `tile` columns and rows, K in `splits`, `deep`: four stage
+// buffers instead of two.
 struct Plan {
   int tile, splits, cols, parts;
-  bool fused;
+  bool fused, deep;
 };
 
 constexpr int kCUs = 256;
@@ -215,19 +216,22 @@ constexpr int kCUs = 256;
 // `shared` per workgroup of a CU that is full; K splits write and read FP32 sums
 // at about 3 TB/s, in one more launch.  Fitted to the tile sizes and splits
 // measured at 24 to 4096 rows of 4096 x 14336, 14336 x 4096, 4096 x 4096 and
-// 2592 x 5003: it picks the fastest of them or one within 10%.
-double tile_cost(int size, int64_t rows, int64_t n, int64_t stages, int64_t splits) {
-  const double alone = size == 4 ? 1.48 : size == 2 ? 0.75 : 0.55, shared = size == 4 ? 2.3 : size == 2 ? 0.85 : 0.385;
+// 2592 x 5003, of which it picks the fastest or one within 10%.
+double tile_cost(int size, bool deep, int64_t rows, int64_t n, int64_t stages, int64_t splits) {
+  const double alone = size == 4 ? 1.48 : size == 2 ? (deep ? 0.52 : 0.72) : 0.30;
+  const double shared = size == 4 ? 2.2 : size == 2 ? (deep ? 0.60 : 0.80) : 0.385;
   const int64_t groups = ((n + 64 * size - 1) / (64 * size)) * ((rows + 64 * size - 1) / (64 * size)) * splits;
-  // whole rounds of the one workgroup of the largest tiles that a CU holds
-  const double load = size == 4 ? double((groups + kCUs - 1) / kCUs) : double(groups) / kCUs;
-  const double each = size == 4 && groups < kCUs / 2 ? alone : std::max(alone, shared * load);
+  // whole rounds where a CU holds one workgroup
+  const bool one = size == 4 || deep;
+  const double load = one ? double((groups + kCUs - 1) / kCUs) : double(groups) / kCUs;
+  // (four buffers' workgroups gain nothing from each other over rounds)
+  const double each = one && groups < kCUs / 2 ? alone : std::max(alone, (deep && load > 1 ? 0.95 : shared) * load);
   const double sums = splits > 1 ? 3.0 + double(rows) * double(n) * 8.0 * double(splits) / 3e6 : 0.0;
   return double((stages + splits - 1) / splits) * each + sums;
 }
 
 Plan plan_of(int64_t rows, int64_t k, int64_t n) {
-  Plan p{0, 1, 1, 1, false};
+  Plan p{0, 1, 1, 1, false, false};
   const int64_t blocks = k / kBlock, stages = (blocks + kStageBlocks - 1) / kStageBlocks;
   // the tile kernel wants whole stages, buffers below 2 GiB and a 32-bit grid
   const bool tiles = rows > 16 && blocks >= kStageBlocks && k <= (int64_t(1) << 22) &&
@@ -237,14 +241,16 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n) {
   // 20.9 (15.3).
   if (tiles && (rows > 64 || (rows + 15) / 16 * double(n) * double(k) > 64e6)) {
     double best = 0;
-    for (const int size : {1, 2, 4}) {
+    for (const int kind : {1, 2, 3, 4}) {  // 3: size 2 with four buffers
+      const int size = kind == 3 ? 2 : kind;
       for (const int splits : {1, 2, 4, 8}) {
         if (splits > 1 && stages < 4 * splits) continue;
-        const double cost = tile_cost(size, rows, n, stages, splits);
+        const double cost = tile_cost(size, kind == 3, rows, n, stages, splits);
         if (!p.tile || cost < best) {
           best = cost;
           p.tile = size;
           p.splits = splits;
+          p.deep = kind == 3;
         }
       }
     }
@@ -264,7 +270,10 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n) {
     p.fused = rows <= 16 && groups_cu * rows * k <= 40960;
   }
 #ifdef MX_TUNE
-  if (g_tile >= 0 && g_tile != 9) p.tile = tiles ? g_tile : 0;
+  if (g_tile >= 0 && g_tile != 9) {
+    p.tile = tiles ? g_tile == 3 ? 2 : g_tile : 0;
+    p.deep = g_tile == 3;
+  }
   if (g_splits) p.splits = g_splits;
   if (g_cols) p.cols = g_cols;
   if (g_parts) p.parts = g_parts;
@@ -314,9 +323,9 @@ SmallArgs small_args(const MatmulArgs& g) {
 }
 
 int launch_matmul(const MatmulArgs& g, const Plan& p, float* part, hipStream_t s) {
-  if (p.tile == 4) return launch_tile<4, 4>(g, p.splits, part, s);
-  if (p.tile == 2) return launch_tile<2, 2>(g, p.splits, part, s);
-  if (p.tile == 1) return launch_tile<1, 1>(g, p.splits, part, s);
+  if (p.tile == 4) return launch_tile<4, 2>(g, p.splits, part, s);
+  if (p.tile == 2) return p.deep ? launch_tile<2, 4>(g, p.splits, part, s) : launch_tile<2, 2>(g, p.splits, part, s);
+  if (p.tile == 1) return launch_tile<1, 4>(g, p.splits, part, s);
   return launch_small<false, vq::kBF16>(small_args(g), p, s);
 }
 

@@ -623,7 +623,7 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   t.hs = base + ws.hs;
   const int64_t bound = (slots / kTileRows + std::min(experts, slots) + 7) / 8 * 8;
   if (bound * std::max((inter + 63) / 64, (hidden + 127) / 128) > INT_MAX) return vq::fail("mxfp4 moe: too many rows");
-  hipLaunchKernelGGL((tile_kernel<2, 2, kGateUp>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
+  hipLaunchKernelGGL((tile_kernel<2, 2, kGateUp, 2>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
   if (int rc = vq::check_launch("mxfp4 moe gate_up")) return rc;
   t.a = base + ws.hq;
   t.as = base + ws.hs;
@@ -633,7 +633,7 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   t.blocks = int(ib);
   t.tiles_n = int((hidden + 127) / 128);
   t.out = base + ws.c3;
-  hipLaunchKernelGGL((tile_kernel<2, 2, kDown>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
+  hipLaunchKernelGGL((tile_kernel<2, 2, kDown, 2>), dim3(unsigned(bound * t.tiles_n)), dim3(kTileThreads), 0, st, t);
   if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
   return sum();
 }

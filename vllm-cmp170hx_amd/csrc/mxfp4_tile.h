@@ -4,24 +4,25 @@
 // One workgroup of four wavefronts (2 x 2) computes 64 kN columns by 64 kM
 // rows, each wavefront 32 kN x 32 kM of v_mfma_scale_f32_32x32x64 tiles (its
 // rate is twice the 16x16x128 form's: 8.9 against 4.6 PFLOP/s in a loop of
-// nothing else).  A stage is 256 k: the 128 code bytes and 8 scale bytes of
-// every row and column.
-//  * Codes come to LDS by DMA, one 128-byte line of a row in eight lanes, the
-//    next stage's while this one is multiplied (two buffers, one barrier a
-//    stage).  A row's eight 16-byte blocks lie in LDS in the order kb ^ (row / 2
-//    & 7), so that the 16 rows that a ds_read_b128 reads at once, all at one kb,
-//    lie on 16 different 16-byte columns of the 64 banks.
+// nothing else).  A stage is 256 k: the 128 code bytes and 8 scale bytes of every
+// row and column, in one of kBufs buffers; one barrier a stage.
+//  * Codes come to LDS by DMA, one 128-byte line of a row in eight lanes, up to
+//    kBufs - 1 stages ahead.  A row's eight 16-byte blocks lie in LDS in the order
+//    kb ^ (row / 2 & 7), so that the 16 rows that a ds_read_b128 reads at once, all
+//    at one kb, lie on 16 different 16-byte columns of the 64 banks.
 //  * A lane of the 32x32x64 form holds one block: row lane & 31, block 2 sub +
 //    (lane >> 5) of the stage's 64-k sub-step `sub`.  Scales come through
-//    registers, a row's even blocks' bytes in one dword and the odd blocks' in
-//    another: a lane reads one dword a row and stage, and the MFMA's byte
-//    selector is `sub`.
+//    registers, a row's even blocks' bytes in one half of its LDS entry and the
+//    odd blocks' in the other: a lane reads one half a row and stage, and the
+//    MFMA's byte selector is `sub`.
 //  * Weights are the A operand, rows the B operand, so that a lane's sums are
 //    of one row: 16 of a 32-column block, the other 16 in lane ^ 32.
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "mxfp4.h"
 
@@ -31,7 +32,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
 constexpr int kTileThreads = 256;
-constexpr int kStageBlocks = 8;                          // 256 k
+constexpr int kStageBlocks = 8;                          // 256 k; the fewest that the kernel takes
 constexpr int kStageBytes = kStageBlocks * kBlockBytes;  // of codes, a row
 
 // f(std::integral_constant<int, i>) for i = first .. last - 1.
@@ -95,7 +96,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, uint3
 // An offset past any buffer: such loads give zeros.
 constexpr uint32_t kPastEnd = 0x80000000u;
 
-// Eight scale bytes of a row of at least eight blocks, from block b0 on (the
+// A stage's scale bytes of a row of at least eight blocks, from block b0 on (the
 // last eight, where fewer are left), as they come from memory,
 __device__ __forceinline__ uint64_t load_scales(const uint8_t* row, int b0, int blocks) {
   uint64_t v;
@@ -154,14 +155,30 @@ __device__ __forceinline__ void store_rows(const float* part, int stride, int la
   }
 }
 
-template <int kN, int kM, int kMode>
-__global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel(TileArgs g) {
+// Workgroups of a size that a CU's LDS (and registers) hold, two at most.
+constexpr int tile_groups(int n, int m, int bufs) { return n * m > 8 || 64 * (n + m) * (kStageBytes * bufs + 16) > 80 * 1024 ? 1 : 2; }
+
+template <int kN, int kM, int kMode, int kBufs>
+__global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile_kernel(TileArgs g) {
   constexpr int kCols = 64 * kN, kRows = 64 * kM, kLines = kCols + kRows;
-  constexpr int kLoadsW = kCols / 32, kLoadsA = kRows / 32;  // 1 KB DMA loads a wavefront and stage
+  constexpr int kLoadRows = 8;  // lines of a 1 KB DMA load
+  constexpr int kLoadsW = kCols / (4 * kLoadRows), kLoadsA = kRows / (4 * kLoadRows);  // loads a wavefront and stage
   constexpr int kLoads = kLoadsW + kLoadsA;
+  static_assert(kBufs == 2 || kBufs == 4, "stage buffers");
   constexpr int kScaleRows = (kLines + kTileThreads - 1) / kTileThreads;
-  __shared__ __attribute__((aligned(1024))) uint8_t buf0[kLines * kStageBytes], buf1[kLines * kStageBytes];
+  // (buffers by name: the compiler then sees that a stage's reads are not of the
+  // buffer that the DMA is filling, and does not wait for it)
+  constexpr int kBufBytes = kLines * kStageBytes;
+  __shared__ __attribute__((aligned(1024))) uint8_t buf0[kBufBytes], buf1[kBufBytes], buf2[kBufs > 2 ? kBufBytes : 16],
+      buf3[kBufs > 2 ? kBufBytes : 16];
   __shared__ __attribute__((aligned(16))) uint2 scale0[kLines], scale1[kLines];
+  const auto buf = [&](auto i_c) -> uint8_t* {
+    constexpr int i = decltype(i_c)::value % kBufs;
+    if constexpr (i == 0) return buf0;
+    else if constexpr (i == 1) return buf1;
+    else if constexpr (i == 2) return buf2;
+    else return buf3;
+  };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = vq::uniform(tid >> 6);
@@ -221,17 +238,19 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
   const __amdgpu_buffer_rsrc_t abuf =
       buffer(g.a + act0 * line, uint32_t(kMode == kGateUp ? g.a_rows : int64_t(nrows)) * uint32_t(line));
 
-  // ---- loads: 1 KB each, 8 lines; a wavefront's first kLoadsW bring weights.
-  // Rows that follow each other: the first one's offset is scalar (a row of the
-  // buffer also where the eight lie past its end: their sums are not stored; the
-  // rest of eight that begin inside it are zeros), and the lane's part has two
-  // values, by the parity of the line's eight.  Scattered rows (kGateUp's
+  // ---- loads: 1 KB each, kLoadRows lines; a wavefront's first kLoadsW bring
+  // weights.  Rows that follow each other: the first one's offset is scalar (a row
+  // of the buffer also where the load's lie past its end: their sums are not
+  // stored; the rest of a load that begins inside it is zeros), and the lane's part
+  // has two values, by the parity of the load's place.  Scattered rows (kGateUp's
   // tokens): an offset a lane and load.
   const uint32_t rline = uint32_t(line);
   const int sub_row = lane >> 3;
-  const auto first_line = [&](int i) { return i < kLoadsW ? 8 * (kLoadsW * wave + i) : kCols + 8 * (kLoadsA * wave + i - kLoadsW); };
-  const auto block_of = [&](int parity) { return (lane & 7) ^ ((4 * parity + (sub_row >> 1)) & 7); };
-  const int kb[2] = {block_of(0), block_of(1)};
+  const auto first_line = [&](int i) {
+    return i < kLoadsW ? kLoadRows * (kLoadsW * wave + i) : kCols + kLoadRows * (kLoadsA * wave + i - kLoadsW);
+  };
+  const auto swizzle_of = [](int l) { return (l >> 1) & 7; };
+  const int kb[2] = {(lane & 7) ^ swizzle_of(sub_row), (lane & 7) ^ swizzle_of(kLoadRows + sub_row)};
   const uint32_t lane_off[2] = {sub_row * rline + kb[0] * kBlockBytes, sub_row * rline + kb[1] * kBlockBytes};
   uint32_t token_off[kMode == kGateUp ? kLoadsA : 1];
   if constexpr (kMode == kGateUp) {
@@ -247,7 +266,7 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
       const int l = first_line(i), half = l / (32 * kN), j = l % (32 * kN) / 32;
       const bool up = j >= kN / 2;
       const int c = c0 + 16 * kN * half + 32 * (up ? j - kN / 2 : j) + (l & 31);
-      return (c < inter ? c : 0) + (up ? inter : 0);  // inter: whole eights
+      return (c < inter ? c : 0) + (up ? inter : 0);  // inter: whole 32s
     }
     return first_line(i) < w_rows ? first_line(i) : 0;
   };
@@ -264,7 +283,7 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
     stages = min(first + g.split_stages, all_stages);
   }
   // DMA load i of stage s (zeros past the last stage)
-  const auto fetch = [&](auto i_c, int s, uint8_t* buf) {
+  const auto fetch = [&](auto i_c, int s, uint8_t* buf) __attribute__((always_inline)) {
     constexpr int i = decltype(i_c)::value;
     const int left = s < stages ? g.blocks - s * kStageBlocks : 0;
     const int parity = (i < kLoadsW ? kLoadsW * wave + i : kLoadsA * wave + i - kLoadsW) & 1;
@@ -276,23 +295,30 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
     __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? wbuf : abuf, (lds_ptr_t)(buf + first_line(i) * kStageBytes), 16,
                                              int(o), row_part + (left > 0 ? s * kStageBytes : 0), 0, 0);
   };
-  uint64_t sreg[kScaleRows];
-  const auto fetch_scales = [&](int s) {
+  uint64_t sreg[kBufs][kScaleRows];  // of the stages on their way
+  const auto fetch_scales = [&](auto set_c, int s) {
+    constexpr int set = decltype(set_c)::value % kBufs;
 #pragma unroll
-    for (int i = 0; i < kScaleRows; ++i) sreg[i] = load_scales(srow[i], s * kStageBlocks, g.blocks);
+    for (int i = 0; i < kScaleRows; ++i) sreg[set][i] = load_scales(srow[i], s * kStageBlocks, g.blocks);
   };
-  // stage s has landed (its loads of this wavefront, then everyone's), and no
-  // wavefront reads the buffer before it any more
-  const auto land = [&](int s, uint2* scales) {
-    vq::wait_vmcnt<0>();
+  // stage s has landed (its loads of this wavefront, behind which kBufs - 2 stages'
+  // stay on their way, then everyone's), and no wavefront reads the stage before it
+  // any more
+  const auto land = [&](auto set_c, int s, uint2* scales) {
+    constexpr int set = decltype(set_c)::value % kBufs;
+    vq::wait_vmcnt<(kBufs - 2) * kLoads>();
     const int b0 = min(s, all_stages - 1) * kStageBlocks;
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i) {
       if (kLines % kTileThreads == 0 || tid + i * kTileThreads < kLines) {
-        scales[tid + i * kTileThreads] = order_scales(sreg[i], b0, g.blocks);
+        scales[tid + i * kTileThreads] = order_scales(sreg[set][i], b0, g.blocks);
       }
     }
-    __syncthreads();
+    // (a barrier that leaves the loads on their way: __syncthreads() waits for them)
+    vq::wait_lgkmcnt0();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
 
   f32x16_t acc[kN][kM];
@@ -304,7 +330,7 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
       for (int k = 0; k < 16; ++k) acc[i][j][k] = 0;
 
   const int wline = 32 * kN * wn + r, aline = kCols + 32 * kM * wm + r;
-  const int swizzle = (r >> 1) & 7;
+  const int swizzle = swizzle_of(r);
   uint32_t sw[2][kN], sa[2][kM];          // this stage's scales and the next one's
   u32x4_t fw[2][kN], fa[2][kM];           // this sub-step's operands and the next one's
   const auto read_scales = [&](const uint2* scales, uint32_t (&w)[kN], uint32_t (&a)[kM]) {
@@ -315,60 +341,81 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
     for (int j = 0; j < kM; ++j) a[j] = words[2 * (aline + 32 * j) + h];
   };
   // operand i of a sub-step: kN of weights, then kM of rows
-  const auto read = [&](auto i_c, const uint8_t* buf, int sub, int set) {
+  const auto read = [&](auto i_c, const uint8_t* buf, int sub, int set) __attribute__((always_inline)) {
     constexpr int i = decltype(i_c)::value;
     const int at = ((2 * sub + h) ^ swizzle) * kBlockBytes;
     if constexpr (i < kN) fw[set][i] = *reinterpret_cast<const u32x4_t*>(buf + (wline + 32 * i) * kStageBytes + at);
     else fa[set][i - kN] = *reinterpret_cast<const u32x4_t*>(buf + (aline + 32 * (i - kN)) * kStageBytes + at);
   };
-  // Sub-step `sub` of a stage, in kN groups of kM MFMAs: beside them the next
-  // sub-step's operands are read (of `next`, at sub-step next_sub) and loads
-  // kFirst .. kLast - 1 of stage s issued into `into`.  A wavefront issues in
-  // order and alone on its SIMD, so loads in one burst would hold up its MFMAs
-  // (16 cycles a load and CU): spread out they cost nothing.
-  const auto step = [&](auto sub_c, auto first_c, auto last_c, int set, const uint8_t* next, int next_sub, int s, uint8_t* into) {
+  // Sub-step `sub` of a stage: between its kN kM MFMAs, one or two at a time, the
+  // next sub-step's operands are read (of `next`, at sub-step next_sub) and loads
+  // kFirst .. kLast - 1 of stage s issued into `into`.  A wavefront issues in order
+  // and alone on its SIMD: what stands between two MFMAs hides behind the first
+  // one's 32 cycles (six or seven instructions), and loads in one burst would hold
+  // up the MFMAs behind them (16 cycles a load and CU).
+  const auto step = [&](auto sub_c, auto first_c, auto last_c, int set, const uint8_t* next, int next_sub, int s,
+                        uint8_t* into) __attribute__((always_inline)) {
     constexpr int sub = decltype(sub_c)::value, kFirst = decltype(first_c)::value, kLast = decltype(last_c)::value;
-    for_each<kN>([&](auto i_c) {
-      constexpr int i = decltype(i_c)::value;
-      constexpr int kReads = kN + kM;
-      for_range<i * kReads / kN, (i + 1) * kReads / kN>([&](auto k) { read(k, next, next_sub, (sub + 1) & 1); });
-      for_range<kFirst + i * (kLast - kFirst) / kN, kFirst + (i + 1) * (kLast - kFirst) / kN>([&](auto k) { fetch(k, s, into); });
+    constexpr int kReads = kN + kM, kSlots = kN * kM;
+    for_each<kSlots>([&](auto slot_c) __attribute__((always_inline)) {
+      constexpr int slot = decltype(slot_c)::value, i = slot / kM, j = slot % kM;
+      for_range<slot * kReads / kSlots, (slot + 1) * kReads / kSlots>([&](auto k) __attribute__((always_inline)) {
+        read(k, next, next_sub, (sub + 1) & 1);
+      });
+      constexpr int kFetch = kLast - kFirst, kTurn = (slot + kSlots / 2) % kSlots;  // in other slots than the reads
+      for_range<kFirst + kTurn * kFetch / kSlots, kFirst + (kTurn + 1) * kFetch / kSlots>(
+          [&](auto k) __attribute__((always_inline)) { fetch(k, s, into); });
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int j = 0; j < kM; ++j) mfma32<sub>(acc[i][j], fw[sub & 1][i], sw[set][i], fa[sub & 1][j], sa[set][j]);
+      mfma32<sub>(acc[i][j], fw[sub & 1][i], sw[set][i], fa[sub & 1][j], sa[set][j]);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  // Stage s from cur.  The barrier comes before the last sub-step, whose
-  // operands are in registers by then: its MFMAs run while the next stage's
-  // first operands are read.
+  // Stage s, the i-th of a round of the buffers.  The barrier comes before the last
+  // sub-step, whose operands are in registers by then: its MFMAs run while the next
+  // stage's first operands are read, and its buffer takes stage s + kBufs: half of
+  // those loads here, the others in the next stage's first sub-steps.
   constexpr int kHalf = kLoads / 2, kMore = kHalf + kLoads / 4;
-  const auto stage = [&](int s, int set, uint8_t* cur, uint8_t* next, uint2* next_scales) {
+  const auto stage = [&](auto i_c, int s) __attribute__((always_inline)) {
+    constexpr int i = decltype(i_c)::value;
     using std::integral_constant;
     constexpr integral_constant<int, 0> c0{};
-    step(c0, integral_constant<int, kHalf>{}, integral_constant<int, kMore>{}, set, cur, 1, s + 1, next);
-    step(integral_constant<int, 1>{}, integral_constant<int, kMore>{}, integral_constant<int, kLoads>{}, set, cur, 2, s + 1, next);
+    constexpr integral_constant<int, i + 1> c1{};
+    uint8_t* const cur = buf(i_c);
+    uint8_t* const next = buf(c1);
+    uint8_t* const prev = buf(integral_constant<int, i + kBufs - 1>{});
+    uint2* const next_scales = i & 1 ? scale0 : scale1;
+    constexpr int set = i & 1;
+    step(c0, integral_constant<int, kHalf>{}, integral_constant<int, kMore>{}, set, cur, 1, s + kBufs - 1, prev);
+    step(integral_constant<int, 1>{}, integral_constant<int, kMore>{}, integral_constant<int, kLoads>{}, set, cur, 2, s + kBufs - 1, prev);
     step(integral_constant<int, 2>{}, c0, c0, set, cur, 3, 0, cur);
-    land(s + 1, next_scales);
-    fetch_scales(s + 2);
+    land(c1, s + 1, next_scales);
+    fetch_scales(i_c, s + kBufs);
     read_scales(next_scales, sw[set ^ 1], sa[set ^ 1]);
-    step(integral_constant<int, 3>{}, c0, integral_constant<int, kHalf>{}, set, next, 0, s + 2, cur);
+    step(integral_constant<int, 3>{}, c0, integral_constant<int, kHalf>{}, set, next, 0, s + kBufs, cur);
   };
-  for_range<0, kLoads>([&](auto k) { fetch(k, first, buf0); });
-  fetch_scales(first);
-  land(first, scale0);
-  fetch_scales(first + 1);
-  for_range<0, kHalf>([&](auto k) { fetch(k, first + 1, buf1); });
+  for_range<0, kBufs - 1>([&](auto b_c) {
+    constexpr int b = decltype(b_c)::value;
+    fetch_scales(b_c, first + b);
+    for_range<0, kLoads>([&](auto k) { fetch(k, first + b, buf(b_c)); });
+  });
+  land(std::integral_constant<int, 0>{}, first, scale0);
+  fetch_scales(std::integral_constant<int, kBufs - 1>{}, first + kBufs - 1);
+  for_range<0, kHalf>([&](auto k) { fetch(k, first + kBufs - 1, buf(std::integral_constant<int, kBufs - 1>{})); });
   read_scales(scale0, sw[0], sa[0]);
   for_range<0, kN + kM>([&](auto k) { read(k, buf0, 0, 0); });
-  // stages in pairs, one buffer each by name: the compiler then sees that a
-  // stage's reads are not of the buffer that the DMA is filling
   int s = first;
-  for (; s + 1 < stages; s += 2) {
-    stage(s, 0, buf0, buf1, scale1);
-    stage(s + 1, 1, buf1, buf0, scale0);
+  for (; s + kBufs <= stages; s += kBufs) {
+    for_range<0, kBufs>([&](auto i) __attribute__((always_inline)) { stage(i, s + decltype(i)::value); });
   }
-  if (s < stages) stage(s, 0, buf0, buf1, scale1);
+  if (s < stages) {
+    stage(std::integral_constant<int, 0>{}, s);
+    if constexpr (kBufs > 2) {
+      if (s + 1 < stages) {
+        stage(std::integral_constant<int, 1>{}, s + 1);
+        if (s + 2 < stages) stage(std::integral_constant<int, 2>{}, s + 2);
+      }
+    }
+  }
   vq::wait_vmcnt<0>();  // the last loads (zeros) are in before their buffers are used again
 
   // ---- results
@@ -410,8 +457,9 @@ __global__ __launch_bounds__(kTileThreads, kN * kM > 8 ? 1 : 2) void tile_kernel
     // each row tile through LDS (a wavefront's own part, rows 16 bytes apart
     // from a bank's multiple), then whole rows of 32 kN columns
     constexpr int kStride = 32 * kN + 4;
-    static_assert(2 * 32 * kStride * 4 <= int(sizeof(buf0)), "two wavefronts' exchange fits a stage buffer");
-    float* part = reinterpret_cast<float*>(wave < 2 ? buf0 : buf1) + (wave & 1) * 32 * kStride;
+    static_assert((4 / kBufs) * 32 * kStride * 4 <= kBufBytes, "the wavefronts' exchanges fit the stage buffers");
+    float* part = kBufs == 2 ? reinterpret_cast<float*>(wave < 2 ? buf0 : buf1) + (wave & 1) * 32 * kStride
+                             : reinterpret_cast<float*>(wave < 2 ? (wave ? buf1 : buf0) : (wave == 2 ? buf2 : buf3));
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kM; ++i) {
