@@ -647,7 +647,8 @@ int moe_balance_loss(const void* logits, int dtype, int64_t rows, int64_t expert
                      int scoring, float* loss, int64_t* counts, float* stats, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
-/* grad [rows][experts] (contiguous, of the logits' dtype) = upstream[0] *
+/* grad [rows][experts] (contiguous, of the logits' dtype, aligned to four elements)
+ * = upstream[0] *
  * dloss/dlogits with the counts constant, zeros in padding rows. */
 int moe_balance_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,
                      const uint8_t* is_padding, int scoring, const float* stats,

@@ -18,10 +18,16 @@
 // much).  A row whose logits leave nothing (all -inf, sigmoids that sum to 0)
 // has p = 0.  Counts are whole numbers, so their atomics give one result in any
 // order; the rows' parts are summed in 64 bits in a fixed order.
+//
+// Bound by the logits' bytes where rows are many: at 65536 rows of 256 in FP32 (64
+// MiB, 14 us at the rate of a large copy) the loss takes 17 us after a count of 12
+// us and before a finish of 5 us, the gradient (twice the bytes) 23 us; at 200 rows
+// of 128 one launch each, which costs less than its call from the host.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "../../include/vllm_mi355x.h"
 #include "common.h"
@@ -31,168 +37,398 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr int kCountThreads = 1024;
 constexpr int kMaxExperts = 1024;
-constexpr int kMaxParts = 64;    // workgroups that count
-constexpr int kMaxGroups = 1024; // workgroups that take rows
+// Workgroups that count: the count and the loss that adds them up took 11.6 + 17.0 us
+// at 65536 rows of 256 with 32, 8.2 + 25.1 us with 64.
+constexpr int kMaxParts = 32;
+constexpr int kLossThreads = 1024, kLossWaves = kLossThreads / 64;
+constexpr int kMaxGroups = 512;  // workgroups of the loss: two a CU, few enough to add up the counts
+constexpr int kGradGroups = 2048;
+// Calls of up to so many logits run in one workgroup and launch (200 rows of 128:
+// the launches cost more than the rows).
+constexpr int kOneLogits = 1 << 15;
 
-__device__ __forceinline__ float wave_sum(float v, int lane) {
-  v += vq::xor_lanes<32>(v, lane);
-  v += vq::xor_lanes<16>(v, lane);
+// ---- a row of logits in the lanes of a wavefront ----------------------------------
+
+// How experts lie in lanes: kLanes lanes a row (64 / kLanes rows a wavefront), four
+// consecutive experts a lane and step, kSteps steps.
+template <int kLanes_, int kSteps_>
+struct Shape {
+  static constexpr int kLanes = kLanes_, kSteps = kSteps_, kRows = 64 / kLanes_;
+};
+
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v, int lane) {
+  if constexpr (kLanes > 32) v += vq::xor_lanes<32>(v, lane);
+  if constexpr (kLanes > 16) v += vq::xor_lanes<16>(v, lane);
   v += vq::xor_lanes<8>(v, lane);
   v += vq::xor_lanes<4>(v, lane);
   v += vq::xor_lanes<2>(v, lane);
   v += vq::xor_lanes<1>(v, lane);
   return v;
 }
+template <int kLanes>
+__device__ __forceinline__ float lanes_max(float v, int lane) {
+  if constexpr (kLanes > 32) v = fmaxf(v, vq::xor_lanes<32>(v, lane));
+  if constexpr (kLanes > 16) v = fmaxf(v, vq::xor_lanes<16>(v, lane));
+  v = fmaxf(v, vq::xor_lanes<8>(v, lane));
+  v = fmaxf(v, vq::xor_lanes<4>(v, lane));
+  v = fmaxf(v, vq::xor_lanes<2>(v, lane));
+  v = fmaxf(v, vq::xor_lanes<1>(v, lane));
+  return v;
+}
 
-// hist[part][E + 1]: the part's slots by expert, and its rows.
-__global__ __launch_bounds__(kThreads) void count_kernel(const int32_t* ids, const uint8_t* padding, int64_t rows, int top_k,
-                                                         int experts, int32_t* hist) {
-  extern __shared__ int count[];
-  for (int e = threadIdx.x; e <= experts; e += kThreads) count[e] = 0;
-  __syncthreads();
-  int mine = 0;
-  for (int64_t t = int64_t(blockIdx.x) * kThreads + threadIdx.x; t < rows; t += int64_t(gridDim.x) * kThreads) {
-    if (padding && padding[t]) continue;
-    ++mine;
-    for (int k = 0; k < top_k; ++k) {
-      const int id = ids[t * top_k + k];
-      if (id >= 0 && id < experts) atomicAdd(&count[id], 1);
+// e^x for x <= 0: 2^y of y = x log2(e) as rounded, corrected by what the rounding
+// took (a relative error of 2^-22 whatever x; of y alone |x| 2^-24).
+__device__ __forceinline__ float exp_nonpositive(float x) {
+  constexpr float kLog2e = 1.44269504f, kLow = 1.925963033e-8f, kLn2 = 0.693147181f;
+  const float y = x * kLog2e;
+  float low = __builtin_fmaf(x, kLog2e, -y) + x * kLow;
+  low = x > -104.0f ? low : 0.0f;  // (infinities have no difference)
+  const float p = __builtin_amdgcn_exp2f(y);
+  return __builtin_fmaf(p, low * kLn2, p);
+}
+
+struct Rows {
+  const void* logits;
+  int64_t stride;
+  const uint8_t* padding;
+  int64_t rows;
+  int experts;
+  bool wide;  // four experts at a time: whole fours, rows on whole fours
+};
+
+template <typename S>
+struct Values {
+  float v[S::kSteps][4];
+};
+
+// Row t's logits (experts past the last are -inf).
+template <typename S, int kDtype>
+__device__ __forceinline__ Values<S> load_row(const Rows& g, int64_t t, int l) {
+  Values<S> o;
+#pragma unroll
+  for (int i = 0; i < S::kSteps; ++i) {
+    const int e = 4 * (S::kLanes * i + l);
+    if (g.wide && e < g.experts) {
+      const int64_t at = t * g.stride + e;
+      if constexpr (kDtype == vq::kFP32) {
+        typedef float f4_t __attribute__((ext_vector_type(4)));
+        const f4_t w = *reinterpret_cast<const f4_t*>(static_cast<const float*>(g.logits) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.v[i][j] = w[j];
+      } else {
+        typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+        const u2_t w = *reinterpret_cast<const u2_t*>(static_cast<const uint16_t*>(g.logits) + at);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint16_t u = uint16_t(w[j >> 1] >> (16 * (j & 1)));
+          o.v[i][j] = kDtype == vq::kBF16 ? vq::bf16_to_f32(u) : vq::f16_to_f32(u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o.v[i][j] = e + j < g.experts ? vq::load_act(g.logits, kDtype, t * g.stride + e + j) : -__builtin_inff();
+      }
     }
   }
-  if (mine) atomicAdd(&count[experts], mine);
-  __syncthreads();
-  for (int e = threadIdx.x; e <= experts; e += kThreads) hist[int64_t(blockIdx.x) * (experts + 1) + e] = count[e];
+  return o;
 }
 
-// counts[e] (+)= the parts' sums; stats (may be null): f_e, then 1/n (0 for no rows).
-__global__ __launch_bounds__(kThreads) void totals_kernel(const int32_t* hist, int parts, int experts, int top_k, bool add,
-                                                          int64_t* counts, float* stats) {
-  int64_t n = 0;
-  for (int p = 0; p < parts; ++p) n += hist[int64_t(p) * (experts + 1) + experts];
-  for (int e = threadIdx.x; e < experts; e += kThreads) {
-    int64_t c = 0;
-    for (int p = 0; p < parts; ++p) c += hist[int64_t(p) * (experts + 1) + e];
-    counts[e] = add ? counts[e] + c : c;
-    if (stats) stats[e] = n ? float(double(c) * experts / (double(n) * top_k)) : 0.0f;
-  }
-  if (stats && threadIdx.x == 0) stats[experts] = n ? float(1.0 / double(n)) : 0.0f;
-}
-
-// The row's probabilities p and, for the gradient, their slopes d (lane holds
-// experts lane + 64 i), and r = sum f p.
-template <int kPer, bool kSigmoid>
-__device__ __forceinline__ float row_terms(const void* logits, int dtype, int64_t at, const float* f, int experts, int lane,
-                                           float (&d)[kPer]) {
-  float l[kPer], z[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int e = lane + 64 * i;
-    l[i] = e < experts ? vq::load_act(logits, dtype, at + e) : -__builtin_inff();
-  }
+// From a row's logits its r = sum f p (in all its lanes), and in place of the
+// logits the slopes p (softmax) or p (1 - sigmoid).  f: LDS, zeros past the last
+// expert up to a whole step.
+template <typename S, bool kSigmoid>
+__device__ __forceinline__ float row_terms(Values<S>& x, const float* f, int l, int lane) {
   float m = 0;
   if constexpr (!kSigmoid) {
-    m = l[0];
+    m = x.v[0][0];
 #pragma unroll
-    for (int i = 1; i < kPer; ++i) m = fmaxf(m, l[i]);
-    m = vq::wave_max(m, lane);
+    for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, x.v[i][j]);
+    m = lanes_max<S::kLanes>(m, lane);
     if (m == -__builtin_inff()) m = 0;
   }
   float sum = 0, dot = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int e = lane + 64 * i;
-    if constexpr (kSigmoid) {
-      const float t = expf(-fabsf(l[i]));
-      const float small = t / (1 + t), large = 1 / (1 + t);
-      z[i] = l[i] >= 0 ? large : small;
-      d[i] = l[i] >= 0 ? small : large;
-    } else {
-      z[i] = expf(l[i] - m);
-      d[i] = 1;
-    }
-    if (e < experts) {
-      sum += z[i];
-      dot += f[e] * z[i];
+  for (int i = 0; i < S::kSteps; ++i) {
+    typedef float f4_t __attribute__((ext_vector_type(4)));
+    const f4_t w = *reinterpret_cast<const f4_t*>(f + 4 * (S::kLanes * i + l));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float z;
+      if constexpr (kSigmoid) {
+        const float a = x.v[i][j], t = exp_nonpositive(-fabsf(a)), large = 1 / (1 + t), small = t * large;
+        z = a >= 0 ? large : small;
+        x.v[i][j] = large * small;
+        if (a != a) z = x.v[i][j] = a;
+      } else {
+        z = x.v[i][j] = exp_nonpositive(x.v[i][j] - m);
+      }
+      sum += z;
+      dot = __builtin_fmaf(w[j], z, dot);
     }
   }
-  sum = wave_sum(sum, lane);
-  dot = wave_sum(dot, lane);
+  sum = lanes_sum<S::kLanes>(sum, lane);
+  dot = lanes_sum<S::kLanes>(dot, lane);
   const float inv = sum == 0 ? 0.0f : 1 / sum;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) d[i] *= z[i] * inv;
+  for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x.v[i][j] *= inv;
   return dot * inv;
 }
 
-// partial[workgroup] = the sum of its rows' r, one row a wavefront.
-template <int kPer, bool kSigmoid>
-__global__ __launch_bounds__(kThreads) void loss_kernel(const void* logits, int dtype, int64_t stride, const uint8_t* padding,
-                                                        int64_t rows, int experts, const float* stats, double* partial) {
-  __shared__ double part[kWaves];
-  const int lane = threadIdx.x & 63, wave = vq::uniform(int(threadIdx.x) >> 6);
-  double sum = 0;
-  float d[kPer];
-  for (int64_t t = int64_t(blockIdx.x) * kWaves + wave; t < rows; t += int64_t(gridDim.x) * kWaves) {
-    if (padding && padding[t]) continue;
-    sum += row_terms<kPer, kSigmoid>(logits, dtype, t * stride, stats, experts, lane, d);
-  }
-  if (lane == 0) part[wave] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double all = 0;
-    for (int w = 0; w < kWaves; ++w) all += part[w];
-    partial[blockIdx.x] = all;
-  }
-}
+// ---- counts ---------------------------------------------------------------------------
 
-__global__ __launch_bounds__(64) void finish_kernel(const double* partial, int groups, const float* inv_n, float* loss) {
-  __shared__ double part[64];
-  double sum = 0;
-  for (int i = threadIdx.x; i < groups; i += 64) sum += partial[i];
-  part[threadIdx.x] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double all = 0;
-    for (int i = 0; i < 64; ++i) all += part[i];
-    loss[0] = float(all * double(inv_n[0]));
-  }
-}
+struct Counting {
+  const int32_t* ids;
+  const uint8_t* padding;
+  int64_t rows;
+  int top_k, experts;
+};
 
-template <int kPer, bool kSigmoid>
-__global__ __launch_bounds__(kThreads) void grad_kernel(const void* logits, int dtype, int64_t stride, const uint8_t* padding,
-                                                        int64_t rows, int experts, const float* stats, const float* upstream,
-                                                        void* grad) {
-  const int lane = threadIdx.x & 63, wave = vq::uniform(int(threadIdx.x) >> 6);
-  const float scale = upstream[0] * stats[experts];
-  float d[kPer];
-  for (int64_t t = int64_t(blockIdx.x) * kWaves + wave; t < rows; t += int64_t(gridDim.x) * kWaves) {
-    const bool counted = !(padding && padding[t]);
-    float r = 0;
-    if (counted) r = row_terms<kPer, kSigmoid>(logits, dtype, t * stride, stats, experts, lane, d);
+// count (LDS, experts + 1 zeros): the slots by expert of rows first, first + step, ...
+// and at its end these rows.
+__device__ __forceinline__ void count_rows(const Counting& g, int64_t first, int64_t step, int* count) {
+  int mine = 0;
+  for (int64_t t = first; t < g.rows; t += step) {
+    const int32_t* ids = g.ids + t * g.top_k;
+    // (the mark and the first ids are on their way together)
+    const bool counted = !(g.padding && g.padding[t]);
+    for (int k0 = 0; k0 < g.top_k; k0 += 8) {
+      int id[8];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int e = lane + 64 * i;
-      if (e < experts) vq::store_act(grad, dtype, t * experts + e, counted ? scale * d[i] * (stats[e] - r) : 0.0f);
+      for (int u = 0; u < 8; ++u) id[u] = ids[min(k0 + u, g.top_k - 1)];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (counted && k0 + u < g.top_k && id[u] >= 0 && id[u] < g.experts) atomicAdd(&count[id[u]], 1);
+      }
+    }
+    mine += counted;
+  }
+  if (mine) atomicAdd(&count[g.experts], mine);
+}
+
+// hist[part][E + 1]: the part's slots by expert, and its rows (an expert's parts in
+// one line make the sums slower: the loss 21.2 us for 17.0).
+__global__ __launch_bounds__(kCountThreads) void count_kernel(Counting g, int32_t* hist) {
+  __shared__ int count[kMaxExperts + 1];
+  for (int e = threadIdx.x; e <= g.experts; e += kCountThreads) count[e] = 0;
+  __syncthreads();
+  count_rows(g, int64_t(blockIdx.x) * kCountThreads + threadIdx.x, int64_t(gridDim.x) * kCountThreads, count);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= g.experts; e += kCountThreads) hist[int64_t(blockIdx.x) * (g.experts + 1) + e] = count[e];
+}
+
+// The parts' sum for entry e, all its loads on their way at once (another XCD
+// wrote them: a trip to memory).
+__device__ __forceinline__ int64_t total_of(const int32_t* hist, int parts, int experts, int e) {
+  int n[kMaxParts];
+#pragma unroll
+  for (int p = 0; p < kMaxParts; ++p) n[p] = hist[int64_t(min(p, parts - 1)) * (experts + 1) + e];
+  int64_t sum = 0;
+#pragma unroll
+  for (int p = 0; p < kMaxParts; ++p) sum += p < parts ? n[p] : 0;
+  return sum;
+}
+
+__global__ __launch_bounds__(kThreads) void totals_kernel(const int32_t* hist, int parts, int experts, bool add, int64_t* counts) {
+  for (int e = threadIdx.x; e < experts; e += kThreads) {
+    const int64_t c = total_of(hist, parts, experts, e);
+    counts[e] = add ? counts[e] + c : c;
+  }
+}
+
+// f_e of c slots, where n rows of top_k count.
+__device__ __forceinline__ float share_of(int64_t c, int64_t n, int top_k, int experts) {
+  return n ? float(double(c) * experts / (double(n) * top_k)) : 0.0f;
+}
+
+// ---- loss -------------------------------------------------------------------------------
+
+// Rows first, first + step, ... of this wavefront (S::kRows at once): the sum of
+// their r, in lane 0 of each row's lanes the row's own.
+template <typename S, int kDtype, bool kSigmoid>
+__device__ __forceinline__ double sum_rows(const Rows& g, int64_t first, int64_t step, const float* f, int lane) {
+  const int l = lane % S::kLanes, sub = lane / S::kLanes;
+  double sum = 0;
+  if (first >= g.rows) return sum;
+  // a row ahead: the next one's logits are on their way while this one's are used
+  const auto row = [&](int64_t t) { return load_row<S, kDtype>(g, min(t, g.rows - 1), l); };
+  const auto kept = [&](int64_t t) { return t < g.rows && !(g.padding && g.padding[t]); };
+  Values<S> next = row(first + sub);
+  bool next_kept = kept(first + sub);
+  for (int64_t t = first + sub; t - sub < g.rows; t += step) {
+    Values<S> x = next;
+    const bool counted = next_kept;
+    if (t - sub + step < g.rows) {
+      next = row(t + step);
+      next_kept = kept(t + step);
+    }
+    const float r = row_terms<S, kSigmoid>(x, f, l, lane);
+    if (counted && l == 0) sum += r;
+  }
+  return sum;
+}
+
+// The sum over a workgroup's `waves` wavefronts, in order (part: as many entries).
+__device__ __forceinline__ double block_sum(double v, double* part, int waves) {
+  for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double sum = 0;
+  for (int w = 0; w < waves; ++w) sum += part[w];
+  return sum;
+}
+
+struct Results {
+  float* loss;
+  int64_t* counts;
+  float* stats;  // f_e, then 1 / n
+};
+
+// All of a small call in one workgroup.
+template <typename S, int kDtype, bool kSigmoid>
+__global__ __launch_bounds__(1024) void one_kernel(Rows g, Counting c, Results out) {
+  __shared__ int count[kMaxExperts + 1];
+  __shared__ __attribute__((aligned(16))) float f[kMaxExperts];
+  __shared__ double part[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
+  for (int e = tid; e <= c.experts; e += 1024) count[e] = 0;
+  __syncthreads();
+  count_rows(c, tid, 1024, count);
+  __syncthreads();
+  const int n = count[c.experts];
+  for (int e = tid; e < kMaxExperts; e += 1024) {
+    f[e] = e < c.experts ? share_of(count[e], n, c.top_k, c.experts) : 0.0f;
+    if (e < c.experts) {
+      out.counts[e] = count[e];
+      out.stats[e] = f[e];
+    }
+  }
+  if (tid == 0) out.stats[c.experts] = n ? float(1.0 / double(n)) : 0.0f;
+  __syncthreads();
+  const double sum = block_sum(sum_rows<S, kDtype, kSigmoid>(g, wave * S::kRows, 16 * S::kRows, f, lane), part, 16);
+  if (tid == 0) out.loss[0] = n ? float(sum / double(n)) : 0.0f;
+}
+
+// partial[workgroup] = the sum of its rows' r.  Every workgroup adds up the parts'
+// counts for itself, an entry a thread (one thread the rows': as many requests to
+// the same lines as there are wavefronts would queue up in L2).  A launch of its
+// own finishes: 512 arrivals at one counter took 10 us.
+template <typename S, int kDtype, bool kSigmoid>
+__global__ __launch_bounds__(kLossThreads) void loss_kernel(Rows g, int top_k, const int32_t* hist, int parts, double* partial) {
+  __shared__ __attribute__((aligned(16))) float f[kMaxExperts];
+  __shared__ double part[kLossWaves];
+  __shared__ int64_t counted;
+  static_assert(kMaxExperts <= kLossThreads, "a thread an expert");
+  const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
+  const int64_t mine = tid < g.experts ? total_of(hist, parts, g.experts, tid) : 0;
+  if (tid == kLossThreads - 1) counted = total_of(hist, parts, g.experts, g.experts);
+  __syncthreads();
+  if (tid < S::kLanes * S::kSteps * 4) f[tid] = tid < g.experts ? share_of(mine, counted, top_k, g.experts) : 0.0f;
+  __syncthreads();
+  const int64_t first = (int64_t(blockIdx.x) * kLossWaves + wave) * S::kRows;
+  const double sum = block_sum(sum_rows<S, kDtype, kSigmoid>(g, first, int64_t(gridDim.x) * kLossWaves * S::kRows, f, lane), part, kLossWaves);
+  if (tid == 0) partial[blockIdx.x] = sum;
+}
+
+__global__ __launch_bounds__(kLossThreads) void finish_kernel(const double* partial, int groups, const int32_t* hist, int parts,
+                                                              int experts, int top_k, Results out) {
+  __shared__ double part[kLossWaves];
+  __shared__ int64_t counted;
+  static_assert(kMaxGroups <= kLossThreads, "a thread a workgroup's sum");
+  const int tid = threadIdx.x;
+  const double one = tid < groups ? partial[tid] : 0.0;
+  const int64_t mine = tid < experts ? total_of(hist, parts, experts, tid) : 0;
+  if (tid == kLossThreads - 1) counted = total_of(hist, parts, experts, experts);
+  const double all = block_sum(one, part, kLossWaves);
+  const int64_t n = counted;
+  if (tid < experts) {
+    out.counts[tid] = mine;
+    out.stats[tid] = share_of(mine, n, top_k, experts);
+  }
+  if (tid == 0) {
+    out.loss[0] = n ? float(all / double(n)) : 0.0f;
+    out.stats[experts] = n ? float(1.0 / double(n)) : 0.0f;
+  }
+}
+
+template <typename S, int kDtype, bool kSigmoid>
+__global__ __launch_bounds__(kThreads) void grad_kernel(Rows g, const float* stats, const float* upstream, void* grad) {
+  __shared__ __attribute__((aligned(16))) float f[kMaxExperts];
+  const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
+  const int l = lane % S::kLanes, sub = lane / S::kLanes;
+  for (int e = tid; e < S::kLanes * S::kSteps * 4; e += kThreads) f[e] = e < g.experts ? stats[e] : 0.0f;
+  __syncthreads();
+  const float scale = upstream[0] * stats[g.experts];
+  // (rows of the gradient lie close: on whole fours where the experts do)
+  const bool wide = g.experts % 4 == 0;
+  for (int64_t t0 = (int64_t(blockIdx.x) * kWaves + wave) * S::kRows; t0 < g.rows; t0 += int64_t(gridDim.x) * kWaves * S::kRows) {
+    const int64_t t = t0 + sub;
+    const bool counted = t < g.rows && !(g.padding && g.padding[t]);
+    Values<S> x = load_row<S, kDtype>(g, t < g.rows ? t : g.rows - 1, l);
+    const float r = row_terms<S, kSigmoid>(x, f, l, lane);
+    if (t >= g.rows) continue;
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) {
+      const int e = 4 * (S::kLanes * i + l);
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = counted ? scale * x.v[i][j] * (f[e + j] - r) : 0.0f;
+      const int64_t at = t * g.experts + e;
+      if (wide && e < g.experts) {
+        if constexpr (kDtype == vq::kFP32) {
+          typedef float f4_t __attribute__((ext_vector_type(4)));
+          *reinterpret_cast<f4_t*>(static_cast<float*>(grad) + at) = f4_t{v[0], v[1], v[2], v[3]};
+        } else {
+          typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+          const auto half = [](float a) {
+            return uint32_t(kDtype == vq::kBF16 ? vq::f32_to_bf16(a) : __builtin_bit_cast(uint16_t, _Float16(a)));
+          };
+          *reinterpret_cast<u2_t*>(static_cast<uint16_t*>(grad) + at) = u2_t{half(v[0]) | (half(v[1]) << 16), half(v[2]) | (half(v[3]) << 16)};
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (e + j < g.experts) vq::store_act(grad, kDtype, at + j, v[j]);
+        }
+      }
     }
   }
 }
 
+// launch(shape, dtype, sigmoid) with the call's as types.
 template <typename F>
-int by_width(int64_t experts, bool sigmoid, const F& launch) {
-  const auto pick = [&](auto per) {
-    if (sigmoid) launch(per, std::true_type{});
-    else launch(per, std::false_type{});
+int dispatch(int64_t experts, int dtype, bool sigmoid, const F& launch) {
+  const auto shaped = [&](auto shape) {
+    const auto typed = [&](auto type) {
+      if (sigmoid) launch(shape, type, std::true_type{});
+      else launch(shape, type, std::false_type{});
+    };
+    if (dtype == vq::kBF16) typed(std::integral_constant<int, vq::kBF16>{});
+    else if (dtype == vq::kFP16) typed(std::integral_constant<int, vq::kFP16>{});
+    else typed(std::integral_constant<int, vq::kFP32>{});
   };
-  if (experts <= 64) pick(std::integral_constant<int, 1>{});
-  else if (experts <= 128) pick(std::integral_constant<int, 2>{});
-  else if (experts <= 256) pick(std::integral_constant<int, 4>{});
-  else if (experts <= 512) pick(std::integral_constant<int, 8>{});
-  else pick(std::integral_constant<int, 16>{});
+  if (experts <= 64) shaped(Shape<16, 1>{});
+  else if (experts <= 128) shaped(Shape<32, 1>{});
+  else if (experts <= 256) shaped(Shape<64, 1>{});
+  else if (experts <= 512) shaped(Shape<64, 2>{});
+  else shaped(Shape<64, 4>{});
   return vq::check_launch("moe balance");
 }
 
-int64_t parts_of(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (rows + kThreads - 1) / kThreads)); }
-int64_t groups_of(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(kMaxGroups, (rows + kWaves - 1) / kWaves)); }
+int rows_at_once(int64_t experts) { return experts <= 64 ? 4 : experts <= 128 ? 2 : 1; }
+int64_t parts_of(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(kMaxParts, (rows + 255) / 256)); }
+int64_t groups_of(int64_t rows, int64_t experts, int64_t waves, int64_t most) {
+  const int64_t each = waves * rows_at_once(experts);
+  return std::max<int64_t>(1, std::min<int64_t>(most, (rows + each - 1) / each));
+}
 
 int check_sizes(int64_t rows, int64_t experts, int64_t top_k) {
   if (rows < 0 || rows > INT_MAX) return vq::fail("moe balance: rows out of range");
@@ -201,14 +437,24 @@ int check_sizes(int64_t rows, int64_t experts, int64_t top_k) {
   return vq::kOk;
 }
 
-int launch_counts(const int32_t* ids, const uint8_t* padding, int64_t rows, int64_t top_k, int64_t experts, bool add,
-                  int64_t* counts, float* stats, int32_t* hist, hipStream_t s) {
-  const int parts = int(parts_of(rows));
-  hipLaunchKernelGGL(count_kernel, dim3(unsigned(parts)), dim3(kThreads), size_t(experts + 1) * sizeof(int), s, ids, padding, rows,
-                     int(top_k), int(experts), hist);
-  if (int rc = vq::check_launch("moe counts")) return rc;
-  hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(kThreads), 0, s, hist, parts, int(experts), int(top_k), add, counts, stats);
+// The workspace: partial sums, then the parts' histograms.
+struct Workspace {
+  double* partial;
+  int32_t* hist;
+  static int64_t bytes(int64_t experts) { return kMaxGroups * 8 + kMaxParts * (experts + 1) * 4; }
+  explicit Workspace(void* base)
+      : partial(static_cast<double*>(base)), hist(reinterpret_cast<int32_t*>(partial + kMaxGroups)) {}
+};
+
+int launch_count(const Counting& c, const Workspace& w, hipStream_t s) {
+  hipLaunchKernelGGL(count_kernel, dim3(unsigned(parts_of(c.rows))), dim3(kCountThreads), 0, s, c, w.hist);
   return vq::check_launch("moe counts");
+}
+
+Rows rows_of(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, const uint8_t* padding) {
+  const int64_t four = 4 * vq::dtype_bytes(dtype);
+  const bool wide = experts % 4 == 0 && stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % four == 0;
+  return {logits, stride, padding, rows, int(experts), wide};
 }
 
 int check_logits(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, int scoring) {
@@ -227,7 +473,7 @@ bool aligned8(const void* p) { return reinterpret_cast<uintptr_t>(p) % 8 == 0; }
 extern "C" int64_t moe_balance_workspace_size(int64_t rows, int64_t experts) {
   using namespace balance;
   if (check_sizes(rows, experts, 1)) return -1;
-  return kMaxGroups * int64_t(sizeof(double)) + parts_of(rows) * (experts + 1) * int64_t(sizeof(int32_t));
+  return Workspace::bytes(experts);
 }
 
 extern "C" int moe_expert_counts(const int32_t* topk_ids, const uint8_t* is_padding, int64_t rows, int64_t top_k, int64_t experts,
@@ -235,9 +481,12 @@ extern "C" int moe_expert_counts(const int32_t* topk_ids, const uint8_t* is_padd
   using namespace balance;
   if (int rc = check_sizes(rows, experts, top_k)) return rc;
   if (!counts || !workspace || (rows > 0 && !topk_ids)) return vq::fail("moe balance: null pointer");
-  if (workspace_bytes < moe_balance_workspace_size(rows, experts) || !aligned8(workspace)) return vq::fail("moe balance: workspace too small or misaligned");
-  int32_t* hist = reinterpret_cast<int32_t*>(static_cast<double*>(workspace) + kMaxGroups);
-  return launch_counts(topk_ids, is_padding, rows, top_k, experts, add != 0, counts, nullptr, hist, static_cast<hipStream_t>(stream));
+  if (workspace_bytes < Workspace::bytes(experts) || !aligned8(workspace)) return vq::fail("moe balance: workspace too small or misaligned");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const Workspace w(workspace);
+  if (int rc = launch_count({topk_ids, is_padding, rows, int(top_k), int(experts)}, w, s)) return rc;
+  hipLaunchKernelGGL(totals_kernel, dim3(1), dim3(kThreads), 0, s, w.hist, int(parts_of(rows)), int(experts), add != 0, counts);
+  return vq::check_launch("moe counts");
 }
 
 extern "C" int moe_balance_loss(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, const int32_t* topk_ids,
@@ -247,18 +496,26 @@ extern "C" int moe_balance_loss(const void* logits, int dtype, int64_t rows, int
   if (int rc = check_sizes(rows, experts, top_k)) return rc;
   if (int rc = check_logits(logits, dtype, rows, experts, stride, scoring)) return rc;
   if (!loss || !counts || !stats || !workspace || (rows > 0 && !topk_ids)) return vq::fail("moe balance: null pointer");
-  if (workspace_bytes < moe_balance_workspace_size(rows, experts) || !aligned8(workspace)) return vq::fail("moe balance: workspace too small or misaligned");
+  if (workspace_bytes < Workspace::bytes(experts) || !aligned8(workspace)) return vq::fail("moe balance: workspace too small or misaligned");
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  double* partial = static_cast<double*>(workspace);
-  int32_t* hist = reinterpret_cast<int32_t*>(partial + kMaxGroups);
-  if (int rc = launch_counts(topk_ids, is_padding, rows, top_k, experts, false, counts, stats, hist, s)) return rc;
-  const int groups = int(groups_of(rows));
-  int rc = by_width(experts, scoring == 1, [&](auto per, auto sigmoid) {
-    hipLaunchKernelGGL((loss_kernel<decltype(per)::value, decltype(sigmoid)::value>), dim3(unsigned(groups)), dim3(kThreads), 0, s,
-                       logits, dtype, stride, is_padding, rows, int(experts), stats, partial);
+  const Counting c{topk_ids, is_padding, rows, int(top_k), int(experts)};
+  const Rows g = rows_of(logits, dtype, rows, experts, stride, is_padding);
+  const Results out{loss, counts, stats};
+  if (rows * experts <= kOneLogits) {
+    return dispatch(experts, dtype, scoring == 1, [&](auto shape, auto type, auto sigmoid) {
+      hipLaunchKernelGGL((one_kernel<decltype(shape), decltype(type)::value, decltype(sigmoid)::value>), dim3(1), dim3(1024), 0, s, g, c, out);
+    });
+  }
+  const Workspace w(workspace);
+  if (int rc = launch_count(c, w, s)) return rc;
+  const unsigned groups = unsigned(groups_of(rows, experts, kLossWaves, kMaxGroups));
+  const int parts = int(parts_of(rows));
+  const int rc = dispatch(experts, dtype, scoring == 1, [&](auto shape, auto type, auto sigmoid) {
+    hipLaunchKernelGGL((loss_kernel<decltype(shape), decltype(type)::value, decltype(sigmoid)::value>), dim3(groups), dim3(kLossThreads), 0,
+                       s, g, int(top_k), w.hist, parts, w.partial);
   });
   if (rc) return rc;
-  hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(64), 0, s, partial, groups, stats + experts, loss);
+  hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(kLossThreads), 0, s, w.partial, int(groups), w.hist, parts, int(experts), int(top_k), out);
   return vq::check_launch("moe balance");
 }
 
@@ -269,10 +526,12 @@ extern "C" int moe_balance_grad(const void* logits, int dtype, int64_t rows, int
   if (int rc = check_logits(logits, dtype, rows, experts, stride, scoring)) return rc;
   if (rows == 0) return vq::kOk;
   if (!stats || !upstream || !grad) return vq::fail("moe balance: null pointer");
+  if (reinterpret_cast<uintptr_t>(grad) % (4 * vq::dtype_bytes(dtype))) return vq::fail("moe balance: grad must be aligned to four elements");
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const unsigned groups = unsigned(std::min<int64_t>((rows + kWaves - 1) / kWaves, 8 * kMaxGroups));
-  return by_width(experts, scoring == 1, [&](auto per, auto sigmoid) {
-    hipLaunchKernelGGL((grad_kernel<decltype(per)::value, decltype(sigmoid)::value>), dim3(groups), dim3(kThreads), 0, s, logits,
-                       dtype, stride, is_padding, rows, int(experts), stats, upstream, grad);
+  const Rows g = rows_of(logits, dtype, rows, experts, stride, is_padding);
+  const unsigned groups = unsigned(groups_of(rows, experts, kWaves, kGradGroups));
+  return dispatch(experts, dtype, scoring == 1, [&](auto shape, auto type, auto sigmoid) {
+    hipLaunchKernelGGL((grad_kernel<decltype(shape), decltype(type)::value, decltype(sigmoid)::value>), dim3(groups), dim3(kThreads), 0, s,
+                       g, stats, upstream, grad);
   });
 }

@@ -104,7 +104,10 @@ struct BalanceLoss : torch::autograd::Function<BalanceLoss> {
     const int64_t rows = logits.size(0), experts = logits.size(1);
     const c10::DeviceGuard guard(logits.device());
     at::Tensor grad = at::empty({rows, experts}, logits.options());
-    const at::Tensor upstream = grads[0].to(logits.device(), at::kFloat).contiguous();
+    // (one FP32 value on the device, as a rule)
+    const at::Tensor& given = grads[0];
+    const at::Tensor upstream = given.scalar_type() == at::kFloat && given.device() == logits.device()
+                                    ? given : given.to(logits.device(), at::kFloat);
     check_status(native_grad(logits.const_data_ptr(), dtype_code(logits.scalar_type()), rows, experts,
                              rows > 1 ? logits.stride(0) : experts,
                              padding.defined() ? static_cast<const uint8_t*>(padding.const_data_ptr()) : nullptr,
