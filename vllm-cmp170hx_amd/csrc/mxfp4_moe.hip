@@ -37,17 +37,21 @@ struct ExpertOf {
   }
 };
 
-// Workgroups 0 .. parts - 1 count the slots; the others quantize the rows of x,
-// four lanes a block.
+// Workgroups 0 .. parts - 1 count the slots (one alone also lists them: no launch
+// for that); the others quantize the rows of x, four lanes a block.
 template <int kDtype>
 __global__ __launch_bounds__(moe::kRowsPartThreads) void count_quantize_kernel(ExpertOf of, moe::RowsLayout lay, int32_t* table,
-                                                                               const void* x, int64_t tokens, int blocks,
+                                                                               int task_rows, const void* x, int64_t tokens, int blocks,
                                                                                int64_t stride, bool wide, uint32_t* codes,
                                                                                uint8_t* scales) {
   extern __shared__ int part_count[];
   const int64_t parts = lay.parts();
   if (blockIdx.x < parts) {
     moe::rows_count_part(of, lay, table, int(blockIdx.x), part_count);
+    if (parts == 1) {
+      __syncthreads();
+      moe::rows_fill_part(lay, table, task_rows, 0, part_count);
+    }
     return;
   }
   const int64_t quarter = int64_t(blockIdx.x - parts) * moe::kRowsPartThreads + threadIdx.x;
@@ -581,18 +585,20 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
     if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
     return sum();
   }
+  const int task_rows = path == 2 ? kTileRows : kTaskRows;
   uint32_t* xq = reinterpret_cast<uint32_t*>(base + ws.xq);
   if (act_dtype == vq::kBF16) {
     hipLaunchKernelGGL(count_quantize_kernel<vq::kBF16>, dim3(unsigned(groups)), dim3(moe::kRowsPartThreads), lds, st, of, lay, table,
-                       x, tokens, int(hb), x_stride, wide, xq, base + ws.xs);
+                       task_rows, x, tokens, int(hb), x_stride, wide, xq, base + ws.xs);
   } else {
     hipLaunchKernelGGL(count_quantize_kernel<vq::kFP16>, dim3(unsigned(groups)), dim3(moe::kRowsPartThreads), lds, st, of, lay, table,
-                       x, tokens, int(hb), x_stride, wide, xq, base + ws.xs);
+                       task_rows, x, tokens, int(hb), x_stride, wide, xq, base + ws.xs);
   }
   if (int rc = vq::check_launch("mxfp4 moe count")) return rc;
-  hipLaunchKernelGGL(fill_kernel, dim3(unsigned(lay.parts())), dim3(moe::kRowsPartThreads), lds, st, lay, table,
-                     path == 2 ? kTileRows : kTaskRows);
-  if (int rc = vq::check_launch("mxfp4 moe fill")) return rc;
+  if (lay.parts() > 1) {
+    hipLaunchKernelGGL(fill_kernel, dim3(unsigned(lay.parts())), dim3(moe::kRowsPartThreads), lds, st, lay, table, task_rows);
+    if (int rc = vq::check_launch("mxfp4 moe fill")) return rc;
+  }
   if (path == 1) {
     const int wgs13 = wgs_of(lay.max_tasks, (ib + 3) / 4), wgs2 = wgs_of(lay.max_tasks, (hidden + 63) / 64);
     if (lay.max_tasks * std::max(wgs13, wgs2) > INT_MAX) return vq::fail("mxfp4 moe: too many rows");

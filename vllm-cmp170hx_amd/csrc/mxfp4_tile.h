@@ -156,7 +156,10 @@ __device__ __forceinline__ void store_rows(const float* part, int stride, int la
 }
 
 // Workgroups of a size that a CU's LDS (and registers) hold, two at most.
-constexpr int tile_groups(int n, int m, int bufs) { return n * m > 8 || 64 * (n + m) * (kStageBytes * bufs + 16) > 80 * 1024 ? 1 : 2; }
+constexpr int tile_groups(int n, int m, int bufs) {
+  const int lds = 64 * (n + m) * (kStageBytes * bufs + 16);
+  return n * m > 8 || lds > 80 * 1024 ? 1 : n * m > 2 || lds > 53 * 1024 ? 2 : 3;
+}
 
 template <int kN, int kM, int kMode, int kBufs>
 __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile_kernel(TileArgs g) {
@@ -201,10 +204,12 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     m0 = int64_t(t % g.tiles_m) * kRows;
     nrows = int(min(int64_t(kRows), g.rows - m0));
   } else {
-    // XCD x takes tasks x, x + 8, ..., a task's columns one after another
-    const int local = int(blockIdx.x >> 3);
-    const int task = local / g.tiles_n * 8 + int(blockIdx.x & 7);
-    if (task >= g.table[0]) return;
+    // XCD x takes a run of tasks, a task's columns one after another: the tasks of
+    // one expert share its weights in L2
+    const int local = int(blockIdx.x >> 3), all = g.table[0], per = (all + 7) / 8;
+    const int task = int(blockIdx.x & 7) * per + local / g.tiles_n;
+    if (local / g.tiles_n >= per) return;
+    if (task >= all) return;
     const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[task];
     wbase = int64_t(vq::uniform(tk.x)) * g.n;
     m0 = vq::uniform(tk.y);
@@ -295,23 +300,25 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? wbuf : abuf, (lds_ptr_t)(buf + first_line(i) * kStageBytes), 16,
                                              int(o), row_part + (left > 0 ? s * kStageBytes : 0), 0, 0);
   };
-  uint64_t sreg[kBufs][kScaleRows];  // of the stages on their way
-  const auto fetch_scales = [&](auto set_c, int s) {
-    constexpr int set = decltype(set_c)::value % kBufs;
+  // Scale bytes come for four stages at a time: a stage's eight bytes of a row by
+  // themselves would ask L2 for as many lines as the codes do.
+  uint64_t scales_now[4][kScaleRows], scales_next[4][kScaleRows];
+  const auto fetch_scales = [&](uint64_t (&to)[4][kScaleRows], int s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kScaleRows; ++i) sreg[set][i] = load_scales(srow[i], s * kStageBlocks, g.blocks);
+    for (int i = 0; i < kScaleRows; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) to[k][i] = load_scales(srow[i], (s + k) * kStageBlocks, g.blocks);
   };
   // stage s has landed (its loads of this wavefront, behind which kBufs - 2 stages'
   // stay on their way, then everyone's), and no wavefront reads the stage before it
   // any more
-  const auto land = [&](auto set_c, int s, uint2* scales) {
-    constexpr int set = decltype(set_c)::value % kBufs;
+  const auto land = [&](const uint64_t (&from)[kScaleRows], int s, uint2* scales) __attribute__((always_inline)) {
     vq::wait_vmcnt<(kBufs - 2) * kLoads>();
     const int b0 = min(s, all_stages - 1) * kStageBlocks;
 #pragma unroll
     for (int i = 0; i < kScaleRows; ++i) {
       if (kLines % kTileThreads == 0 || tid + i * kTileThreads < kLines) {
-        scales[tid + i * kTileThreads] = order_scales(sreg[set][i], b0, g.blocks);
+        scales[tid + i * kTileThreads] = order_scales(from[i], b0, g.blocks);
       }
     }
     // (a barrier that leaves the loads on their way: __syncthreads() waits for them)
@@ -370,12 +377,12 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  // Stage s, the i-th of a round of the buffers.  The barrier comes before the last
+  // Stage s, the i-th of a round of four.  The barrier comes before the last
   // sub-step, whose operands are in registers by then: its MFMAs run while the next
   // stage's first operands are read, and its buffer takes stage s + kBufs: half of
   // those loads here, the others in the next stage's first sub-steps.
   constexpr int kHalf = kLoads / 2, kMore = kHalf + kLoads / 4;
-  const auto stage = [&](auto i_c, int s) __attribute__((always_inline)) {
+  const auto stage = [&](auto i_c, auto whole_c, int s) __attribute__((always_inline)) {
     constexpr int i = decltype(i_c)::value;
     using std::integral_constant;
     constexpr integral_constant<int, 0> c0{};
@@ -388,32 +395,32 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     step(c0, integral_constant<int, kHalf>{}, integral_constant<int, kMore>{}, set, cur, 1, s + kBufs - 1, prev);
     step(integral_constant<int, 1>{}, integral_constant<int, kMore>{}, integral_constant<int, kLoads>{}, set, cur, 2, s + kBufs - 1, prev);
     step(integral_constant<int, 2>{}, c0, c0, set, cur, 3, 0, cur);
-    land(c1, s + 1, next_scales);
-    fetch_scales(i_c, s + kBufs);
+    land(i < 3 ? scales_now[(i + 1) & 3] : scales_next[0], s + 1, next_scales);
+    if constexpr (i == 0 && decltype(whole_c)::value) fetch_scales(scales_next, s + 4);
     read_scales(next_scales, sw[set ^ 1], sa[set ^ 1]);
     step(integral_constant<int, 3>{}, c0, integral_constant<int, kHalf>{}, set, next, 0, s + kBufs, cur);
   };
+  fetch_scales(scales_now, first);
   for_range<0, kBufs - 1>([&](auto b_c) {
-    constexpr int b = decltype(b_c)::value;
-    fetch_scales(b_c, first + b);
-    for_range<0, kLoads>([&](auto k) { fetch(k, first + b, buf(b_c)); });
+    for_range<0, kLoads>([&](auto k) { fetch(k, first + decltype(b_c)::value, buf(b_c)); });
   });
-  land(std::integral_constant<int, 0>{}, first, scale0);
-  fetch_scales(std::integral_constant<int, kBufs - 1>{}, first + kBufs - 1);
+  land(scales_now[0], first, scale0);
   for_range<0, kHalf>([&](auto k) { fetch(k, first + kBufs - 1, buf(std::integral_constant<int, kBufs - 1>{})); });
   read_scales(scale0, sw[0], sa[0]);
   for_range<0, kN + kM>([&](auto k) { read(k, buf0, 0, 0); });
   int s = first;
-  for (; s + kBufs <= stages; s += kBufs) {
-    for_range<0, kBufs>([&](auto i) __attribute__((always_inline)) { stage(i, s + decltype(i)::value); });
+  for (; s + 4 <= stages; s += 4) {
+    for_range<0, 4>([&](auto i) __attribute__((always_inline)) { stage(i, std::true_type{}, s + decltype(i)::value); });
+#pragma unroll
+    for (int i = 0; i < kScaleRows; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) scales_now[k][i] = scales_next[k][i];
   }
   if (s < stages) {
-    stage(std::integral_constant<int, 0>{}, s);
-    if constexpr (kBufs > 2) {
-      if (s + 1 < stages) {
-        stage(std::integral_constant<int, 1>{}, s + 1);
-        if (s + 2 < stages) stage(std::integral_constant<int, 2>{}, s + 2);
-      }
+    stage(std::integral_constant<int, 0>{}, std::false_type{}, s);
+    if (s + 1 < stages) {
+      stage(std::integral_constant<int, 1>{}, std::false_type{}, s + 1);
+      if (s + 2 < stages) stage(std::integral_constant<int, 2>{}, std::false_type{}, s + 2);
     }
   }
   vq::wait_vmcnt<0>();  // the last loads (zeros) are in before their buffers are used again
