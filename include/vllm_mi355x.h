@@ -609,9 +609,9 @@ int mxfp4_linear(const void* x, int x_dtype, int64_t rows, int64_t k, int64_t x_
  * up rows), w2 [experts][hidden][inter]; topk_ids int32 [tokens][top_k];
  * expert_map int32 [map_size] global id -> local expert (map_size 0: none).
  * Slots outside [0, experts) add nothing.  limit L > 0 (infinity: no clamp).
- * hidden and inter multiples of 32, at most 1024 experts.  workspace:
- * mxfp4_moe_workspace_size bytes, 16-byte aligned; calls that share one must
- * be on one stream.
+ * hidden and inter multiples of 32 up to 65536, at most 1024 experts.  out may be
+ * x and overlaps no other argument.  workspace: mxfp4_moe_workspace_size bytes,
+ * 16-byte aligned, of its own; calls that share one must be on one stream.
  */
 int64_t mxfp4_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int64_t inter,
                                  int64_t experts);

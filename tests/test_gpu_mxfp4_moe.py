@@ -54,7 +54,15 @@ def check(layer, got, x, ids, weights, dtype, limit=math.inf):
 CASES = [  # experts, hidden, inter, topk, tokens
     (1, 32, 32, 1, 1), (4, 64, 32, 2, 3), (8, 256, 96, 2, 1), (8, 288, 160, 8, 1), (16, 128, 64, 3, 2),
     (16, 512, 256, 4, 5), (8, 416, 224, 2, 40), (4, 256, 128, 1, 70), (64, 128, 64, 6, 33), (3, 160, 96, 3, 150),
-    (2, 384, 320, 1, 300), (40, 96, 32, 5, 20), (128, 64, 32, 8, 17), (300, 64, 32, 4, 30)]
+    (2, 384, 320, 1, 300), (40, 96, 32, 5, 20), (128, 64, 32, 8, 17), (300, 64, 32, 4, 30),
+    # few rows' kernels: several tasks of 16 rows an expert, listed and looked for; whole
+    # blocks a wavefront, by expert and by slot; more than eight and 64 slots a token
+    (64, 128, 64, 6, 200), (8, 160, 96, 2, 100), (64, 256, 512, 2, 40), (128, 64, 512, 2, 62), (32, 128, 64, 20, 2),
+    (100, 64, 32, 64, 1), (100, 64, 32, 65, 1),
+    # rows so long that LDS holds fewer than 16 (and one)
+    (2, 8192, 64, 1, 30), (4, 96, 8192, 1, 80), (2, 8192, 64, 2, 600), (1, 65536, 32, 1, 2), (1, 32, 65536, 1, 2),
+    # tiles: several an expert, a few rows of many experts, sizes that end inside a stage
+    (2, 256, 256, 1, 700), (3, 288, 416, 2, 450), (200, 256, 256, 8, 150)]
 
 
 @pytest.mark.parametrize("experts,hidden,inter,topk,tokens", CASES)
@@ -195,6 +203,41 @@ def test_streams_workspace_and_graph(mx, device, tokens):
         again = layer.run(mx, *sets[i])
         torch.cuda.synchronize()
         assert torch.equal(out, want[i]) and torch.equal(again, want[i])
+
+
+def test_a_graph_outlives_its_workspace(mx, device):
+    """Calls captured with a workspace, which later calls replace by larger ones
+    and whose memory others then write; two graphs replayed in turn; the output
+    in the place of the input."""
+    print("moe graphs and a workspace", flush=True)
+    rng = np.random.default_rng(8)
+    layer = Layer(rng, 8, 256, 128, device)
+    def call(tokens):
+        ids, weights = routing(rng, tokens, 8, 2)
+        return (torch.from_numpy(rng.standard_normal((tokens, 256))).bfloat16().to(device),
+                torch.from_numpy(weights).to(device), torch.from_numpy(ids).to(device))
+    small, large = call(5), call(90)
+    want = [layer.run(mx, *small), layer.run(mx, *large)]
+    ws, graphs, outs = {}, [], []
+    layer.run(mx, *small, workspace=ws)
+    torch.cuda.synchronize()
+    for args in (small, large):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(layer.run(mx, *args, workspace=ws))
+        graphs.append(graph)
+    layer.run(mx, *call(600), workspace=ws)
+    taken = [torch.full((1 << 16,), 255, dtype=torch.uint8, device=device) for _ in range(64)]
+    for i in (0, 1, 1, 0):
+        outs[i].zero_()
+        graphs[i].replay()
+        layer.run(mx, *large, workspace=ws)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want[i])
+    assert all(bool((t == 255).all()) for t in taken)
+    for args, y in zip((small, large), want):
+        x = args[0].clone()
+        assert layer.run(mx, x, *args[1:], output=x) is x and torch.equal(x, y)
 
 
 def test_router_load_and_experts_together(mx, device):

@@ -86,7 +86,9 @@ def _moe(x=1 << 40, dt=0, tokens=2, stride=64, w13=1 << 41, s13=1 << 42, w2=1 <<
     ({"experts": 1025}, "1024"), ({"topk": 0}, "range"), ({"tokens": 1 << 31}, "range"),
     ({"stride": 32}, "stride"), ({"limit": float("nan")}, "limit"), ({"limit": 0.0}, "limit"),
     ({"w2": 0}, "null"), ({"mapn": 4}, "null"), ({"w13": (1 << 41) + 8}, "16-byte"), ({"x": (1 << 40) + 1}, "aligned"),
-    ({"wb": 64}, "workspace"), ({"ws": (1 << 48) + 4}, "workspace")])
+    ({"wb": 64}, "workspace"), ({"ws": (1 << 48) + 4}, "workspace"), ({"hidden": 65568}, "65536"),
+    ({"inter": 1 << 17}, "65536"), ({"ws": 1 << 41}, "overlap"), ({"ws": 1 << 47}, "overlap"), ({"ws": 1 << 40}, "overlap"),
+    ({"out": 1 << 43}, "overlap"), ({"out": 1 << 45}, "overlap"), ({"out": 1 << 42}, "overlap")])
 def test_moe_refusals(lib, change, word):
     assert lib.mxfp4_moe(*_moe(**change)) == 1 and word in _err(lib)
 

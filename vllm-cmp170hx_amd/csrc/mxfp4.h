@@ -153,13 +153,4 @@ __device__ __forceinline__ float scale_value(uint32_t b) {
   return b == 255u ? __builtin_nanf("") : b == 0 ? __builtin_bit_cast(float, 0x00400000u) : __builtin_bit_cast(float, b << 23);
 }
 
-// acc += A B over 128 k: A 16 rows, B 16 columns, lane (r = lane & 15, q = lane
-// >> 4) holding the block of k 32 q .. 32 q + 31 of row / column r and its scale
-// byte; lane's acc[i] is row 4 q + i, column r.
-__device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, uint32_t sa, const u32x4_t& b, uint32_t sb, const f32x4_t& acc) {
-  const i32x8_t av{int(a[0]), int(a[1]), int(a[2]), int(a[3]), 0, 0, 0, 0};
-  const i32x8_t bv{int(b[0]), int(b[1]), int(b[2]), int(b[3]), 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, int(sa), 0, int(sb));
-}
-
 }  // namespace mx

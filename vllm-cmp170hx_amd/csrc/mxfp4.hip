@@ -196,10 +196,6 @@ int launch_tile(const MatmulArgs& g, int splits, float* part, hipStream_t s) {
 
 // ---- which kernel ------------------------------------------------------------
 
-#ifdef MX_TUNE
-int g_tile = 0, g_splits = 0, g_parts = 0, g_cols = 0, g_fuse = -1;
-#endif
-
 // How a product runs.  tile 0: the few-rows kernel, `cols` column tiles and
 // `parts` parts of K a workgroup, `fused`: it quantizes x itself; else the tile
 // kernel with 64 `tile` columns and rows, K in `splits`, `deep`: four stage
@@ -269,16 +265,6 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n) {
     const int64_t groups_cu = ((groups + p.cols - 1) / p.cols + kCUs - 1) / kCUs;
     p.fused = rows <= 16 && groups_cu * rows * k <= 40960;
   }
-#ifdef MX_TUNE
-  if (g_tile >= 0 && g_tile != 9) {
-    p.tile = tiles ? g_tile == 3 ? 2 : g_tile : 0;
-    p.deep = g_tile == 3;
-  }
-  if (g_splits) p.splits = g_splits;
-  if (g_cols) p.cols = g_cols;
-  if (g_parts) p.parts = g_parts;
-  if (g_fuse >= 0) p.fused = g_fuse;
-#endif
   if (p.splits > 1) p.splits = int((stages + (stages + p.splits - 1) / p.splits - 1) / ((stages + p.splits - 1) / p.splits));
   return p;
 }
@@ -504,13 +490,3 @@ extern "C" int mxfp4_linear(const void* x, int x_dtype, int64_t rows, int64_t k,
   packed.as = scales;
   return launch_matmul(packed, p, reinterpret_cast<float*>(codes + packed_bytes(rows, k)), s);
 }
-
-#ifdef MX_TUNE
-extern "C" void mx_plan(int tile, int splits, int cols, int parts, int fuse) {
-  mx::g_tile = tile;
-  mx::g_splits = splits;
-  mx::g_cols = cols;
-  mx::g_parts = parts;
-  mx::g_fuse = fuse;
-}
-#endif

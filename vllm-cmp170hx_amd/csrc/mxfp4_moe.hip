@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <utility>
 
 #include "../../include/vllm_mi355x.h"
 #include "moe_rows.h"
@@ -18,11 +19,9 @@ namespace mx {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMaxSize = 65536;  // hidden and intermediate: a row fits LDS
 constexpr int kTaskRows = 16;
 constexpr int kTileRows = 128;  // rows of a task on the tile kernel
-#ifdef MX_TUNE
-int g_moe_force = -1, g_split = 1024, g_target = 1024;
-#endif
 
 // The local expert of a slot: through the map where the call brings one, -1
 // outside [0, experts).
@@ -82,6 +81,7 @@ struct SmallMoeArgs {
   const uint8_t *a, *as;    // their codes and scales
   const uint8_t *w, *ws;    // [experts][n][k]
   int slots, top_k;
+  int pass;                 // rows that a workgroup takes at a time, 16 or what LDS holds
   int by_slot;              // kScan: workgroups go by slot, the first of an expert's does the work
   const int32_t* table;
   int64_t tasks, sorted;    // offsets in the table
@@ -91,8 +91,14 @@ struct SmallMoeArgs {
   uint8_t *h, *hs;          // [slots][inter]
   float* c3;                // [slots][n]
   void* out;
-  int out_dtype;
 };
+
+// Rows of `chunks` chunks that the kernels below take at a time.
+int rows_at_once(int64_t slots, int64_t chunks) {
+  constexpr int64_t kLds = 56 * 1024;  // beside the list of slots
+  static_assert(small_bytes(1, kMaxSize / kBlock / kChunk) <= kLds, "one row fits");
+  return int(std::min({slots, int64_t(16), kLds / small_bytes(1, chunks)}));
+}
 
 // The expert and the slots of workgroup `index`, in slot order; count 0: no work.
 // kScan: from the ids themselves (list: LDS of kScanSlots entries); else a task of
@@ -116,7 +122,6 @@ __device__ __forceinline__ RowsOf rows_of(const SmallMoeArgs& g, int index, int3
     if (threadIdx.x < 64) {
       const int lane = threadIdx.x;
       int n = 0;
-      bool later = false;  // an earlier slot's workgroup has this expert
       constexpr int kEach = 4;
       for (int s0 = 0; s0 < g.slots; s0 += 64 * kEach) {
         int id[kEach];
@@ -133,8 +138,8 @@ __device__ __forceinline__ RowsOf rows_of(const SmallMoeArgs& g, int index, int3
           n += __popcll(all);
         }
       }
-      if (g.by_slot) later = list[0] != index;
-      if (lane == 0) *count = later ? 0 : n;
+      // (by slot: an expert's first one has the work)
+      if (lane == 0) *count = g.by_slot && list[0] != index ? 0 : n;
     }
     __syncthreads();
     return {e, vq::uniform(*count), list};
@@ -169,8 +174,8 @@ __global__ __launch_bounds__(1024, 4) void gate_up_split_kernel(SmallMoeArgs g) 
     return o;
   };
   float* sums = reinterpret_cast<float*>(lds);
-  for (int m0 = 0; m0 < rows.count; m0 += 16) {
-    const int here = min(rows.count - m0, 16);
+  for (int m0 = 0; m0 < rows.count; m0 += g.pass) {
+    const int here = min(rows.count - m0, g.pass);
     f32x4_t acc{0, 0, 0, 0};
     ChunkOperand a = weights(part), b = weights(part + parts);
     quantize_to_lds<kDtype>(g.x, [&](int m) { return int64_t(rows.slots[m0 + m] / g.top_k) * g.stride; }, here, g.blocks, chunks,
@@ -277,8 +282,8 @@ __global__ __launch_bounds__(256, 4) void gate_up_kernel(SmallMoeArgs g, int wgs
     wt = w + row * line;
     wst = ws + row * g.blocks;
   };
-  for (int m0 = 0; m0 < rows.count; m0 += 16) {
-    const int here = min(rows.count - m0, 16);
+  for (int m0 = 0; m0 < rows.count; m0 += g.pass) {
+    const int here = min(rows.count - m0, g.pass);
     WeightStream<decltype(base)> stream{base, 4 * mine, chunks, g.blocks, q, 0, 0, {}};
     stream.start();
     if (m0) __syncthreads();
@@ -347,8 +352,8 @@ __global__ __launch_bounds__(256, 4) void down_kernel(SmallMoeArgs g, int wgs) {
     wt = w + row * line;
     wst = ws + row * g.blocks;
   };
-  for (int m0 = 0; m0 < rows.count; m0 += 16) {
-    const int here = min(rows.count - m0, 16);
+  for (int m0 = 0; m0 < rows.count; m0 += g.pass) {
+    const int here = min(rows.count - m0, g.pass);
     WeightStream<decltype(base)> stream{base, mine, chunks, g.blocks, q, 0, 0, {}};
     stream.start();
     if (m0) __syncthreads();
@@ -465,8 +470,8 @@ Workspace workspace_of(int64_t tokens, int64_t top_k, int64_t hidden, int64_t in
 extern "C" int64_t mxfp4_moe_workspace_size(int64_t tokens, int64_t top_k, int64_t hidden, int64_t inter, int64_t experts) {
   using namespace mx;
   if (tokens < 0 || top_k <= 0 || tokens > INT_MAX / top_k || hidden <= 0 || inter <= 0 || hidden % kBlock != 0 ||
-      inter % kBlock != 0 || hidden > (1 << 24) || inter > (1 << 24) || experts <= 0 || experts > moe::kRowsMaxExperts) {
-    vq::fail("mxfp4 moe: sizes out of range (hidden and intermediate multiples of 32, at most 1024 experts)");
+      inter % kBlock != 0 || hidden > kMaxSize || inter > kMaxSize || experts <= 0 || experts > moe::kRowsMaxExperts) {
+    vq::fail("mxfp4 moe: sizes out of range (hidden and intermediate multiples of 32 up to 65536, at most 1024 experts)");
     return -1;
   }
   return workspace_of(tokens, top_k, hidden, inter, experts).total;
@@ -489,7 +494,15 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   if (!aligned(w13, 16) || !aligned(w2, 16)) return vq::fail("mxfp4 moe: codes must be 16-byte aligned");
   if (!aligned(x, 2) || !aligned(out, 2) || !aligned(topk_ids, 4) || !aligned(topk_w, 4)) return vq::fail("mxfp4 moe: misaligned pointer");
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) return vq::fail("mxfp4 moe: workspace too small or not 16-byte aligned");
-  const int64_t slots = tokens * top_k;
+  const int64_t slots = tokens * top_k, codes = experts * inter * hidden;  // of w13, bytes
+  for (const auto& other : {std::pair<const void*, int64_t>{x, ((tokens - 1) * x_stride + hidden) * 2}, {w13, codes}, {s13, codes / 16},
+                            {w2, codes / 2}, {s2, codes / 32}, {topk_ids, slots * 4}, {topk_w, slots * 4}, {expert_map, map_size * 4}}) {
+    if (vq::overlaps(workspace, need, other.first, other.second)) return vq::fail("mxfp4 moe: the workspace must not overlap another argument");
+    if (other.first != x && vq::overlaps(out, tokens * hidden * 2, other.first, other.second)) {
+      return vq::fail("mxfp4 moe: out must not overlap the weights or the routing");
+    }
+  }
+  if (vq::overlaps(workspace, need, out, tokens * hidden * 2)) return vq::fail("mxfp4 moe: the workspace must not overlap another argument");
   const Workspace ws = workspace_of(tokens, top_k, hidden, inter, experts);
   const moe::RowsLayout lay = layout_of(slots, experts);
   uint8_t* base = static_cast<uint8_t*>(workspace);
@@ -502,17 +515,16 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   if (groups > INT_MAX || sums > INT_MAX) return vq::fail("mxfp4 moe: too many rows");
   const bool wide = aligned(x, 16) && x_stride % 8 == 0;
   const size_t lds = size_t(experts) * sizeof(int);
-  // 0 few slots (each workgroup looks through them), 1 tasks of 16 rows, 2 tiles
+  const int64_t chunks = (hb + kChunk - 1) / kChunk, chunks2 = (ib + kChunk - 1) / kChunk;
+  // Tiles where more than 16 rows may meet at an expert, which the few rows' kernels
+  // would take one pass over its weights after another, or where it may expect ten (a
+  // map says how many share the slots); whole stages and buffers below 2 GiB.  In us,
+  // few rows' kernels and tiles, 128 experts of 2048 x 768, eight a token: 8 tokens
+  // 44 and 53, 16 evenly routed 64 and 74, routed by a power law 66 and 55, 64 evenly
+  // 82 and 91, by the power law 152 and 84; 8 experts of 4096 x 14336, two a token: 16
+  // tokens 162 and 179, 32 198 and 180.
   const bool can_tile = hb >= kStageBlocks && ib >= kStageBlocks && hidden * inter < (int64_t(1) << 31) && tokens * hidden / 2 < (int64_t(1) << 31);
-  const int64_t small_rows = std::min<int64_t>(slots, 16), chunks = (hb + kChunk - 1) / kChunk;
-  const bool can_scan = slots <= kScanSlots && small_bytes(small_rows, chunks) <= 56 * 1024 &&
-                        small_bytes(small_rows, (ib + kChunk - 1) / kChunk) <= 56 * 1024;
-  // rows an expert held here may expect (a map says how many share the slots)
-  const double rows_each = double(slots) / double(std::max(experts, map_size));
-  int path = can_tile && rows_each >= 10 ? 2 : can_scan ? 0 : 1;
-#ifdef MX_TUNE
-  if (g_moe_force >= 0) path = g_moe_force;
-#endif
+  const bool tile = can_tile && (tokens > 16 || slots >= 10 * std::max(experts, map_size));
   SmallMoeArgs m{};
   m.of = of;
   m.x = x;
@@ -524,6 +536,7 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   m.ws = s13;
   m.slots = int(slots);
   m.top_k = int(top_k);
+  m.pass = rows_at_once(slots, chunks);
   m.table = table;
   m.tasks = lay.tasks();
   m.sorted = lay.sorted();
@@ -535,15 +548,9 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   m.hs = base + ws.hs;
   m.c3 = reinterpret_cast<float*>(base + ws.c3);
   m.out = out;
-  m.out_dtype = act_dtype;
-  const size_t rows2 = size_t(small_bytes(small_rows, (ib + kChunk - 1) / kChunk));
-  int64_t split_blocks = 1024, target = 1024;
-#ifdef MX_TUNE
-  split_blocks = g_split;
-  target = g_target;
-#endif
-  // workgroups an expert: about `target` in all
-  const auto wgs_of = [&](int64_t units, int64_t most) { return int(std::max<int64_t>(1, std::min(most, target / units))); };
+  const size_t rows13 = size_t(small_bytes(m.pass, chunks)), rows2 = size_t(small_bytes(rows_at_once(slots, chunks2), chunks2));
+  // workgroups an expert: about four a CU in all
+  const auto wgs_of = [&](int64_t units, int64_t most) { return int(std::max<int64_t>(1, std::min(most, 1024 / units))); };
   const int parts = chunks >= 8 ? 4 : chunks >= 2 ? 2 : 1;
   const size_t sums_lds = size_t(parts) * 4 * 16 * 20 * sizeof(float);
   const auto second = [&](SmallMoeArgs& a) {
@@ -551,16 +558,16 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
     a.ws = s2;
     a.n = int(hidden);
     a.blocks = int(ib);
+    a.pass = rows_at_once(slots, chunks2);
   };
   const auto sum = [&] {
     hipLaunchKernelGGL(slot_sum_kernel, dim3(unsigned(sums)), dim3(kThreads), 0, st, m.c3, of, tokens, int(top_k), int(hidden), out, act_dtype);
     return vq::check_launch("mxfp4 moe sum");
   };
-  if (path == 0) {
+  if (!tile && slots <= kScanSlots) {
     m.by_slot = slots < experts;
     const int64_t units = m.by_slot ? slots : experts;
-    const size_t rows13 = size_t(small_bytes(small_rows, chunks));
-    if (units * ib < split_blocks) {
+    if (units * ib < 1024) {
       const size_t need13 = std::max<size_t>(sums_lds, rows13);
       const dim3 grid13(unsigned(units * ib)), block13(256 * parts);
       if (act_dtype == vq::kBF16) hipLaunchKernelGGL(gate_up_split_kernel<vq::kBF16>, grid13, block13, need13, st, m);
@@ -585,7 +592,7 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
     if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
     return sum();
   }
-  const int task_rows = path == 2 ? kTileRows : kTaskRows;
+  const int task_rows = tile ? kTileRows : kTaskRows;
   uint32_t* xq = reinterpret_cast<uint32_t*>(base + ws.xq);
   if (act_dtype == vq::kBF16) {
     hipLaunchKernelGGL(count_quantize_kernel<vq::kBF16>, dim3(unsigned(groups)), dim3(moe::kRowsPartThreads), lds, st, of, lay, table,
@@ -599,11 +606,11 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
     hipLaunchKernelGGL(fill_kernel, dim3(unsigned(lay.parts())), dim3(moe::kRowsPartThreads), lds, st, lay, table, task_rows);
     if (int rc = vq::check_launch("mxfp4 moe fill")) return rc;
   }
-  if (path == 1) {
+  if (!tile) {
     const int wgs13 = wgs_of(lay.max_tasks, (ib + 3) / 4), wgs2 = wgs_of(lay.max_tasks, (hidden + 63) / 64);
     if (lay.max_tasks * std::max(wgs13, wgs2) > INT_MAX) return vq::fail("mxfp4 moe: too many rows");
     hipLaunchKernelGGL((gate_up_kernel<false, vq::kBF16>), dim3(unsigned(lay.max_tasks * wgs13)), dim3(256),
-                       size_t(small_bytes(small_rows, chunks)), st, m, wgs13);
+                       rows13, st, m, wgs13);
     if (int rc = vq::check_launch("mxfp4 moe gate_up")) return rc;
     second(m);
     hipLaunchKernelGGL(down_kernel<false>, dim3(unsigned(lay.max_tasks * wgs2)), dim3(256), rows2, st, m, wgs2);
@@ -643,11 +650,3 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
   if (int rc = vq::check_launch("mxfp4 moe down")) return rc;
   return sum();
 }
-
-#ifdef MX_TUNE
-extern "C" void mx_moe_force(int f) { mx::g_moe_force = f; }
-#endif
-
-#ifdef MX_TUNE
-extern "C" void mx_moe_tune(int s, int t) { mx::g_split = s; mx::g_target = t; }
-#endif

@@ -20,7 +20,9 @@ namespace mx {
 
 constexpr int kChunk = 16;  // blocks, 512 k
 
-// acc += A B over 128 k, as mfma16, with B's scale byte kByte.
+// acc += A B over 128 k: A 16 rows, B 16 columns, lane (r = lane & 15, q = lane
+// >> 4) holding the block of k 32 q .. 32 q + 31 of row / column r, its scale in
+// byte 0 of sa and byte kByte of sb; lane's acc[i] is row 4 q + i, column r.
 template <int kByte>
 __device__ __forceinline__ f32x4_t mfma16_byte(const u32x4_t& a, uint32_t sa, const u32x4_t& b, uint32_t sb, const f32x4_t& acc) {
   const i32x8_t av{int(a[0]), int(a[1]), int(a[2]), int(a[3]), 0, 0, 0, 0};

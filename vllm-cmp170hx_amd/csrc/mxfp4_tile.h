@@ -156,10 +156,7 @@ __device__ __forceinline__ void store_rows(const float* part, int stride, int la
 }
 
 // Workgroups of a size that a CU's LDS (and registers) hold, two at most.
-constexpr int tile_groups(int n, int m, int bufs) {
-  const int lds = 64 * (n + m) * (kStageBytes * bufs + 16);
-  return n * m > 8 || lds > 80 * 1024 ? 1 : n * m > 2 || lds > 53 * 1024 ? 2 : 3;
-}
+constexpr int tile_groups(int n, int m, int bufs) { return n * m > 8 || 64 * (n + m) * (kStageBytes * bufs + 16) > 80 * 1024 ? 1 : 2; }
 
 template <int kN, int kM, int kMode, int kBufs>
 __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile_kernel(TileArgs g) {

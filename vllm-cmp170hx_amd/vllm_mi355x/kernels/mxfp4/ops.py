@@ -66,10 +66,12 @@ def fused_mxfp4_moe(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Ten
 
     hidden_states [M, K] bf16 or fp16; w1 [E, 2 N, K / 2] (gate rows 0..N-1, up
     rows N..2N-1) and w2 [E, K, N / 2] codes with their scales; K and N
-    multiples of 32.  topk_weights / topk_ids [M, topk]; expert_map: global id
+    multiples of 32 up to 65536, at most 1024 experts.  topk_weights / topk_ids [M, topk]; expert_map: global id
     -> local expert or -1.  Slots routed outside the local experts add nothing.
     workspace: a dict that keeps the call's scratch; calls that share one must
-    be on one stream."""
+    be on one stream.  (A captured call has scratch of its graph's own: a later
+    call may replace the dict's by a larger one, the graph's has to stay.)
+    output: contiguous, like hidden_states, which it may be."""
     ops = _lib()
     ids = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.to(torch.int32)
     weights = topk_weights if topk_weights.dtype == torch.float32 else topk_weights.float()
@@ -78,6 +80,8 @@ def fused_mxfp4_moe(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Ten
     out = output if output is not None else torch.empty_like(
         hidden_states, memory_format=torch.contiguous_format)
     need = ops.mxfp4_moe_workspace(hidden_states, w1, w2, ids)
+    if workspace is not None and torch.cuda.is_current_stream_capturing():
+        workspace = None
     scratch = None if workspace is None else workspace.get("mxfp4")
     if scratch is None or scratch.numel() < need or scratch.device != hidden_states.device:
         scratch = torch.empty(need, dtype=torch.uint8, device=hidden_states.device)
