@@ -20,8 +20,8 @@
 // order; the rows' parts are summed in 64 bits in a fixed order.
 //
 // Bound by the logits' bytes where rows are many: at 65536 rows of 256 in FP32 (64
-// MiB, 14 us at the rate of a large copy) the loss takes 17 us after a count of 12
-// us and before a finish of 5 us, the gradient (twice the bytes) 23 us; at 200 rows
+// MiB, 14 us at the rate of a large copy) the loss takes 17 us after a count of 6
+// us and before a finish of 4 us, the gradient (twice the bytes) 23 us; at 200 rows
 // of 128 one launch each, which costs less than its call from the host.
 #include <hip/hip_runtime.h>
 
@@ -39,8 +39,8 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kCountThreads = 1024;
 constexpr int kMaxExperts = 1024;
-// Workgroups that count: the count and the loss that adds them up took 11.6 + 17.0 us
-// at 65536 rows of 256 with 32, 8.2 + 25.1 us with 64.
+// Workgroups that count: the count and the loss that adds them up take 6.3 + 17.2 us
+// at 65536 rows of 256 with 32, 10.0 + 16.9 us with 16 (the loss with 64: 25.1).
 constexpr int kMaxParts = 32;
 constexpr int kLossThreads = 1024, kLossWaves = kLossThreads / 64;
 constexpr int kMaxGroups = 512;  // workgroups of the loss: two a CU, few enough to add up the counts
@@ -191,24 +191,29 @@ struct Counting {
   int top_k, experts;
 };
 
-// count (LDS, experts + 1 zeros): the slots by expert of rows first, first + step, ...
-// and at its end these rows.
-__device__ __forceinline__ void count_rows(const Counting& g, int64_t first, int64_t step, int* count) {
+// count (LDS, experts + 1 zeros): the slots first, first + step, ... by expert, and at
+// its end the rows that these begin.  Slot by slot, so that a wavefront's loads are of
+// neighbours; eight slots at once, their loads on their way together.
+__device__ __forceinline__ void count_slots(const Counting& g, int64_t first, int64_t step, int* count) {
+  constexpr int kEach = 8;
+  const int64_t slots = g.rows * g.top_k;
   int mine = 0;
-  for (int64_t t = first; t < g.rows; t += step) {
-    const int32_t* ids = g.ids + t * g.top_k;
-    // (the mark and the first ids are on their way together)
-    const bool counted = !(g.padding && g.padding[t]);
-    for (int k0 = 0; k0 < g.top_k; k0 += 8) {
-      int id[8];
+  for (int64_t s0 = first; s0 < slots; s0 += kEach * step) {
+    int id[kEach];
+    uint32_t row[kEach];
+    bool counted[kEach];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) id[u] = ids[min(k0 + u, g.top_k - 1)];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        if (counted && k0 + u < g.top_k && id[u] >= 0 && id[u] < g.experts) atomicAdd(&count[id[u]], 1);
-      }
+    for (int u = 0; u < kEach; ++u) {
+      const uint32_t s = uint32_t(min(s0 + u * step, slots - 1));  // (slots fit 31 bits)
+      row[u] = s / uint32_t(g.top_k);
+      id[u] = g.ids[s];
+      counted[u] = s0 + u * step < slots && !(g.padding && g.padding[row[u]]);
     }
-    mine += counted;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      if (counted[u] && id[u] >= 0 && id[u] < g.experts) atomicAdd(&count[id[u]], 1);
+      mine += counted[u] && row[u] * uint32_t(g.top_k) == uint32_t(s0 + u * step);
+    }
   }
   if (mine) atomicAdd(&count[g.experts], mine);
 }
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(kCountThreads) void count_kernel(Counting g, int32_
   __shared__ int count[kMaxExperts + 1];
   for (int e = threadIdx.x; e <= g.experts; e += kCountThreads) count[e] = 0;
   __syncthreads();
-  count_rows(g, int64_t(blockIdx.x) * kCountThreads + threadIdx.x, int64_t(gridDim.x) * kCountThreads, count);
+  count_slots(g, int64_t(blockIdx.x) * kCountThreads + threadIdx.x, int64_t(gridDim.x) * kCountThreads, count);
   __syncthreads();
   for (int e = threadIdx.x; e <= g.experts; e += kCountThreads) hist[int64_t(blockIdx.x) * (g.experts + 1) + e] = count[e];
 }
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(1024) void one_kernel(Rows g, Counting c, Results o
   const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
   for (int e = tid; e <= c.experts; e += 1024) count[e] = 0;
   __syncthreads();
-  count_rows(c, tid, 1024, count);
+  count_slots(c, tid, 1024, count);
   __syncthreads();
   const int n = count[c.experts];
   for (int e = tid; e < kMaxExperts; e += 1024) {
