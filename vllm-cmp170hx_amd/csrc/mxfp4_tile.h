@@ -120,11 +120,11 @@ __device__ __forceinline__ void mfma32(f32x16_t& acc, const u32x4_t& a, uint32_t
 }
 
 // 32 rows of 32 kN columns from LDS to the output, eight columns a lane (n a
-// multiple of eight, rows 16-byte aligned).  sorted: the rows' slots, whose
-// router weights multiply them.
+// multiple of eight, rows 16-byte aligned).  slots (LDS): the rows' slots and their
+// router weights, which multiply them.
 template <int kN, int kDtype>
 __device__ __forceinline__ void store_rows(const float* part, int stride, int lane, int mt, int nrows, int ct, const TileArgs& g,
-                                           int64_t m0, const int32_t* sorted) {
+                                           int64_t m0, const int2* slots) {
   constexpr int kChunks = 4 * kN;  // of eight columns, a row
   const int ch = lane % kChunks, r0 = lane / kChunks;
   const int c = ct + 8 * ch;
@@ -137,9 +137,9 @@ __device__ __forceinline__ void store_rows(const float* part, int stride, int la
     if (m >= nrows || c >= g.n) continue;
     int64_t row = m0 + m;
     float weight = 1;
-    if (sorted) {
-      row = sorted[m];
-      weight = g.topk_w[row];
+    if (slots) {
+      row = slots[m].x;
+      weight = __builtin_bit_cast(float, slots[m].y);
     }
     const int64_t at = row * g.n + c;
     if constexpr (kDtype == vq::kFP32) {
@@ -201,13 +201,12 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     m0 = int64_t(t % g.tiles_m) * kRows;
     nrows = int(min(int64_t(kRows), g.rows - m0));
   } else {
-    // XCD x takes a run of tasks, a task's columns one after another: the tasks of
-    // one expert share its weights in L2
-    const int local = int(blockIdx.x >> 3), all = g.table[0], per = (all + 7) / 8;
-    const int task = int(blockIdx.x & 7) * per + local / g.tiles_n;
-    if (local / g.tiles_n >= per) return;
-    if (task >= all) return;
-    const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[task];
+    // XCD x takes a run of tasks (entries x, x + 8, ...), a task's columns one after
+    // another: the tasks of one expert share its weights in L2
+    const int local = int(blockIdx.x >> 3), mine = local / g.tiles_n;
+    const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[mine * 8 + int(blockIdx.x & 7)];
+    const int all = g.table[0], run = (all + 7) / 8;
+    if (mine >= run || int(blockIdx.x & 7) * run + mine >= all) return;
     wbase = int64_t(vq::uniform(tk.x)) * g.n;
     m0 = vq::uniform(tk.y);
     nrows = vq::uniform(tk.z);
@@ -231,6 +230,7 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     if constexpr (kMode == kGateUp) return sorted[t] / g.top_k;
     return t;
   };
+  static_assert(kMode != kDown || kRows <= kTileThreads, "a thread a row");
   const int64_t act0 = kMode == kGateUp ? 0 : m0;
   const int64_t line = int64_t(g.blocks) * kBlockBytes;
   // this tile's weight rows from the first one's address on
@@ -284,6 +284,11 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     first = int(blockIdx.y) * g.split_stages;
     stages = min(first + g.split_stages, all_stages);
   }
+  // kDown: the rows' slots, and (below, behind the first loads) their weights, for the end
+  __shared__ int2 slots[kMode == kDown ? kRows : 1];
+  int slot = 0;
+  float slot_weight = 0;
+  if constexpr (kMode == kDown) slot = sorted[min(tid, nrows - 1)];
   // DMA load i of stage s (zeros past the last stage)
   const auto fetch = [&](auto i_c, int s, uint8_t* buf) __attribute__((always_inline)) {
     constexpr int i = decltype(i_c)::value;
@@ -401,6 +406,7 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
   for_range<0, kBufs - 1>([&](auto b_c) {
     for_range<0, kLoads>([&](auto k) { fetch(k, first + decltype(b_c)::value, buf(b_c)); });
   });
+  if constexpr (kMode == kDown) slot_weight = g.topk_w[slot];
   land(scales_now[0], first, scale0);
   for_range<0, kHalf>([&](auto k) { fetch(k, first + kBufs - 1, buf(std::integral_constant<int, kBufs - 1>{})); });
   read_scales(scale0, sw[0], sa[0]);
@@ -464,6 +470,9 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     static_assert((4 / kBufs) * 32 * kStride * 4 <= kBufBytes, "the wavefronts' exchanges fit the stage buffers");
     float* part = kBufs == 2 ? reinterpret_cast<float*>(wave < 2 ? buf0 : buf1) + (wave & 1) * 32 * kStride
                              : reinterpret_cast<float*>(wave < 2 ? (wave ? buf1 : buf0) : (wave == 2 ? buf2 : buf3));
+    if constexpr (kMode == kDown) {
+      if (tid < kRows) slots[tid] = make_int2(slot, __builtin_bit_cast(int, slot_weight));
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kM; ++i) {
@@ -496,7 +505,7 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
           }
         }
       } else {
-        store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, o0, sorted);
+        store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, o0, slots);
       }
     }
   }
