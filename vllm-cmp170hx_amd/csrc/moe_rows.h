@@ -67,11 +67,8 @@ __device__ __forceinline__ int rows_height(int c, int tasks) {
 // this part's rows of the expert begin).  Every expert's first row (a scan of the summed
 // histograms, the same in each workgroup) plus the rows of the parts before
 // this one place the part's slots; workgroup 0 also writes the tasks.  Experts
-// e0 .. e1 - 1 (a contiguous run) belong to one thread.  spread: task i of n lies at
-// i % p * 8 + i / p, p = ceil(n / 8) (of max_tasks at least 8 p): entries x, x + 8, ...
-// are a run of tasks, for an XCD to read without n.
-__device__ __forceinline__ void rows_fill_part(const RowsLayout& lay, int32_t* table, int task_rows, int part, int* first,
-                                               bool spread = false) {
+// e0 .. e1 - 1 (a contiguous run) belong to one thread.
+__device__ __forceinline__ void rows_fill_part(const RowsLayout& lay, int32_t* table, int task_rows, int part, int* first) {
   __shared__ int wave_rows[kRowsPartThreads / 64], wave_tasks[kRowsPartThreads / 64];
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -125,12 +122,6 @@ __device__ __forceinline__ void rows_fill_part(const RowsLayout& lay, int32_t* t
     task += wave_tasks[w];
   }
   if (part == 0 && tid == kRowsPartThreads - 1) table[0] = task + tasks;
-  int run = 1;  // p
-  if (spread) {
-    int all = 0;
-    for (int w = 0; w < kRowsPartThreads / 64; ++w) all += wave_tasks[w];
-    run = max((all + 7) / 8, 1);
-  }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = e0 + i;
@@ -139,9 +130,7 @@ __device__ __forceinline__ void rows_fill_part(const RowsLayout& lay, int32_t* t
       if (part == 0) {
         const int h = rows_height(total[i], rows_tasks(total[i], task_rows));
         for (int r = 0; r < total[i]; r += h) {
-          const int at = spread ? task % run * 8 + task / run : task;
-          reinterpret_cast<int4*>(table + lay.tasks())[at] = make_int4(e, row + r, min(h, total[i] - r), 0);
-          ++task;
+          reinterpret_cast<int4*>(table + lay.tasks())[task++] = make_int4(e, row + r, min(h, total[i] - r), 0);
         }
       }
       row += total[i];

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(moe::kRowsPartThreads) void count_quantize_kernel(E
     moe::rows_count_part(of, lay, table, int(blockIdx.x), part_count);
     if (parts == 1) {
       __syncthreads();
-      moe::rows_fill_part(lay, table, task_rows, 0, part_count, task_rows == kTileRows);
+      moe::rows_fill_part(lay, table, task_rows, 0, part_count);
     }
     return;
   }
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(moe::kRowsPartThreads) void count_quantize_kernel(E
 
 __global__ __launch_bounds__(moe::kRowsPartThreads) void fill_kernel(moe::RowsLayout lay, int32_t* table, int task_rows) {
   extern __shared__ int first[];
-  moe::rows_fill_part(lay, table, task_rows, int(blockIdx.x), first, task_rows == kTileRows);
+  moe::rows_fill_part(lay, table, task_rows, int(blockIdx.x), first);
 }
 
 // ---- few rows an expert ---------------------------------------------------------
@@ -443,7 +443,7 @@ struct Workspace {
   int64_t xq, xs, hq, hs, c3, table, total;
 };
 
-moe::RowsLayout layout_of(int64_t slots, int64_t experts) { return {slots, experts, slots / 16 + std::min(experts, slots) + 8}; }
+moe::RowsLayout layout_of(int64_t slots, int64_t experts) { return {slots, experts, slots / 16 + std::min(experts, slots)}; }
 
 Workspace workspace_of(int64_t tokens, int64_t top_k, int64_t hidden, int64_t inter, int64_t experts) {
   const int64_t slots = tokens * top_k;

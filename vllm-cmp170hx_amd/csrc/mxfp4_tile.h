@@ -201,12 +201,13 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
     m0 = int64_t(t % g.tiles_m) * kRows;
     nrows = int(min(int64_t(kRows), g.rows - m0));
   } else {
-    // XCD x takes a run of tasks (entries x, x + 8, ...), a task's columns one after
-    // another: the tasks of one expert share its weights in L2
-    const int local = int(blockIdx.x >> 3), mine = local / g.tiles_n;
-    const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[mine * 8 + int(blockIdx.x & 7)];
-    const int all = g.table[0], run = (all + 7) / 8;
-    if (mine >= run || int(blockIdx.x & 7) * run + mine >= all) return;
+    // XCD x takes a run of tasks, a task's columns one after another: the tasks of
+    // one expert share its weights in L2
+    const int local = int(blockIdx.x >> 3), all = g.table[0], per = (all + 7) / 8;
+    const int task = int(blockIdx.x & 7) * per + local / g.tiles_n;
+    if (local / g.tiles_n >= per) return;
+    if (task >= all) return;
+    const int4 tk = reinterpret_cast<const int4*>(g.table + g.tasks)[task];
     wbase = int64_t(vq::uniform(tk.x)) * g.n;
     m0 = vq::uniform(tk.y);
     nrows = vq::uniform(tk.z);
