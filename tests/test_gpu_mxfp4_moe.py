@@ -58,7 +58,7 @@ CASES = [  # experts, hidden, inter, topk, tokens
     # few rows' kernels: several tasks of 16 rows an expert, listed and looked for; whole
     # blocks a wavefront, by expert and by slot; more than eight and 64 slots a token
     (64, 128, 64, 6, 200), (8, 160, 96, 2, 100), (64, 256, 512, 2, 40), (128, 64, 512, 2, 62), (32, 128, 64, 20, 2),
-    (100, 64, 32, 64, 1), (100, 64, 32, 65, 1),
+    (100, 64, 32, 64, 1), (100, 64, 32, 65, 1), (100, 64, 32, 40, 2), (4, 64, 2080, 2, 1), (6, 64, 4128, 1, 4),
     # rows so long that LDS holds fewer than 16 (and one)
     (2, 8192, 64, 1, 30), (4, 96, 8192, 1, 80), (2, 8192, 64, 2, 600), (1, 65536, 32, 1, 2), (1, 32, 65536, 1, 2),
     # tiles: several an expert, a few rows of many experts, sizes that end inside a stage

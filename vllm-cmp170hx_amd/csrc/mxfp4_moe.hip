@@ -373,12 +373,13 @@ __global__ __launch_bounds__(256, 4) void down_kernel(SmallMoeArgs g, int wgs) {
   }
 }
 
-// down and the slot sum for one token by 16 columns, a wavefront a slot: where
-// tokens are few, their experts' weights are read a token at a time (those two
-// share come from L2) and the slot rows never leave the workgroup.
+// down and the slot sum for one token by 16 columns, `parts` wavefronts a slot (chunk c
+// of K multiplied by part c % parts): where tokens are few, their experts' weights are
+// read a token at a time (those two share come from L2) and the slot rows never leave
+// the workgroup.
 template <int kDtype>
-__global__ __launch_bounds__(512, 4) void down_sum_kernel(SmallMoeArgs g) {
-  extern __shared__ float part[];  // [top_k][16]
+__global__ __launch_bounds__(1024, 4) void down_sum_kernel(SmallMoeArgs g, int parts) {
+  extern __shared__ float sums[];  // [top_k][parts][16]
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = vq::uniform(int(threadIdx.x) >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -386,8 +387,9 @@ __global__ __launch_bounds__(512, 4) void down_sum_kernel(SmallMoeArgs g) {
   const int n0 = int(blockIdx.x) % groups * 16;
   const int token = int(blockIdx.x) / groups;
   const int chunks = (g.blocks + kChunk - 1) / kChunk;
-  for (int k = wave; k < g.top_k; k += waves) {
-    const int64_t slot = int64_t(token) * g.top_k + k;
+  for (int i = wave; i < g.top_k * parts; i += waves) {
+    const int64_t slot = int64_t(token) * g.top_k + i / parts;
+    const int part = i % parts;
     const int e = vq::uniform(g.of(slot));
     f32x4_t acc{0, 0, 0, 0};
     if (e >= 0) {
@@ -396,26 +398,34 @@ __global__ __launch_bounds__(512, 4) void down_sum_kernel(SmallMoeArgs g) {
       const uint8_t* ws = g.ws + wrow * g.blocks;
       const uint8_t* x = g.h + slot * g.blocks * kBlockBytes;
       const uint8_t* xs = g.hs + slot * g.blocks;
-      ChunkOperand a = load_chunk(w, ws, 0, g.blocks, q), ax = load_chunk(x, xs, 0, g.blocks, q);
-      for (int c = 0; c < chunks; ++c) {
-        ChunkOperand next{}, nx{};
-        if (c + 1 < chunks) {
-          next = load_chunk(w, ws, c + 1, g.blocks, q);
-          nx = load_chunk(x, xs, c + 1, g.blocks, q);
+      const auto load = [&](int c, ChunkOperand& a, ChunkOperand& ax) {
+        a = ax = ChunkOperand{};
+        if (c < chunks) {
+          a = load_chunk(w, ws, c, g.blocks, q);
+          ax = load_chunk(x, xs, c, g.blocks, q);
         }
+      };
+      ChunkOperand a, ax;
+      load(part, a, ax);
+      for (int c = part; c < chunks; c += parts) {
+        ChunkOperand next, nx;
+        load(c + parts, next, nx);
         multiply_loaded(a, ax, acc);
         a = next;
         ax = nx;
       }
       acc = acc * g.topk_w[slot];
     }
-    if (r == 0) *reinterpret_cast<f32x4_t*>(part + k * 16 + 4 * q) = acc;
+    if (r == 0) *reinterpret_cast<f32x4_t*>(sums + i * 16 + 4 * q) = acc;
   }
   __syncthreads();
   if (threadIdx.x >= 16) return;
   float sum = 0;
   for (int k = 0; k < g.top_k; ++k) {
-    if (g.of(int64_t(token) * g.top_k + k) >= 0) sum += part[k * 16 + threadIdx.x];
+    if (g.of(int64_t(token) * g.top_k + k) < 0) continue;
+    float one = 0;
+    for (int p = 0; p < parts; ++p) one += sums[(k * parts + p) * 16 + threadIdx.x];
+    sum += one;
   }
   vq::store_act(g.out, kDtype, int64_t(token) * g.n + n0 + threadIdx.x, sum);
 }
@@ -580,11 +590,18 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
     }
     if (int rc = vq::check_launch("mxfp4 moe gate_up")) return rc;
     second(m);
-    if (tokens <= 4 && top_k <= 64) {
-      const dim3 grid(unsigned(tokens * (hidden / 16))), block(unsigned(64 * std::min<int64_t>(top_k, 8)));
-      const size_t bytes = size_t(top_k) * 16 * sizeof(float);
-      if (act_dtype == vq::kBF16) hipLaunchKernelGGL(down_sum_kernel<vq::kBF16>, grid, block, bytes, st, m);
-      else hipLaunchKernelGGL(down_sum_kernel<vq::kFP16>, grid, block, bytes, st, m);
+    // A token at a time while experts are hardly shared: in us, a token at a time and
+    // an expert at a time, 128 experts of 2048 x 768, eight a token: 4 tokens 25 and 30,
+    // 12 58 and 61, 16 67 and 65; 8 experts of 4096 x 14336, two a token: 2 tokens 78 and
+    // 86, 4 126 and 119.  K split where slots are few (the same 8 experts, one token: 51
+    // for 65).
+    if ((m.by_slot || tokens == 1) && top_k <= 64) {
+      int split = 1;
+      while (2 * split * std::min<int64_t>(top_k, 8) <= 16 && 4 * split <= chunks2) split *= 2;
+      const dim3 grid(unsigned(tokens * (hidden / 16))), block(unsigned(64 * split * std::min<int64_t>(top_k, 8)));
+      const size_t bytes = size_t(top_k) * split * 16 * sizeof(float);
+      if (act_dtype == vq::kBF16) hipLaunchKernelGGL(down_sum_kernel<vq::kBF16>, grid, block, bytes, st, m, split);
+      else hipLaunchKernelGGL(down_sum_kernel<vq::kFP16>, grid, block, bytes, st, m, split);
       return vq::check_launch("mxfp4 moe down");
     }
     const int wgs = wgs_of(units, (hidden + 63) / 64);
