@@ -20,8 +20,9 @@
 // order; the rows' parts are summed in 64 bits in a fixed order.
 //
 // Bound by the logits' bytes where rows are many: at 65536 rows of 256 in FP32 (64
-// MiB, 14 us at the rate of a large copy) the loss takes 17 us after a count of 6
-// us and before a finish of 4 us, the gradient (twice the bytes) 23 us; at 200 rows
+// MiB, 14 us at the rate of a large copy) the loss takes 17 us (sigmoids,
+// with padding marked, 18) after a count of 6 to 7 us and before a finish of 4 us, the
+// gradient (twice the bytes) 23 to 24 us; at 200 rows
 // of 128 one launch each, which costs less than its call from the host.
 #include <hip/hip_runtime.h>
 
@@ -161,7 +162,8 @@ __device__ __forceinline__ float row_terms(Values<S>& x, const float* f, int l, 
     for (int j = 0; j < 4; ++j) {
       float z;
       if constexpr (kSigmoid) {
-        const float a = x.v[i][j], t = exp_nonpositive(-fabsf(a)), large = 1 / (1 + t), small = t * large;
+        // (the reciprocal of 1 .. 2 as the hardware rounds it, off by one step at most)
+        const float a = x.v[i][j], t = exp_nonpositive(-fabsf(a)), large = __builtin_amdgcn_rcpf(1 + t), small = t * large;
         z = a >= 0 ? large : small;
         x.v[i][j] = large * small;
         if (a != a) z = x.v[i][j] = a;
@@ -201,18 +203,23 @@ __device__ __forceinline__ void count_slots(const Counting& g, int64_t first, in
   for (int64_t s0 = first; s0 < slots; s0 += kEach * step) {
     int id[kEach];
     uint32_t row[kEach];
-    bool counted[kEach];
+    uint8_t mark[kEach];
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
       const uint32_t s = uint32_t(min(s0 + u * step, slots - 1));  // (slots fit 31 bits)
       row[u] = s / uint32_t(g.top_k);
       id[u] = g.ids[s];
-      counted[u] = s0 + u * step < slots && !(g.padding && g.padding[row[u]]);
+      mark[u] = 0;
+    }
+    if (g.padding) {
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) mark[u] = g.padding[row[u]];
     }
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
-      if (counted[u] && id[u] >= 0 && id[u] < g.experts) atomicAdd(&count[id[u]], 1);
-      mine += counted[u] && row[u] * uint32_t(g.top_k) == uint32_t(s0 + u * step);
+      const bool counted = s0 + u * step < slots && !mark[u];
+      if (counted && id[u] >= 0 && id[u] < g.experts) atomicAdd(&count[id[u]], 1);
+      mine += counted && row[u] * uint32_t(g.top_k) == uint32_t(s0 + u * step);
     }
   }
   if (mine) atomicAdd(&count[g.experts], mine);
@@ -264,15 +271,15 @@ __device__ __forceinline__ double sum_rows(const Rows& g, int64_t first, int64_t
   if (first >= g.rows) return sum;
   // a row ahead: the next one's logits are on their way while this one's are used
   const auto row = [&](int64_t t) { return load_row<S, kDtype>(g, min(t, g.rows - 1), l); };
-  const auto kept = [&](int64_t t) { return t < g.rows && !(g.padding && g.padding[t]); };
+  const auto mark = [&](int64_t t) { return g.padding ? g.padding[min(t, g.rows - 1)] : uint8_t(0); };
   Values<S> next = row(first + sub);
-  bool next_kept = kept(first + sub);
+  uint8_t next_mark = mark(first + sub);
   for (int64_t t = first + sub; t - sub < g.rows; t += step) {
     Values<S> x = next;
-    const bool counted = next_kept;
+    const bool counted = t < g.rows && !next_mark;
     if (t - sub + step < g.rows) {
       next = row(t + step);
-      next_kept = kept(t + step);
+      next_mark = mark(t + step);
     }
     const float r = row_terms<S, kSigmoid>(x, f, l, lane);
     if (counted && l == 0) sum += r;
@@ -376,7 +383,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Rows g, const float* sta
   const bool wide = g.experts % 4 == 0;
   for (int64_t t0 = (int64_t(blockIdx.x) * kWaves + wave) * S::kRows; t0 < g.rows; t0 += int64_t(gridDim.x) * kWaves * S::kRows) {
     const int64_t t = t0 + sub;
-    const bool counted = t < g.rows && !(g.padding && g.padding[t]);
+    const bool counted = t < g.rows && !(g.padding && g.padding[min(t, g.rows - 1)]);
     Values<S> x = load_row<S, kDtype>(g, t < g.rows ? t : g.rows - 1, l);
     const float r = row_terms<S, kSigmoid>(x, f, l, lane);
     if (t >= g.rows) continue;

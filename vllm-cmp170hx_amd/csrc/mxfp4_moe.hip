@@ -38,6 +38,8 @@ struct ExpertOf {
 
 // Workgroups 0 .. parts - 1 count the slots (one alone also lists them: no launch
 // for that); the others quantize the rows of x, four lanes a block.
+// 2048 tokens of 2048 and 16384 slots 6 us, 300 tokens of 2592 with their list 5 us (in
+// two launches 4.9 + 4.8).
 template <int kDtype>
 __global__ __launch_bounds__(moe::kRowsPartThreads) void count_quantize_kernel(ExpertOf of, moe::RowsLayout lay, int32_t* table,
                                                                                int task_rows, const void* x, int64_t tokens, int blocks,
@@ -149,7 +151,10 @@ __device__ __forceinline__ RowsOf rows_of(const SmallMoeArgs& g, int index, int3
 // gate | up and the SwiGLU for the rows of one expert, 16 at a time, by one block
 // of 32 columns of h: wavefront (tile = wave % 4: gate 0, gate 1, up 0, up 1; part
 // = wave / 4 of K).  Its sums meet in LDS; one wavefront forms h, four lanes a row.
-// For calls of few blocks, whose time is one block's.
+// For calls of few blocks, whose time is one block's: in us of the call, these and
+// whole blocks a wavefront (gate_up_kernel), 1152 blocks of 2048 33 and 38, 1792 blocks
+// of 4096 91 and 78.  One token, eight of 128 experts of 2048 x 768: 6.6 us for 13 MB, the
+// list, one chain of loads and the sums.
 template <int kDtype>
 __global__ __launch_bounds__(1024, 4) void gate_up_split_kernel(SmallMoeArgs g) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -257,9 +262,11 @@ struct WeightStream {
   }
 };
 
-// gate | up and the SwiGLU for the rows of one expert, 16 at a time: the rows in
-// LDS, a wavefront whole blocks of 32 columns of h (four weight tiles each), one
-// after another with no barrier between.  `wgs` workgroups an expert.
+// gate | up and the SwiGLU for the rows of one expert, 16 (or g.pass) at a time: the rows
+// in LDS, a wavefront whole blocks of 32 columns of h (four weight tiles each), one after
+// another with no barrier between.  `wgs` workgroups an expert.  Bound by the weight
+// stream: 8 tokens, eight of 128 experts of 2048 x 768 each, 25 us for the 87 MB of 52
+// experts.
 template <bool kScan, int kDtype>
 __global__ __launch_bounds__(256, 4) void gate_up_kernel(SmallMoeArgs g, int wgs) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(256, 4) void gate_up_kernel(SmallMoeArgs g, int wgs
 }
 
 // down for the rows of one expert: the rows of h in LDS, a wavefront 16 columns
-// after another; the weighted slot rows.
+// after another; the weighted slot rows.  16 tokens of the layer above 22 us (69 MB).
 template <bool kScan>
 __global__ __launch_bounds__(256, 4) void down_kernel(SmallMoeArgs g, int wgs) {
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -376,7 +383,8 @@ __global__ __launch_bounds__(256, 4) void down_kernel(SmallMoeArgs g, int wgs) {
 // down and the slot sum for one token by 16 columns, `parts` wavefronts a slot (chunk c
 // of K multiplied by part c % parts): where tokens are few, their experts' weights are
 // read a token at a time (those two share come from L2) and the slot rows never leave
-// the workgroup.
+// the workgroup.  One token, eight experts of 2048 x 768: 5 us (6.7 MB), two of 4096 x
+// 14336: 15 us (62 MB; 29 without parts).
 template <int kDtype>
 __global__ __launch_bounds__(1024, 4) void down_sum_kernel(SmallMoeArgs g, int parts) {
   extern __shared__ float sums[];  // [top_k][parts][16]
@@ -430,7 +438,8 @@ __global__ __launch_bounds__(1024, 4) void down_sum_kernel(SmallMoeArgs g, int p
   vq::store_act(g.out, kDtype, int64_t(token) * g.n + n0 + threadIdx.x, sum);
 }
 
-// out[t][c] = RN(sum over t's slots with a local expert, in slot order).
+// out[t][c] = RN(sum over t's slots with a local expert, in slot order).  2048 tokens of
+// eight slots of 2048: 22.5 us, 142 MB at 6.3 TB/s (the slot rows were just written).
 __global__ __launch_bounds__(kThreads) void slot_sum_kernel(const float* in, ExpertOf of, int64_t tokens, int top_k, int hidden,
                                                             void* out, int dtype) {
   const int64_t i = (int64_t(blockIdx.x) * kThreads + threadIdx.x) * 4;
