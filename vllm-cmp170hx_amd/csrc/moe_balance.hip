@@ -20,10 +20,10 @@
 // order; the rows' parts are summed in 64 bits in a fixed order.
 //
 // Bound by the logits' bytes where rows are many: at 65536 rows of 256 in FP32 (64
-// MiB, 14 us at the rate of a large copy) the loss takes 17 us (sigmoids,
-// with padding marked, 18) after a count of 6 to 7 us and before a finish of 4 us, the
-// gradient (twice the bytes) 23 to 24 us; at 200 rows
-// of 128 one launch each, which costs less than its call from the host.
+// MiB, 14 us at the rate of a large copy) the loss takes 17 us (sigmoids, with
+// padding marked, 18) after a count of 6 to 7 us and before a finish of 4 us, the
+// gradient (twice the bytes) 23 to 24 us; at 200 rows of 128 one launch each, which
+// costs less than its call from the host.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

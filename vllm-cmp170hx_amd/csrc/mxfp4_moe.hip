@@ -380,24 +380,24 @@ __global__ __launch_bounds__(256, 4) void down_kernel(SmallMoeArgs g, int wgs) {
   }
 }
 
-// down and the slot sum for one token by 16 columns, `parts` wavefronts a slot (chunk c
-// of K multiplied by part c % parts): where tokens are few, their experts' weights are
+// down and the slot sum for one token by 16 columns, 2^log_parts wavefronts a slot (chunk
+// c of K multiplied by part c % parts, of at least as many chunks): where tokens are few, their experts' weights are
 // read a token at a time (those two share come from L2) and the slot rows never leave
 // the workgroup.  One token, eight experts of 2048 x 768: 5 us (6.7 MB), two of 4096 x
 // 14336: 15 us (62 MB; 29 without parts).
 template <int kDtype>
-__global__ __launch_bounds__(1024, 4) void down_sum_kernel(SmallMoeArgs g, int parts) {
+__global__ __launch_bounds__(1024, 4) void down_sum_kernel(SmallMoeArgs g, int log_parts) {
   extern __shared__ float sums[];  // [top_k][parts][16]
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = vq::uniform(int(threadIdx.x) >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int groups = g.n / 16;
+  const int groups = g.n / 16, parts = 1 << log_parts;
   const int n0 = int(blockIdx.x) % groups * 16;
   const int token = int(blockIdx.x) / groups;
   const int chunks = (g.blocks + kChunk - 1) / kChunk;
-  for (int i = wave; i < g.top_k * parts; i += waves) {
-    const int64_t slot = int64_t(token) * g.top_k + i / parts;
-    const int part = i % parts;
+  for (int i = wave; i < g.top_k << log_parts; i += waves) {
+    const int64_t slot = int64_t(token) * g.top_k + (i >> log_parts);
+    const int part = i & (parts - 1);
     const int e = vq::uniform(g.of(slot));
     f32x4_t acc{0, 0, 0, 0};
     if (e >= 0) {
@@ -406,18 +406,13 @@ __global__ __launch_bounds__(1024, 4) void down_sum_kernel(SmallMoeArgs g, int p
       const uint8_t* ws = g.ws + wrow * g.blocks;
       const uint8_t* x = g.h + slot * g.blocks * kBlockBytes;
       const uint8_t* xs = g.hs + slot * g.blocks;
-      const auto load = [&](int c, ChunkOperand& a, ChunkOperand& ax) {
-        a = ax = ChunkOperand{};
-        if (c < chunks) {
-          a = load_chunk(w, ws, c, g.blocks, q);
-          ax = load_chunk(x, xs, c, g.blocks, q);
-        }
-      };
-      ChunkOperand a, ax;
-      load(part, a, ax);
+      ChunkOperand a = load_chunk(w, ws, part, g.blocks, q), ax = load_chunk(x, xs, part, g.blocks, q);
       for (int c = part; c < chunks; c += parts) {
-        ChunkOperand next, nx;
-        load(c + parts, next, nx);
+        ChunkOperand next{}, nx{};
+        if (c + parts < chunks) {
+          next = load_chunk(w, ws, c + parts, g.blocks, q);
+          nx = load_chunk(x, xs, c + parts, g.blocks, q);
+        }
         multiply_loaded(a, ax, acc);
         a = next;
         ax = nx;
@@ -428,18 +423,15 @@ __global__ __launch_bounds__(1024, 4) void down_sum_kernel(SmallMoeArgs g, int p
   }
   __syncthreads();
   if (threadIdx.x >= 16) return;
-  float sum = 0;
-  for (int k = 0; k < g.top_k; ++k) {
-    if (g.of(int64_t(token) * g.top_k + k) < 0) continue;
-    float one = 0;
-    for (int p = 0; p < parts; ++p) one += sums[(k * parts + p) * 16 + threadIdx.x];
-    sum += one;
-  }
+  float sum = 0;  // (masked slots: zeros)
+#pragma unroll 4
+  for (int i = 0; i < g.top_k << log_parts; ++i) sum += sums[i * 16 + threadIdx.x];
   vq::store_act(g.out, kDtype, int64_t(token) * g.n + n0 + threadIdx.x, sum);
 }
 
 // out[t][c] = RN(sum over t's slots with a local expert, in slot order).  2048 tokens of
-// eight slots of 2048: 22.5 us, 142 MB at 6.3 TB/s (the slot rows were just written).
+// eight slots of 2048: 22 us, 142 MB at 6.4 TB/s (the slot rows were just written); 64
+// tokens 4.6 us (5.8 with a slot's load behind the one before).
 __global__ __launch_bounds__(kThreads) void slot_sum_kernel(const float* in, ExpertOf of, int64_t tokens, int top_k, int hidden,
                                                             void* out, int dtype) {
   const int64_t i = (int64_t(blockIdx.x) * kThreads + threadIdx.x) * 4;
@@ -447,11 +439,20 @@ __global__ __launch_bounds__(kThreads) void slot_sum_kernel(const float* in, Exp
   const int64_t t = i / hidden;
   const int64_t c = i - t * hidden;
   f32x4_t sum{0, 0, 0, 0};
-  for (int k = 0; k < top_k; ++k) {
-    if (of(t * top_k + k) < 0) continue;
-    const f32x4_t v = *reinterpret_cast<const f32x4_t*>(in + (t * top_k + k) * hidden + c);
+  constexpr int kEach = 4;  // slots whose loads are on their way together
+  for (int k0 = 0; k0 < top_k; k0 += kEach) {
+    f32x4_t v[kEach];
+    bool local[kEach];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j] += v[j];
+    for (int u = 0; u < kEach; ++u) {
+      const int64_t slot = t * top_k + min(k0 + u, top_k - 1);
+      v[u] = *reinterpret_cast<const f32x4_t*>(in + slot * hidden + c);  // (of a masked slot whatever lies there)
+      local[u] = k0 + u < top_k && of(slot) >= 0;
+    }
+#pragma unroll
+    for (int u = 0; u < kEach; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = local[u] ? sum[j] + v[u][j] : sum[j];
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) vq::store_act(out, dtype, i + j, sum[j]);
@@ -605,10 +606,10 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
     // 86, 4 126 and 119.  K split where slots are few (the same 8 experts, one token: 51
     // for 65).
     if ((m.by_slot || tokens == 1) && top_k <= 64) {
-      int split = 1;
-      while (2 * split * std::min<int64_t>(top_k, 8) <= 16 && 4 * split <= chunks2) split *= 2;
-      const dim3 grid(unsigned(tokens * (hidden / 16))), block(unsigned(64 * split * std::min<int64_t>(top_k, 8)));
-      const size_t bytes = size_t(top_k) * split * 16 * sizeof(float);
+      int split = 0;  // log2
+      while ((2 << split) * std::min<int64_t>(top_k, 8) <= 16 && 4 << split <= chunks2) ++split;
+      const dim3 grid(unsigned(tokens * (hidden / 16))), block(unsigned((64 << split) * std::min<int64_t>(top_k, 8)));
+      const size_t bytes = (size_t(top_k) << split) * 16 * sizeof(float);
       if (act_dtype == vq::kBF16) hipLaunchKernelGGL(down_sum_kernel<vq::kBF16>, grid, block, bytes, st, m, split);
       else hipLaunchKernelGGL(down_sum_kernel<vq::kFP16>, grid, block, bytes, st, m, split);
       return vq::check_launch("mxfp4 moe down");
