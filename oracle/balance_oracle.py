@@ -1,6 +1,6 @@
 """CPU statement of the router's load-balance loss and its gradient, FP64 NumPy.
 
-TEST INFRASTRUCTURE ONLY.  Only tests/ may import this module, as the checker;
+TEST INFRASTRUCTURE ONLY.  Only tests/ may import this module;
 the product path (vllm-cmp170hx_amd/) never does.
 
 Pinned by even routing giving 1, by all rows on one expert, and the gradient by

@@ -1,7 +1,7 @@
 """CPU statement of MXFP4 (blocks of 32, E2M1 codes under an E8M0 scale byte),
 its product and the routed experts in it, in FP64 NumPy.
 
-TEST INFRASTRUCTURE ONLY.  Only tests/ may import this module, as the checker;
+TEST INFRASTRUCTURE ONLY.  Only tests/ may import this module;
 the product path (vllm-cmp170hx_amd/) never does.
 
 Pinned by closed forms (tests/test_oracle_mxfp4.py): every code's value, the
