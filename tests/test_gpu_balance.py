@@ -57,7 +57,7 @@ def check(moe, logits, ids, padding, sigmoid, device, upstream=1.0):
 
 @pytest.mark.parametrize("rows,experts,topk", [(1, 1, 1), (1, 8, 2), (3, 5, 4), (64, 64, 6), (200, 128, 8), (7, 65, 3),
                                                (300, 257, 8), (33, 512, 10), (5, 1000, 8), (2, 1024, 1), (5000, 40, 2), (2500, 256, 8),
-                                               (9000, 16, 4)])
+                                               (9000, 16, 4), (256, 128, 8), (257, 128, 8)])
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("sigmoid", [False, True])
 def test_matches_the_oracle(moe, device, rows, experts, topk, dtype, sigmoid):

@@ -62,7 +62,7 @@ CASES = [  # experts, hidden, inter, topk, tokens
     # rows so long that LDS holds fewer than 16 (and one)
     (2, 8192, 64, 1, 30), (4, 96, 8192, 1, 80), (2, 8192, 64, 2, 600), (1, 65536, 32, 1, 2), (1, 32, 65536, 1, 2),
     # tiles: several an expert, a few rows of many experts, sizes that end inside a stage
-    (2, 256, 256, 1, 700), (3, 288, 416, 2, 450), (200, 256, 256, 8, 150)]
+    (2, 256, 256, 1, 700), (3, 288, 416, 2, 450), (200, 256, 256, 8, 150), (16, 256, 288, 4, 16), (16, 256, 288, 4, 17)]
 
 
 @pytest.mark.parametrize("experts,hidden,inter,topk,tokens", CASES)
@@ -79,12 +79,13 @@ def test_matches_the_oracle(mx, device, experts, hidden, inter, topk, tokens, dt
     check(layer, got, x, ids, weights, TYPES[dtype], limit)
 
 
+@pytest.mark.parametrize("hidden,inter", [(192, 96), (288, 320)])
 @pytest.mark.parametrize("tokens", [1, 6, 90])
-def test_expert_map_masked_slots_and_repeats(mx, device, tokens):
+def test_expert_map_masked_slots_and_repeats(mx, device, tokens, hidden, inter):
     """A part of the layer's experts, ids out of range, one expert twice in a
     row, rows with no slot left (zeros), all slots on one expert."""
     rng = np.random.default_rng(tokens)
-    layer = Layer(rng, 6, 192, 96, device)
+    layer = Layer(rng, 6, hidden, inter, device)
     emap = np.array([-1, 3, 0, -1, 5, 2, 77, 1, 4, -5], np.int32)
     ids = rng.integers(-2, 12, (tokens, 4)).astype(np.int32)
     ids[0] = [1, 1, 4, 4]
@@ -93,7 +94,7 @@ def test_expert_map_masked_slots_and_repeats(mx, device, tokens):
         ids[2] = [0, 3, 6, 11]
     weights = rng.random((tokens, 4)).astype(np.float32)
     local = np.where((ids >= 0) & (ids < len(emap)), emap[np.clip(ids, 0, len(emap) - 1)], -1)
-    x = torch.from_numpy(rng.standard_normal((tokens, 192))).bfloat16().to(device)
+    x = torch.from_numpy(rng.standard_normal((tokens, hidden))).bfloat16().to(device)
     tw = torch.from_numpy(weights).to(device)
     got = layer.run(mx, x, tw, torch.from_numpy(ids).to(device), expert_map=torch.from_numpy(emap).to(device))
     check(layer, got, x, local, weights, torch.bfloat16)
@@ -107,10 +108,11 @@ def test_expert_map_masked_slots_and_repeats(mx, device, tokens):
     check(layer, layer.run(mx, x, tw, one), x, np.full((tokens, 4), 5), weights, torch.bfloat16)
 
 
-def test_rows_do_not_depend_on_each_other(mx, device):
+@pytest.mark.parametrize("inter", [128, 288])
+def test_rows_do_not_depend_on_each_other(mx, device, inter):
     """A NaN row, and one of infinities, leave the other rows' bits; row strides."""
     rng = np.random.default_rng(0)
-    layer = Layer(rng, 8, 256, 128, device)
+    layer = Layer(rng, 8, 256, inter, device)
     ids, weights = routing(rng, 50, 8, 2)
     ti, tw = torch.from_numpy(ids).to(device), torch.from_numpy(weights).to(device)
     wide = torch.from_numpy(rng.standard_normal((50, 300))).bfloat16().to(device)
@@ -128,16 +130,19 @@ def test_rows_do_not_depend_on_each_other(mx, device):
     assert torch.equal(got[keep], clean[keep])
 
 
-def test_weights_with_a_nan_expert(mx, device):
+@pytest.mark.parametrize("size,copies", [(128, 1), (256, 1), (256, 7)])
+def test_weights_with_a_nan_expert(mx, device, size, copies):
     rng = np.random.default_rng(2)
-    layer = Layer(rng, 4, 128, 64, device)
-    ids = torch.tensor([[0, 1], [2, 3], [1, 2]], dtype=torch.int32, device=device)
-    tw = torch.full((3, 2), 0.5, device=device)
-    x = torch.from_numpy(rng.standard_normal((3, 128))).half().to(device)
+    layer = Layer(rng, 4, size, size, device)
+    ids = torch.tensor([[0, 1], [2, 3], [1, 2]] * copies, dtype=torch.int32, device=device)
+    tw = torch.full((3 * copies, 2), 0.5, device=device)
+    x = torch.from_numpy(rng.standard_normal((3 * copies, size)) * 0.1).half().to(device)
     clean = layer.run(mx, x, tw, ids)
+    assert torch.isfinite(clean).all()
     layer.s13[3, 10, 1] = 255  # a gate row: h's block is NaN, and so every output
     got = layer.run(mx, x, tw, ids)
-    assert torch.isnan(got[1]).all() and torch.equal(got[[0, 2]], clean[[0, 2]])
+    hit = torch.arange(3 * copies, device=device) % 3 == 1
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], clean[~hit])
 
 
 def test_refusals(mx, device):
@@ -164,13 +169,14 @@ def test_refusals(mx, device):
     assert mx.fused_mxfp4_moe(*ok, output=out) is out
 
 
-@pytest.mark.parametrize("tokens", [1, 3, 64, 200])
-def test_streams_workspace_and_graph(mx, device, tokens):
+@pytest.mark.parametrize("inter", [128, 256])
+@pytest.mark.parametrize("tokens", [1, 3, 64, 200, 700])
+def test_streams_workspace_and_graph(mx, device, tokens, inter):
     """Equal bits on another stream, with a workspace that a larger call left,
     and on every replay of a graph with new inputs and new routing."""
-    print(f"moe graph T={tokens}", flush=True)
+    print(f"moe graph T={tokens} I={inter}", flush=True)
     rng = np.random.default_rng(tokens + 1)
-    layer = Layer(rng, 16, 256, 128, device)
+    layer = Layer(rng, 16, 256, inter, device)
     sets = []
     for _ in range(3):
         ids, weights = routing(rng, tokens, 16, 4)
@@ -205,13 +211,14 @@ def test_streams_workspace_and_graph(mx, device, tokens):
         assert torch.equal(out, want[i]) and torch.equal(again, want[i])
 
 
-def test_a_graph_outlives_its_workspace(mx, device):
+@pytest.mark.parametrize("inter", [128, 256])
+def test_a_graph_outlives_its_workspace(mx, device, inter):
     """Calls captured with a workspace, which later calls replace by larger ones
     and whose memory others then write; two graphs replayed in turn; the output
     in the place of the input."""
     print("moe graphs and a workspace", flush=True)
     rng = np.random.default_rng(8)
-    layer = Layer(rng, 8, 256, 128, device)
+    layer = Layer(rng, 8, 256, inter, device)
     def call(tokens):
         ids, weights = routing(rng, tokens, 8, 2)
         return (torch.from_numpy(rng.standard_normal((tokens, 256))).bfloat16().to(device),

@@ -6,6 +6,7 @@ A packed tensor [..., k] is a pair of contiguous uint8 tensors: codes
 is free.  Outputs and scratch come from torch's allocator on the current stream,
 so calls on several streams, and captured ones, do not share memory (the fused
 MoE's workspace aside, which is the caller's).  Failed checks raise RuntimeError.
+These are operators for inference: outputs carry no gradient.
 """
 
 from __future__ import annotations
