@@ -1,8 +1,8 @@
 """A router's load: slots per expert, and the load-balance loss with its
 gradient (no counterpart in the reference).
 
-Both take what moe_route gives: logits [M, E] and topk_ids [M, topk], where
-padding rows hold -1.  Failed checks raise RuntimeError.
+Both take what moe_route gives: logits [M, E] and topk_ids [M, topk] (int32, or
+another type of such values), where padding rows hold -1.  Failed checks raise RuntimeError.
 """
 
 from __future__ import annotations

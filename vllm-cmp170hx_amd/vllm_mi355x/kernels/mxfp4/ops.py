@@ -67,8 +67,8 @@ def fused_mxfp4_moe(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Ten
 
     hidden_states [M, K] bf16 or fp16; w1 [E, 2 N, K / 2] (gate rows 0..N-1, up
     rows N..2N-1) and w2 [E, K, N / 2] codes with their scales; K and N
-    multiples of 32 up to 65536, at most 1024 experts.  topk_weights / topk_ids [M, topk]; expert_map: global id
-    -> local expert or -1.  Slots routed outside the local experts add nothing.
+    multiples of 32 up to 65536, at most 1024 experts.  topk_weights / topk_ids [M, topk] (FP32 and int32, or
+    other types of such values); expert_map: global id -> local expert or -1.  Slots routed outside the local experts add nothing.
     workspace: a dict that keeps the call's scratch; calls that share one must
     be on one stream.  (A captured call has scratch of its graph's own: a later
     call may replace the dict's by a larger one, the graph's has to stay.)
