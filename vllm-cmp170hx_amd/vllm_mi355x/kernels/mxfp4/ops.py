@@ -81,7 +81,7 @@ def fused_mxfp4_moe(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Ten
     out = output if output is not None else torch.empty_like(
         hidden_states, memory_format=torch.contiguous_format)
     need = ops.mxfp4_moe_workspace(hidden_states, w1, w2, ids)
-    if workspace is not None and torch.cuda.is_current_stream_capturing():
+    if workspace is not None and hidden_states.is_cuda and torch.cuda.is_current_stream_capturing():
         workspace = None
     scratch = None if workspace is None else workspace.get("mxfp4")
     if scratch is None or scratch.numel() < need or scratch.device != hidden_states.device:
