@@ -151,7 +151,8 @@ def test_linear_matches_the_oracle(mx, device, rows, k, n, dtype):
 
 @pytest.mark.parametrize("rows,k,n,out", [
     (1500, 288, 2200, torch.bfloat16), (1500, 320, 2205, torch.float32), (3600, 288, 3730, torch.bfloat16),
-    (3585, 512, 3704, torch.float32), (3600, 544, 3704, torch.float16), (1290, 800, 2304, torch.float16)])
+    (3585, 512, 3704, torch.float32), (3600, 544, 3704, torch.float16), (1290, 800, 2304, torch.float16),
+    (3600, 4128, 3733, torch.bfloat16), (3590, 2080, 3729, torch.float32)])
 def test_many_tiles(mx, device, rows, k, n, out):
     """Enough tiles of every size, ragged on each side, ends of k inside a stage."""
     print(f"tiles {rows}x{k}x{n} {out}", flush=True)

@@ -184,7 +184,6 @@ int launch_tile(const MatmulArgs& g, int splits, float* part, hipStream_t s) {
   t.blocks = g.blocks;
   t.out = splits > 1 ? part : g.out;
   t.out_dtype = splits > 1 ? int(vq::kFP32) : g.out_dtype;
-  t.wide = g.n % 8 == 0 && aligned(t.out, 16);
   t.tiles_n = int((g.n + 64 * kSize - 1) / (64 * kSize));
   t.tiles_m = int((g.rows + 64 * kSize - 1) / (64 * kSize));
   const int stages = (g.blocks + kStageBlocks - 1) / kStageBlocks;
@@ -217,16 +216,18 @@ constexpr int kCUs = 256;
 // `shared` per workgroup of a CU that is full; K splits write and read FP32 sums
 // at about 3 TB/s, in one more launch.  Fitted to the tile sizes and splits
 // measured at 24 to 4096 rows of 4096 x 14336, 14336 x 4096, 4096 x 4096 and
-// 2592 x 5003, of which it picks the fastest or one within 10%.
-double tile_cost(int size, bool deep, int64_t rows, int64_t n, int64_t stages, int64_t splits) {
-  const double alone = size == 4 ? 1.48 : size == 2 ? (deep ? 0.52 : 0.72) : 0.30;
-  const double shared = size == 4 ? 2.2 : size == 2 ? (deep ? 0.60 : 0.80) : 0.385;
+// 2592 x 5003, of which it picks the fastest or one within 10%.  `lines`: rows of codes
+// begin on 128-byte lines; the others' stages take longer, most of all the largest
+// tiles' (1500 rows of 2592 x 5003: 38 us, 26 on 128 x 128).
+double tile_cost(int size, bool deep, bool lines, int64_t rows, int64_t n, int64_t stages, int64_t splits) {
+  const double alone = size == 4 ? (lines ? 1.48 : 2.4) : size == 2 ? (deep ? 0.52 : 0.72) * (lines ? 1 : 1.12) : lines ? 0.30 : 0.33;
+  const double shared = (size == 4 ? 2.2 : size == 2 ? (deep ? 0.60 : 0.80) : 0.385) * (lines ? 1 : 1.25);
   const int64_t groups = ((n + 64 * size - 1) / (64 * size)) * ((rows + 64 * size - 1) / (64 * size)) * splits;
   // whole rounds where a CU holds one workgroup
   const bool one = size == 4 || deep;
   const double load = one ? double((groups + kCUs - 1) / kCUs) : double(groups) / kCUs;
   // (four buffers' workgroups gain nothing from each other over rounds)
-  const double each = one && groups < kCUs / 2 ? alone : std::max(alone, (deep && load > 1 ? 0.95 : shared) * load);
+  const double each = one && groups < kCUs / 2 ? alone : std::max(alone, (deep && load > 1 ? (lines ? 0.95 : 1.19) : shared) * load);
   const double sums = splits > 1 ? 3.0 + double(rows) * double(n) * 8.0 * double(splits) / 3e6 : 0.0;
   return double((stages + splits - 1) / splits) * each + sums;
 }
@@ -246,7 +247,7 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n) {
       const int size = kind == 3 ? 2 : kind;
       for (const int splits : {1, 2, 4, 8}) {
         if (splits > 1 && stages < 4 * splits) continue;
-        const double cost = tile_cost(size, kind == 3, rows, n, stages, splits);
+        const double cost = tile_cost(size, kind == 3, k % (2 * 128) == 0, rows, n, stages, splits);
         if (!p.tile || cost < best) {
           best = cost;
           p.tile = size;

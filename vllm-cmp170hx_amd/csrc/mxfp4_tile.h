@@ -66,7 +66,6 @@ struct TileArgs {
   int blocks;
   void* out;              // kDense: [rows][n] of out_dtype; kDown: FP32 [slots][n]
   int out_dtype;
-  int wide;               // kDense: n a multiple of eight, out 16-byte aligned
   int tiles_n, tiles_m;   // kDense: workgroups; else tiles_n alone
   int split_stages;       // kDense: stages of one split of K (gridDim.y splits, whose
                           // sums go to FP32 [split][rows][n] at out)
@@ -127,8 +126,9 @@ __device__ __forceinline__ void mfma32(f32x16_t& acc, const u32x4_t& a, uint32_t
   acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc, 4, 4, kSub, int(sa), kSub, int(sb));
 }
 
-// 32 rows of 32 kN columns from LDS to the output, eight columns a lane (n a
-// multiple of eight, rows 16-byte aligned).  slots (LDS): the rows' slots and their
+// 32 rows of 32 kN columns from LDS to the output, eight columns a lane, in 16-byte
+// stores whatever the rows' alignment (1500 x 2592 x 5003 on 128 x 128 tiles: 26 us,
+// with an element a store 33).  slots (LDS): the rows' slots and their
 // router weights, which multiply them.
 template <int kN, int kDtype>
 __device__ __forceinline__ void store_rows(const float* part, int stride, int lane, int mt, int nrows, int ct, const TileArgs& g,
@@ -150,15 +150,16 @@ __device__ __forceinline__ void store_rows(const float* part, int stride, int la
       weight = __builtin_bit_cast(float, slots[m].y);
     }
     const int64_t at = row * g.n + c;
-    if constexpr (kDtype == vq::kFP32) {
-      float* out = static_cast<float*>(g.out) + at;
-      *reinterpret_cast<f32x4_t*>(out) = lo * weight;
-      *reinterpret_cast<f32x4_t*>(out + 4) = hi * weight;
+    if (c + 8 > g.n) {  // the last columns
+      for (int q = 0; q < g.n - c; ++q) vq::store_act(g.out, kDtype, at + q, part[mr * stride + 8 * ch + q] * weight);
+    } else if constexpr (kDtype == vq::kFP32) {
+      const f32x4_t v[2] = {lo * weight, hi * weight};
+      __builtin_memcpy(static_cast<float*>(g.out) + at, v, 32);
     } else {
       u32x4_t w;
 #pragma unroll
       for (int q = 0; q < 4; ++q) w[q] = pack16<kDtype>((q < 2 ? lo : hi)[2 * (q & 1)], (q < 2 ? lo : hi)[2 * (q & 1) + 1]);
-      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(g.out) + at) = w;
+      __builtin_memcpy(static_cast<uint16_t*>(g.out) + at, &w, 16);
     }
   }
 }
@@ -498,21 +499,9 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
       const int mt = 32 * (kM * wm + i), ct = c0 + 32 * kN * wn;
       const int64_t o0 = kMode == kDense ? m0 + int64_t(blockIdx.y) * g.rows : m0;  // first output row
       if constexpr (kMode == kDense) {
-        if (g.wide) {
-          if (g.out_dtype == vq::kBF16) store_rows<kN, vq::kBF16>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
-          else if (g.out_dtype == vq::kFP16) store_rows<kN, vq::kFP16>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
-          else store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
-        } else {
-          // rows of any alignment: 64 consecutive elements a store, or fewer
-          constexpr int kSpan = 32 * kN < 64 ? 32 * kN : 64;
-          const int c = lane % kSpan;
-#pragma unroll 8
-          for (int k = 0; k < 32 * 32 * kN / 64; ++k) {
-            const int mr = k * 64 / (32 * kN) + (kSpan < 64 ? lane / kSpan : 0), cc = k * 64 % (32 * kN) + c;
-            const float v = part[mr * kStride + cc];
-            if (mt + mr < nrows && ct + cc < g.n) vq::store_act(g.out, g.out_dtype, (o0 + mt + mr) * g.n + ct + cc, v);
-          }
-        }
+        if (g.out_dtype == vq::kBF16) store_rows<kN, vq::kBF16>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
+        else if (g.out_dtype == vq::kFP16) store_rows<kN, vq::kFP16>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
+        else store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, o0, nullptr);
       } else {
         store_rows<kN, vq::kFP32>(part, kStride, lane, mt, nrows, ct, g, o0, slots);
       }
