@@ -638,8 +638,9 @@ int moe_expert_counts(const int32_t* topk_ids, const uint8_t* is_padding, int64_
  * loss = sum_e f_e P_e over the n counted rows: f_e = counts_e experts / (n
  * top_k), P_e the mean of p_te, p_t = softmax (scoring 0) of the row's logits or
  * their sigmoids divided by the sum of these (scoring 1).  A row whose logits
- * leave nothing (all -infinity) has p = 0; no counted row: loss 0.  Even load
- * gives 1.  logits [rows][experts] of dtype, row stride `stride`.  stats
+ * leave nothing has p = 0: all of them -infinity or, with scoring 1, below -708.396
+ * (sigmoids below 2^-1022; masks of a type's lowest value are).  A p below 2^-66 may
+ * count as 0.  No counted row: loss 0.  Even load gives 1.  logits [rows][experts] of dtype, row stride `stride`.  stats
  * [experts + 1]: f_e, then 1 / n (0 for n = 0), for moe_balance_grad.
  */
 int moe_balance_loss(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,

@@ -15,9 +15,10 @@
 //
 // come from the counts and the row alone.  The forward reads the logits once
 // and the backward once more (keeping the probabilities would write and read as
-// much).  A row whose logits leave nothing (all -inf, sigmoids that sum to 0)
-// has p = 0.  Counts are whole numbers, so their atomics give one result in any
-// order; the rows' parts are summed in 64 bits in a fixed order.
+// much).  A row whose logits leave nothing has p = 0: all of them -inf or, with
+// sigmoids, below kNothing.  A p below 2^-66 may count as 0.  Counts are whole
+// numbers, so their atomics give one result in any order; the rows' parts are
+// summed in 64 bits in a fixed order.
 //
 // Bound by the logits' bytes where rows are many: at 65536 rows of 256 in FP32 (64
 // MiB, 14 us at the rate of a large copy) the loss takes 17 us (sigmoids, with
@@ -80,15 +81,30 @@ __device__ __forceinline__ float lanes_max(float v, int lane) {
   return v;
 }
 
-// e^x for x <= 0: 2^y of y = x log2(e) as rounded, corrected by what the rounding
-// took (a relative error of 2^-22 whatever x; of y alone |x| 2^-24).
-__device__ __forceinline__ float exp_nonpositive(float x) {
-  constexpr float kLog2e = 1.44269504f, kLow = 1.925963033e-8f, kLn2 = 0.693147181f;
+constexpr float kLog2e = 1.44269504f;
+
+// A row whose logits all lie below it, masks among them, leaves nothing with
+// sigmoids: they are below 2^-1022, the smallest that 64 bits hold in full.
+constexpr float kNothing = -708.396f;
+
+// e^x / 2^k for x <= 0 and a whole k, 0 or at least x log2(e): 2^(y - k) of y = x
+// log2(e) as rounded (its difference to k is exact), corrected by what the rounding
+// took.  Off by 2^-22 of it whatever x (by y alone |x| 2^-24); 0 where it is below
+// 2^-126.
+__device__ __forceinline__ float exp_nonpositive(float x, float k = 0) {
+#pragma clang fp contract(off)  // (y - k is of the rounded y)
+  constexpr float kLow = 1.925963033e-8f, kLn2 = 0.693147181f;
   const float y = x * kLog2e;
-  float low = __builtin_fmaf(x, kLog2e, -y) + x * kLow;
-  low = x > -104.0f ? low : 0.0f;  // (infinities have no difference)
-  const float p = __builtin_amdgcn_exp2f(y);
+  float low = __builtin_fmaf(x, kLow, __builtin_fmaf(x, kLog2e, -y));
+  low = x > -2048.0f ? low : 0.0f;  // (infinities have no difference)
+  const float p = __builtin_amdgcn_exp2f(y - k);
   return __builtin_fmaf(p, low * kLn2, p);
+}
+
+// a b rounded by itself, whatever is added to it (r: the same in loss and gradient).
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
 }
 
 struct Rows {
@@ -138,22 +154,23 @@ __device__ __forceinline__ Values<S> load_row(const Rows& g, int64_t t, int l) {
   return o;
 }
 
-// From a row's logits its r = sum f p (in all its lanes), and in place of the
-// logits the slopes p (softmax) or p (1 - sigmoid).  f: LDS, zeros past the last
-// expert up to a whole step.
+template <typename S>
+__device__ __forceinline__ float row_max(const Values<S>& x, int lane) {
+  float m = x.v[0][0];
+#pragma unroll
+  for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, x.v[i][j]);
+  return lanes_max<S::kLanes>(m, lane);
+}
+
+// A row's r from z = e^l / e^shift (softmax) or the sigmoid / 2^shift, and `sum`, z's
+// sum (both in all its lanes); in place of the logits the slopes p (softmax) or p (1 -
+// sigmoid).
 template <typename S, bool kSigmoid>
-__device__ __forceinline__ float row_terms(Values<S>& x, const float* f, int l, int lane) {
-  float m = 0;
-  if constexpr (!kSigmoid) {
-    m = x.v[0][0];
-#pragma unroll
-    for (int i = 0; i < S::kSteps; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) m = fmaxf(m, x.v[i][j]);
-    m = lanes_max<S::kLanes>(m, lane);
-    if (m == -__builtin_inff()) m = 0;
-  }
-  float sum = 0, dot = 0;
+__device__ __forceinline__ float shifted_terms(Values<S>& x, const float* f, int l, int lane, float shift, float& sum) {
+  float dot = 0;
+  sum = 0;
 #pragma unroll
   for (int i = 0; i < S::kSteps; ++i) {
     typedef float f4_t __attribute__((ext_vector_type(4)));
@@ -162,13 +179,14 @@ __device__ __forceinline__ float row_terms(Values<S>& x, const float* f, int l, 
     for (int j = 0; j < 4; ++j) {
       float z;
       if constexpr (kSigmoid) {
+        const float a = x.v[i][j], u = exp_nonpositive(-fabsf(a), shift), t = __builtin_amdgcn_ldexpf(u, int(shift));
         // (the reciprocal of 1 .. 2 as the hardware rounds it, off by one step at most)
-        const float a = x.v[i][j], t = exp_nonpositive(-fabsf(a)), large = __builtin_amdgcn_rcpf(1 + t), small = t * large;
+        const float large = __builtin_amdgcn_rcpf(1 + t), small = u * large;
         z = a >= 0 ? large : small;
         x.v[i][j] = large * small;
         if (a != a) z = x.v[i][j] = a;
       } else {
-        z = x.v[i][j] = exp_nonpositive(x.v[i][j] - m);
+        z = x.v[i][j] = exp_nonpositive(x.v[i][j] - shift);
       }
       sum += z;
       dot = __builtin_fmaf(w[j], z, dot);
@@ -181,7 +199,35 @@ __device__ __forceinline__ float row_terms(Values<S>& x, const float* f, int l, 
   for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) x.v[i][j] *= inv;
-  return dot * inv;
+  return product(dot, inv);
+}
+
+// From a row's logits its r = sum f p (in all its lanes), and in place of the
+// logits the slopes.  f: LDS, zeros past the last expert up to a whole step.
+// again(): the logits once more.
+template <typename S, bool kSigmoid, typename Again>
+__device__ __forceinline__ float row_terms(Values<S>& x, const float* f, int l, int lane, const Again& again) {
+  float sum;
+  if constexpr (kSigmoid) {
+    float r = shifted_terms<S, true>(x, f, l, lane, 0.0f, sum);
+    // A row of tiny sigmoids alone (logits below -41) holds them over 2^k, about the
+    // largest: p does not change by that, and none of weight is lost below 2^-126.
+    // Such rows are read and computed again: 65536 of 256 cost the loss 41 us for 27, so
+    // that rows in whose sums those below 2^-126 weigh nothing are left as they are;
+    // their logits kept in registers would cost all rows a microsecond.
+    const bool small = sum < 0x1p-60f;
+    if (__builtin_expect(__any(small), 0)) {
+      x = again();
+      const float m = row_max(x, lane);
+      const float k = small && m < 0 && m >= kNothing ? __builtin_ceilf(m * kLog2e) : 0.0f;
+      r = shifted_terms<S, true>(x, f, l, lane, k, sum);
+    }
+    return r;
+  } else {
+    float m = row_max(x, lane);
+    if (m == -__builtin_inff()) m = 0;
+    return shifted_terms<S, false>(x, f, l, lane, m, sum);
+  }
 }
 
 // ---- counts ---------------------------------------------------------------------------
@@ -281,7 +327,7 @@ __device__ __forceinline__ double sum_rows(const Rows& g, int64_t first, int64_t
       next = row(t + step);
       next_mark = mark(t + step);
     }
-    const float r = row_terms<S, kSigmoid>(x, f, l, lane);
+    const float r = row_terms<S, kSigmoid>(x, f, l, lane, [&] { return row(t); });
     if (counted && l == 0) sum += r;
   }
   return sum;
@@ -384,8 +430,9 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Rows g, const float* sta
   for (int64_t t0 = (int64_t(blockIdx.x) * kWaves + wave) * S::kRows; t0 < g.rows; t0 += int64_t(gridDim.x) * kWaves * S::kRows) {
     const int64_t t = t0 + sub;
     const bool counted = t < g.rows && !(g.padding && g.padding[min(t, g.rows - 1)]);
-    Values<S> x = load_row<S, kDtype>(g, t < g.rows ? t : g.rows - 1, l);
-    const float r = row_terms<S, kSigmoid>(x, f, l, lane);
+    const auto row = [&] { return load_row<S, kDtype>(g, t < g.rows ? t : g.rows - 1, l); };
+    Values<S> x = row();
+    const float r = row_terms<S, kSigmoid>(x, f, l, lane, row);
     if (t >= g.rows) continue;
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i) {
