@@ -47,9 +47,13 @@ constexpr int kMaxParts = 32;
 constexpr int kLossThreads = 1024, kLossWaves = kLossThreads / 64;
 constexpr int kMaxGroups = 512;  // workgroups of the loss: two a CU, few enough to add up the counts
 constexpr int kGradGroups = 2048;
-// Calls of up to so many logits run in one workgroup and launch (200 rows of 128:
-// the launches cost more than the rows).
+// Calls of up to so many logits, whose rows a workgroup takes in up to so many steps
+// (of one, two or four rows a wavefront), run in one workgroup and launch: a step
+// costs 0.9 us, the launches of the others 12 whatever their rows.  In us, one workgroup
+// and several: 512 rows of 8 12.1 and 12.7, 1024 18.9 and 12.7, 4096 59.7 and 12.7; 256
+// rows of 128 11.4 and 11.8; 128 rows of 256 11.1 and 12.2.
 constexpr int kOneLogits = 1 << 15;
+constexpr int kOneSteps = 8;
 
 // ---- a row of logits in the lanes of a wavefront ----------------------------------
 
@@ -560,7 +564,7 @@ extern "C" int moe_balance_loss(const void* logits, int dtype, int64_t rows, int
   const Counting c{topk_ids, is_padding, rows, int(top_k), int(experts)};
   const Rows g = rows_of(logits, dtype, rows, experts, stride, is_padding);
   const Results out{loss, counts, stats};
-  if (rows * experts <= kOneLogits) {
+  if (rows * experts <= kOneLogits && rows <= kOneSteps * 16 * rows_at_once(experts)) {
     return dispatch(experts, dtype, scoring == 1, [&](auto shape, auto type, auto sigmoid) {
       hipLaunchKernelGGL((one_kernel<decltype(shape), decltype(type)::value, decltype(sigmoid)::value>), dim3(1), dim3(1024), 0, s, g, c, out);
     });
