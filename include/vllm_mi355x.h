@@ -589,6 +589,12 @@ int mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, int64_t rows, int64_
                  const uint8_t* w, const uint8_t* w_scales, int64_t n, void* out, int out_dtype,
                  void* workspace, int64_t workspace_bytes, void* stream);
 
+/* How the two products run at a size, for tests: plan[0] the tile's rows and
+ * columns (0: the few rows' kernel), plan[1] its stage buffers, plan[2] the K splits;
+ * of the few rows' kernel plan[3] a workgroup's column tiles, plan[4] its parts of K,
+ * plan[5] whether mxfp4_linear quantizes x in it. */
+int mxfp4_matmul_plan(int64_t rows, int64_t k, int64_t n, int32_t* plan);
+
 /*
  * mxfp4_matmul of x as mxfp4_quantize quantizes it (x [rows][k] of VQ_BF16,
  * VQ_FP16 or VQ_FP32, row stride x_stride): the same codes, products and

@@ -448,6 +448,20 @@ extern "C" int64_t mxfp4_matmul_workspace_size(int64_t rows, int64_t k, int64_t 
   return split_bytes(plan_of(rows, k, n), rows, n);
 }
 
+extern "C" int mxfp4_matmul_plan(int64_t rows, int64_t k, int64_t n, int32_t* plan) {
+  using namespace mx;
+  if (!plan) return vq::fail("mxfp4: null pointer");
+  if (mxfp4_matmul_workspace_size(rows, k, n) < 0) return vq::kInvalidArgument;
+  const Plan p = plan_of(rows, k, n);
+  plan[0] = 64 * p.tile;
+  plan[1] = p.tile == 1 || p.deep ? 4 : p.tile ? 2 : 0;
+  plan[2] = p.splits;
+  plan[3] = p.cols;
+  plan[4] = p.parts;
+  plan[5] = p.fused;
+  return vq::kOk;
+}
+
 extern "C" int64_t mxfp4_linear_workspace_size(int64_t rows, int64_t k, int64_t n) {
   using namespace mx;
   if (rows < 0 || n < 0 || k <= 0 || k % kBlock != 0 || !sane(rows, k) || !sane(rows, n)) {

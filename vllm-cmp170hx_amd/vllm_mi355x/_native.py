@@ -148,6 +148,7 @@ SIGNATURES = {
         c_vp, c_vp, c_i64, c_vp, c_int,          # w, w_scales, n, out, out_dtype
         c_vp, c_i64, c_vp,                       # workspace, bytes, stream
     ]),
+    "mxfp4_matmul_plan": (c_int, [c_i64, c_i64, c_i64, c_vp]),
     "mxfp4_linear_workspace_size": (c_i64, [c_i64, c_i64, c_i64]),
     "mxfp4_linear": (c_int, [
         c_vp, c_int, c_i64, c_i64, c_i64,        # x, x_dtype, rows, k, x_stride
