@@ -216,7 +216,7 @@ constexpr int kCUs = 256;
 // `shared` per workgroup of a CU that is full; K splits write and read FP32 sums
 // at about 3 TB/s, in one more launch.  Fitted to the tile sizes and splits
 // measured at 24 to 4096 rows of 4096 x 14336, 14336 x 4096, 4096 x 4096 and
-// 2592 x 5003, of which it picks the fastest or one within 10%.  `lines`: rows of codes
+// 2592 x 5003: at 52 sizes the fastest, or one within 12% of it, is picked.  `lines`: rows of codes
 // begin on 128-byte lines; the others' stages take longer, most of all the largest
 // tiles' (1500 rows of 2592 x 5003: 38 us, 26 on 128 x 128).
 double tile_cost(int size, bool deep, bool lines, int64_t rows, int64_t n, int64_t stages, int64_t splits) {
@@ -240,7 +240,8 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n) {
                      ((n + 63) / 64) * ((rows + 63) / 64) <= INT_MAX / 8;
   // A group of 16 rows reads the weights once more, from L2: 20 rows of 2592 x
   // 5003 10.6 us (tiles 13.0), 64 rows 11.4 (13.9), but 20 rows of 4096 x 14336
-  // 20.9 (15.3).
+  // 20.9 (15.3).  Near the border the product alone may lose a fifth by it (40 rows
+  // of 4096 x 4096 10.2, on tiles 8.4).
   if (tiles && (rows > 64 || (rows + 15) / 16 * double(n) * double(k) > 64e6)) {
     double best = 0;
     for (const int kind : {1, 2, 3, 4}) {  // 3: size 2 with four buffers

@@ -37,11 +37,11 @@ def moe_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, scoring: str 
     mark, P_e the mean of the rows' probabilities: softmax of the logits, or
     (scoring "sigmoid") their sigmoids over the row's sum.  counts: int64 [E].
 
-    Differentiable once in the logits (bf16, fp16 or fp32, any row stride), in
-    reverse mode (a forward-mode tangent raises); the counts are constants.  A row
-    whose logits are all -inf (with sigmoids: below -708.396, masks of the type's
-    lowest value among them) adds nothing.  To capture a backward pass into a graph,
-    let go of eager losses of the same leaves first, as for any operator of torch."""
+    Differentiable once in the logits (bf16, fp16 or fp32; rows in one stride, not
+    overlapping), in reverse mode (a forward-mode tangent raises); the counts are
+    constants.  A row whose logits are all -inf (with sigmoids: below -708.396, masks of
+    the type's lowest value among them) adds nothing.  To capture a backward pass into a
+    graph, let go of eager losses of the same leaves first, as for any operator of torch."""
     if scoring not in _SCORING:
         raise ValueError(f"unknown scoring {scoring!r}")
     _native.load_torch()
