@@ -580,7 +580,7 @@ int mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, 
 /*
  * out [rows][n] = RN_out(sum_k a[r][k] w[n][k]) of MXFP4 a [rows][k] and w
  * [n][k], products exact and summed in FP32 on the matrix cores.  The order
- * of the sums, and so the last bits, depend on rows, k and n alone.
+ * of the sums, and so the last bits, depend on rows, k and n alone.  k up to 2^32.
  * workspace: mxfp4_matmul_workspace_size(rows, k, n) bytes, 16-byte aligned
  * (null where that is 0), used by one call at a time.
  */

@@ -346,12 +346,16 @@ bool sane(int64_t rows, int64_t cols) {
   return rows >= 0 && cols >= 0 && (rows == 0 || cols <= (int64_t(1) << 60) / std::max<int64_t>(rows, 1));
 }
 
+// The longest sum of a product: a row's blocks, and what the kernels count in them, fit
+// 32 bits.
+constexpr int64_t kMaxK = int64_t(1) << 32;
+
 bool known_dtype(int dtype) { return dtype == vq::kBF16 || dtype == vq::kFP16 || dtype == vq::kFP32; }
 
 int check_product(int64_t rows, int64_t k, int64_t n, const uint8_t* w, const uint8_t* w_scales, int out_dtype, const void* out) {
   if (!known_dtype(out_dtype)) return vq::fail("mxfp4: out must be BF16, FP16 or FP32");
   if (rows < 0 || n < 0 || k <= 0 || k % kBlock != 0) return vq::fail("mxfp4: k must be a positive multiple of 32");
-  if (!sane(rows, k) || !sane(n, k) || !sane(rows, n)) return vq::fail("mxfp4: sizes out of range");
+  if (k > kMaxK || !sane(rows, k) || !sane(n, k) || !sane(rows, n)) return vq::fail("mxfp4: sizes out of range");
   if (rows == 0 || n == 0) return vq::kOk;
   if (!w || !w_scales || !out) return vq::fail("mxfp4: null pointer");
   if (!aligned(w, 16)) return vq::fail("mxfp4: codes must be 16-byte aligned");
@@ -442,8 +446,8 @@ extern "C" int mxfp4_matmul(const uint8_t* a, const uint8_t* a_scales, int64_t r
 
 extern "C" int64_t mxfp4_matmul_workspace_size(int64_t rows, int64_t k, int64_t n) {
   using namespace mx;
-  if (rows < 0 || n < 0 || k <= 0 || k % kBlock != 0 || !sane(rows, k) || !sane(rows, n)) {
-    vq::fail("mxfp4: k must be a positive multiple of 32, sizes not negative");
+  if (rows < 0 || n < 0 || k <= 0 || k % kBlock != 0 || k > kMaxK || !sane(rows, k) || !sane(rows, n)) {
+    vq::fail("mxfp4: k must be a positive multiple of 32 up to 2^32, sizes not negative");
     return -1;
   }
   return split_bytes(plan_of(rows, k, n), rows, n);
@@ -465,8 +469,8 @@ extern "C" int mxfp4_matmul_plan(int64_t rows, int64_t k, int64_t n, int32_t* pl
 
 extern "C" int64_t mxfp4_linear_workspace_size(int64_t rows, int64_t k, int64_t n) {
   using namespace mx;
-  if (rows < 0 || n < 0 || k <= 0 || k % kBlock != 0 || !sane(rows, k) || !sane(rows, n)) {
-    vq::fail("mxfp4: k must be a positive multiple of 32, sizes not negative");
+  if (rows < 0 || n < 0 || k <= 0 || k % kBlock != 0 || k > kMaxK || !sane(rows, k) || !sane(rows, n)) {
+    vq::fail("mxfp4: k must be a positive multiple of 32 up to 2^32, sizes not negative");
     return -1;
   }
   const Plan p = plan_of(rows, k, n);
