@@ -631,6 +631,7 @@ int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, co
  * Up to 1024 experts; rows with is_padding[t] != 0 (optional uint8 [rows]) are
  * left out.  No counterparts in the reference.  workspace:
  * moe_balance_workspace_size bytes, 8-byte aligned, used by one call at a time.
+ * Arrays lie on their elements and outputs overlap no other (but for grad, below).
  */
 int64_t moe_balance_workspace_size(int64_t rows, int64_t experts);
 
@@ -654,9 +655,9 @@ int moe_balance_loss(const void* logits, int dtype, int64_t rows, int64_t expert
                      int scoring, float* loss, int64_t* counts, float* stats, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
-/* grad [rows][experts] (contiguous, of the logits' dtype, aligned to four elements)
- * = upstream[0] *
- * dloss/dlogits with the counts constant, zeros in padding rows. */
+/* grad [rows][experts] (contiguous, of the logits' dtype, aligned to four elements; it
+ * may be contiguous logits) = upstream[0] * dloss/dlogits with the counts constant,
+ * zeros in padding rows. */
 int moe_balance_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,
                      const uint8_t* is_padding, int scoring, const float* stats,
                      const float* upstream, void* grad, void* stream);

@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/vllm_mi355x.h"
@@ -530,6 +531,33 @@ int check_logits(const void* logits, int dtype, int64_t rows, int64_t experts, i
 
 bool aligned8(const void* p) { return reinterpret_cast<uintptr_t>(p) % 8 == 0; }
 
+// A call's arrays: no output may overlap another array, and each lies on its elements.
+struct Span {
+  const void* p;
+  int64_t bytes, element;
+};
+int check_spans(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  for (const Span* a = outputs.begin(); a != outputs.end(); ++a) {
+    for (const Span* b = outputs.begin(); b != a; ++b) {
+      if (vq::overlaps(a->p, a->bytes, b->p, b->bytes)) return vq::fail("moe balance: arguments must not overlap");
+    }
+    for (const Span& b : inputs) {
+      if (vq::overlaps(a->p, a->bytes, b.p, b.bytes)) return vq::fail("moe balance: arguments must not overlap");
+    }
+  }
+  for (const auto* list : {&outputs, &inputs}) {
+    for (const Span& a : *list) {
+      if (reinterpret_cast<uintptr_t>(a.p) % uintptr_t(a.element)) return vq::fail("moe balance: misaligned pointer");
+    }
+  }
+  return vq::kOk;
+}
+
+// Bytes from the first logit to the last.
+int64_t logits_bytes(int dtype, int64_t rows, int64_t experts, int64_t stride) {
+  return rows > 0 ? ((rows - 1) * stride + experts) * vq::dtype_bytes(dtype) : 0;
+}
+
 }  // namespace
 }  // namespace balance
 
@@ -545,6 +573,10 @@ extern "C" int moe_expert_counts(const int32_t* topk_ids, const uint8_t* is_padd
   if (int rc = check_sizes(rows, experts, top_k)) return rc;
   if (!counts || !workspace || (rows > 0 && !topk_ids)) return vq::fail("moe balance: null pointer");
   if (workspace_bytes < Workspace::bytes(experts) || !aligned8(workspace)) return vq::fail("moe balance: workspace too small or misaligned");
+  if (int rc = check_spans({{counts, experts * 8, 8}, {workspace, Workspace::bytes(experts), 8}},
+                           {{topk_ids, rows * top_k * 4, 4}, {is_padding, rows, 1}})) {
+    return rc;
+  }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Workspace w(workspace);
   if (int rc = launch_count({topk_ids, is_padding, rows, int(top_k), int(experts)}, w, s)) return rc;
@@ -560,6 +592,11 @@ extern "C" int moe_balance_loss(const void* logits, int dtype, int64_t rows, int
   if (int rc = check_logits(logits, dtype, rows, experts, stride, scoring)) return rc;
   if (!loss || !counts || !stats || !workspace || (rows > 0 && !topk_ids)) return vq::fail("moe balance: null pointer");
   if (workspace_bytes < Workspace::bytes(experts) || !aligned8(workspace)) return vq::fail("moe balance: workspace too small or misaligned");
+  if (int rc = check_spans({{loss, 4, 4}, {counts, experts * 8, 8}, {stats, (experts + 1) * 4, 4}, {workspace, Workspace::bytes(experts), 8}},
+                           {{logits, logits_bytes(dtype, rows, experts, stride), vq::dtype_bytes(dtype)},
+                            {topk_ids, rows * top_k * 4, 4}, {is_padding, rows, 1}})) {
+    return rc;
+  }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Counting c{topk_ids, is_padding, rows, int(top_k), int(experts)};
   const Rows g = rows_of(logits, dtype, rows, experts, stride, is_padding);
@@ -590,6 +627,14 @@ extern "C" int moe_balance_grad(const void* logits, int dtype, int64_t rows, int
   if (rows == 0) return vq::kOk;
   if (!stats || !upstream || !grad) return vq::fail("moe balance: null pointer");
   if (reinterpret_cast<uintptr_t>(grad) % (4 * vq::dtype_bytes(dtype))) return vq::fail("moe balance: grad must be aligned to four elements");
+  // (in place of contiguous logits a row is read whole before it is written)
+  const bool in_place = grad == logits && (rows == 1 || stride == experts);
+  if (int rc = check_spans({{grad, rows * experts * vq::dtype_bytes(dtype), 1}},
+                           {{in_place ? nullptr : logits, logits_bytes(dtype, rows, experts, stride), 1}, {is_padding, rows, 1},
+                            {stats, (experts + 1) * 4, 4}, {upstream, 4, 4}})) {
+    return rc;
+  }
+  if (reinterpret_cast<uintptr_t>(logits) % uintptr_t(vq::dtype_bytes(dtype))) return vq::fail("moe balance: misaligned pointer");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Rows g = rows_of(logits, dtype, rows, experts, stride, is_padding);
   const unsigned groups = unsigned(groups_of(rows, experts, kWaves, kGradGroups));

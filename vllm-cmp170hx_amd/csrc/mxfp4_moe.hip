@@ -515,7 +515,7 @@ extern "C" int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x
     return vq::fail("mxfp4 moe: null pointer");
   }
   if (!aligned(w13, 16) || !aligned(w2, 16)) return vq::fail("mxfp4 moe: codes must be 16-byte aligned");
-  if (!aligned(x, 2) || !aligned(out, 2) || !aligned(topk_ids, 4) || !aligned(topk_w, 4)) return vq::fail("mxfp4 moe: misaligned pointer");
+  if (!aligned(x, 2) || !aligned(out, 2) || !aligned(topk_ids, 4) || !aligned(topk_w, 4) || !aligned(expert_map, 4)) return vq::fail("mxfp4 moe: misaligned pointer");
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16)) return vq::fail("mxfp4 moe: workspace too small or not 16-byte aligned");
   const int64_t slots = tokens * top_k, codes = experts * inter * hidden;  // of w13, bytes
   for (const auto& other : {std::pair<const void*, int64_t>{x, ((tokens - 1) * x_stride + hidden) * 2}, {w13, codes}, {s13, codes / 16},

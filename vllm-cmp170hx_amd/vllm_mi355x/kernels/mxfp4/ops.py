@@ -3,9 +3,10 @@ a byte, the even element in the low nibble) under one E8M0 scale byte.
 
 A packed tensor [..., k] is a pair of contiguous uint8 tensors: codes
 [..., k / 2] and scales [..., k / 32].  k is a multiple of 32 (up to 2^32 in
-products); every other size is free.  Outputs and scratch come from torch's allocator on the current stream,
-so calls on several streams, and captured ones, do not share memory (the fused
-MoE's workspace aside, which is the caller's).  Failed checks raise RuntimeError.
+products); every other size is free.  Outputs and scratch come from torch's
+allocator on the current stream, so calls on several streams, and captured ones,
+do not share memory (the fused MoE's workspace aside, which is the caller's).
+Failed checks raise RuntimeError.
 These are operators for inference: outputs carry no gradient.
 """
 
