@@ -1,5 +1,6 @@
 """The fused MXFP4 MoE where a task's rows just fit LDS, or just do not: tasks of 16
-rows and a few more, of rows up to 7168 elements and above.  Tolerance as the oracle
+rows and a few more, of rows up to 7168 elements and above; and few tokens whose slots are
+many to an expert, or more than a workgroup lists.  Tolerance as the oracle
 gives it, then half a step of the type."""
 
 import numpy as np
@@ -19,7 +20,9 @@ def mx():
 
 @pytest.mark.parametrize("experts,hidden,inter,topk,tokens", [(2, 6656, 32, 1, 40), (2, 7168, 32, 1, 40), (2, 7200, 32, 1, 40),
                                                               (1, 7168, 64, 1, 16), (1, 7168, 64, 1, 17), (2, 64, 7168, 2, 33),
-                                                              (3, 6688, 32, 2, 700), (40, 7168, 32, 8, 8)])
+                                                              (3, 6688, 32, 2, 700), (40, 7168, 32, 8, 8),
+                                                              # tiles for few tokens, many to an expert; long lists of few tokens
+                                                              (4, 256, 288, 4, 12), (2, 512, 256, 2, 16), (200, 64, 32, 100, 12)])
 def test_rows_that_just_fit(mx, device, experts, hidden, inter, topk, tokens):
     print(f"moe rows E={experts} H={hidden} I={inter} k={topk} T={tokens}", flush=True)
     rng = np.random.default_rng(hidden + tokens)
