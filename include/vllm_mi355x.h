@@ -627,6 +627,37 @@ int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, co
               const int32_t* expert_map, int64_t map_size, int64_t hidden, int64_t inter,
               float limit, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- routing from logits ---------------------------------------------------------
+ * No counterparts in the reference (moe_route's selection is of its own logits, without
+ * groups or gradient).  Up to 1024 experts, 64 slots a row, 64 groups.
+ */
+
+/*
+ * topk_weights / topk_ids [rows][top_k]: each row's experts and their weights from its
+ * logits [rows][experts] of dtype, row stride `stride`.  Score: softmax (scoring 0) or
+ * sigmoid (1); key: score + bias (FP32 [experts]), in 64 bits, or without a bias
+ * (null) the logit.  groups > 1: of `groups` runs of equally many experts the
+ * topk_groups best stay open, a group's score being its largest key or, with a bias,
+ * the sum of its two largest.  The top_k largest keys, largest first, equals by the
+ * lower number.  Weights: scale times the score, or with renormalize its share of the
+ * chosen ones' sum.  Not chosen: experts 708.396 or more below 0 (softmax: below the
+ * row's largest logit), -infinity among them, or with a bias of -infinity or NaN; slots
+ * left over hold -1 and weight 0, as rows with is_padding[t] != 0 (optional uint8
+ * [rows]) do, whose logits are not looked at.  A row with a NaN (softmax: or
+ * +infinity) has weights NaN, its experts chosen without that one.
+ */
+int moe_route_logits(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,
+                     const float* bias, int64_t top_k, int64_t groups, int64_t topk_groups,
+                     int scoring, int renormalize, float scale, const uint8_t* is_padding,
+                     float* topk_weights, int32_t* topk_ids, void* stream);
+
+/* grad [rows][experts] (contiguous, of the logits' dtype, aligned to four elements) =
+ * the gradient in the logits of sum upstream topk_weights (FP32 [rows][top_k]), the
+ * choice constant; weights and ids as moe_route_logits gave them. */
+int moe_route_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,
+                   const float* topk_weights, const int32_t* topk_ids, int64_t top_k, int scoring,
+                   int renormalize, float scale, const float* upstream, void* grad, void* stream);
+
 /* ---- a router's load -----------------------------------------------------------
  * Up to 1024 experts; rows with is_padding[t] != 0 (optional uint8 [rows]) are
  * left out.  No counterparts in the reference.  workspace:

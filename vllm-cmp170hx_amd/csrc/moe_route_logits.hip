@@ -1,0 +1,662 @@
+// Routing from a router's logits: the experts of each row, by groups where asked, and
+// their weights, with the weights' gradient.
+//
+// s_e is the softmax or the sigmoid of the row's logit l_e, the key of an expert its
+// score plus its bias; without a bias the logit orders as its score does and is the
+// key.  A group of consecutive experts scores its largest key, with a bias its two
+// largest's sum; the best groups stay open, and of their experts the best are chosen,
+// always the lower number of equals.  Over the chosen (c the scale)
+//
+//   w_j = c s_j, or renormalized c s_j / S, S their sum,
+//
+// and with g the weights' gradient, the choice constant, d_e = dL/dl_e:
+//
+//   softmax, renormalized:  w_e (g_e - sum_j w_j g_j / c)            of chosen experts
+//   sigmoid, renormalized:  w_e (1 - s_e) (g_e - sum_j w_j g_j / c)
+//   sigmoid:                w_e (1 - s_e) g_e
+//   softmax:                [chosen] w_e g_e - s_e sum_j w_j g_j     of all experts.
+//
+// An expert is masked, and not chosen, where its score is below 2^-1022 of the
+// largest possible (logits 708.396 below 0 or, for softmax, the row's largest; -inf
+// among them) or its bias is -inf or NaN.  Slots left over hold -1 and weight 0.  A row
+// with a NaN (softmax: or +inf) has weights NaN, its experts chosen without that one.
+//
+// Keys with a bias are FP32 sums, off by up to 2^-20; where two that decide the
+// choice or its order lie closer than their errors, the wavefront's rows are keyed and
+// chosen again in 64 bits, so that the choice is always that of 64-bit keys.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <initializer_list>
+#include <type_traits>
+
+#include "../../include/vllm_mi355x.h"
+#include "common.h"
+#include "moe_logits.h"
+
+namespace route {
+namespace {
+
+using logits::exp_nonpositive;
+using logits::kLog2e;
+using logits::kNothing;
+using logits::lanes_max;
+using logits::lanes_sum;
+using logits::load_row;
+using logits::Rows;
+using logits::Shape;
+using logits::Values;
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxSlots = 64;   // a lane a slot
+constexpr int kMaxGroups = 64;  // a bit a group
+constexpr unsigned kMaxGrid = 2048;
+
+struct Choice {
+  const float* bias;
+  int top_k, groups, topk_groups;  // groups 1: none
+  int group_experts;
+  int group_lanes;  // lanes that hold a group in one step, a power of two; 0: groups lie otherwise
+  bool renormalize;
+  float scale;
+  float* weights;
+  int32_t* ids;
+};
+
+__device__ __forceinline__ float minus_inf() { return -__builtin_inff(); }
+
+template <int d>
+__device__ __forceinline__ int xor_int(int v, int lane) {
+  return __builtin_bit_cast(int, vq::xor_lanes<d>(__builtin_bit_cast(float, v), lane));
+}
+template <int d>
+__device__ __forceinline__ float xor_key(float v, int lane) { return vq::xor_lanes<d>(v, lane); }
+template <int d>
+__device__ __forceinline__ double xor_key(double v, int lane) { return __shfl_xor(v, d); }
+
+template <int kLanes>
+__device__ __forceinline__ int lanes_min(int v, int lane) {
+  if constexpr (kLanes > 32) v = min(v, xor_int<32>(v, lane));
+  if constexpr (kLanes > 16) v = min(v, xor_int<16>(v, lane));
+  v = min(v, xor_int<8>(v, lane));
+  v = min(v, xor_int<4>(v, lane));
+  v = min(v, xor_int<2>(v, lane));
+  return min(v, xor_int<1>(v, lane));
+}
+__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
+template <int kLanes, typename Key>
+__device__ __forceinline__ Key keys_max(Key v, int lane) {
+  if constexpr (kLanes > 32) v = larger(v, xor_key<32>(v, lane));
+  if constexpr (kLanes > 16) v = larger(v, xor_key<16>(v, lane));
+  v = larger(v, xor_key<8>(v, lane));
+  v = larger(v, xor_key<4>(v, lane));
+  v = larger(v, xor_key<2>(v, lane));
+  return larger(v, xor_key<1>(v, lane));
+}
+
+// The two largest of a run of keys.
+template <typename Key>
+struct Top2 {
+  Key first, second;
+  __device__ __forceinline__ void add(Key k) {
+    second = larger(second, smaller(first, k));
+    first = larger(first, k);
+  }
+  template <int d>
+  __device__ __forceinline__ void join(int lane) {
+    const Key a = xor_key<d>(first, lane), b = xor_key<d>(second, lane);
+    second = larger(smaller(first, a), larger(second, b));
+    first = larger(first, a);
+  }
+};
+
+// What lies in LDS for groups that do not fill whole lanes of a step: the
+// wavefront's rows of keys, and the groups of four neighbouring experts, a byte each.
+template <typename S>
+struct GroupSpace {
+  static constexpr int kPadded = 4 * S::kLanes * S::kSteps;
+  double* keys;            // [kRows][kPadded], FP32 ones in its first half
+  const uint32_t* group4;  // [kPadded / 4]
+};
+
+// Keys of closed groups become -inf.  error: what an FP32 key may be off by at most,
+// apart from its own rounding; doubt: set where it may decide (64-bit keys: never).
+template <typename S, bool kTwo, typename Key>
+__device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Choice& c, const GroupSpace<S>& space, int l, int lane,
+                                             float error, bool& doubt) {
+  const Key none = minus_inf();
+  const bool in_lanes = c.group_lanes > 0;
+  Key score[S::kSteps];
+  float size = 0;  // of the keys that scores are made of
+  const auto finish = [&](const Top2<Key>& t) {
+    if constexpr (std::is_same<Key, float>::value && kTwo) {
+      const float a = fabsf(t.first), b = fabsf(t.second);
+      size = fmaxf(size, fmaxf(a < __builtin_inff() ? a : 0.0f, b < __builtin_inff() ? b : 0.0f));
+    }
+    return kTwo && t.second > none ? t.first + t.second : t.first;
+  };
+  const int shift = in_lanes ? __builtin_ctz(c.group_lanes) : 0;
+  const auto group_at = [&](int i) { return in_lanes ? (S::kLanes * i + l) >> shift : l; };
+  if (in_lanes) {
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) {
+      Top2<Key> t{key[i][0], none};
+#pragma unroll
+      for (int j = 1; j < 4; ++j) t.add(key[i][j]);
+      if (c.group_lanes > 1) t.template join<1>(lane);
+      if (c.group_lanes > 2) t.template join<2>(lane);
+      if (c.group_lanes > 4) t.template join<4>(lane);
+      if (c.group_lanes > 8) t.template join<8>(lane);
+      if constexpr (S::kLanes > 16) {
+        if (c.group_lanes > 16) t.template join<16>(lane);
+      }
+      if constexpr (S::kLanes > 32) {
+        if (c.group_lanes > 32) t.template join<32>(lane);
+      }
+      score[i] = finish(t);
+    }
+  } else {
+    // lane g takes group g, its keys from LDS (each lane from a place of its own on)
+    Key* rows = reinterpret_cast<Key*>(space.keys);
+    Key* row = rows + (lane / S::kLanes) * GroupSpace<S>::kPadded;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) row[4 * (S::kLanes * i + l) + j] = key[i][j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    Top2<Key> t{none, none};
+    if (l < c.groups) {
+      int at = l % c.group_experts;
+      for (int n = 0; n < c.group_experts; ++n) {
+        t.add(row[l * c.group_experts + at]);
+        at = at + 1 == c.group_experts ? 0 : at + 1;
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) score[i] = none;
+    score[0] = finish(t);
+  }
+  float tolerance = 0;
+  if constexpr (std::is_same<Key, float>::value && kTwo) {
+    // four keys decide between two scores, each off by its error and half a step
+    tolerance = 4 * error + lanes_max<S::kLanes>(size, lane) * 0x1p-21f;
+  }
+  uint64_t open = 0;
+  Key last = none;
+  for (int q = 0;; ++q) {
+    Key m = score[0];
+#pragma unroll
+    for (int i = 1; i < S::kSteps; ++i) m = larger(m, score[i]);
+    m = keys_max<S::kLanes>(m, lane);
+    if (q == c.topk_groups) {
+      if constexpr (std::is_same<Key, float>::value && kTwo) doubt = doubt || last - m <= tolerance;
+      break;
+    }
+    int g = INT_MAX;
+#pragma unroll
+    for (int i = S::kSteps - 1; i >= 0; --i) g = score[i] == m ? group_at(i) : g;
+    g = lanes_min<S::kLanes>(g, lane);
+    if (m > none) open |= uint64_t(1) << (g & 63);
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) score[i] = group_at(i) == g ? none : score[i];
+    last = m;
+  }
+#pragma unroll
+  for (int i = 0; i < S::kSteps; ++i) {
+    if (in_lanes) {
+      const bool kept = (open >> (group_at(i) & 63)) & 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) key[i][j] = kept ? key[i][j] : none;
+    } else {
+      const uint32_t four = space.group4[S::kLanes * i + l];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) key[i][j] = (open >> (four >> (8 * j) & 63)) & 1 ? key[i][j] : none;
+    }
+  }
+}
+
+// Slot l's expert, or -1, in lane l of the row's lanes; the keys are used up.
+template <typename S, bool kBias, typename Key>
+__device__ __forceinline__ int choose(Key (&key)[S::kSteps][4], const Choice& c, const GroupSpace<S>& space, int l, int lane, float error,
+                                      bool& doubt) {
+  const Key none = minus_inf();
+  constexpr bool kDoubt = kBias && std::is_same<Key, float>::value;
+  if (c.groups > 1) close_groups<S, kBias>(key, c, space, l, lane, error, doubt);
+  int mine = -1;
+  Key last = none;
+  for (int k = 0;; ++k) {
+    if (!kDoubt && k == c.top_k) break;
+    Key m = key[0][0];
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = larger(m, key[i][j]);
+    m = keys_max<S::kLanes>(m, lane);
+    if constexpr (kDoubt) {
+      // (both off by their errors and half a step)
+      doubt = doubt || (k > 0 && last - m <= 2 * error + fabsf(last) * 0x1p-22f);
+      if (k == c.top_k) break;
+      last = m;
+    }
+    int e = INT_MAX;
+#pragma unroll
+    for (int i = S::kSteps - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = 3; j >= 0; --j) e = key[i][j] == m ? 4 * S::kLanes * i + j : e;
+    e = lanes_min<S::kLanes>(e == INT_MAX ? e : e + 4 * l, lane);
+    if (l == k && m > none) mine = e;
+    const int here = e - 4 * l;
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) key[i][j] = here == 4 * S::kLanes * i + j ? none : key[i][j];
+  }
+  return mine;
+}
+
+// 1 / (1 + e^-x), off by 2^-21 of it.
+__device__ __forceinline__ float sigmoid_of(float x) {
+  const float u = exp_nonpositive(-fabsf(x)), large = __builtin_amdgcn_rcpf(1 + u);
+  return x >= 0 ? large : u * large;
+}
+
+template <typename S, int kDtype, bool kSigmoid, bool kBias>
+__global__ __launch_bounds__(kThreads) void choose_kernel(Rows g, Choice c) {
+  constexpr int kPadded = GroupSpace<S>::kPadded;
+  __shared__ __attribute__((aligned(16))) float bias[kBias ? kPadded : 4];
+  __shared__ uint32_t group4[kPadded / 4];
+  __shared__ double rows[kWaves][S::kRows * kPadded];
+  typedef float f4_t __attribute__((ext_vector_type(4)));
+  const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
+  const int l = lane % S::kLanes, sub = lane / S::kLanes;
+  if constexpr (kBias) {
+    for (int e = tid; e < kPadded; e += kThreads) bias[e] = e < g.experts ? c.bias[e] : minus_inf();
+  }
+  if (c.groups > 1 && !c.group_lanes) {
+    for (int q = tid; q < kPadded / 4; q += kThreads) {
+      uint32_t four = 0;
+      for (int j = 0; j < 4; ++j) four |= uint32_t(min((4 * q + j) / c.group_experts, c.groups - 1)) << (8 * j);
+      group4[q] = four;
+    }
+  }
+  __syncthreads();
+  const GroupSpace<S> space{rows[wave], group4};
+  const int64_t step = int64_t(gridDim.x) * kWaves * S::kRows;
+  const int64_t first = (int64_t(blockIdx.x) * kWaves + wave) * S::kRows;
+  if (first >= g.rows) return;
+  // a row ahead: the next one's logits are on their way while this one's are used
+  const auto row = [&](int64_t t) { return load_row<S, kDtype>(g, min(t, g.rows - 1), l); };
+  const auto mark = [&](int64_t t) { return g.padding ? g.padding[min(t, g.rows - 1)] : uint8_t(0); };
+  Values<S> next = row(first + sub);
+  uint8_t next_mark = mark(first + sub);
+  for (int64_t t = first + sub; t - sub < g.rows; t += step) {
+    Values<S> x = next;
+    const bool padding = next_mark;
+    if (t - sub + step < g.rows) {
+      next = row(t + step);
+      next_mark = mark(t + step);
+    }
+    // what poisons a row becomes -inf
+    bool bad = false;
+    float largest = minus_inf();
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float& v = x.v[i][j];
+        const bool b = kSigmoid ? v != v : !(v < __builtin_inff());
+        bad = bad || b;
+        v = b ? minus_inf() : v;
+        if (!kSigmoid) largest = fmaxf(largest, v);
+      }
+    const uint64_t bads = __ballot(bad);
+    const bool poisoned = (S::kLanes == 64 ? bads : (bads >> (S::kLanes * sub)) & ((uint64_t(1) << (S::kLanes & 63)) - 1)) != 0;
+    float lowest = kNothing;  // logits from here on count
+    if constexpr (!kSigmoid) {
+      largest = lanes_max<S::kLanes>(largest, lane);
+      if (largest == minus_inf()) largest = 0;
+      lowest = 0;
+    }
+    const auto masked = [&](float v) { return kSigmoid ? !(v >= lowest) : !(v - largest >= kNothing); };
+    // the softmax's sum
+    float sum = 0;
+    float inv = 0;
+    if (!kSigmoid && (kBias || !c.renormalize)) {
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += exp_nonpositive(x.v[i][j] - largest);
+      sum = lanes_sum<S::kLanes>(sum, lane);
+      inv = sum > 0 ? 1 / sum : 0.0f;
+    }
+    // an FP32 score's error: a sigmoid's 2^-21; a softmax's that of its sum too (up to 22
+    // additions in a row), and none is larger than 1 / sum
+    const float error = kSigmoid ? 0x1p-21f : 0x1p-19f * inv;
+    bool doubt = false;
+    int mine;
+    {
+      float key[S::kSteps][4];
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i) {
+        f4_t b{0, 0, 0, 0};
+        if constexpr (kBias) b = *reinterpret_cast<const f4_t*>(bias + 4 * (S::kLanes * i + l));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = x.v[i][j];
+          float k = v;
+          if constexpr (kBias) k = (kSigmoid ? sigmoid_of(v) : exp_nonpositive(v - largest) * inv) + b[j];
+          key[i][j] = masked(v) || !(k > minus_inf()) ? minus_inf() : k;
+        }
+      }
+      mine = choose<S, kBias>(key, c, space, l, lane, error, doubt);
+    }
+    if constexpr (kBias) {
+      doubt = doubt && !padding;
+      if (__builtin_expect(__any(doubt), 0)) {
+        double key[S::kSteps][4], total = 0;
+        const Values<S> again = row(t);  // (kept in registers it would cost all rows)
+#pragma unroll
+        for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = again.v[i][j];
+            const bool b = kSigmoid ? v != v : !(v < __builtin_inff());
+            const double d = b ? -__builtin_inf() : double(v);
+            key[i][j] = kSigmoid ? 1 / (1 + exp(-d)) : exp(d - double(largest));
+            total += key[i][j];
+          }
+        if constexpr (!kSigmoid) {
+#pragma unroll
+          for (int d = S::kLanes / 2; d > 0; d /= 2) total += __shfl_xor(total, d);
+        }
+#pragma unroll
+        for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = again.v[i][j], b = bias[4 * (S::kLanes * i + l) + j];
+            const double k = (kSigmoid ? key[i][j] : key[i][j] / total) + double(b);
+            const bool out = v != v || (!kSigmoid && v == __builtin_inff()) || masked(v) || !(k > -__builtin_inf());
+            key[i][j] = out ? -__builtin_inf() : k;
+          }
+        bool none = false;
+        const int exact = choose<S, true>(key, c, space, l, lane, 0.0f, none);
+        if (doubt) mine = exact;
+      }
+    }
+    // slot l's weight in lane l
+    const bool chosen = l < c.top_k && mine >= 0;
+    const float v = chosen ? vq::load_act(g.logits, kDtype, min(t, g.rows - 1) * g.stride + mine) : minus_inf();
+    float w = 0;
+    if (c.renormalize) {
+      // over the largest chosen one's size, so that shares do not depend on where logits lie
+      float top = lanes_max<S::kLanes>(v, lane);
+      if (top == minus_inf()) top = 0;
+      if constexpr (kSigmoid) {
+        const float k = top < 0 ? __builtin_ceilf(top * kLog2e) : 0.0f;
+        const float u = exp_nonpositive(-fabsf(v));
+        w = (v >= 0 ? 1.0f : exp_nonpositive(v, k)) / (1 + u);
+      } else {
+        w = exp_nonpositive(v - top);
+      }
+      w = chosen ? w : 0.0f;
+      const float all = lanes_sum<S::kLanes>(w, lane);
+      w = all > 0 ? w / all : 0.0f;
+    } else if (chosen) {
+      if constexpr (kSigmoid) {
+        const float u = exp_nonpositive(-fabsf(v));
+        w = (v >= 0 ? 1.0f : u) / (1 + u);
+      } else {
+        w = exp_nonpositive(v - largest) / sum;
+      }
+    }
+    w *= c.scale;
+    if (poisoned) w = chosen ? __builtin_nanf("") : 0.0f;
+    if (t < g.rows && l < c.top_k) {
+      c.weights[t * c.top_k + l] = padding || !chosen ? 0.0f : w;
+      c.ids[t * c.top_k + l] = padding || !chosen ? -1 : mine;
+    }
+  }
+}
+
+struct Slots {
+  const float* weights;
+  const int32_t* ids;
+  const float* upstream;
+  int top_k;
+  bool renormalize;
+  float scale;
+};
+
+template <typename S, int kDtype, bool kSigmoid>
+__global__ __launch_bounds__(kThreads) void grad_kernel(Rows g, Slots c, void* grad) {
+  constexpr int kPadded = 4 * S::kLanes * S::kSteps;
+  // the chosen experts' parts, zeros between the rows' turns
+  __shared__ __attribute__((aligned(16))) float parts[kWaves][S::kRows * kPadded];
+  typedef float f4_t __attribute__((ext_vector_type(4)));
+  const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
+  const int l = lane % S::kLanes, sub = lane / S::kLanes;
+  float* part = parts[wave] + sub * kPadded;
+#pragma unroll
+  for (int i = 0; i < S::kSteps; ++i) *reinterpret_cast<f4_t*>(part + 4 * (S::kLanes * i + l)) = f4_t{0, 0, 0, 0};
+  const bool wide = g.experts % 4 == 0;  // (rows of the gradient lie close)
+  const bool dense = !kSigmoid && !c.renormalize;
+  const float over = c.scale != 0 ? 1 / c.scale : 0.0f;
+  const int64_t step = int64_t(gridDim.x) * kWaves * S::kRows;
+  for (int64_t t0 = (int64_t(blockIdx.x) * kWaves + wave) * S::kRows; t0 < g.rows; t0 += step) {
+    const int64_t t = t0 + sub, at = min(t, g.rows - 1);
+    int e = -1;
+    float w = 0, up = 0;
+    if (l < c.top_k) {
+      e = c.ids[at * c.top_k + l];
+      w = c.weights[at * c.top_k + l];
+      up = c.upstream[at * c.top_k + l];
+    }
+    const bool chosen = e >= 0 && e < g.experts;
+    if (!chosen) w = up = 0;
+    float d = w * up;
+    const float all = lanes_sum<S::kLanes>(d, lane);
+    if (c.renormalize) d = w * (up - all * over);
+    if constexpr (kSigmoid) {
+      // 1 - sigmoid of the logit is the sigmoid of its opposite
+      const float v = chosen ? vq::load_act(g.logits, kDtype, at * g.stride + e) : 0.0f;
+      d *= sigmoid_of(-v);
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (chosen) part[e] = d;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float out[S::kSteps][4];
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) {
+      const f4_t p = *reinterpret_cast<const f4_t*>(part + 4 * (S::kLanes * i + l));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[i][j] = p[j];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (chosen) part[e] = 0;
+    if (dense) {
+      const uint64_t any = __ballot(chosen);
+      const bool used = (S::kLanes == 64 ? any : (any >> (S::kLanes * sub)) & ((uint64_t(1) << (S::kLanes & 63)) - 1)) != 0;
+      const Values<S> x = load_row<S, kDtype>(g, at, l);
+      float m = logits::row_max(x, lane), sum = 0;
+      if (m == minus_inf()) m = 0;
+      float z[S::kSteps][4];
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += z[i][j] = exp_nonpositive(x.v[i][j] - m);
+      sum = lanes_sum<S::kLanes>(sum, lane);
+      const float share = all / sum;
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[i][j] = used ? out[i][j] - z[i][j] * share : 0.0f;  // (rows that chose nothing may hold anything)
+    }
+    if (t >= g.rows) continue;
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) {
+      const int e0 = 4 * (S::kLanes * i + l);
+      const int64_t to = t * g.experts + e0;
+      if (wide && e0 < g.experts) {
+        if constexpr (kDtype == vq::kFP32) {
+          *reinterpret_cast<f4_t*>(static_cast<float*>(grad) + to) = f4_t{out[i][0], out[i][1], out[i][2], out[i][3]};
+        } else {
+          typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+          const auto half = [](float a) {
+            return uint32_t(kDtype == vq::kBF16 ? vq::f32_to_bf16(a) : __builtin_bit_cast(uint16_t, _Float16(a)));
+          };
+          *reinterpret_cast<u2_t*>(static_cast<uint16_t*>(grad) + to) =
+              u2_t{half(out[i][0]) | (half(out[i][1]) << 16), half(out[i][2]) | (half(out[i][3]) << 16)};
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (e0 + j < g.experts) vq::store_act(grad, kDtype, to + j, out[i][j]);
+        }
+      }
+    }
+  }
+}
+
+// launch(shape, dtype, sigmoid) for rows of `experts` whose lanes hold `slots` slots
+// (and groups) at least.
+template <typename F>
+int dispatch(int64_t experts, int64_t slots, int dtype, bool sigmoid, const F& launch) {
+  const auto shaped = [&](auto shape) {
+    const auto typed = [&](auto type) {
+      if (sigmoid) launch(shape, type, std::true_type{});
+      else launch(shape, type, std::false_type{});
+    };
+    if (dtype == vq::kBF16) typed(std::integral_constant<int, vq::kBF16>{});
+    else if (dtype == vq::kFP16) typed(std::integral_constant<int, vq::kFP16>{});
+    else typed(std::integral_constant<int, vq::kFP32>{});
+  };
+  if (slots <= 16 && experts <= 64) shaped(Shape<16, 1>{});
+  else if (slots <= 16 && experts <= 128) shaped(Shape<16, 2>{});
+  else if (slots <= 16 && experts <= 256) shaped(Shape<16, 4>{});
+  else if (experts <= 256) shaped(Shape<64, 1>{});
+  else if (slots <= 32 && experts <= 512) shaped(Shape<32, 4>{});
+  else shaped(Shape<64, 4>{});
+  return vq::check_launch("moe_route_logits");
+}
+
+template <typename S>
+unsigned grid_of(int64_t rows) {
+  const int64_t each = kWaves * S::kRows;
+  return unsigned(std::max<int64_t>(1, std::min<int64_t>(kMaxGrid, (rows + each - 1) / each)));
+}
+
+Rows rows_of(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, const uint8_t* padding) {
+  const int64_t four = 4 * vq::dtype_bytes(dtype);
+  const bool wide = experts % 4 == 0 && stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % four == 0;
+  return {logits, stride, padding, rows, int(experts), wide};
+}
+
+int check_call(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, int64_t top_k, int scoring, float scale) {
+  if (dtype != vq::kBF16 && dtype != vq::kFP16 && dtype != vq::kFP32) return vq::fail("moe_route_logits: logits must be BF16, FP16 or FP32");
+  if (rows < 0 || rows > INT_MAX) return vq::fail("moe_route_logits: rows out of range");
+  if (experts <= 0 || experts > kMaxExperts) return vq::fail("moe_route_logits: between 1 and 1024 experts");
+  if (top_k <= 0 || top_k > kMaxSlots || top_k > experts) return vq::fail("moe_route_logits: topk must be between 1 and 64, and at most the experts");
+  if (scoring != 0 && scoring != 1) return vq::fail("moe_route_logits: scoring must be softmax (0) or sigmoid (1)");
+  if (!(scale > -__builtin_inff() && scale < __builtin_inff())) return vq::fail("moe_route_logits: the scale must be finite");
+  if (stride < 0 || (rows > 1 && stride < experts) || stride > (int64_t(1) << 31)) return vq::fail("moe_route_logits: row stride out of range");
+  if (rows > 0 && !logits) return vq::fail("moe_route_logits: null pointer");
+  return vq::kOk;
+}
+
+// A call's arrays: no output may overlap another array, and each lies on its elements.
+struct Span {
+  const void* p;
+  int64_t bytes, element;
+};
+int check_spans(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  for (const Span* a = outputs.begin(); a != outputs.end(); ++a) {
+    for (const Span* b = outputs.begin(); b != a; ++b) {
+      if (vq::overlaps(a->p, a->bytes, b->p, b->bytes)) return vq::fail("moe_route_logits: arguments must not overlap");
+    }
+    for (const Span& b : inputs) {
+      if (vq::overlaps(a->p, a->bytes, b.p, b.bytes)) return vq::fail("moe_route_logits: arguments must not overlap");
+    }
+  }
+  for (const auto* list : {&outputs, &inputs}) {
+    for (const Span& a : *list) {
+      if (reinterpret_cast<uintptr_t>(a.p) % uintptr_t(a.element)) return vq::fail("moe_route_logits: misaligned pointer");
+    }
+  }
+  return vq::kOk;
+}
+
+int64_t logits_bytes(int dtype, int64_t rows, int64_t experts, int64_t stride) {
+  return rows > 0 ? ((rows - 1) * stride + experts) * vq::dtype_bytes(dtype) : 0;
+}
+
+}  // namespace
+}  // namespace route
+
+extern "C" int moe_route_logits(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, const float* bias,
+                                int64_t top_k, int64_t groups, int64_t topk_groups, int scoring, int renormalize, float scale,
+                                const uint8_t* is_padding, float* topk_weights, int32_t* topk_ids, void* stream) {
+  using namespace route;
+  if (int rc = check_call(logits, dtype, rows, experts, stride, top_k, scoring, scale)) return rc;
+  if (groups <= 0 || groups > kMaxGroups || experts % groups) return vq::fail("moe_route_logits: up to 64 groups of equal size");
+  if (topk_groups <= 0 || topk_groups > groups) return vq::fail("moe_route_logits: topk_groups must be between 1 and the groups");
+  if (top_k > topk_groups * (experts / groups)) return vq::fail("moe_route_logits: topk experts do not fit topk_groups groups");
+  if (rows == 0) return vq::kOk;
+  if (!topk_weights || !topk_ids) return vq::fail("moe_route_logits: null pointer");
+  const int64_t slots = rows * top_k;
+  if (int rc = check_spans({{topk_weights, slots * 4, 4}, {topk_ids, slots * 4, 4}},
+                           {{logits, logits_bytes(dtype, rows, experts, stride), vq::dtype_bytes(dtype)},
+                            {bias, experts * 4, 4}, {is_padding, rows, 1}})) {
+    return rc;
+  }
+  if (topk_groups == groups) groups = topk_groups = 1;  // all are open
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const Rows g = rows_of(logits, dtype, rows, experts, stride, is_padding);
+  Choice c{bias, int(top_k), int(groups), int(topk_groups), int(experts / groups), 0, renormalize != 0, scale, topk_weights, topk_ids};
+  return dispatch(experts, std::max(top_k, groups), dtype, scoring == 1, [&](auto shape, auto type, auto sigmoid) {
+    using S = decltype(shape);
+    const int lanes = c.group_experts / 4;
+    if (c.group_experts % 4 == 0 && lanes <= S::kLanes && (lanes & (lanes - 1)) == 0) c.group_lanes = lanes;
+    if (bias) {
+      hipLaunchKernelGGL((choose_kernel<S, decltype(type)::value, decltype(sigmoid)::value, true>), dim3(grid_of<S>(rows)), dim3(kThreads), 0,
+                         s, g, c);
+    } else {
+      hipLaunchKernelGGL((choose_kernel<S, decltype(type)::value, decltype(sigmoid)::value, false>), dim3(grid_of<S>(rows)), dim3(kThreads), 0,
+                         s, g, c);
+    }
+  });
+}
+
+extern "C" int moe_route_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, const float* topk_weights,
+                              const int32_t* topk_ids, int64_t top_k, int scoring, int renormalize, float scale, const float* upstream,
+                              void* grad, void* stream) {
+  using namespace route;
+  if (int rc = check_call(logits, dtype, rows, experts, stride, top_k, scoring, scale)) return rc;
+  if (rows == 0) return vq::kOk;
+  if (!topk_weights || !topk_ids || !upstream || !grad) return vq::fail("moe_route_logits: null pointer");
+  const int64_t slots = rows * top_k, bytes = vq::dtype_bytes(dtype);
+  if (int rc = check_spans({{grad, rows * experts * bytes, 4 * bytes}},
+                           {{logits, logits_bytes(dtype, rows, experts, stride), bytes},
+                            {topk_weights, slots * 4, 4}, {topk_ids, slots * 4, 4}, {upstream, slots * 4, 4}})) {
+    return rc;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const Rows g = rows_of(logits, dtype, rows, experts, stride, nullptr);
+  const Slots c{topk_weights, topk_ids, upstream, int(top_k), renormalize != 0, scale};
+  return dispatch(experts, top_k, dtype, scoring == 1, [&](auto shape, auto type, auto sigmoid) {
+    using S = decltype(shape);
+    hipLaunchKernelGGL((grad_kernel<S, decltype(type)::value, decltype(sigmoid)::value>), dim3(grid_of<S>(rows)), dim3(kThreads), 0, s, g, c,
+                       grad);
+  });
+}

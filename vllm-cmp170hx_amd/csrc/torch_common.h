@@ -17,5 +17,6 @@ void check_status(int status);
 // dlopen handle); false when one is missing.
 bool bind_mxfp4(void* library);
 bool bind_balance(void* library);
+bool bind_route(void* library);
 
 }  // namespace vq_torch

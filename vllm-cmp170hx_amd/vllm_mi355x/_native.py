@@ -14,7 +14,7 @@ import threading
 LIBRARY_NAME = "libvllm_mi355x.so"
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIBRARY_NAME)
 # The host-only operator implementations (csrc/torch_ops.cpp, torch_mxfp4.cpp,
-# torch_balance.cpp) and the torch
+# torch_balance.cpp, torch_route.cpp) and the torch
 # custom classes the reference's loader requires (csrc/torch_classes.cpp).
 TORCH_CLASSES_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                   "libvllm_mi355x_torch.so")
@@ -176,6 +176,17 @@ SIGNATURES = {
     "moe_balance_grad": (c_int, [
         c_vp, c_int, c_i64, c_i64, c_i64,        # logits, dtype, rows, experts, stride
         c_vp, c_int, c_vp, c_vp, c_vp, c_vp,     # is_padding, scoring, stats, upstream, grad, stream
+    ]),
+    "moe_route_logits": (c_int, [
+        c_vp, c_int, c_i64, c_i64, c_i64,        # logits, dtype, rows, experts, stride
+        c_vp, c_i64, c_i64, c_i64,               # bias, top_k, groups, topk_groups
+        c_int, c_int, ctypes.c_float, c_vp,      # scoring, renormalize, scale, is_padding
+        c_vp, c_vp, c_vp,                        # topk_weights, topk_ids, stream
+    ]),
+    "moe_route_grad": (c_int, [
+        c_vp, c_int, c_i64, c_i64, c_i64,        # logits, dtype, rows, experts, stride
+        c_vp, c_vp, c_i64, c_int, c_int,         # topk_weights, topk_ids, top_k, scoring, renormalize
+        ctypes.c_float, c_vp, c_vp, c_vp,        # scale, upstream, grad, stream
     ]),
     "moe_split_align": (c_int, [
         c_vp, c_i64, c_i64, c_vp, c_vp, c_i64,  # topk_ids, numel, num_experts, expert_map, cover, rows

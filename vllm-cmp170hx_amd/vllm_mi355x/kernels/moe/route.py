@@ -84,3 +84,36 @@ def moe_route(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, 
             expert_ids.numel(), ntpp.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
     _native.check(status)
     return logits, topk_w, topk_ids, sorted_ids, expert_ids, ntpp
+
+
+def moe_route_logits(logits: torch.Tensor, topk: int, bias: torch.Tensor | None = None,
+                     num_groups: int = 1, topk_groups: int = 1, renormalize: bool = True,
+                     routed_scaling_factor: float = 1.0, is_padding: torch.Tensor | None = None,
+                     scoring: str = "sigmoid") -> tuple[torch.Tensor, torch.Tensor]:
+    """(topk_weights fp32 [M, topk], topk_ids int32 [M, topk]) from a router's logits
+    [M, E] (bf16, fp16 or fp32; rows in one stride, not overlapping; E up to 1024), as the
+    fused MoE calls and moe_balance_loss take them.  No counterpart in the reference.
+
+    Scores are the logits' softmax or sigmoids; an expert's key is its score plus its bias
+    (fp32 [E]) in 64 bits, or without a bias the logit itself, and the topk (up to 64)
+    largest keys are chosen, largest first, equals by the lower expert.  num_groups > 1 (up
+    to 64): of so many runs of equally many experts only the topk_groups best are open; a
+    group's score is its largest key, or with a bias its two largest's sum.  Weights: the
+    chosen scores (the bias has no part in them), over their sum if renormalize, times
+    routed_scaling_factor.
+
+    Masked experts are not chosen: logits of -inf or 708.396 or more below 0 (softmax: below
+    the row's largest), biases of -inf or NaN.  Slots left over, and the rows that is_padding
+    (bool [M]) marks, hold id -1 and weight 0.  A row with a NaN (softmax: or +inf) has
+    weights NaN.
+
+    The weights are differentiable once in the logits, in reverse mode (a forward-mode
+    tangent raises), the choice and the bias constants.  Failed checks raise RuntimeError.
+    To capture a backward pass into a graph, let go of eager results of the same leaves
+    first, as for any operator of torch."""
+    if scoring not in _SCORING:
+        raise ValueError(f"unknown scoring {scoring!r}")
+    _native.load_torch()
+    return torch.ops._vllm_mi355x.moe_route_logits(
+        logits, bias, int(topk), int(num_groups), int(topk_groups), _SCORING[scoring],
+        bool(renormalize), float(routed_scaling_factor), is_padding)
