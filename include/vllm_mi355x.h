@@ -627,6 +627,57 @@ int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, co
               const int32_t* expert_map, int64_t map_size, int64_t hidden, int64_t inter,
               float limit, void* out, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- dense linear layers ---------------------------------------------------------
+ * Plain 16-bit weights: routers, shared experts, layers that a quantized model leaves
+ * as they are.  No counterparts in the reference.
+ */
+
+/* Activations. */
+#define VQ_ACT_NONE 0
+#define VQ_ACT_RELU 1
+#define VQ_ACT_GELU 2 /* of the error function */
+#define VQ_ACT_GELU_TANH 3
+#define VQ_ACT_SILU 4
+#define VQ_ACT_SWIGLU 5 /* gated: w has n gate rows, then n up rows */
+
+/*
+ * out [rows][n] = RN_out(act(x W^T + bias) + residual): x [rows][k] and w [lines][k] of
+ * dtype (VQ_BF16 or VQ_FP16; row strides in elements, no alignment beyond the
+ * element's), lines = n, with VQ_ACT_SWIGLU 2 n: SiLU(min(g, L)) clamp(u, -L, L), L = limit
+ * > 0 (infinity: no clamp).  FP32 sums of exact products; bias [lines] (or null) and
+ * residual [rows][n] (or null) of any of the three types; out contiguous, of any of them;
+ * it may be a contiguous residual of its type.  z (or null): contiguous [rows][lines] of
+ * dtype, x W^T + bias for dense_linear_grad (with a limit, infinities for what lies
+ * outside).  The order of the sums, and so the last bits, depend on the sizes alone.  k
+ * up to 2^21.  workspace: dense_linear_workspace_size bytes of the same x, w and strides,
+ * 16-byte aligned (null where that is 0), used by one call at a time.
+ */
+int64_t dense_linear_workspace_size(const void* x, int64_t rows, int64_t k, int64_t x_stride,
+                                    const void* w, int64_t n, int64_t w_stride, int activation);
+int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride,
+                 const void* w, int64_t n, int64_t w_stride, const void* bias, int bias_dtype,
+                 int activation, float limit, const void* residual, int residual_dtype,
+                 int64_t residual_stride, void* out, int out_dtype, void* z, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/* How it runs at a size, for tests: plan[0] the tile's rows and lines (0: the few rows'
+ * kernel), plan[1] the K splits, plan[2] the wavefronts of the few rows' workgroups. */
+int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int32_t* plan);
+
+/*
+ * From dy, the gradient of out ([rows][n] of any of the three types): dx [rows][k] and dw
+ * [lines][k] (contiguous, of dtype) and dbias [lines]; each may be null.  z as dense_linear
+ * left it (with VQ_ACT_NONE null).  The gradient of z is rounded to dtype, in FP16 over a
+ * power of two of the whole, before its products.  At least one row.
+ */
+int64_t dense_linear_grad_workspace_size(int64_t rows, int64_t k, int64_t n, int activation,
+                                         int need_x, int need_w, int need_bias);
+int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride,
+                      const void* w, int64_t n, int64_t w_stride, const void* z, int activation,
+                      float limit, const void* dy, int dy_dtype, int64_t dy_stride, void* dx,
+                      void* dw, void* dbias, int bias_dtype, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 /* ---- routing from logits ---------------------------------------------------------
  * No counterparts in the reference (moe_route's selection is of its own logits, without
  * groups or gradient).  Up to 1024 experts, 64 slots a row, 64 groups.

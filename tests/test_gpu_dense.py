@@ -1,0 +1,300 @@
+"""The dense linear layer on the GPU against the FP64 oracle, whose bounds count the FP32
+sums' roundings, the functions' and, for gradients, the rounding of what is kept to x's
+type; then half a step of the output's type."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import dense_oracle as D
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+ACTIVATIONS = [None, "relu", "gelu", "gelu_tanh", "silu", "swiglu"]
+
+
+@pytest.fixture(scope="module")
+def linear():
+    from vllm_mi355x.kernels.dense import dense_linear
+    return dense_linear
+
+
+def normal(rng, shape, dtype, device, scale=1.0):
+    return torch.from_numpy(rng.standard_normal(shape) * scale).to(TYPES[dtype]).to(device)
+
+
+def exact(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def close(got, want, tol, what):
+    info = torch.finfo(got.dtype)
+    got = got.detach().double().cpu().numpy()
+    want = want.reshape(got.shape)
+    tol = tol.reshape(got.shape)
+    tol = tol + info.eps / 2 * (np.abs(want) + tol) + info.smallest_normal * info.eps
+    off = np.abs(got - want) - tol
+    assert (off <= 0).all(), f"{what}: {np.count_nonzero(off > 0)} of {off.size}, max excess {off.max():.3g}"
+
+
+def check(linear, x, w, bias=None, activation=None, residual=None, out_dtype=None, limit=None, dy=None):
+    """One call, and with dy its gradients; returns y and the gradients."""
+    lim = np.inf if limit is None else limit
+    flat = exact(x).reshape(-1, x.shape[-1])
+    n = len(w) // 2 if activation == "swiglu" else len(w)
+    res = None if residual is None else exact(residual).reshape(-1, n)
+    want, tol = D.forward(flat, exact(w), exact(bias), activation, res, lim)
+    with torch.no_grad():
+        y = linear(x, w, bias, activation, residual, out_dtype, limit)
+    assert y.shape == (*x.shape[:-1], n) and y.dtype == (out_dtype or x.dtype) and y.is_contiguous() and not y.requires_grad
+    close(y, want, tol, "y")
+    if dy is None:
+        return y, None
+    leaves = {name: t.detach().requires_grad_() for name, t in (("x", x), ("w", w), ("bias", bias), ("residual", residual)) if t is not None}
+    again = linear(leaves["x"], leaves["w"], leaves.get("bias"), activation, leaves.get("residual"), out_dtype, limit)
+    assert torch.equal(again, y)
+    grads = dict(zip(leaves, torch.autograd.grad(again, list(leaves.values()), dy)))
+    wants, _ = D.backward(flat, exact(w), exact(bias), activation, exact(dy).reshape(-1, n), torch.finfo(x.dtype).eps, lim)
+    for name, g in grads.items():
+        assert g.shape == leaves[name].shape and g.dtype == leaves[name].dtype
+        if name == "residual":
+            assert torch.equal(g, dy.to(g.dtype))
+        else:
+            close(g, *wants[name], name)
+    return y, grads
+
+
+SIZES = [(1, 1, 1), (1, 7, 3), (1, 64, 16), (2, 129, 17), (3, 4096, 40), (5, 200, 33), (16, 512, 64), (17, 130, 50), (20, 1000, 100),
+         (33, 72, 31), (64, 640, 96), (65, 64, 65), (65, 8, 200), (100, 200, 130), (130, 1024, 256), (200, 72, 48), (300, 333, 129),
+         (257, 1096, 520), (70, 8192, 64)]
+
+
+@pytest.mark.parametrize("rows,k,n", SIZES)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_matches_the_oracle(linear, device, rows, k, n, dtype, activation):
+    print(f"dense {rows}x{k}x{n} {dtype} {activation}", flush=True)
+    rng = np.random.default_rng(rows * 31 + k + n)
+    lines = 2 * n if activation == "swiglu" else n
+    x, w = normal(rng, (rows, k), dtype, device), normal(rng, (lines, k), dtype, device, k ** -0.5)
+    bias = normal(rng, lines, dtype, device)
+    residual = normal(rng, (rows, n), dtype, device)
+    dy = normal(rng, (rows, n), dtype, device)
+    check(linear, x, w, bias, activation, residual, dy=dy)
+    check(linear, x, w, activation=activation, out_dtype=torch.float32, dy=dy.float() * 1e-6)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_types_of_bias_residual_and_output(linear, device, rows, dtype):
+    rng = np.random.default_rng(rows)
+    x, w = normal(rng, (rows, 96), dtype, device), normal(rng, (75, 96), dtype, device, 0.1)
+    for b in TYPES:
+        for r in TYPES:
+            for o in TYPES:
+                check(linear, x, w, normal(rng, 75, b, device), "silu", normal(rng, (rows, 75), r, device), TYPES[o],
+                      dy=normal(rng, (rows, 75), o, device))
+
+
+@pytest.mark.parametrize("rows", [1, 12, 50, 300])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_clamped_gate(linear, device, rows, dtype):
+    """Values on both sides of the limit and near it; a limit that the type does not hold."""
+    rng = np.random.default_rng(rows)
+    x, w = normal(rng, (rows, 80), dtype, device), normal(rng, (2 * 70, 80), dtype, device, 0.3)
+    bias = normal(rng, 2 * 70, "fp32", device)
+    dy = normal(rng, (rows, 70), dtype, device)
+    for limit in (1.0, 2.003, 7.0):
+        check(linear, x, w, bias, "swiglu", None, None, limit, dy)
+
+
+def test_strides_and_axes(linear, device):
+    """Rows of larger buffers, off 16 bytes, in one run over leading axes; slices of weights and
+    residuals."""
+    rng = np.random.default_rng(5)
+    for rows in (4, 40, 200):
+        for dtype in ("bf16", "fp16"):
+            wide, weights = normal(rng, (rows, 300), dtype, device), normal(rng, (90, 280), dtype, device, 0.1)
+            res, dy = normal(rng, (rows, 200), dtype, device), normal(rng, (rows, 90), dtype, device)
+            for x0, w0, k in ((0, 0, 256), (8, 16, 64), (1, 0, 99), (3, 5, 160), (0, 1, 128), (2, 0, 255)):
+                check(linear, wide[:, x0:x0 + k], weights[:, w0:w0 + k], None, "gelu", res[:, 7:97], dy=dy)
+            x = wide[:, :64].reshape(2, rows // 2, 64)
+            check(linear, x, weights[:, :64], None, None, res[:, :90].reshape(2, rows // 2, 90), dy=dy.reshape(2, rows // 2, 90))
+            check(linear, wide.view(2, rows // 2, 300)[..., :50], weights[:, :50], dy=dy.reshape(2, rows // 2, 90))
+    check(linear, wide[0, :64], weights[:, :64], None, "relu", res[0, :90], dy=dy[0])
+    # upstream gradients as autograd gives them
+    x, w = wide[:, :64].detach().requires_grad_(), weights[:, :64].detach().requires_grad_()
+    y = linear(x, w)
+    a = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)
+    b = torch.autograd.grad(y, (x, w), torch.ones_like(y), retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    up = torch.randn(90, 200, device=device).to(y.dtype)
+    a = torch.autograd.grad(y, (x, w), up.t(), retain_graph=True)
+    b = torch.autograd.grad(y, (x, w), up.t().contiguous())
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_single_gradients(linear, device):
+    """Each input's gradient by itself has the bits it has beside the others."""
+    rng = np.random.default_rng(7)
+    t = {"x": normal(rng, (100, 72), "bf16", device), "w": normal(rng, (60, 72), "bf16", device), "bias": normal(rng, 60, "fp32", device),
+         "residual": normal(rng, (100, 60), "fp16", device)}
+    dy = normal(rng, (100, 60), "bf16", device)
+
+    def grads(names):
+        leaf = {k: v.detach().requires_grad_(k in names) for k, v in t.items()}
+        y = linear(leaf["x"], leaf["w"], leaf["bias"], "silu", leaf["residual"])
+        return dict(zip(names, torch.autograd.grad(y, [leaf[k] for k in names], dy)))
+
+    every = grads(list(t))
+    for name in t:
+        assert torch.equal(grads([name])[name], every[name])
+
+
+def test_out_and_in_place(linear, device):
+    rng = np.random.default_rng(8)
+    for rows in (3, 90, 400):
+        x, w, res = normal(rng, (rows, 2048), "bf16", device), normal(rng, (64, 2048), "bf16", device, 0.02), normal(rng, (rows, 64), "fp32", device)
+        want = linear(x, w, None, "silu", res, torch.float32)
+        out = torch.full_like(res, float("nan"))
+        assert linear(x, w, None, "silu", res, out=out) is out and torch.equal(out, want)
+        place = res.clone()
+        linear(x, w, None, "silu", place, out=place)
+        assert torch.equal(place, want)
+
+
+def test_nothing(linear, device):
+    x, w = torch.empty(0, 16, device=device, dtype=torch.bfloat16), torch.randn(6, 16, device=device).bfloat16()
+    leaf, weight, bias = x.requires_grad_(), w.requires_grad_(), torch.zeros(6, device=device, requires_grad=True)
+    y = linear(leaf, weight, bias, "gelu")
+    assert y.shape == (0, 6)
+    dx, dw, db = torch.autograd.grad(y, (leaf, weight, bias), torch.empty_like(y))
+    assert dx.shape == (0, 16) and not dw.any() and not db.any()
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_not_numbers_stay_in_their_rows(linear, device, rows):
+    """NaN and infinities reach their own rows' outputs (and columns, from W) and no others."""
+    rng = np.random.default_rng(9)
+    for activation in ACTIVATIONS:
+        lines = 2 * 40 if activation == "swiglu" else 40
+        x, w = normal(rng, (rows, 128), "bf16", device), normal(rng, (lines, 128), "bf16", device, 0.1)
+        good = linear(x, w, None, activation)
+        bad = x.clone()
+        bad[rows // 2, 5] = float("nan")
+        y = linear(bad, w, None, activation)
+        keep = torch.arange(rows, device=device) != rows // 2
+        assert torch.isnan(y[rows // 2]).all() and torch.equal(y[keep], good[keep])
+        worse = w.clone()
+        worse[3, 7] = float("inf")
+        y = linear(x, worse, None, activation)
+        keep = torch.arange(40, device=device) != 3
+        assert torch.equal(y[:, keep], good[:, keep])
+
+
+def test_tiny_and_large_gradients_in_fp16(linear, device):
+    """FP32 gradients far below FP16's range, and gate gradients above it."""
+    rng = np.random.default_rng(10)
+    x, w = normal(rng, (200, 64), "fp16", device), normal(rng, (96, 64), "fp16", device, 0.1)
+    for scale in (1e-12, 1e-7, 1e4, 1e9):
+        dy = normal(rng, (200, 96), "fp32", device, scale)
+        leaf = x.detach().requires_grad_()
+        weight = w.detach().requires_grad_()
+        bias = torch.zeros(96, device=device, requires_grad=True)
+        y = linear(leaf, weight, bias, "silu", out_dtype=torch.float32)
+        db, = torch.autograd.grad(y, bias, dy)
+        wants, _ = D.backward(exact(x), exact(w), np.zeros(96), "silu", exact(dy), torch.finfo(torch.float16).eps)
+        close(db, *wants["bias"], "bias")
+    gate = normal(rng, (2 * 30, 64), "fp16", device, 3.0)
+    check(linear, x, gate, None, "swiglu", None, torch.float32, None, normal(rng, (200, 30), "fp32", device, 1e-4))
+
+
+def test_gradient_by_differences(linear, device):
+    """Against central differences of the 64-bit loss; bf16's roundings of z and dz are
+    2^-9 of each of the 24 (or 6) terms."""
+    rng = np.random.default_rng(12)
+    for activation in ACTIVATIONS:
+        lines = 2 * 24 if activation == "swiglu" else 24
+        x, w = normal(rng, (6, 16), "bf16", device), normal(rng, (lines, 16), "bf16", device, 0.3)
+        dy = normal(rng, (6, 24), "bf16", device)
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        dx, dw = torch.autograd.grad(linear(a, b, None, activation), (a, b), dy)
+        fx, fw, fy = exact(x), exact(w), exact(dy)
+        bounds, _ = D.backward(fx, fw, None, activation, fy, torch.finfo(torch.bfloat16).eps)
+        for name, arr, grad in (("x", fx, dx), ("w", fw, dw)):
+            for at in ((0, 0), (3, 7), (5, 15)):
+                old = arr[at]
+                arr[at] = old + 1e-6
+                up = (D.forward(fx, fw, None, activation, None)[0] * fy).sum()
+                arr[at] = old - 1e-6
+                diff = (up - (D.forward(fx, fw, None, activation, None)[0] * fy).sum()) / 2e-6
+                arr[at] = old
+                tol = bounds[name][1][at] + 1e-6
+                assert abs(grad[at].item() - diff) <= tol + 2.0 ** -8 * (abs(diff) + tol)
+
+
+def test_refusals(linear, device):
+    x, w = torch.zeros(6, 16, device=device).half(), torch.zeros(8, 16, device=device).half()
+    b, r = torch.zeros(8, device=device).half(), torch.zeros(6, 8, device=device).half()
+    for call in (lambda: linear(x.float(), w.float()), lambda: linear(x, w.bfloat16()), lambda: linear(x.cpu(), w.cpu()), lambda: linear(x, w.cpu()),
+                 lambda: linear(x, w[0]), lambda: linear(x, w[:, :15]), lambda: linear(x.t(), w), lambda: linear(x, w.t()),
+                 lambda: linear(x[:1].expand(6, 16), w), lambda: linear(x, w[:1].expand(8, 16)), lambda: linear(x, w, b[:7]),
+                 lambda: linear(x, w, b.double()), lambda: linear(x, w, b.cpu()), lambda: linear(x, w, b[None]),
+                 lambda: linear(x, w, torch.zeros(16, device=device)[::2]), lambda: linear(x, w, residual=r[:5]), lambda: linear(x, w, residual=r[0]),
+                 lambda: linear(x, w, residual=r.double()), lambda: linear(x, w, residual=r.cpu()), lambda: linear(x, w, residual=r[:1].expand(6, 8)),
+                 lambda: linear(x, w, out_dtype=torch.float64), lambda: linear(x, w[:7], activation="swiglu"),
+                 lambda: linear(x, w, activation="swiglu", clamp_limit=0.0), lambda: linear(x, w, activation="swiglu", clamp_limit=float("nan")),
+                 lambda: linear(x, w, out=r.float(), out_dtype=torch.float16), lambda: linear(x, w, out=r[:5]), lambda: linear(x, w, out=x[:, :8]),
+                 lambda: linear(x, w, out=r.t().contiguous().t()), lambda: linear(x[:, :0], w[:, :0]), lambda: linear(x, w[:0]),
+                 lambda: linear(x, w.requires_grad_(), out=r)):
+        with pytest.raises(RuntimeError):
+            call()
+            pytest.fail("taken")
+    w = w.detach()
+    for call in (lambda: linear(x, w, activation="tanh"), lambda: linear(x, w, clamp_limit=7.0)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        leaf = x.clone().requires_grad_()
+        torch.autograd.grad(linear(leaf, w).sum(), leaf, create_graph=True)
+
+
+@pytest.mark.parametrize("rows", [1, 30, 300])
+@pytest.mark.parametrize("activation", ["gelu", "swiglu"])
+def test_graph_and_streams(linear, device, rows, activation):
+    """Forward and backward captured, replayed with new inputs between eager work, and
+    eager calls on two streams at once: equal bits."""
+    rng = np.random.default_rng(rows)
+    lines = 2 * 72 if activation == "swiglu" else 72
+    sets = [(normal(rng, (rows, 1000), "fp16", device), normal(rng, (lines, 1000), "fp16", device, 0.03), normal(rng, lines, "fp16", device),
+             normal(rng, (rows, 72), "fp16", device), normal(rng, (rows, 72), "fp16", device)) for _ in range(3)]
+
+    def step(x, w, b, r, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = linear(*leaves[:3], activation, leaves[3])
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = [step(*s) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = step(*sets[0])
+    second = step(*sets[1])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for got, w in ((first, want[0]), (second, want[1])):
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
+    static = tuple(t.clone() for t in sets[0])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for i in (1, 2, 0, 1):
+        for dst, src in zip(static, sets[i]):
+            dst.copy_(src)
+        graph.replay()
+        again = step(*sets[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+        assert all(torch.equal(a, b) for a, b in zip(again, want[i]))

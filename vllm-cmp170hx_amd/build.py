@@ -34,7 +34,7 @@ SOURCES = [("exl3_gemv_part.hip", f"exl3_gemv_part{p}", [f"-DVQ_GEMV_PART={p}"])
            ("exl3_linear.hip", "exl3_linear", []), ("exl3_moe.hip", "exl3_moe", []),
            ("exl3_ple.hip", "exl3_ple", []), ("mxfp4.hip", "mxfp4", []),
            ("mxfp4_moe.hip", "mxfp4_moe", []), ("moe_balance.hip", "moe_balance", []),
-           ("moe_route_logits.hip", "moe_route_logits", []),
+           ("moe_route_logits.hip", "moe_route_logits", []), ("dense.hip", "dense", []),
            ("common.cpp", "common", [])]
 
 ARCH = "gfx950"
@@ -95,19 +95,20 @@ def _check_undefined(library: str) -> None:
     res = subprocess.run([nm, "-u", "-C", library], capture_output=True, text=True)
     bad = [line.strip() for line in res.stdout.splitlines()
            if "__device_stub__" in line or any(ns in line for ns in ("exl3::", "marlin::", "vq::", "mx::", "moe::",
-                                                                    "balance::", "route::", "logits::"))]
+                                                                    "balance::", "route::", "logits::", "dense::"))]
     if bad:
         os.remove(library)
         raise RuntimeError("linked library has undefined project symbols:\n  " + "\n  ".join(bad[:10]))
 
 
 TORCH_LIBRARY_PATH = os.path.join(PACKAGE, "libvllm_mi355x_torch.so")
-TORCH_SOURCES = ["torch_classes", "torch_ops", "torch_mxfp4", "torch_balance", "torch_route"]
+TORCH_SOURCES = ["torch_classes", "torch_ops", "torch_mxfp4", "torch_balance", "torch_route",
+                 "torch_dense"]
 
 
 def build_torch_classes(verbose: bool = False) -> str:
     """libvllm_mi355x_torch.so: the operators' host side (csrc/torch_ops.cpp,
-    torch_mxfp4.cpp, torch_balance.cpp, torch_route.cpp) and the torch custom classes the
+    torch_mxfp4.cpp, torch_balance.cpp, torch_route.cpp, torch_dense.cpp) and the torch custom classes the
     reference's loader requires (csrc/torch_classes.cpp): host-only, built with
     g++ against the installed torch, one process a source."""
     import torch

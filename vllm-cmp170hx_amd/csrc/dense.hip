@@ -1,0 +1,677 @@
+// The dense linear layer: few rows, many rows (dense_tile.h), the sum of K splits, and
+// the gradient.
+//
+// With dy the gradient of y and z = x W^T + b,
+//
+//   dz = dy act'(z)   (gated: dg = dy clamp(u) silu'(g) where g <= L, du = dy silu(min(g, L))
+//                      where |u| <= L)
+//   dx = dz W,   dW = dz^T x,   db = sum over rows of dz,
+//
+// so two more products, whose sums run over the lines and over the rows.  Both run on
+// the tiles of dense_tile.h, which want what is summed over to lie together: W and x
+// are transposed into the workspace, dz is written both ways.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <initializer_list>
+
+#include "../../include/vllm_mi355x.h"
+#include "common.h"
+#include "dense.h"
+#include "dense_tile.h"
+
+namespace dense {
+namespace {
+
+constexpr int64_t kMaxK = 1 << 21;       // 256 rows of a tile stay below 2^31 bytes
+constexpr int64_t kMaxStride = 1 << 22;
+constexpr int64_t kMaxSize = int64_t(1) << 30;  // rows, lines
+
+// ---- few rows ---------------------------------------------------------------------
+//
+// W is read once, from memory to the registers of the wavefront that multiplies it: a
+// wavefront holds 16 lines (a gated activation: 16 gate and the 16 up lines of the same
+// columns), per step 128 k, in which lane (r = lane & 15, q = lane >> 4) loads the
+// chunks 4 j + q (j < 4) of line r and of x's row r and multiplies them in four
+// v_mfma_16x16x32.  K is split over the wavefronts of a workgroup, whose sums meet in
+// LDS and are added in order.
+
+constexpr int kSmallRows = 16;  // of one B operand
+constexpr int kStepChunks = 16;
+
+template <bool kBf16>
+__device__ __forceinline__ u32x4_t load_chunk(const uint16_t* row, int64_t b, int64_t k) {
+  u32x4_t v{0, 0, 0, 0};
+  if (kChunk * b + kChunk <= k) {
+    __builtin_memcpy(&v, row + kChunk * b, 16);  // (of any alignment)
+  } else if (kChunk * b < k) {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      if (kChunk * b + i < k) w[i / 2] |= uint32_t(row[kChunk * b + i]) << (16 * (i & 1));
+    }
+    v = u32x4_t{w[0], w[1], w[2], w[3]};
+  }
+  return v;
+}
+
+template <int kTiles, bool kGated, bool kBf16>
+__global__ __launch_bounds__(1024) void small_kernel(Operand x, Operand w, int64_t k, Epilogue e) {
+  constexpr int kOps = kGated ? 2 : 1;
+  extern __shared__ __attribute__((aligned(16))) float sums[];  // [wave][kOps][kTiles][64 lanes][4]
+  const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6), waves = int(blockDim.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int64_t c0 = int64_t(blockIdx.x) * 16;
+  const int64_t line = min(c0 + r, e.n - 1);
+  const uint16_t* wrow[kOps];
+#pragma unroll
+  for (int o = 0; o < kOps; ++o) wrow[o] = w.p + (line + o * e.n) * w.stride;
+  const uint16_t* xrow[kTiles];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) xrow[t] = x.p + min(int64_t(kSmallRows * t + r), x.rows - 1) * x.stride;
+  f32x4_t acc[kOps][kTiles];
+#pragma unroll
+  for (int o = 0; o < kOps; ++o)
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) acc[o][t] = f32x4_t{0, 0, 0, 0};
+  const int64_t steps = (k + kChunk * kStepChunks - 1) / (kChunk * kStepChunks);
+  for (int64_t s = wave; s < steps; s += waves) {
+    u32x4_t a[kOps][4], b[kTiles][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t at = s * kStepChunks + 4 * j + q;
+#pragma unroll
+      for (int o = 0; o < kOps; ++o) a[o][j] = load_chunk<kBf16>(wrow[o], at, k);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) b[t][j] = load_chunk<kBf16>(xrow[t], at, k);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int o = 0; o < kOps; ++o)
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) mfma16<kBf16>(acc[o][t], a[o][j], b[t][j]);
+  }
+#pragma unroll
+  for (int o = 0; o < kOps; ++o)
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+      *reinterpret_cast<f32x4_t*>(sums + (((wave * kOps + o) * kTiles + t) * 64 + lane) * 4) = acc[o][t];
+  __syncthreads();
+  for (int t = wave; t < kTiles; t += waves) {
+    float v[4], u[4];
+#pragma unroll
+    for (int o = 0; o < kOps; ++o) {
+      f32x4_t all{0, 0, 0, 0};
+      for (int from = 0; from < waves; ++from) all += *reinterpret_cast<const f32x4_t*>(sums + (((from * kOps + o) * kTiles + t) * 64 + lane) * 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) (o ? u : v)[i] = all[i];
+    }
+    const int64_t m = kSmallRows * t + r;
+    if (m < x.rows) finish_columns<4>(e, m, c0 + 4 * q, v, u);
+  }
+}
+
+// ---- the sum of K splits --------------------------------------------------------------
+
+__global__ __launch_bounds__(256) void finish_kernel(const float* sums, int splits, int64_t rows, Epilogue e) {
+  const bool gated = e.activation == kSwiglu;
+  const int64_t lines = gated ? 2 * e.n : e.n, eighths = (e.n + 7) / 8;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * eighths; i += int64_t(gridDim.x) * 256) {
+    const int64_t m = i / eighths, c = i % eighths * 8;
+    float v[8], u[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = u[q] = 0;
+    for (int s = 0; s < splits; ++s) {
+      float a[8];
+      const float* from = sums + (s * rows + m) * lines + c;
+      load_columns<8>(from, vq::kFP32, 0, e.n - c, a);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += a[q];
+      if (gated) {
+        load_columns<8>(from + e.n, vq::kFP32, 0, e.n - c, a);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) u[q] += a[q];
+      }
+    }
+    finish_columns<8>(e, m, c, v, u);
+  }
+}
+
+// ---- operands that do not lie as the tiles want them -----------------------------------
+
+// out [rows][stride] = in's rows of k, zeros up to whole chunks.
+__global__ __launch_bounds__(256) void pack_kernel(Operand in, int64_t k, uint16_t* out, int64_t stride) {
+  const int64_t chunks = stride / kChunk;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < in.rows * chunks; i += int64_t(gridDim.x) * 256) {
+    const int64_t m = i / chunks, b = i % chunks;
+    *reinterpret_cast<u32x4_t*>(out + m * stride + kChunk * b) = load_chunk<true>(in.p + m * in.stride, b, k);
+  }
+}
+
+// A 64 x 64 part of a transposition through LDS: rows of 64 elements and one dword more.
+constexpr int kPart = 64, kPartStride = kPart + 2;
+
+// out [k][out_stride] = the transpose of in [rows][k], zeros up to whole chunks of rows.
+__global__ __launch_bounds__(256) void transpose_kernel(Operand in, int64_t k, uint16_t* out, int64_t out_stride) {
+  __shared__ uint16_t part[kPart * kPartStride];
+  const int64_t m0 = int64_t(blockIdx.y) * kPart, k0 = int64_t(blockIdx.x) * kPart;
+  const int ch = threadIdx.x & 7, row = threadIdx.x >> 3;
+#pragma unroll
+  for (int i = 0; i < kPart; i += 32) {
+    const int64_t m = m0 + row + i;
+    u32x4_t v{0, 0, 0, 0};
+    if (m < in.rows) v = load_chunk<true>(in.p + m * in.stride, k0 / kChunk + ch, k);
+    uint32_t* to = reinterpret_cast<uint32_t*>(part + (row + i) * kPartStride + kChunk * ch);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[j] = v[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPart; i += 32) {
+    const int64_t line = k0 + row + i, m = m0 + kChunk * ch;
+    u32x4_t v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint16_t* from = part + (kChunk * ch + 2 * j) * kPartStride + row + i;
+      v[j] = uint32_t(from[0]) | (uint32_t(from[kPartStride]) << 16);
+    }
+    if (line < k && m < out_stride) *reinterpret_cast<u32x4_t*>(out + line * out_stride + m) = v;
+  }
+}
+
+// ---- the gradient of z ------------------------------------------------------------------
+
+struct Slopes {
+  const void* dy;  // [rows][n], stride dy_stride
+  int dy_dtype;
+  int64_t dy_stride;
+  const uint16_t* z;  // [rows][lines], or null without an activation
+  int dtype, activation;
+  float limit;
+  int64_t rows, n, lines;
+};
+
+// Slopes are 0 or 1 from here on (z may be an infinity, having been rounded to FP16).
+constexpr float kFar = 104.0f;
+
+// dz at row m, lines c .. c + 7 (of which `valid` exist).
+__device__ __forceinline__ void slopes8(const Slopes& g, int64_t m, int64_t c, float (&v)[8]) {
+  const int64_t valid = m < g.rows ? g.lines - c : 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] = 0;
+  if (valid <= 0) return;
+  if (g.activation == kSwiglu) {
+    // (eight lines may begin in the gate half and end in the up half)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      if (q >= valid) continue;
+      const bool up = c + q >= g.n;
+      const int64_t col = up ? c + q - g.n : c + q;
+      const float a = vq::load_act(g.z, g.dtype, m * g.lines + col), b = vq::load_act(g.z, g.dtype, m * g.lines + g.n + col);
+      const float dy = vq::load_act(g.dy, g.dy_dtype, m * g.dy_stride + col);
+      // (kept as infinities where they lie outside)
+      const bool clamped = g.limit < __builtin_inff();
+      const float gate = clamp_above(a, g.limit);
+      if (up) v[q] = clamped && fabsf(b) == __builtin_inff() ? 0.0f : dy * silu(gate < -kFar ? -kFar : gate);
+      else v[q] = clamped && a == __builtin_inff() ? 0.0f : dy * clamp_both(b, g.limit) * silu_slope(clamp_both(gate, kFar));
+    }
+    return;
+  }
+  float dy[8];
+  load_columns<8>(g.dy, g.dy_dtype, m * g.dy_stride + c, valid, dy);
+  if (g.z) {
+    float z[8];
+    load_columns<8>(g.z, g.dtype, m * g.lines + c, valid, z);
+    const auto each = [&](float (*f)(float)) __attribute__((always_inline)) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = dy[q] * f(clamp_both(z[q], kFar));
+    };
+    switch (g.activation) {
+      case kRelu: each(relu_slope); break;
+      case kGelu: each(gelu_slope); break;
+      case kGeluTanh: each(gelu_tanh_slope); break;
+      default: each(silu_slope); break;
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = dy[q];
+  }
+}
+
+// FP16 holds dz over a power of two that brings its largest magnitude to 2^13 .. 2^14:
+// gradients of a mean are often below what FP16 holds, and products with up lines may be
+// above.  top: the FP32 bits of that magnitude.
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  const int e = int(top >> 23);
+  if (e == 0 || e == 255) return 1.0f;  // nothing, or no number
+  return __builtin_amdgcn_ldexpf(1.0f, min(13 - (e - 127), 126));
+}
+
+__global__ void clear_kernel(uint32_t* top) {
+  if (threadIdx.x == 0) *top = 0;
+}
+
+__global__ __launch_bounds__(256) void top_kernel(Slopes g, uint32_t* top) {
+  const int64_t eighths = (g.lines + 7) / 8;
+  uint32_t most = 0;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < g.rows * eighths; i += int64_t(gridDim.x) * 256) {
+    float v[8];
+    slopes8(g, i / eighths, i % eighths * 8, v);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) most = max(most, __builtin_bit_cast(uint32_t, v[q]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) most = max(most, uint32_t(__shfl_xor(int(most), d)));
+  if ((threadIdx.x & 63) == 0 && most) atomicMax(top, most);  // (the largest, in any order)
+}
+
+__global__ void factor_kernel(const uint32_t* top, float* factor) {
+  if (threadIdx.x == 0) *factor = 1 / scale_of(*top);
+}
+
+// dz of 64 rows and 64 lines: by rows (stride `ld`, zeros up to whole chunks of lines), by
+// lines (stride `ldt`, zeros up to whole chunks of rows), and the lines' sums over these rows.
+__global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* top, uint16_t* dz, int64_t ld, uint16_t* dzt, int64_t ldt,
+                                                     float* partial) {
+  __shared__ uint16_t part[kPart * kPartStride];
+  __shared__ float sum[32][kPart + 1];
+  const int64_t m0 = int64_t(blockIdx.y) * kPart, c0 = int64_t(blockIdx.x) * kPart;
+  const int ch = threadIdx.x & 7, row = threadIdx.x >> 3;
+  const float scale = top ? scale_of(*top) : 1.0f;
+  float mine[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) mine[q] = 0;
+#pragma unroll
+  for (int i = 0; i < kPart; i += 32) {
+    const int64_t m = m0 + row + i, c = c0 + kChunk * ch;
+    float v[8];
+    slopes8(g, m, c, v);
+    u32x4_t w;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) mine[q] += v[q];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack16(g.dtype, v[2 * j] * scale, v[2 * j + 1] * scale);
+    if (dz && m < g.rows && c < ld) *reinterpret_cast<u32x4_t*>(dz + m * ld + c) = w;
+    uint32_t* to = reinterpret_cast<uint32_t*>(part + (row + i) * kPartStride + kChunk * ch);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) to[j] = w[j];
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) sum[row][kChunk * ch + q] = mine[q];
+  __syncthreads();
+  if (dzt) {
+#pragma unroll
+    for (int i = 0; i < kPart; i += 32) {
+      const int64_t line = c0 + row + i, m = m0 + kChunk * ch;
+      u32x4_t v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint16_t* from = part + (kChunk * ch + 2 * j) * kPartStride + row + i;
+        v[j] = uint32_t(from[0]) | (uint32_t(from[kPartStride]) << 16);
+      }
+      if (line < g.lines && m < ldt) *reinterpret_cast<u32x4_t*>(dzt + line * ldt + m) = v;
+    }
+  }
+  if (partial && threadIdx.x < kPart && c0 + threadIdx.x < g.lines) {
+    float all = 0;
+    for (int i = 0; i < 32; ++i) all += sum[i][threadIdx.x];
+    partial[int64_t(blockIdx.y) * g.lines + c0 + threadIdx.x] = all;
+  }
+}
+
+// db = the parts' sums, in order.
+__global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t parts, int64_t lines, void* out, int dtype) {
+  const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (c >= lines) return;
+  float all = 0;
+  for (int64_t p = 0; p < parts; ++p) all += partial[p * lines + c];
+  vq::store_act(out, dtype, c, all);
+}
+
+// ---- how a product runs -----------------------------------------------------------------
+
+int64_t up_to(int64_t v, int64_t step) { return (v + step - 1) / step * step; }
+int64_t parts_of(int64_t v, int64_t step) { return (v + step - 1) / step; }
+
+struct Plan {
+  int tile;  // 64 tile rows and lines; 0: the few rows' kernel
+  int splits;
+  int waves;  // of the few rows' kernel
+};
+
+constexpr int kCus = 256;
+
+Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated) {
+  const int64_t lines = gated ? 2 * n : n;
+  if (rows <= 64) {
+    const int64_t steps = parts_of(k, kChunk * kStepChunks);
+    // (up to 64 KB of sums)
+    return {0, 1, steps >= 16 && !(gated && rows > 32) ? 16 : steps >= 8 ? 8 : 4};
+  }
+  const int64_t stages = parts_of(k, kChunk * kStageChunks);
+  Plan best{4, 1, 0};
+  double least = 0;
+  for (int tile : {4, 2, 1}) {
+    if (gated && tile == 1) continue;
+    const int64_t tiles = parts_of(rows, 64 * tile) * parts_of(lines, 64 * tile);
+    const int64_t places = kCus * (tile == 4 ? 1 : 2);
+    for (int64_t splits = 1; splits <= 16 && splits <= std::max<int64_t>(1, stages / 4); ++splits) {
+      const double rounds = double(parts_of(tiles * splits, places));
+      const double stage = tile == 4 ? 1.0 : tile == 2 ? 0.7 : 0.4;
+      double cost = rounds * (4 + double(parts_of(stages, splits)) * stage);
+      if (splits > 1) cost += 4 + double(splits) * double(rows) * double(lines) * 8 / 4e6;
+      if (least == 0 || cost < least) {
+        least = cost;
+        best = {tile, int(splits), 0};
+      }
+    }
+  }
+  return best;
+}
+
+bool direct(const Operand& o, int64_t k) { return aligned(o.p, 16) && o.stride % kChunk == 0 && k % kChunk == 0 && o.stride <= kMaxStride; }
+
+int64_t sums_bytes(const Plan& p, int64_t rows, int64_t lines) { return p.splits > 1 ? p.splits * rows * lines * 4 : 0; }
+
+template <int kTiles>
+void launch_small(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, bool bf16, int waves, hipStream_t s) {
+  const bool gated = e.activation == kSwiglu;
+  const dim3 grid(unsigned(parts_of(e.n, 16))), block(unsigned(64 * waves));
+  const size_t lds = size_t(waves) * (gated ? 2 : 1) * kTiles * 64 * 16;
+  if (gated) {
+    if (bf16) hipLaunchKernelGGL((small_kernel<kTiles, true, true>), grid, block, lds, s, x, w, k, e);
+    else hipLaunchKernelGGL((small_kernel<kTiles, true, false>), grid, block, lds, s, x, w, k, e);
+  } else {
+    if (bf16) hipLaunchKernelGGL((small_kernel<kTiles, false, true>), grid, block, lds, s, x, w, k, e);
+    else hipLaunchKernelGGL((small_kernel<kTiles, false, false>), grid, block, lds, s, x, w, k, e);
+  }
+}
+
+template <int kSize, int kBufs>
+void launch_tile(TileArgs& t, bool bf16, int64_t splits, hipStream_t s) {
+  const bool gated = t.e.activation == kSwiglu;
+  const int64_t total = int64_t(t.tiles_n) * t.tiles_m;
+  const dim3 grid(unsigned(up_to(total, 8)), unsigned(splits)), block(kTileThreads);
+  if constexpr (kSize >= 2) {
+    if (gated) {
+      if (bf16) hipLaunchKernelGGL((tile_kernel<kSize, kSize, true, kBufs, true>), grid, block, 0, s, t);
+      else hipLaunchKernelGGL((tile_kernel<kSize, kSize, true, kBufs, false>), grid, block, 0, s, t);
+      return;
+    }
+  }
+  if (bf16) hipLaunchKernelGGL((tile_kernel<kSize, kSize, false, kBufs, true>), grid, block, 0, s, t);
+  else hipLaunchKernelGGL((tile_kernel<kSize, kSize, false, kBufs, false>), grid, block, 0, s, t);
+}
+
+// x [rows][k] times W's transpose, finished by e; sums: the plan's K splits' room.
+int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, bool bf16, float* sums, const Plan& p, hipStream_t s) {
+  if (p.tile == 0) {
+    if (x.rows <= 16) launch_small<1>(x, w, k, e, bf16, p.waves, s);
+    else if (x.rows <= 32) launch_small<2>(x, w, k, e, bf16, p.waves, s);
+    else launch_small<4>(x, w, k, e, bf16, p.waves, s);
+    return vq::check_launch("dense_linear");
+  }
+  const bool gated = e.activation == kSwiglu;
+  const int64_t side = 64 * p.tile, stages = parts_of(k, kChunk * kStageChunks);
+  const int64_t tiles_n = parts_of(e.n, gated ? side / 2 : side), tiles_m = parts_of(x.rows, side);
+  if (tiles_n * tiles_m > INT_MAX / 2) return vq::fail("dense_linear: too many rows and columns");
+  const int64_t split = parts_of(stages, p.splits);
+  TileArgs t{x, w, int(parts_of(k, kChunk)), int(tiles_n), int(tiles_m), int(split), sums, e};
+  const int64_t splits = parts_of(stages, split);  // (none without a stage)
+  if (p.tile == 4) launch_tile<4, 2>(t, bf16, splits, s);
+  else if (p.tile == 2) launch_tile<2, 2>(t, bf16, splits, s);
+  else launch_tile<1, 4>(t, bf16, splits, s);
+  if (int rc = vq::check_launch("dense_linear")) return rc;
+  if (splits == 1) return vq::kOk;
+  const int64_t groups = parts_of(x.rows * parts_of(e.n, 8), 256);
+  hipLaunchKernelGGL(finish_kernel, dim3(unsigned(std::min<int64_t>(groups, 8192))), dim3(256), 0, s, sums, int(splits), x.rows, e);
+  return vq::check_launch("dense_linear");
+}
+
+int pack(Operand& o, int64_t k, uint16_t* to, hipStream_t s) {
+  const int64_t stride = up_to(k, kChunk), groups = parts_of(o.rows * (stride / kChunk), 256);
+  hipLaunchKernelGGL(pack_kernel, dim3(unsigned(std::min<int64_t>(groups, 16384))), dim3(256), 0, s, o, k, to, stride);
+  o.p = to;
+  o.stride = stride;
+  return vq::check_launch("dense_linear");
+}
+
+int transpose(const Operand& o, int64_t k, uint16_t* to, int64_t stride, hipStream_t s) {
+  hipLaunchKernelGGL(transpose_kernel, dim3(unsigned(parts_of(k, kPart)), unsigned(parts_of(o.rows, kPart))), dim3(256), 0, s, o, k, to, stride);
+  return vq::check_launch("dense_linear");
+}
+
+int check_sizes(int64_t rows, int64_t k, int64_t n, int activation) {
+  if (rows < 0 || rows > kMaxSize) return vq::fail("dense_linear: rows out of range");
+  if (k <= 0 || k > kMaxK) return vq::fail("dense_linear: k must be between 1 and 2^21");
+  if (n <= 0 || n > kMaxSize) return vq::fail("dense_linear: columns out of range");
+  if (activation < kNone || activation > kSwiglu) return vq::fail("dense_linear: unknown activation");
+  return vq::kOk;
+}
+
+bool is_half(int dtype) { return dtype == vq::kBF16 || dtype == vq::kFP16; }
+bool is_float(int dtype) { return is_half(dtype) || dtype == vq::kFP32; }
+
+int check_inputs(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t w_stride, float limit) {
+  if (!is_half(dtype)) return vq::fail("dense_linear: x and the weights must be BF16 or FP16");
+  if (!x || !w) return vq::fail("dense_linear: null pointer");
+  if (x_stride < 0 || (rows > 1 && x_stride < k) || x_stride > (int64_t(1) << 40) || w_stride < k || w_stride > (int64_t(1) << 40)) {
+    return vq::fail("dense_linear: row stride out of range");
+  }
+  if (!(limit > 0)) return vq::fail("dense_linear: the clamp limit must be positive");
+  return vq::kOk;
+}
+
+struct Span {
+  const void* p;
+  int64_t bytes, element;
+};
+int check_spans(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  for (const Span* a = outputs.begin(); a != outputs.end(); ++a) {
+    for (const Span* b = outputs.begin(); b != a; ++b) {
+      if (vq::overlaps(a->p, a->bytes, b->p, b->bytes)) return vq::fail("dense_linear: arguments must not overlap");
+    }
+    for (const Span& b : inputs) {
+      if (vq::overlaps(a->p, a->bytes, b.p, b.bytes)) return vq::fail("dense_linear: arguments must not overlap");
+    }
+  }
+  for (const auto* list : {&outputs, &inputs}) {
+    for (const Span& a : *list) {
+      if (reinterpret_cast<uintptr_t>(a.p) % uintptr_t(a.element)) return vq::fail("dense_linear: misaligned pointer");
+    }
+  }
+  return vq::kOk;
+}
+int64_t span_bytes(int64_t rows, int64_t cols, int64_t stride, int dtype) {
+  return rows > 0 ? ((rows - 1) * stride + cols) * vq::dtype_bytes(dtype) : 0;
+}
+
+// The forward's workspace: the K splits' sums, then packed operands.
+struct Room {
+  int64_t sums, x, w, bytes;
+  Room(int64_t rows, int64_t k, int64_t lines, const Plan& p, bool pack_x, bool pack_w) {
+    const int64_t row = up_to(k, kChunk) * 2;
+    sums = up_to(sums_bytes(p, rows, lines), 256);
+    x = pack_x ? up_to(rows * row, 256) : 0;
+    w = pack_w ? up_to(lines * row, 256) : 0;
+    bytes = sums + x + w;
+  }
+};
+
+// The gradient's: the sums (of either product), then the operands by what they are summed over.
+struct GradRoom {
+  Plan px, pw;
+  int64_t sums, wt, xt, dz, dzt, partial, top, bytes;
+  GradRoom(int64_t rows, int64_t k, int64_t lines, bool need_x, bool need_w, bool need_bias) {
+    px = plan_of(rows, lines, k, false);
+    pw = plan_of(lines, rows, k, false);
+    const int64_t ld = up_to(lines, kChunk) * 2, ldt = up_to(rows, kChunk) * 2;
+    sums = up_to(std::max(need_x ? sums_bytes(px, rows, k) : 0, need_w ? sums_bytes(pw, lines, k) : 0), 256);
+    wt = need_x ? up_to(k * ld, 256) : 0;
+    xt = need_w ? up_to(k * ldt, 256) : 0;
+    dz = need_x ? up_to(rows * ld, 256) : 0;
+    dzt = need_w ? up_to(lines * ldt, 256) : 0;
+    partial = need_bias ? up_to(parts_of(rows, kPart) * lines * 4, 256) : 0;
+    top = 256;
+    bytes = sums + wt + xt + dz + dzt + partial + top;
+  }
+};
+
+}  // namespace
+}  // namespace dense
+
+extern "C" int64_t dense_linear_workspace_size(const void* x, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t n,
+                                               int64_t w_stride, int activation) {
+  using namespace dense;
+  if (check_sizes(rows, k, n, activation)) return -1;
+  if (rows == 0) return 0;
+  const bool gated = activation == kSwiglu;
+  const int64_t lines = gated ? 2 * n : n;
+  const Plan p = plan_of(rows, k, n, gated);
+  const bool tiles = p.tile != 0;
+  const Operand xo{static_cast<const uint16_t*>(x), rows, x_stride}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
+  return Room(rows, k, lines, p, tiles && !direct(xo, k), tiles && !direct(wo, k)).bytes;
+}
+
+extern "C" int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int32_t* plan) {
+  using namespace dense;
+  if (int rc = check_sizes(rows, k, n, activation)) return rc;
+  if (!plan) return vq::fail("dense_linear: null pointer");
+  const Plan p = plan_of(rows, k, n, activation == kSwiglu);
+  plan[0] = 64 * p.tile;
+  plan[1] = p.splits;
+  plan[2] = p.waves;
+  return vq::kOk;
+}
+
+extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t n, int64_t w_stride,
+                            const void* bias, int bias_dtype, int activation, float limit, const void* residual, int residual_dtype,
+                            int64_t residual_stride, void* out, int out_dtype, void* z, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  using namespace dense;
+  if (int rc = check_sizes(rows, k, n, activation)) return rc;
+  if (!is_float(out_dtype) || (bias && !is_float(bias_dtype)) || (residual && !is_float(residual_dtype))) {
+    return vq::fail("dense_linear: bias, residual and output must be BF16, FP16 or FP32");
+  }
+  if (rows == 0) return vq::kOk;
+  if (int rc = check_inputs(x, dtype, rows, k, x_stride, w, w_stride, limit)) return rc;
+  if (!out) return vq::fail("dense_linear: null pointer");
+  if (residual && (residual_stride < 0 || (rows > 1 && residual_stride < n))) return vq::fail("dense_linear: residual stride out of range");
+  const bool gated = activation == kSwiglu;
+  const int64_t lines = gated ? 2 * n : n;
+  Operand xo{static_cast<const uint16_t*>(x), rows, rows > 1 ? x_stride : k}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
+  const Plan p = plan_of(rows, k, n, gated);
+  const bool pack_x = p.tile && !direct(xo, k), pack_w = p.tile && !direct(wo, k);
+  const Room room(rows, k, lines, p, pack_x, pack_w);
+  if (room.bytes && (!workspace || workspace_bytes < room.bytes || !aligned(workspace, 16))) {
+    return vq::fail("dense_linear: workspace too small or misaligned");
+  }
+  // (the output may be the residual: an element is read before it is written, by the same lane)
+  const bool in_place = residual == out && residual_dtype == out_dtype && (rows == 1 || residual_stride == n);
+  if (int rc = check_spans({{out, rows * n * vq::dtype_bytes(out_dtype), vq::dtype_bytes(out_dtype)},
+                            {z, z ? rows * lines * 2 : 0, 2},
+                            {workspace, room.bytes, 1}},
+                           {{x, span_bytes(rows, k, xo.stride, dtype), 2},
+                            {w, span_bytes(lines, k, w_stride, dtype), 2},
+                            {bias, bias ? lines * vq::dtype_bytes(bias_dtype) : 0, bias ? vq::dtype_bytes(bias_dtype) : 1},
+                            {in_place ? nullptr : residual, residual ? span_bytes(rows, n, residual_stride, residual_dtype) : 0,
+                             residual ? vq::dtype_bytes(residual_dtype) : 1}})) {
+    return rc;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  float* sums = reinterpret_cast<float*>(at);
+  at += room.sums;
+  if (pack_x) {
+    if (int rc = pack(xo, k, reinterpret_cast<uint16_t*>(at), s)) return rc;
+  }
+  at += room.x;
+  if (pack_w) {
+    if (int rc = pack(wo, k, reinterpret_cast<uint16_t*>(at), s)) return rc;
+  }
+  const Epilogue e{bias, bias_dtype, activation, limit, residual, residual_dtype, residual_stride, out, out_dtype, n, z, dtype, nullptr};
+  return product(xo, wo, k, e, dtype == vq::kBF16, sums, p, s);
+}
+
+extern "C" int64_t dense_linear_grad_workspace_size(int64_t rows, int64_t k, int64_t n, int activation, int need_x, int need_w, int need_bias) {
+  using namespace dense;
+  if (check_sizes(rows, k, n, activation)) return -1;
+  if (rows == 0) return 0;
+  return GradRoom(rows, k, activation == kSwiglu ? 2 * n : n, need_x, need_w, need_bias).bytes;
+}
+
+extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t n,
+                                 int64_t w_stride, const void* z, int activation, float limit, const void* dy, int dy_dtype,
+                                 int64_t dy_stride, void* dx, void* dw, void* dbias, int bias_dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  using namespace dense;
+  if (int rc = check_sizes(rows, k, n, activation)) return rc;
+  if (!is_float(dy_dtype) || (dbias && !is_float(bias_dtype))) return vq::fail("dense_linear: bias and output must be BF16, FP16 or FP32");
+  if (rows == 0) return vq::fail("dense_linear: no rows have no gradient to compute");
+  if (int rc = check_inputs(x, dtype, rows, k, x_stride, w, w_stride, limit)) return rc;
+  if (!dy || (activation != kNone && !z)) return vq::fail("dense_linear: null pointer");
+  if (dy_stride < 0 || (rows > 1 && dy_stride < n)) return vq::fail("dense_linear: gradient stride out of range");
+  const int64_t lines = activation == kSwiglu ? 2 * n : n;
+  const GradRoom room(rows, k, lines, dx, dw, dbias);
+  if (!workspace || workspace_bytes < room.bytes || !aligned(workspace, 16)) return vq::fail("dense_linear: workspace too small or misaligned");
+  const Operand xo{static_cast<const uint16_t*>(x), rows, rows > 1 ? x_stride : k}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
+  if (int rc = check_spans({{dx, dx ? rows * k * 2 : 0, 2},
+                            {dw, dw ? lines * k * 2 : 0, 2},
+                            {dbias, dbias ? lines * vq::dtype_bytes(bias_dtype) : 0, dbias ? vq::dtype_bytes(bias_dtype) : 1},
+                            {workspace, room.bytes, 1}},
+                           {{x, span_bytes(rows, k, xo.stride, dtype), 2},
+                            {w, span_bytes(lines, k, w_stride, dtype), 2},
+                            {z, activation != kNone ? rows * lines * 2 : 0, 2},
+                            {dy, span_bytes(rows, n, dy_stride, dy_dtype), vq::dtype_bytes(dy_dtype)}})) {
+    return rc;
+  }
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t* at = static_cast<uint8_t*>(workspace);
+  const auto take = [&](int64_t bytes) {
+    uint8_t* p = bytes ? at : nullptr;
+    at += bytes;
+    return p;
+  };
+  float* sums = reinterpret_cast<float*>(take(room.sums));
+  uint16_t* wt = reinterpret_cast<uint16_t*>(take(room.wt));
+  uint16_t* xt = reinterpret_cast<uint16_t*>(take(room.xt));
+  uint16_t* dz = reinterpret_cast<uint16_t*>(take(room.dz));
+  uint16_t* dzt = reinterpret_cast<uint16_t*>(take(room.dzt));
+  float* partial = reinterpret_cast<float*>(take(room.partial));
+  uint32_t* top = reinterpret_cast<uint32_t*>(take(room.top));
+  float* factor = reinterpret_cast<float*>(top) + 1;
+  const int64_t ld = up_to(lines, kChunk), ldt = up_to(rows, kChunk);
+  const Slopes g{dy, dy_dtype, rows > 1 ? dy_stride : n, activation == kNone ? nullptr : static_cast<const uint16_t*>(z), dtype, activation, limit,
+                 rows, n, lines};
+  const bool scaled = dtype == vq::kFP16 && (dx || dw);
+  if (scaled) {
+    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(64), 0, s, top);
+    const int64_t groups = parts_of(rows * parts_of(lines, 8), 256);
+    hipLaunchKernelGGL(top_kernel, dim3(unsigned(std::min<int64_t>(groups, 2048))), dim3(256), 0, s, g, top);
+    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(64), 0, s, top, factor);
+    if (int rc = vq::check_launch("dense_linear gradient")) return rc;
+  }
+  hipLaunchKernelGGL(slopes_kernel, dim3(unsigned(parts_of(lines, kPart)), unsigned(parts_of(rows, kPart))), dim3(256), 0, s, g,
+                     scaled ? top : nullptr, dz, ld, dzt, ldt, partial);
+  if (int rc = vq::check_launch("dense_linear gradient")) return rc;
+  if (dbias) {
+    hipLaunchKernelGGL(bias_kernel, dim3(unsigned(parts_of(lines, 256))), dim3(256), 0, s, partial, parts_of(rows, kPart), lines, dbias,
+                       bias_dtype);
+    if (int rc = vq::check_launch("dense_linear gradient")) return rc;
+  }
+  const bool bf16 = dtype == vq::kBF16;
+  const auto plain = [&](void* out) {
+    return Epilogue{nullptr, 0, kNone, __builtin_inff(), nullptr, 0, 0, out, dtype, k, nullptr, 0, scaled ? factor : nullptr};
+  };
+  if (dx) {
+    if (int rc = transpose(wo, k, wt, ld, s)) return rc;
+    if (int rc = product({dz, rows, ld}, {wt, k, ld}, lines, plain(dx), bf16, sums, room.px, s)) return rc;
+  }
+  if (dw) {
+    if (int rc = transpose(xo, k, xt, ldt, s)) return rc;
+    if (int rc = product({dzt, lines, ldt}, {xt, k, ldt}, rows, plain(dw), bf16, sums, room.pw, s)) return rc;
+  }
+  return vq::kOk;
+}

@@ -18,5 +18,6 @@ void check_status(int status);
 bool bind_mxfp4(void* library);
 bool bind_balance(void* library);
 bool bind_route(void* library);
+bool bind_dense(void* library);
 
 }  // namespace vq_torch

@@ -1,0 +1,308 @@
+// The dense linear layer (kernels/dense/ops.py) in host-only C++: tensor checks, outputs
+// and scratch from torch's allocator (so of the current stream, and of a graph's pool
+// under capture), the C-ABI calls on torch's current stream, and the gradient as an
+// autograd node that calls operators of its own below autograd.
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/Tensor.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
+#include <dlfcn.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "../../include/vllm_mi355x.h"
+#include "torch_common.h"
+
+namespace {
+
+using vq_torch::check_status;
+using vq_torch::dtype_code;
+using vq_torch::stream_of;
+
+decltype(&dense_linear) native_linear = nullptr;
+decltype(&dense_linear_workspace_size) native_workspace = nullptr;
+decltype(&dense_linear_grad) native_grad = nullptr;
+decltype(&dense_linear_grad_workspace_size) native_grad_workspace = nullptr;
+decltype(&vllm_mi355x_last_error) native_error = nullptr;
+
+constexpr const char* kWhat = "dense_linear";
+constexpr int64_t kSwiglu = 5;
+
+bool is_float(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat; }
+
+template <typename Size>
+std::vector<Size> with_last(c10::ArrayRef<Size> sizes, const Size& last) {
+  std::vector<Size> v = sizes.vec();
+  v.back() = last;
+  return v;
+}
+
+// t as rows of its last axis at one row stride; stride -1: they do not lie so.
+struct Rows {
+  int64_t rows, k, stride;
+};
+Rows rows_of(const at::Tensor& t) {
+  const int64_t k = t.size(-1);
+  const int64_t rows = k ? t.numel() / k : 0;
+  if (rows == 0) return {0, k, k};
+  if (k > 1 && t.stride(-1) != 1) return {rows, k, -1};
+  int64_t stride = k, count = 1;
+  bool first = true;
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (first) stride = t.stride(d);
+    else if (t.stride(d) != stride * count) return {rows, k, -1};
+    first = false;
+    count *= t.size(d);
+  }
+  return {rows, k, rows > 1 && stride < k ? -1 : stride};
+}
+
+// What needs no data; sizes may be symbolic.
+void check_kinds(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                 const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, kWhat, ": x must be BF16 or FP16");
+  TORCH_CHECK(w.scalar_type() == x.scalar_type(), kWhat, ": the weights must have x's type");
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2, kWhat, ": x must be [..., k], the weights [n, k]");
+  TORCH_CHECK(is_float(out_dtype), kWhat, ": out_dtype must be BF16, FP16 or FP32");
+  TORCH_CHECK(activation >= 0 && activation <= kSwiglu, kWhat, ": unknown activation");
+  TORCH_CHECK(limit > 0, kWhat, ": clamp_limit must be positive");
+  TORCH_CHECK(!bias || (bias->dim() == 1 && is_float(bias->scalar_type())), kWhat, ": bias must be BF16, FP16 or FP32, a value a weight row");
+  TORCH_CHECK(!residual || (residual->dim() == x.dim() && is_float(residual->scalar_type())), kWhat,
+              ": residual must be BF16, FP16 or FP32 of the output's shape");
+  for (const at::Tensor* t : {&w, bias ? &*bias : nullptr, residual ? &*residual : nullptr}) {
+    TORCH_CHECK(!t || t->device() == x.device(), kWhat, ": tensors must be on x's device");
+  }
+}
+
+int64_t columns_of(const at::Tensor& w, int64_t activation) {
+  TORCH_CHECK(activation != kSwiglu || w.size(0) % 2 == 0, kWhat, ": a gated activation needs gate and up rows in equal number");
+  return activation == kSwiglu ? w.size(0) / 2 : w.size(0);
+}
+
+void run(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+         const std::optional<at::Tensor>& residual, double limit, const at::Tensor& out, const at::Tensor& z) {
+  TORCH_CHECK(x.is_cuda(), kWhat, ": x must be on a GPU");
+  const Rows r = rows_of(x);
+  TORCH_CHECK(r.k > 0 && w.size(1) == r.k && w.size(0) > 0, kWhat, ": the weights must be [n, k] of x's k = ", r.k);
+  TORCH_CHECK(r.stride >= 0, kWhat, ": x needs unit stride along its last axis and leading axes that are one run of rows, not overlapping");
+  TORCH_CHECK((r.k == 1 || w.stride(1) == 1) && (w.size(0) == 1 || w.stride(0) >= r.k), kWhat,
+              ": the weights need unit inner stride and rows that do not overlap");
+  const int64_t n = columns_of(w, activation);
+  TORCH_CHECK(!bias || (bias->size(0) == w.size(0) && bias->is_contiguous()), kWhat, ": bias must be contiguous, a value a weight row");
+  Rows res{0, 0, 0};
+  if (residual) {
+    TORCH_CHECK(residual->sizes() == out.sizes(), kWhat, ": residual must have the output's shape");
+    res = rows_of(*residual);
+    TORCH_CHECK(res.stride >= 0, kWhat, ": residual needs unit stride along its last axis and leading axes that are one run of rows, not overlapping");
+  }
+  const c10::DeviceGuard guard(x.device());
+  const int64_t w_stride = w.size(0) > 1 ? w.stride(0) : r.k;
+  const int64_t bytes = native_workspace(x.const_data_ptr(), r.rows, r.k, r.stride, w.const_data_ptr(), n, w_stride, int(activation));
+  if (bytes < 0) TORCH_CHECK(false, native_error());
+  const at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check_status(native_linear(x.const_data_ptr(), dtype_code(x.scalar_type()), r.rows, r.k, r.stride, w.const_data_ptr(), n, w_stride,
+                             bias ? bias->const_data_ptr() : nullptr, bias ? dtype_code(bias->scalar_type()) : 0, int(activation),
+                             static_cast<float>(limit), residual ? residual->const_data_ptr() : nullptr,
+                             residual ? dtype_code(residual->scalar_type()) : 0, res.stride, out.mutable_data_ptr(),
+                             dtype_code(out.scalar_type()), z.defined() ? z.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), bytes,
+                             stream_of(x)));
+}
+
+at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                  const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
+  check_kinds(x, w, bias, activation, residual, out_dtype, limit);
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor out = at::empty(with_last(x.sizes(), columns_of(w, activation)), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
+  run(x, w, bias, activation, residual, limit, out, at::Tensor());
+  return out;
+}
+
+void linear_out(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                const std::optional<at::Tensor>& residual, double limit, const at::Tensor& out) {
+  check_kinds(x, w, bias, activation, residual, out.scalar_type(), limit);
+  TORCH_CHECK(out.is_contiguous() && out.device() == x.device() && out.sizes().vec() == with_last(x.sizes(), columns_of(w, activation)), kWhat,
+              ": out must be a contiguous [..., n] on x's GPU");
+  run(x, w, bias, activation, residual, limit, out, at::Tensor());
+}
+
+// (y, z): z is what the gradient needs beside x and w, x w^T + bias in x's type (nothing
+// without an activation).
+std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                                           const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
+  check_kinds(x, w, bias, activation, residual, out_dtype, limit);
+  const c10::DeviceGuard guard(x.device());
+  const int64_t n = columns_of(w, activation), k = x.size(-1);
+  TORCH_CHECK(k > 0, kWhat, ": the weights must be [n, k] of x's k = 0");
+  at::Tensor out = at::empty(with_last(x.sizes(), n), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor z = at::empty({activation ? x.numel() / k : 0, w.size(0)}, x.options().memory_format(at::MemoryFormat::Contiguous));
+  run(x, w, bias, activation, residual, limit, out, activation ? z : at::Tensor());
+  return {out, z};
+}
+
+// (dx, dw, dbias) from dy; those not asked for are empty.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient(const at::Tensor& x, const at::Tensor& w, const at::Tensor& z, int64_t activation,
+                                                        double limit, const at::Tensor& given, bool need_x, bool need_w,
+                                                        std::optional<at::ScalarType> bias_dtype) {
+  check_kinds(x, w, std::nullopt, activation, std::nullopt, given.scalar_type(), limit);
+  TORCH_CHECK(x.is_cuda() && given.device() == x.device() && z.device() == x.device(), kWhat, ": the gradient's tensors must be on x's GPU");
+  const int64_t n = columns_of(w, activation);
+  const Rows r = rows_of(x);
+  TORCH_CHECK(r.stride >= 0 && w.size(1) == r.k && given.numel() == r.rows * n &&
+                  (!activation || (z.is_contiguous() && z.numel() == r.rows * w.size(0) && z.scalar_type() == x.scalar_type())),
+              kWhat, ": the gradient's tensors must be the forward's");
+  const c10::DeviceGuard guard(x.device());
+  const auto nothing = [&] { return at::empty({0}, x.options()); };
+  const auto like = [&](const at::Tensor& t) {
+    return r.rows ? at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)) : at::zeros(t.sizes(), t.options());
+  };
+  at::Tensor dx = need_x ? like(x) : nothing(), dw = need_w ? like(w) : nothing();
+  at::Tensor db = !bias_dtype ? nothing()
+                  : r.rows    ? at::empty({w.size(0)}, x.options().dtype(*bias_dtype))
+                              : at::zeros({w.size(0)}, x.options().dtype(*bias_dtype));
+  if (r.rows == 0) return {dx, dw, db};
+  // (autograd gives broadcast and transposed gradients too)
+  const at::Tensor dy = rows_of(given).stride >= 0 ? given : given.contiguous();
+  const int64_t bytes = native_grad_workspace(r.rows, r.k, n, int(activation), need_x, need_w, bias_dtype.has_value());
+  if (bytes < 0) TORCH_CHECK(false, native_error());
+  const at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check_status(native_grad(x.const_data_ptr(), dtype_code(x.scalar_type()), r.rows, r.k, r.stride, w.const_data_ptr(), n,
+                           w.size(0) > 1 ? w.stride(0) : r.k, activation ? z.const_data_ptr() : nullptr, int(activation),
+                           static_cast<float>(limit), dy.const_data_ptr(), dtype_code(dy.scalar_type()), rows_of(dy).stride,
+                           need_x ? dx.mutable_data_ptr() : nullptr, need_w ? dw.mutable_data_ptr() : nullptr,
+                           bias_dtype ? db.mutable_data_ptr() : nullptr, bias_dtype ? dtype_code(*bias_dtype) : 0, ws.mutable_data_ptr(), bytes,
+                           stream_of(x)));
+  return {dx, dw, db};
+}
+
+template <typename F>
+c10::TypedOperatorHandle<F> handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+struct DenseLinear : torch::autograd::Function<DenseLinear> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const std::optional<at::Tensor>& bias, int64_t activation, const std::optional<at::Tensor>& residual,
+                            at::ScalarType out_dtype, double limit) {
+    static const auto op = handle<decltype(::forward)>("_vllm_mi355x::dense_linear_forward");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, z] = op.call(x, w, bias, activation, residual, out_dtype, limit);
+    // (x and w both: their types and sizes are those of the gradients)
+    ctx->save_for_backward({x, w, z});
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["limit"] = limit;
+    ctx->saved_data["x"] = x.requires_grad();
+    ctx->saved_data["w"] = w.requires_grad();
+    ctx->saved_data["bias"] = bias && bias->requires_grad() ? int64_t(bias->scalar_type()) : int64_t(-1);
+    ctx->saved_data["residual"] = residual && residual->requires_grad() ? int64_t(residual->scalar_type()) : int64_t(-1);
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(7);
+    if (!grads[0].defined()) return out;
+    TORCH_CHECK(!c10::GradMode::is_enabled(), kWhat, ": its gradient has no gradient (create_graph)");
+    static const auto op = handle<decltype(::gradient)>("_vllm_mi355x::dense_linear_grad");
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
+    const int64_t bias = ctx->saved_data["bias"].toInt(), residual = ctx->saved_data["residual"].toInt();
+    const bool need_x = ctx->saved_data["x"].toBool(), need_w = ctx->saved_data["w"].toBool();
+    if (residual >= 0) out[4] = grads[0].to(at::ScalarType(residual));
+    if (need_x || need_w || bias >= 0) {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      auto [dx, dw, db] = op.call(saved[0], saved[1], saved[2], ctx->saved_data["activation"].toInt(), ctx->saved_data["limit"].toDouble(),
+                                  grads[0], need_x, need_w, bias >= 0 ? std::optional<at::ScalarType>(at::ScalarType(bias)) : std::nullopt);
+      if (need_x) out[0] = dx;
+      if (need_w) out[1] = dw;
+      if (bias >= 0) out[2] = db;
+    }
+    return out;
+  }
+};
+
+at::Tensor linear_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                           const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
+  bool needs = false;
+  for (const at::Tensor* t : {&x, &w, bias ? &*bias : nullptr, residual ? &*residual : nullptr}) {
+    if (!t) continue;
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), kWhat, ": no forward-mode derivative");
+    needs = needs || t->requires_grad();
+  }
+  if (!needs || !c10::GradMode::is_enabled()) {
+    static const auto op = handle<decltype(linear)>("_vllm_mi355x::dense_linear");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return op.call(x, w, bias, activation, residual, out_dtype, limit);
+  }
+  return DenseLinear::apply(x, w, bias, activation, residual, out_dtype, limit);
+}
+
+// Shapes alone, for tracing.
+at::Tensor linear_meta(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                       const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
+  check_kinds(x, w, bias, activation, residual, out_dtype, limit);
+  const c10::SymInt lines = w.sym_size(0);
+  return at::empty_symint(with_last(x.sym_sizes(), activation == kSwiglu ? lines / 2 : lines), x.options().dtype(out_dtype));
+}
+void linear_out_meta(const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&, int64_t, const std::optional<at::Tensor>&, double,
+                     const at::Tensor&) {}
+std::tuple<at::Tensor, at::Tensor> forward_meta(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
+                                                int64_t activation, const std::optional<at::Tensor>& residual, at::ScalarType out_dtype,
+                                                double limit) {
+  at::Tensor y = linear_meta(x, w, bias, activation, residual, out_dtype, limit);
+  const c10::SymInt rows = activation ? x.sym_numel() / x.sym_size(-1) : c10::SymInt(0);
+  return {y, at::empty_symint({rows, w.sym_size(0)}, x.options())};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient_meta(const at::Tensor& x, const at::Tensor& w, const at::Tensor&, int64_t, double,
+                                                             const at::Tensor&, bool need_x, bool need_w,
+                                                             std::optional<at::ScalarType> bias_dtype) {
+  const auto nothing = [&] { return at::empty({0}, x.options()); };
+  return {need_x ? at::empty_symint(x.sym_sizes(), x.options()) : nothing(), need_w ? at::empty_symint(w.sym_sizes(), w.options()) : nothing(),
+          bias_dtype ? at::empty_symint({w.sym_size(0)}, x.options().dtype(*bias_dtype)) : nothing()};
+}
+
+template <typename F>
+bool find(void* library, const char* name, F& f) {
+  f = reinterpret_cast<F>(dlsym(library, name));
+  return f != nullptr;
+}
+
+}  // namespace
+
+bool vq_torch::bind_dense(void* library) {
+  return find(library, "dense_linear", native_linear) && find(library, "dense_linear_workspace_size", native_workspace) &&
+         find(library, "dense_linear_grad", native_grad) && find(library, "dense_linear_grad_workspace_size", native_grad_workspace) &&
+         find(library, "vllm_mi355x_last_error", native_error);
+}
+
+TORCH_LIBRARY_FRAGMENT(_vllm_mi355x, m) {
+  m.def("dense_linear(Tensor x, Tensor w, Tensor? bias, int activation, Tensor? residual, ScalarType out_dtype, float limit) -> Tensor");
+  m.def("dense_linear_out(Tensor x, Tensor w, Tensor? bias, int activation, Tensor? residual, float limit, Tensor(a!) out) -> ()");
+  m.def(
+      "dense_linear_forward(Tensor x, Tensor w, Tensor? bias, int activation, Tensor? residual, ScalarType out_dtype, float limit) "
+      "-> (Tensor, Tensor)");
+  m.def(
+      "dense_linear_grad(Tensor x, Tensor w, Tensor z, int activation, float limit, Tensor dy, bool need_x, bool need_w, "
+      "ScalarType? bias_dtype) -> (Tensor, Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(_vllm_mi355x, CUDA, m) {
+  m.impl("dense_linear", &linear);
+  m.impl("dense_linear_out", &linear_out);
+  m.impl("dense_linear_forward", &forward);
+  m.impl("dense_linear_grad", &gradient);
+}
+TORCH_LIBRARY_IMPL(_vllm_mi355x, Meta, m) {
+  m.impl("dense_linear", &linear_meta);
+  m.impl("dense_linear_out", &linear_out_meta);
+  m.impl("dense_linear_forward", &forward_meta);
+  m.impl("dense_linear_grad", &gradient_meta);
+}
+TORCH_LIBRARY_IMPL(_vllm_mi355x, Autograd, m) {
+  m.impl("dense_linear", &linear_autograd);
+  m.impl("dense_linear_out", torch::CppFunction::makeFallthrough());
+}

@@ -5,8 +5,8 @@
 //    torch's current stream (schemas: vllm_mi355x/kernels/exl3/_C.py);
 //  * _vllm_mi355x::marlin_moe, the launches of one fused Marlin MoE call on the
 //    path and buffers that kernels/marlin_moe/fused.py chose.
-// (The MXFP4 operators, the router's load and routing from logits: torch_mxfp4.cpp,
-// torch_balance.cpp, torch_route.cpp.)
+// (The MXFP4 operators, the router's load, routing from logits and the dense layer:
+// torch_mxfp4.cpp, torch_balance.cpp, torch_route.cpp, torch_dense.cpp.)
 // From Python the same checks and calls took longer than the kernels of a small
 // call: a 5120 x 512 linear of one row 21.6 us a call (6 on the GPU), 10.2
 // with its operator here; the fused MoE of 48 tokens 85 us of host work for four
@@ -302,7 +302,8 @@ extern "C" int vllm_mi355x_torch_bind(void* library) {
                    find(library, "marlin_moe_w13_act", native_w13_act) &&
                    find(library, "marlin_moe_w2_sum", native_w2_sum) && find(library, "marlin_moe_rows", native_rows) &&
                    find(library, "moe_sum", native_sum) && find(library, "vllm_mi355x_last_error", native_last_error) &&
-                   vq_torch::bind_mxfp4(library) && vq_torch::bind_balance(library) && vq_torch::bind_route(library);
+                   vq_torch::bind_mxfp4(library) && vq_torch::bind_balance(library) && vq_torch::bind_route(library) &&
+                   vq_torch::bind_dense(library);
   return all ? 0 : 1;
 }
 

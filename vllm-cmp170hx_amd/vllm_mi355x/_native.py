@@ -14,7 +14,7 @@ import threading
 LIBRARY_NAME = "libvllm_mi355x.so"
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIBRARY_NAME)
 # The host-only operator implementations (csrc/torch_ops.cpp, torch_mxfp4.cpp,
-# torch_balance.cpp, torch_route.cpp) and the torch
+# torch_balance.cpp, torch_route.cpp, torch_dense.cpp) and the torch
 # custom classes the reference's loader requires (csrc/torch_classes.cpp).
 TORCH_CLASSES_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)),
                                   "libvllm_mi355x_torch.so")
@@ -187,6 +187,29 @@ SIGNATURES = {
         c_vp, c_int, c_i64, c_i64, c_i64,        # logits, dtype, rows, experts, stride
         c_vp, c_vp, c_i64, c_int, c_int,         # topk_weights, topk_ids, top_k, scoring, renormalize
         ctypes.c_float, c_vp, c_vp, c_vp,        # scale, upstream, grad, stream
+    ]),
+    "dense_linear_workspace_size": (c_i64, [
+        c_vp, c_i64, c_i64, c_i64,               # x, rows, k, x_stride
+        c_vp, c_i64, c_i64, c_int,               # w, n, w_stride, activation
+    ]),
+    "dense_linear": (c_int, [
+        c_vp, c_int, c_i64, c_i64, c_i64,        # x, dtype, rows, k, x_stride
+        c_vp, c_i64, c_i64, c_vp, c_int,         # w, n, w_stride, bias, bias_dtype
+        c_int, ctypes.c_float,                   # activation, limit
+        c_vp, c_int, c_i64, c_vp, c_int,         # residual, dtype, stride, out, out_dtype
+        c_vp, c_vp, c_i64, c_vp,                 # z, workspace, bytes, stream
+    ]),
+    "dense_linear_plan": (c_int, [c_i64, c_i64, c_i64, c_int, c_vp]),
+    "dense_linear_grad_workspace_size": (c_i64, [
+        c_i64, c_i64, c_i64, c_int, c_int, c_int, c_int,  # rows, k, n, activation, need x, w, bias
+    ]),
+    "dense_linear_grad": (c_int, [
+        c_vp, c_int, c_i64, c_i64, c_i64,        # x, dtype, rows, k, x_stride
+        c_vp, c_i64, c_i64, c_vp,                # w, n, w_stride, z
+        c_int, ctypes.c_float,                   # activation, limit
+        c_vp, c_int, c_i64,                      # dy, dy_dtype, dy_stride
+        c_vp, c_vp, c_vp, c_int,                 # dx, dw, dbias, bias_dtype
+        c_vp, c_i64, c_vp,                       # workspace, bytes, stream
     ]),
     "moe_split_align": (c_int, [
         c_vp, c_i64, c_i64, c_vp, c_vp, c_i64,  # topk_ids, numel, num_experts, expert_map, cover, rows
