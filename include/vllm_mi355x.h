@@ -646,9 +646,8 @@ int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, co
  * element's), lines = n, with VQ_ACT_SWIGLU 2 n: SiLU(min(g, L)) clamp(u, -L, L), L = limit
  * > 0 (infinity: no clamp).  FP32 sums of exact products; bias [lines] (or null) and
  * residual [rows][n] (or null) of any of the three types; out contiguous, of any of them;
- * it may be a contiguous residual of its type.  z (or null): contiguous [rows][lines] of
- * dtype, x W^T + bias for dense_linear_grad (with a limit, infinities for what lies
- * outside).  The order of the sums, and so the last bits, depend on the sizes alone.  k
+ * it may be a contiguous residual of its type.  z (or null): contiguous FP32 [rows][lines],
+ * x W^T + bias for dense_linear_grad.  The order of the sums, and so the last bits, depend on the sizes alone.  k
  * up to 2^21.  workspace: dense_linear_workspace_size bytes of the same x, w and strides,
  * 16-byte aligned (null where that is 0), used by one call at a time.
  */
@@ -657,7 +656,7 @@ int64_t dense_linear_workspace_size(const void* x, int64_t rows, int64_t k, int6
 int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride,
                  const void* w, int64_t n, int64_t w_stride, const void* bias, int bias_dtype,
                  int activation, float limit, const void* residual, int residual_dtype,
-                 int64_t residual_stride, void* out, int out_dtype, void* z, void* workspace,
+                 int64_t residual_stride, void* out, int out_dtype, float* z, void* workspace,
                  int64_t workspace_bytes, void* stream);
 
 /* How it runs at a size, for tests: plan[0] the tile's rows and lines (0: the few rows'
@@ -673,7 +672,7 @@ int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int32_
 int64_t dense_linear_grad_workspace_size(int64_t rows, int64_t k, int64_t n, int activation,
                                          int need_x, int need_w, int need_bias);
 int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride,
-                      const void* w, int64_t n, int64_t w_stride, const void* z, int activation,
+                      const void* w, int64_t n, int64_t w_stride, const float* z, int activation,
                       float limit, const void* dy, int dy_dtype, int64_t dy_stride, void* dx,
                       void* dw, void* dbias, int bias_dtype, void* workspace,
                       int64_t workspace_bytes, void* stream);

@@ -87,10 +87,10 @@ def forward(x, w, bias, activation, residual, limit=np.inf):
 
 def backward(x, w, bias, activation, dy, eps, limit=np.inf):
     """({"x", "w", "bias"}: (gradient, what it may be off by before it is rounded to its type),
-    dz), where z is kept and dz rounded with steps of eps (relative, half of which is lost)."""
+    dz), where dz is rounded with steps of eps (relative, half of which is lost)."""
     z, off = products(x, w, bias)
     half = eps / 2
-    off_z = off + half * np.abs(z) * (activation is not None)
+    off_z = off
     if activation == GATED:
         n = len(w) // 2
         g, u = np.minimum(z[:, :n], limit), np.clip(z[:, n:], -limit, limit)

@@ -39,8 +39,10 @@ struct Epilogue {
   void* out;  // [rows][n]
   int out_dtype;
   int64_t n;
-  void* z;  // x W^T + b for the gradient, [rows][lines] of z_dtype, or null
-  int z_dtype;
+  // x W^T + b for the gradient, [rows][lines], or null.  (In 16 bits its rounding would add as
+  // much to gradients as that of dz: of 4096 rows through 4096 x 28672 gated, in BF16, 1.7
+  // times the result's own rounding for 1.4.)
+  float* z;
   const float* factor;  // multiplies the sums, or null
 };
 
@@ -117,18 +119,11 @@ __device__ __forceinline__ float silu_slope(float z) {
 __device__ __forceinline__ float clamp_above(float v, float limit) { return v > limit ? limit : v; }
 __device__ __forceinline__ float clamp_both(float v, float limit) { return v > limit ? limit : (v < -limit ? -limit : v); }
 
-// What the gradient keeps of a clamped value: infinity where it lies outside (rounded, it
-// might not), and otherwise a number that FP16 holds.
-__device__ __forceinline__ float kept(float v, float limit, int dtype) {
-  return v > limit ? __builtin_inff() : (dtype == vq::kFP16 ? clamp_both(v, 65504.0f) : v);
-}
-
 // Columns c .. c + kC - 1 of a row from its sums (u: of a gated activation's up lines).
-template <int kC>
+template <int kC, bool kGated>
 __device__ __forceinline__ void finish_columns(const Epilogue& e, int64_t row, int64_t c, float (&v)[kC], float (&u)[kC]) {
   const int64_t valid = e.n - c;
   if (valid <= 0) return;
-  const bool gated = e.activation == kSwiglu;
   if (e.factor) {
     const float f = *e.factor;
 #pragma unroll
@@ -139,22 +134,16 @@ __device__ __forceinline__ void finish_columns(const Epilogue& e, int64_t row, i
     load_columns<kC>(e.bias, e.bias_dtype, c, valid, b);
 #pragma unroll
     for (int q = 0; q < kC; ++q) v[q] += b[q];
-    if (gated) {
+    if constexpr (kGated) {
       load_columns<kC>(e.bias, e.bias_dtype, e.n + c, valid, b);
 #pragma unroll
       for (int q = 0; q < kC; ++q) u[q] += b[q];
     }
   }
-  if (gated) {
+  if constexpr (kGated) {
     if (e.z) {
-      float a[kC], b[kC];
-#pragma unroll
-      for (int q = 0; q < kC; ++q) {
-        a[q] = kept(v[q], e.limit, e.z_dtype);
-        b[q] = u[q] < 0 ? -kept(-u[q], e.limit, e.z_dtype) : kept(u[q], e.limit, e.z_dtype);
-      }
-      store_columns<kC>(e.z, e.z_dtype, row * 2 * e.n + c, valid, a);
-      store_columns<kC>(e.z, e.z_dtype, row * 2 * e.n + e.n + c, valid, b);
+      store_columns<kC>(e.z, vq::kFP32, row * 2 * e.n + c, valid, v);
+      store_columns<kC>(e.z, vq::kFP32, row * 2 * e.n + e.n + c, valid, u);
     }
 #pragma unroll
     for (int q = 0; q < kC; ++q) {
@@ -162,7 +151,7 @@ __device__ __forceinline__ void finish_columns(const Epilogue& e, int64_t row, i
       v[q] = g * sigmoid(g) * clamp_both(u[q], e.limit);
     }
   } else {
-    if (e.z) store_columns<kC>(e.z, e.z_dtype, row * e.n + c, valid, v);
+    if (e.z) store_columns<kC>(e.z, vq::kFP32, row * e.n + c, valid, v);
     const auto each = [&](float (*f)(float)) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < kC; ++q) v[q] = f(v[q]);

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(1024) void small_kernel(Operand x, Operand w, int64
       for (int i = 0; i < 4; ++i) (o ? u : v)[i] = all[i];
     }
     const int64_t m = kSmallRows * t + r;
-    if (m < x.rows) finish_columns<4>(e, m, c0 + 4 * q, v, u);
+    if (m < x.rows) finish_columns<4, kGated>(e, m, c0 + 4 * q, v, u);
   }
 }
 
@@ -135,7 +135,8 @@ __global__ __launch_bounds__(256) void finish_kernel(const float* sums, int spli
         for (int q = 0; q < 8; ++q) u[q] += a[q];
       }
     }
-    finish_columns<8>(e, m, c, v, u);
+    if (gated) finish_columns<8, true>(e, m, c, v, u);
+    else finish_columns<8, false>(e, m, c, v, u);
   }
 }
 
@@ -187,43 +188,39 @@ struct Slopes {
   const void* dy;  // [rows][n], stride dy_stride
   int dy_dtype;
   int64_t dy_stride;
-  const uint16_t* z;  // [rows][lines], or null without an activation
+  const float* z;  // [rows][lines], or null without an activation
   int dtype, activation;
   float limit;
   int64_t rows, n, lines;
 };
 
-// Slopes are 0 or 1 from here on (z may be an infinity, having been rounded to FP16).
+// Slopes are 0 or 1 from here on.
 constexpr float kFar = 104.0f;
 
-// dz at row m, lines c .. c + 7 (of which `valid` exist).
-__device__ __forceinline__ void slopes8(const Slopes& g, int64_t m, int64_t c, float (&v)[8]) {
-  const int64_t valid = m < g.rows ? g.lines - c : 0;
+// dz at row m of columns c .. c + 7 (zeros past the last): of z's lines there, with a gated
+// activation v of the gate lines and u of the up lines.
+template <bool kGated>
+__device__ __forceinline__ void slopes8(const Slopes& g, int64_t m, int64_t c, float (&v)[8], float (&u)[8]) {
+  const int64_t valid = m < g.rows ? g.n - c : 0;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] = 0;
+  for (int q = 0; q < 8; ++q) v[q] = u[q] = 0;
   if (valid <= 0) return;
-  if (g.activation == kSwiglu) {
-    // (eight lines may begin in the gate half and end in the up half)
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      if (q >= valid) continue;
-      const bool up = c + q >= g.n;
-      const int64_t col = up ? c + q - g.n : c + q;
-      const float a = vq::load_act(g.z, g.dtype, m * g.lines + col), b = vq::load_act(g.z, g.dtype, m * g.lines + g.n + col);
-      const float dy = vq::load_act(g.dy, g.dy_dtype, m * g.dy_stride + col);
-      // (kept as infinities where they lie outside)
-      const bool clamped = g.limit < __builtin_inff();
-      const float gate = clamp_above(a, g.limit);
-      if (up) v[q] = clamped && fabsf(b) == __builtin_inff() ? 0.0f : dy * silu(gate < -kFar ? -kFar : gate);
-      else v[q] = clamped && a == __builtin_inff() ? 0.0f : dy * clamp_both(b, g.limit) * silu_slope(clamp_both(gate, kFar));
-    }
-    return;
-  }
   float dy[8];
   load_columns<8>(g.dy, g.dy_dtype, m * g.dy_stride + c, valid, dy);
-  if (g.z) {
+  if constexpr (kGated) {
+    float a[8], b[8];
+    load_columns<8>(g.z, vq::kFP32, m * g.lines + c, valid, a);
+    load_columns<8>(g.z, vq::kFP32, m * g.lines + g.n + c, valid, b);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      // (an infinite gate has slope 0 or 1, and nothing or all of it passes)
+      const float gate = clamp_above(a[q], g.limit);
+      v[q] = a[q] > g.limit ? 0.0f : dy[q] * clamp_both(b[q], g.limit) * silu_slope(clamp_both(gate, kFar));
+      u[q] = fabsf(b[q]) > g.limit ? 0.0f : dy[q] * silu(gate < -kFar ? -kFar : gate);
+    }
+  } else if (g.z) {
     float z[8];
-    load_columns<8>(g.z, g.dtype, m * g.lines + c, valid, z);
+    load_columns<8>(g.z, vq::kFP32, m * g.lines + c, valid, z);
     const auto each = [&](float (*f)(float)) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] = dy[q] * f(clamp_both(z[q], kFar));
@@ -253,14 +250,19 @@ __global__ void clear_kernel(uint32_t* top) {
   if (threadIdx.x == 0) *top = 0;
 }
 
+template <bool kGated>
 __global__ __launch_bounds__(256) void top_kernel(Slopes g, uint32_t* top) {
-  const int64_t eighths = (g.lines + 7) / 8;
+  const int64_t eighths = (g.n + 7) / 8;
   uint32_t most = 0;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < g.rows * eighths; i += int64_t(gridDim.x) * 256) {
-    float v[8];
-    slopes8(g, i / eighths, i % eighths * 8, v);
+    float v[8], u[8];
+    slopes8<kGated>(g, i / eighths, i % eighths * 8, v, u);
 #pragma unroll
     for (int q = 0; q < 8; ++q) most = max(most, __builtin_bit_cast(uint32_t, v[q]) & 0x7fffffffu);
+    if constexpr (kGated) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) most = max(most, __builtin_bit_cast(uint32_t, u[q]) & 0x7fffffffu);
+    }
   }
 #pragma unroll
   for (int d = 32; d > 0; d /= 2) most = max(most, uint32_t(__shfl_xor(int(most), d)));
@@ -271,53 +273,83 @@ __global__ void factor_kernel(const uint32_t* top, float* factor) {
   if (threadIdx.x == 0) *factor = 1 / scale_of(*top);
 }
 
-// dz of 64 rows and 64 lines: by rows (stride `ld`, zeros up to whole chunks of lines), by
-// lines (stride `ldt`, zeros up to whole chunks of rows), and the lines' sums over these rows.
+// dz of 64 rows and 64 columns (gated: of the gate and of the up lines): by rows (stride
+// `ld`, zeros up to whole chunks of lines), by lines (stride `ldt`, zeros up to whole
+// chunks of rows), and the lines' sums over these rows.
+template <bool kGated>
 __global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* top, uint16_t* dz, int64_t ld, uint16_t* dzt, int64_t ldt,
                                                      float* partial) {
-  __shared__ uint16_t part[kPart * kPartStride];
-  __shared__ float sum[32][kPart + 1];
+  constexpr int kHalves = kGated ? 2 : 1;
+  __shared__ uint16_t part[kHalves][kPart * kPartStride];
+  __shared__ float sum[kHalves][32][kPart + 1];
   const int64_t m0 = int64_t(blockIdx.y) * kPart, c0 = int64_t(blockIdx.x) * kPart;
   const int ch = threadIdx.x & 7, row = threadIdx.x >> 3;
+  const int64_t c = c0 + kChunk * ch;
   const float scale = top ? scale_of(*top) : 1.0f;
-  float mine[8];
+  float mine[kHalves][8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) mine[q] = 0;
+  for (int o = 0; o < kHalves; ++o)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) mine[o][q] = 0;
 #pragma unroll
   for (int i = 0; i < kPart; i += 32) {
-    const int64_t m = m0 + row + i, c = c0 + kChunk * ch;
-    float v[8];
-    slopes8(g, m, c, v);
-    u32x4_t w;
+    const int64_t m = m0 + row + i;
+    float v[2][8];
+    slopes8<kGated>(g, m, c, v[0], v[1]);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) mine[q] += v[q];
+    for (int o = 0; o < kHalves; ++o) {
+      uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack16(g.dtype, v[2 * j] * scale, v[2 * j + 1] * scale);
-    if (dz && m < g.rows && c < ld) *reinterpret_cast<u32x4_t*>(dz + m * ld + c) = w;
-    uint32_t* to = reinterpret_cast<uint32_t*>(part + (row + i) * kPartStride + kChunk * ch);
+      for (int q = 0; q < 8; ++q) mine[o][q] += v[o][q];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) to[j] = w[j];
+      for (int j = 0; j < 4; ++j) w[j] = pack16(g.dtype, v[o][2 * j] * scale, v[o][2 * j + 1] * scale);
+      if (dz && m < g.rows && c < g.n) {
+        const int64_t at = o * g.n + c;
+        uint16_t* to = dz + m * ld + at;
+        if (c + kChunk <= g.n) {
+          __builtin_memcpy(to, w, 16);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            if (c + q < g.n) to[q] = uint16_t(w[q / 2] >> (16 * (q & 1)));
+          }
+        }
+        if (o == kHalves - 1 && c + kChunk >= g.n) {
+          for (int64_t past = g.lines; past < ld; ++past) dz[m * ld + past] = 0;
+        }
+      }
+      uint32_t* to = reinterpret_cast<uint32_t*>(part[o] + (row + i) * kPartStride + kChunk * ch);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[j] = w[j];
+    }
   }
 #pragma unroll
-  for (int q = 0; q < 8; ++q) sum[row][kChunk * ch + q] = mine[q];
+  for (int o = 0; o < kHalves; ++o)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) sum[o][row][kChunk * ch + q] = mine[o][q];
   __syncthreads();
   if (dzt) {
 #pragma unroll
-    for (int i = 0; i < kPart; i += 32) {
-      const int64_t line = c0 + row + i, m = m0 + kChunk * ch;
-      u32x4_t v;
+    for (int o = 0; o < kHalves; ++o)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint16_t* from = part + (kChunk * ch + 2 * j) * kPartStride + row + i;
-        v[j] = uint32_t(from[0]) | (uint32_t(from[kPartStride]) << 16);
+      for (int i = 0; i < kPart; i += 32) {
+        const int64_t col = c0 + row + i, m = m0 + kChunk * ch;
+        u32x4_t v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint16_t* from = part[o] + (kChunk * ch + 2 * j) * kPartStride + row + i;
+          v[j] = uint32_t(from[0]) | (uint32_t(from[kPartStride]) << 16);
+        }
+        if (col < g.n && m < ldt) *reinterpret_cast<u32x4_t*>(dzt + (o * g.n + col) * ldt + m) = v;
       }
-      if (line < g.lines && m < ldt) *reinterpret_cast<u32x4_t*>(dzt + line * ldt + m) = v;
-    }
   }
-  if (partial && threadIdx.x < kPart && c0 + threadIdx.x < g.lines) {
-    float all = 0;
-    for (int i = 0; i < 32; ++i) all += sum[i][threadIdx.x];
-    partial[int64_t(blockIdx.y) * g.lines + c0 + threadIdx.x] = all;
+  if (partial && threadIdx.x < kHalves * kPart) {
+    const int o = threadIdx.x / kPart, col = threadIdx.x % kPart;
+    if (c0 + col < g.n) {
+      float all = 0;
+      for (int i = 0; i < 32; ++i) all += sum[o][i][col];
+      partial[int64_t(blockIdx.y) * g.lines + o * g.n + c0 + col] = all;
+    }
   }
 }
 
@@ -389,20 +421,20 @@ void launch_small(const Operand& x, const Operand& w, int64_t k, const Epilogue&
   }
 }
 
-template <int kSize, int kBufs>
+template <typename T>
 void launch_tile(TileArgs& t, bool bf16, int64_t splits, hipStream_t s) {
   const bool gated = t.e.activation == kSwiglu;
   const int64_t total = int64_t(t.tiles_n) * t.tiles_m;
-  const dim3 grid(unsigned(up_to(total, 8)), unsigned(splits)), block(kTileThreads);
-  if constexpr (kSize >= 2) {
+  const dim3 grid(unsigned(up_to(total, 8)), unsigned(splits)), block(T::kThreads);
+  if constexpr (T::kN >= 2) {
     if (gated) {
-      if (bf16) hipLaunchKernelGGL((tile_kernel<kSize, kSize, true, kBufs, true>), grid, block, 0, s, t);
-      else hipLaunchKernelGGL((tile_kernel<kSize, kSize, true, kBufs, false>), grid, block, 0, s, t);
+      if (bf16) hipLaunchKernelGGL((tile_kernel<T, true, true>), grid, block, 0, s, t);
+      else hipLaunchKernelGGL((tile_kernel<T, true, false>), grid, block, 0, s, t);
       return;
     }
   }
-  if (bf16) hipLaunchKernelGGL((tile_kernel<kSize, kSize, false, kBufs, true>), grid, block, 0, s, t);
-  else hipLaunchKernelGGL((tile_kernel<kSize, kSize, false, kBufs, false>), grid, block, 0, s, t);
+  if (bf16) hipLaunchKernelGGL((tile_kernel<T, false, true>), grid, block, 0, s, t);
+  else hipLaunchKernelGGL((tile_kernel<T, false, false>), grid, block, 0, s, t);
 }
 
 // x [rows][k] times W's transpose, finished by e; sums: the plan's K splits' room.
@@ -420,9 +452,9 @@ int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, bo
   const int64_t split = parts_of(stages, p.splits);
   TileArgs t{x, w, int(parts_of(k, kChunk)), int(tiles_n), int(tiles_m), int(split), sums, e};
   const int64_t splits = parts_of(stages, split);  // (none without a stage)
-  if (p.tile == 4) launch_tile<4, 2>(t, bf16, splits, s);
-  else if (p.tile == 2) launch_tile<2, 2>(t, bf16, splits, s);
-  else launch_tile<1, 4>(t, bf16, splits, s);
+  if (p.tile == 4) launch_tile<Tile<2, 4, 4, 2, 2>>(t, bf16, splits, s);
+  else if (p.tile == 2) launch_tile<Tile<2, 2, 2, 2, 2>>(t, bf16, splits, s);
+  else launch_tile<Tile<2, 2, 1, 1, 4>>(t, bf16, splits, s);
   if (int rc = vq::check_launch("dense_linear")) return rc;
   if (splits == 1) return vq::kOk;
   const int64_t groups = parts_of(x.rows * parts_of(e.n, 8), 256);
@@ -548,7 +580,7 @@ extern "C" int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activat
 
 extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t n, int64_t w_stride,
                             const void* bias, int bias_dtype, int activation, float limit, const void* residual, int residual_dtype,
-                            int64_t residual_stride, void* out, int out_dtype, void* z, void* workspace, int64_t workspace_bytes,
+                            int64_t residual_stride, void* out, int out_dtype, float* z, void* workspace, int64_t workspace_bytes,
                             void* stream) {
   using namespace dense;
   if (int rc = check_sizes(rows, k, n, activation)) return rc;
@@ -571,7 +603,7 @@ extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, i
   // (the output may be the residual: an element is read before it is written, by the same lane)
   const bool in_place = residual == out && residual_dtype == out_dtype && (rows == 1 || residual_stride == n);
   if (int rc = check_spans({{out, rows * n * vq::dtype_bytes(out_dtype), vq::dtype_bytes(out_dtype)},
-                            {z, z ? rows * lines * 2 : 0, 2},
+                            {z, z ? rows * lines * 4 : 0, 4},
                             {workspace, room.bytes, 1}},
                            {{x, span_bytes(rows, k, xo.stride, dtype), 2},
                             {w, span_bytes(lines, k, w_stride, dtype), 2},
@@ -591,7 +623,7 @@ extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, i
   if (pack_w) {
     if (int rc = pack(wo, k, reinterpret_cast<uint16_t*>(at), s)) return rc;
   }
-  const Epilogue e{bias, bias_dtype, activation, limit, residual, residual_dtype, residual_stride, out, out_dtype, n, z, dtype, nullptr};
+  const Epilogue e{bias, bias_dtype, activation, limit, residual, residual_dtype, residual_stride, out, out_dtype, n, z, nullptr};
   return product(xo, wo, k, e, dtype == vq::kBF16, sums, p, s);
 }
 
@@ -603,7 +635,7 @@ extern "C" int64_t dense_linear_grad_workspace_size(int64_t rows, int64_t k, int
 }
 
 extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t n,
-                                 int64_t w_stride, const void* z, int activation, float limit, const void* dy, int dy_dtype,
+                                 int64_t w_stride, const float* z, int activation, float limit, const void* dy, int dy_dtype,
                                  int64_t dy_stride, void* dx, void* dw, void* dbias, int bias_dtype, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   using namespace dense;
@@ -613,7 +645,8 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
   if (int rc = check_inputs(x, dtype, rows, k, x_stride, w, w_stride, limit)) return rc;
   if (!dy || (activation != kNone && !z)) return vq::fail("dense_linear: null pointer");
   if (dy_stride < 0 || (rows > 1 && dy_stride < n)) return vq::fail("dense_linear: gradient stride out of range");
-  const int64_t lines = activation == kSwiglu ? 2 * n : n;
+  const bool gated = activation == kSwiglu;
+  const int64_t lines = gated ? 2 * n : n;
   const GradRoom room(rows, k, lines, dx, dw, dbias);
   if (!workspace || workspace_bytes < room.bytes || !aligned(workspace, 16)) return vq::fail("dense_linear: workspace too small or misaligned");
   const Operand xo{static_cast<const uint16_t*>(x), rows, rows > 1 ? x_stride : k}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
@@ -623,7 +656,7 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
                             {workspace, room.bytes, 1}},
                            {{x, span_bytes(rows, k, xo.stride, dtype), 2},
                             {w, span_bytes(lines, k, w_stride, dtype), 2},
-                            {z, activation != kNone ? rows * lines * 2 : 0, 2},
+                            {z, activation != kNone ? rows * lines * 4 : 0, 4},
                             {dy, span_bytes(rows, n, dy_stride, dy_dtype), vq::dtype_bytes(dy_dtype)}})) {
     return rc;
   }
@@ -643,18 +676,20 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
   uint32_t* top = reinterpret_cast<uint32_t*>(take(room.top));
   float* factor = reinterpret_cast<float*>(top) + 1;
   const int64_t ld = up_to(lines, kChunk), ldt = up_to(rows, kChunk);
-  const Slopes g{dy, dy_dtype, rows > 1 ? dy_stride : n, activation == kNone ? nullptr : static_cast<const uint16_t*>(z), dtype, activation, limit,
+  const Slopes g{dy, dy_dtype, rows > 1 ? dy_stride : n, activation == kNone ? nullptr : z, dtype, activation, limit,
                  rows, n, lines};
   const bool scaled = dtype == vq::kFP16 && (dx || dw);
   if (scaled) {
     hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(64), 0, s, top);
-    const int64_t groups = parts_of(rows * parts_of(lines, 8), 256);
-    hipLaunchKernelGGL(top_kernel, dim3(unsigned(std::min<int64_t>(groups, 2048))), dim3(256), 0, s, g, top);
+    const dim3 grid(unsigned(std::min<int64_t>(parts_of(rows * parts_of(n, 8), 256), 2048)));
+    if (gated) hipLaunchKernelGGL(top_kernel<true>, grid, dim3(256), 0, s, g, top);
+    else hipLaunchKernelGGL(top_kernel<false>, grid, dim3(256), 0, s, g, top);
     hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(64), 0, s, top, factor);
     if (int rc = vq::check_launch("dense_linear gradient")) return rc;
   }
-  hipLaunchKernelGGL(slopes_kernel, dim3(unsigned(parts_of(lines, kPart)), unsigned(parts_of(rows, kPart))), dim3(256), 0, s, g,
-                     scaled ? top : nullptr, dz, ld, dzt, ldt, partial);
+  const dim3 parts(unsigned(parts_of(n, kPart)), unsigned(parts_of(rows, kPart)));
+  if (gated) hipLaunchKernelGGL(slopes_kernel<true>, parts, dim3(256), 0, s, g, scaled ? top : nullptr, dz, ld, dzt, ldt, partial);
+  else hipLaunchKernelGGL(slopes_kernel<false>, parts, dim3(256), 0, s, g, scaled ? top : nullptr, dz, ld, dzt, ldt, partial);
   if (int rc = vq::check_launch("dense_linear gradient")) return rc;
   if (dbias) {
     hipLaunchKernelGGL(bias_kernel, dim3(unsigned(parts_of(lines, 256))), dim3(256), 0, s, partial, parts_of(rows, kPart), lines, dbias,
@@ -663,7 +698,7 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
   }
   const bool bf16 = dtype == vq::kBF16;
   const auto plain = [&](void* out) {
-    return Epilogue{nullptr, 0, kNone, __builtin_inff(), nullptr, 0, 0, out, dtype, k, nullptr, 0, scaled ? factor : nullptr};
+    return Epilogue{nullptr, 0, kNone, __builtin_inff(), nullptr, 0, 0, out, dtype, k, nullptr, scaled ? factor : nullptr};
   };
   if (dx) {
     if (int rc = transpose(wo, k, wt, ld, s)) return rc;

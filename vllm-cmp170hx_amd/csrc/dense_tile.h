@@ -1,7 +1,7 @@
 // Many rows of the dense linear layer: tiles of the product through LDS.
 //
-// One workgroup of four wavefronts (2 x 2) computes 64 kN lines of W by 64 kM rows
-// of x, each wavefront 32 kN x 32 kM of v_mfma_f32_32x32x16 tiles.  A stage is 64 k: 128
+// A workgroup of four or eight wavefronts computes kCols lines of W by kRows rows of x, each
+// wavefront 32 kN x 32 kM of v_mfma_f32_32x32x16 tiles.  A stage is 64 k: 128
 // bytes of every row and line, in one of kBufs buffers, one barrier a stage.
 //  * Rows come to LDS by DMA, one 128-byte line in eight lanes, up to kBufs - 1 stages
 //    ahead.  A line's eight 16-byte chunks lie in LDS in the order chunk ^ (line / 2 &
@@ -22,7 +22,6 @@ namespace dense {
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
-constexpr int kTileThreads = 256;
 constexpr int kStageChunks = 8;  // 64 k
 constexpr int kChunkBytes = 16;
 constexpr int kStageBytes = kStageChunks * kChunkBytes;  // a line
@@ -52,22 +51,31 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, uint3
 // An offset past any buffer: such loads give zeros.
 constexpr uint32_t kPastEnd = 0x80000000u;
 
-// Workgroups of a size that a CU's LDS (and registers) hold, two at most.
-constexpr int tile_groups(int n, int m, int bufs) { return n * m > 8 || 64 * (n + m) * kStageBytes * bufs > 80 * 1024 ? 1 : 2; }
+// A workgroup's kWn x kWm wavefronts, each of 32 kN lines by 32 kM rows, and its stage buffers.
+template <int kWn_, int kWm_, int kN_, int kM_, int kBufs_>
+struct Tile {
+  static constexpr int kWn = kWn_, kWm = kWm_, kN = kN_, kM = kM_, kBufs = kBufs_;
+  static constexpr int kWaves = kWn * kWm, kThreads = 64 * kWaves;
+  static constexpr int kCols = 32 * kN * kWn, kRows = 32 * kM * kWm, kLines = kCols + kRows;
+  // workgroups that a CU's LDS holds, two at most
+  static constexpr int kGroups = kLines * kStageBytes * kBufs > 80 * 1024 ? 1 : 2;
+};
 
-template <int kN, int kM, bool kGated, int kBufs, bool kBf16>
-__global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile_kernel(TileArgs g) {
-  constexpr int kCols = 64 * kN, kRows = 64 * kM, kLines = kCols + kRows;
+template <typename T, bool kGated, bool kBf16>
+__global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_kernel(TileArgs g) {
+  constexpr int kN = T::kN, kM = T::kM, kBufs = T::kBufs, kWaves = T::kWaves;
+  constexpr int kCols = T::kCols, kRows = T::kRows, kLines = T::kLines;
   constexpr int kLoadRows = 8;  // lines of a 1 KB DMA load
-  constexpr int kLoadsW = kCols / (4 * kLoadRows), kLoadsX = kRows / (4 * kLoadRows);  // loads a wavefront and stage
+  constexpr int kLoadsW = kCols / (kWaves * kLoadRows), kLoadsX = kRows / (kWaves * kLoadRows);  // loads a wavefront and stage
   constexpr int kLoads = kLoadsW + kLoadsX;
-  static_assert(kBufs == 2 || kBufs == 4, "stage buffers");
-  static_assert(!kGated || kN >= 2, "a gate and an up block a wavefront");
+  static_assert(kBufs >= 2 && kBufs <= 4, "stage buffers");
+  static_assert(kLoadsW * kWaves * kLoadRows == kCols && kLoadsX * kWaves * kLoadRows == kRows, "whole loads");
+  static_assert(!kGated || (kN >= 2 && kLoadRows * kLoadsW <= 16 * kN), "a wavefront loads gate or up lines alone");
   // (buffers by name: the compiler then sees that a stage's reads are not of the
   // buffer that the DMA is filling, and does not wait for it)
   constexpr int kBufBytes = kLines * kStageBytes;
   __shared__ __attribute__((aligned(1024))) uint8_t buf0[kBufBytes], buf1[kBufBytes], buf2[kBufs > 2 ? kBufBytes : 16],
-      buf3[kBufs > 2 ? kBufBytes : 16];
+      buf3[kBufs > 3 ? kBufBytes : 16];
   const auto buf = [&](auto i_c) -> uint8_t* {
     constexpr int i = decltype(i_c)::value % kBufs;
     if constexpr (i == 0) return buf0;
@@ -79,7 +87,7 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = vq::uniform(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
-  const int wn = wave & 1, wm = wave >> 1;
+  const int wn = wave % T::kWn, wm = wave / T::kWn;
 
   // XCD x (workgroups x, x + 8, ...) takes a run of tiles, rows first: it fetches few
   // lines of W and its L2 keeps them for all the rows
@@ -94,14 +102,15 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
   const uint32_t wline = uint32_t(g.w.stride) * 2, xline = uint32_t(g.x.stride) * 2;
   // Loads: 1 KB each, 8 lines, of which the first one's offset is scalar and the lane's part
   // has two values, by the parity of the load's place.  A wavefront's first kLoadsW
-  // bring lines of W: with a gated activation all gate (wavefronts 0 and 2) or all up lines.
-  const bool up = kGated && (wave & 1);
+  // bring lines of W: with a gated activation all gate or all up lines.
+  const int w_first = kLoadRows * kLoadsW * wave;
+  const bool up = kGated && w_first % (32 * kN) >= 16 * kN;
   const uint32_t line_bytes = uint32_t(g.chunks) * kChunkBytes;
   const __amdgpu_buffer_rsrc_t wbuf = buffer(g.w.p + (c0 + (up ? g.e.n : 0)) * g.w.stride, uint32_t(ncols - 1) * wline + line_bytes);
   const __amdgpu_buffer_rsrc_t xbuf = buffer(g.x.p + m0 * g.x.stride, uint32_t(nrows - 1) * xline + line_bytes);
   const int sub_row = lane >> 3;
   const auto first_line = [&](int i) {
-    return i < kLoadsW ? kLoadRows * (kLoadsW * wave + i) : kCols + kLoadRows * (kLoadsX * wave + i - kLoadsW);
+    return i < kLoadsW ? w_first + kLoadRows * i : kCols + kLoadRows * (kLoadsX * wave + i - kLoadsW);
   };
   const auto swizzle_of = [](int l) { return (l >> 1) & 7; };
   const int kb[2] = {(lane & 7) ^ swizzle_of(sub_row), (lane & 7) ^ swizzle_of(kLoadRows + sub_row)};
@@ -114,7 +123,7 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
       return l < nrows ? l : 0;
     }
     l = first_line(i);
-    if constexpr (kGated) l = 16 * kN * (wave >> 1) + l % (16 * kN);
+    if constexpr (kGated) l = l / (32 * kN) * (16 * kN) + l % (16 * kN);
     return l < ncols ? l : 0;
   };
   const uint32_t wlane[2] = {sub_row * wline + kb[0] * kChunkBytes, sub_row * wline + kb[1] * kChunkBytes};
@@ -211,23 +220,19 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
   for (; s + kBufs <= stages; s += kBufs) {
     for_range<0, kBufs>([&](auto i) __attribute__((always_inline)) { stage(i, s + decltype(i)::value); });
   }
-  if (s < stages) {
-    stage(std::integral_constant<int, 0>{}, s);
-    if constexpr (kBufs > 2) {
-      if (s + 1 < stages) {
-        stage(std::integral_constant<int, 1>{}, s + 1);
-        if (s + 2 < stages) stage(std::integral_constant<int, 2>{}, s + 2);
-      }
-    }
-  }
+  for_range<0, kBufs - 1>([&](auto i) __attribute__((always_inline)) {
+    if (s + decltype(i)::value < stages) stage(i, s + decltype(i)::value);
+  });
   vq::wait_vmcnt<0>();  // the last loads (zeros) are in before their buffers are used again
 
-  // Results: each row tile through LDS (a wavefront's own part, rows 16 bytes apart
-  // from a bank's multiple), then eight columns of a row a lane.
-  constexpr int kStride = 32 * kN + 4;
-  static_assert((4 / kBufs) * 32 * kStride * 4 <= kBufBytes, "the wavefronts' exchanges fit the stage buffers");
-  float* part = kBufs == 2 ? reinterpret_cast<float*>(wave < 2 ? buf0 : buf1) + (wave & 1) * 32 * kStride
-                           : reinterpret_cast<float*>(wave < 2 ? (wave ? buf1 : buf0) : (wave == 2 ? buf2 : buf3));
+  // Results: each row tile through LDS (a wavefront's own part, four columns a chunk, the
+  // chunks in an order by the row), then four columns of a row a lane.
+  constexpr int kStride = 32 * kN;
+  const auto exchange_at = [](int row, int chunk) { return row * kStride + 4 * (chunk ^ (kN > 1 ? row & 15 : (row >> 1) & 7)); };
+  constexpr int kEach = (kWaves + kBufs - 1) / kBufs;  // exchanges in one buffer
+  static_assert(kEach * 32 * kStride * 4 <= kBufBytes, "the wavefronts' exchanges fit the stage buffers");
+  const int in = wave / kEach;
+  float* part = reinterpret_cast<float*>(in == 0 ? buf0 : in == 1 ? buf1 : in == 2 ? buf2 : buf3) + wave % kEach * 32 * kStride;
   __syncthreads();
   const bool split = gridDim.y > 1;
   constexpr int kWave = kGated ? 16 * kN : 32 * kN;  // a wavefront's output columns
@@ -244,37 +249,29 @@ __global__ __launch_bounds__(kTileThreads, tile_groups(kN, kM, kBufs)) void tile
           f32x4_t v;
 #pragma unroll
           for (int q = 0; q < 4; ++q) v[q] = acc[j][row_tile][4 * p + q];
-          *reinterpret_cast<f32x4_t*>(part + r * kStride + 32 * j + 8 * p + 4 * h) = v;
+          *reinterpret_cast<f32x4_t*>(part + exchange_at(r, 8 * j + 2 * p + h)) = v;
         }
       }
     });
     const int mt = 32 * (kM * wm + i);
     const int64_t ct = c0 + kWave * wn;
-    constexpr int kChunksRow = kWave / 8;  // of eight columns
-    const int ch = lane % kChunksRow, r0 = lane / kChunksRow;
+    constexpr int kChunksRow = kWave / 4;  // of four columns
+    const int chunk = lane % kChunksRow, r0 = lane / kChunksRow;
 #pragma unroll 1
     for (int k = 0; k < kChunksRow / 2; ++k) {
       const int mr = r0 + k * (64 / kChunksRow), m = mt + mr;
-      float v[8], u[8];
-#pragma unroll
-      for (int d = 0; d < 8; d += 4) {
-        const float* at = part + mr * kStride + 8 * ch + d;
-        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(at), b = *reinterpret_cast<const f32x4_t*>(at + (kGated ? 16 * kN : 0));
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          v[d + q] = a[q];
-          u[d + q] = b[q];
-        }
-      }
-      const int64_t c = ct + 8 * ch;
+      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk));
+      const f32x4_t b = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk + (kGated ? 4 * kN : 0)));
+      const int64_t c = ct + 4 * chunk;
       if (m >= nrows || c >= g.e.n) continue;
+      float v[4] = {a[0], a[1], a[2], a[3]}, u[4] = {b[0], b[1], b[2], b[3]};
       if (split) {
         const int64_t lines = kGated ? 2 * g.e.n : g.e.n;
         float* to = g.sums + (int64_t(blockIdx.y) * g.x.rows + m0 + m) * lines + c;
-        store_columns<8>(to, vq::kFP32, 0, g.e.n - c, v);
-        if constexpr (kGated) store_columns<8>(to + g.e.n, vq::kFP32, 0, g.e.n - c, u);
+        store_columns<4>(to, vq::kFP32, 0, g.e.n - c, v);
+        if constexpr (kGated) store_columns<4>(to + g.e.n, vq::kFP32, 0, g.e.n - c, u);
       } else {
-        finish_columns<8>(g.e, m0 + m, c, v, u);
+        finish_columns<4, kGated>(g.e, m0 + m, c, v, u);
       }
     }
   }

@@ -112,7 +112,7 @@ void run(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tenso
                              bias ? bias->const_data_ptr() : nullptr, bias ? dtype_code(bias->scalar_type()) : 0, int(activation),
                              static_cast<float>(limit), residual ? residual->const_data_ptr() : nullptr,
                              residual ? dtype_code(residual->scalar_type()) : 0, res.stride, out.mutable_data_ptr(),
-                             dtype_code(out.scalar_type()), z.defined() ? z.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(), bytes,
+                             dtype_code(out.scalar_type()), z.defined() ? z.mutable_data_ptr<float>() : nullptr, ws.mutable_data_ptr(), bytes,
                              stream_of(x)));
 }
 
@@ -133,7 +133,7 @@ void linear_out(const at::Tensor& x, const at::Tensor& w, const std::optional<at
   run(x, w, bias, activation, residual, limit, out, at::Tensor());
 }
 
-// (y, z): z is what the gradient needs beside x and w, x w^T + bias in x's type (nothing
+// (y, z): z is what the gradient needs beside x and w, x w^T + bias in FP32 (nothing
 // without an activation).
 std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
                                            const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
@@ -142,7 +142,7 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor
   const int64_t n = columns_of(w, activation), k = x.size(-1);
   TORCH_CHECK(k > 0, kWhat, ": the weights must be [n, k] of x's k = 0");
   at::Tensor out = at::empty(with_last(x.sizes(), n), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
-  at::Tensor z = at::empty({activation ? x.numel() / k : 0, w.size(0)}, x.options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor z = at::empty({activation ? x.numel() / k : 0, w.size(0)}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
   run(x, w, bias, activation, residual, limit, out, activation ? z : at::Tensor());
   return {out, z};
 }
@@ -156,7 +156,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient(const at::Tensor& x, con
   const int64_t n = columns_of(w, activation);
   const Rows r = rows_of(x);
   TORCH_CHECK(r.stride >= 0 && w.size(1) == r.k && given.numel() == r.rows * n &&
-                  (!activation || (z.is_contiguous() && z.numel() == r.rows * w.size(0) && z.scalar_type() == x.scalar_type())),
+                  (!activation || (z.is_contiguous() && z.numel() == r.rows * w.size(0) && z.scalar_type() == at::kFloat)),
               kWhat, ": the gradient's tensors must be the forward's");
   const c10::DeviceGuard guard(x.device());
   const auto nothing = [&] { return at::empty({0}, x.options()); };
@@ -174,7 +174,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient(const at::Tensor& x, con
   if (bytes < 0) TORCH_CHECK(false, native_error());
   const at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
   check_status(native_grad(x.const_data_ptr(), dtype_code(x.scalar_type()), r.rows, r.k, r.stride, w.const_data_ptr(), n,
-                           w.size(0) > 1 ? w.stride(0) : r.k, activation ? z.const_data_ptr() : nullptr, int(activation),
+                           w.size(0) > 1 ? w.stride(0) : r.k, activation ? z.const_data_ptr<float>() : nullptr, int(activation),
                            static_cast<float>(limit), dy.const_data_ptr(), dtype_code(dy.scalar_type()), rows_of(dy).stride,
                            need_x ? dx.mutable_data_ptr() : nullptr, need_w ? dw.mutable_data_ptr() : nullptr,
                            bias_dtype ? db.mutable_data_ptr() : nullptr, bias_dtype ? dtype_code(*bias_dtype) : 0, ws.mutable_data_ptr(), bytes,
@@ -256,7 +256,7 @@ std::tuple<at::Tensor, at::Tensor> forward_meta(const at::Tensor& x, const at::T
                                                 double limit) {
   at::Tensor y = linear_meta(x, w, bias, activation, residual, out_dtype, limit);
   const c10::SymInt rows = activation ? x.sym_numel() / x.sym_size(-1) : c10::SymInt(0);
-  return {y, at::empty_symint({rows, w.sym_size(0)}, x.options())};
+  return {y, at::empty_symint({rows, w.sym_size(0)}, x.options().dtype(at::kFloat))};
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient_meta(const at::Tensor& x, const at::Tensor& w, const at::Tensor&, int64_t, double,
                                                              const at::Tensor&, bool need_x, bool need_w,
