@@ -659,8 +659,9 @@ int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_st
                  int64_t residual_stride, void* out, int out_dtype, float* z, void* workspace,
                  int64_t workspace_bytes, void* stream);
 
-/* How it runs at a size, for tests: plan[0] the tile's rows and lines (0: the few rows'
- * kernel), plan[1] the K splits, plan[2] the wavefronts of the few rows' workgroups. */
+/* How it runs at a size, for tests: plan[0] 0 on tiles of plan[1] rows and plan[2] lines, K in
+ * plan[3] splits; 1 (16 rows at most) with K over plan[3] wavefronts; 2 (eight at most)
+ * with plan[2] lines a wavefront, K over plan[3]. */
 int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int32_t* plan);
 
 /*

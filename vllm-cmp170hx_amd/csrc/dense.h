@@ -61,13 +61,13 @@ __device__ __forceinline__ uint32_t pack16(int dtype, float a, float b) {
 // loads and stores of 16 bytes whatever their alignment.
 template <int kC>
 __device__ __forceinline__ void load_columns(const void* p, int dtype, int64_t at, int64_t valid, float (&v)[kC]) {
-  if (valid < kC) {
+  if (kC == 1 || valid < kC) {
 #pragma unroll
     for (int q = 0; q < kC; ++q) v[q] = q < valid ? vq::load_act(p, dtype, at + q) : 0.0f;
   } else if (dtype == vq::kFP32) {
     __builtin_memcpy(v, static_cast<const float*>(p) + at, 4 * kC);
   } else {
-    uint32_t w[kC / 2];
+    uint32_t w[(kC + 1) / 2];
     __builtin_memcpy(w, static_cast<const uint16_t*>(p) + at, 2 * kC);
 #pragma unroll
     for (int q = 0; q < kC; ++q) {
@@ -78,7 +78,7 @@ __device__ __forceinline__ void load_columns(const void* p, int dtype, int64_t a
 }
 template <int kC>
 __device__ __forceinline__ void store_columns(void* p, int dtype, int64_t at, int64_t valid, const float (&v)[kC]) {
-  if (valid < kC) {
+  if (kC == 1 || valid < kC) {
 #pragma unroll
     for (int q = 0; q < kC; ++q) {
       if (q < valid) vq::store_act(p, dtype, at + q, v[q]);
@@ -86,7 +86,7 @@ __device__ __forceinline__ void store_columns(void* p, int dtype, int64_t at, in
   } else if (dtype == vq::kFP32) {
     __builtin_memcpy(static_cast<float*>(p) + at, v, 4 * kC);
   } else {
-    uint32_t w[kC / 2];
+    uint32_t w[(kC + 1) / 2];
 #pragma unroll
     for (int q = 0; q < kC / 2; ++q) w[q] = pack16(dtype, v[2 * q], v[2 * q + 1]);
     __builtin_memcpy(static_cast<uint16_t*>(p) + at, w, 2 * kC);

@@ -28,17 +28,32 @@ constexpr int64_t kMaxK = 1 << 21;       // 256 rows of a tile stay below 2^31 b
 constexpr int64_t kMaxStride = 1 << 22;
 constexpr int64_t kMaxSize = int64_t(1) << 30;  // rows, lines
 
-// ---- few rows ---------------------------------------------------------------------
+// ---- eight rows at most -------------------------------------------------------------
 //
-// W is read once, from memory to the registers of the wavefront that multiplies it: a
-// wavefront holds 16 lines (a gated activation: 16 gate and the 16 up lines of the same
-// columns), per step 128 k, in which lane (r = lane & 15, q = lane >> 4) loads the
-// chunks 4 j + q (j < 4) of line r and of x's row r and multiplies them in four
-// v_mfma_16x16x32.  K is split over the wavefronts of a workgroup, whose sums meet in
-// LDS and are added in order.
+// A wavefront takes kLines lines of W (a gated activation: a gate line and its up line), its
+// lanes 512 k of each at a time, 16 bytes a lane and load: a line streams from memory
+// as it lies.  x comes from the caches, its chunks held for all the wavefront's lines; products are
+// v_dot2 with FP32 sums, a lane's own until the end.  Where lines are few, `parts` wavefronts
+// of a workgroup share them, every parts-th 512 k each, and add up in LDS.
 
-constexpr int kSmallRows = 16;  // of one B operand
-constexpr int kStepChunks = 16;
+constexpr int kGemvRows = 8, kGemvWaves = 8, kGemvStep = 64 * kChunk;
+
+template <bool kBf16>
+__device__ __forceinline__ float dot8(const u32x4_t& a, const u32x4_t& b, float sum) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kBf16) {
+      typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+      const uint32_t ai = a[i], bi = b[i];
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, ai), __builtin_bit_cast(bf16x2_t, bi), sum, false);
+    } else {
+      typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+      const uint32_t ai = a[i], bi = b[i];
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, ai), __builtin_bit_cast(half2_t, bi), sum, false);
+    }
+  }
+  return sum;
+}
 
 template <bool kBf16>
 __device__ __forceinline__ u32x4_t load_chunk(const uint16_t* row, int64_t b, int64_t k) {
@@ -56,10 +71,104 @@ __device__ __forceinline__ u32x4_t load_chunk(const uint16_t* row, int64_t b, in
   return v;
 }
 
-template <int kTiles, bool kGated, bool kBf16>
+__device__ __forceinline__ float wave_sum(float v, int lane) {
+  v += vq::xor_lanes<32>(v, lane);
+  v += vq::xor_lanes<16>(v, lane);
+  v += vq::xor_lanes<8>(v, lane);
+  v += vq::xor_lanes<4>(v, lane);
+  v += vq::xor_lanes<2>(v, lane);
+  return v + vq::xor_lanes<1>(v, lane);
+}
+
+template <int kRows, int kLines, bool kGated, bool kBf16>
+__global__ __launch_bounds__(64 * kGemvWaves) void gemv_kernel(Operand x, Operand w, int64_t k, int parts, Epilogue e) {
+  static_assert(!kGated || kLines == 2, "a gate and an up line");
+  constexpr int kCols = kGated ? 1 : kLines;
+  constexpr int kAhead = kRows * kLines > 8 ? 2 : 4;  // steps whose loads are on their way together
+  __shared__ float sums[kGemvWaves][kLines][kRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
+  const int part = wave % parts, set = wave / parts;
+  const int64_t c = (int64_t(blockIdx.x) * (kGemvWaves / parts) + set) * kCols;
+  const uint16_t* wrow[kLines];
+#pragma unroll
+  for (int l = 0; l < kLines; ++l) wrow[l] = w.p + (min(c + (kGated ? 0 : l), e.n - 1) + (kGated && l ? e.n : 0)) * w.stride;
+  const uint16_t* xrow[kRows];
+#pragma unroll
+  for (int m = 0; m < kRows; ++m) xrow[m] = x.p + min(int64_t(m), x.rows - 1) * x.stride;
+  float acc[kLines][kRows];
+#pragma unroll
+  for (int l = 0; l < kLines; ++l)
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) acc[l][m] = 0;
+  const int64_t chunks = (k + kChunk - 1) / kChunk;
+  if (c < e.n) {
+    for (int64_t b = 64 * part + lane; b < chunks; b += 64 * kAhead * parts) {
+      u32x4_t a[kAhead][kLines], v[kAhead][kRows];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+#pragma unroll
+        for (int l = 0; l < kLines; ++l) a[i][l] = load_chunk<kBf16>(wrow[l], b + 64 * i * parts, k);
+#pragma unroll
+        for (int m = 0; m < kRows; ++m) v[i][m] = load_chunk<kBf16>(xrow[m], b + 64 * i * parts, k);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int l = 0; l < kLines; ++l)
+#pragma unroll
+          for (int m = 0; m < kRows; ++m) acc[l][m] = dot8<kBf16>(a[i][l], v[i][m], acc[l][m]);
+    }
+  }
+  // lane m keeps row m's
+  float mine[kLines];
+#pragma unroll
+  for (int l = 0; l < kLines; ++l) {
+    mine[l] = 0;
+#pragma unroll
+    for (int m = 0; m < kRows; ++m) {
+      const float all = wave_sum(acc[l][m], lane);
+      if (lane == m) mine[l] = all;
+    }
+  }
+  if (parts > 1) {
+    if (lane < kRows) {
+#pragma unroll
+      for (int l = 0; l < kLines; ++l) sums[wave][l][lane] = mine[l];
+    }
+    __syncthreads();
+    if (part || lane >= kRows) return;
+#pragma unroll
+    for (int l = 0; l < kLines; ++l) {
+      mine[l] = 0;
+      for (int p = 0; p < parts; ++p) mine[l] += sums[wave + p][l][lane];
+    }
+  }
+  if (lane >= kRows || lane >= x.rows || c >= e.n) return;
+  float v[kCols], u[kCols];
+#pragma unroll
+  for (int q = 0; q < kCols; ++q) {
+    v[q] = mine[q];
+    u[q] = kGated ? mine[1] : 0.0f;
+  }
+  finish_columns<kCols, kGated>(e, lane, c, v, u);
+}
+
+// ---- nine to 16 rows ------------------------------------------------------------------
+//
+// W is read once, from memory to the registers of the wavefront that multiplies it: a
+// wavefront holds 16 lines (a gated activation: 16 gate and the 16 up lines of the same
+// columns), per step 128 k, in which lane (r = lane & 15, q = lane >> 4) loads the
+// chunks 4 j + q (j < 4) of line r and of x's row r and multiplies them in four
+// v_mfma_16x16x32.  K is split over the wavefronts of a workgroup, whose sums meet in
+// LDS and are added in order.
+
+constexpr int kSmallRows = 16;  // of one B operand
+constexpr int kStepChunks = 16;
+
+template <bool kGated, bool kBf16>
 __global__ __launch_bounds__(1024) void small_kernel(Operand x, Operand w, int64_t k, Epilogue e) {
   constexpr int kOps = kGated ? 2 : 1;
-  extern __shared__ __attribute__((aligned(16))) float sums[];  // [wave][kOps][kTiles][64 lanes][4]
+  __shared__ __attribute__((aligned(16))) float sums[16][kOps][64 * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6), waves = int(blockDim.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int64_t c0 = int64_t(blockIdx.x) * 16;
@@ -67,50 +176,38 @@ __global__ __launch_bounds__(1024) void small_kernel(Operand x, Operand w, int64
   const uint16_t* wrow[kOps];
 #pragma unroll
   for (int o = 0; o < kOps; ++o) wrow[o] = w.p + (line + o * e.n) * w.stride;
-  const uint16_t* xrow[kTiles];
+  const uint16_t* xrow = x.p + min(int64_t(r), x.rows - 1) * x.stride;
+  f32x4_t acc[kOps];
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) xrow[t] = x.p + min(int64_t(kSmallRows * t + r), x.rows - 1) * x.stride;
-  f32x4_t acc[kOps][kTiles];
-#pragma unroll
-  for (int o = 0; o < kOps; ++o)
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) acc[o][t] = f32x4_t{0, 0, 0, 0};
+  for (int o = 0; o < kOps; ++o) acc[o] = f32x4_t{0, 0, 0, 0};
   const int64_t steps = (k + kChunk * kStepChunks - 1) / (kChunk * kStepChunks);
   for (int64_t s = wave; s < steps; s += waves) {
-    u32x4_t a[kOps][4], b[kTiles][4];
+    u32x4_t a[kOps][4], b[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t at = s * kStepChunks + 4 * j + q;
 #pragma unroll
       for (int o = 0; o < kOps; ++o) a[o][j] = load_chunk<kBf16>(wrow[o], at, k);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) b[t][j] = load_chunk<kBf16>(xrow[t], at, k);
+      b[j] = load_chunk<kBf16>(xrow, at, k);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int o = 0; o < kOps; ++o)
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) mfma16<kBf16>(acc[o][t], a[o][j], b[t][j]);
+      for (int o = 0; o < kOps; ++o) mfma16<kBf16>(acc[o], a[o][j], b[j]);
   }
 #pragma unroll
-  for (int o = 0; o < kOps; ++o)
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-      *reinterpret_cast<f32x4_t*>(sums + (((wave * kOps + o) * kTiles + t) * 64 + lane) * 4) = acc[o][t];
+  for (int o = 0; o < kOps; ++o) *reinterpret_cast<f32x4_t*>(&sums[wave][o][4 * lane]) = acc[o];
   __syncthreads();
-  for (int t = wave; t < kTiles; t += waves) {
-    float v[4], u[4];
+  if (wave) return;
+  float v[4], u[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int o = 0; o < kOps; ++o) {
-      f32x4_t all{0, 0, 0, 0};
-      for (int from = 0; from < waves; ++from) all += *reinterpret_cast<const f32x4_t*>(sums + (((from * kOps + o) * kTiles + t) * 64 + lane) * 4);
+  for (int o = 0; o < kOps; ++o) {
+    f32x4_t all{0, 0, 0, 0};
+    for (int from = 0; from < waves; ++from) all += *reinterpret_cast<const f32x4_t*>(&sums[from][o][4 * lane]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) (o ? u : v)[i] = all[i];
-    }
-    const int64_t m = kSmallRows * t + r;
-    if (m < x.rows) finish_columns<4, kGated>(e, m, c0 + 4 * q, v, u);
+    for (int i = 0; i < 4; ++i) (o ? u : v)[i] = all[i];
   }
+  if (r < x.rows) finish_columns<4, kGated>(e, r, c0 + 4 * q, v, u);
 }
 
 // ---- the sum of K splits --------------------------------------------------------------
@@ -367,36 +464,59 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t
 int64_t up_to(int64_t v, int64_t step) { return (v + step - 1) / step * step; }
 int64_t parts_of(int64_t v, int64_t step) { return (v + step - 1) / step; }
 
+// The tiles, and for the choice between them what they take in us: a round of workgroups
+// `start`, and a stage `alone` on a card hardly filled or `full` on a full one.
+struct Shape {
+  int lines, rows, places;  // places: workgroups that the card holds
+  double start, alone, full;
+};
+constexpr int kCus = 256, kShapes = 4;
+constexpr Shape kShape[kShapes] = {{256, 256, kCus, 10.95, 0.38, 1.6},
+                                   {256, 128, kCus, 8.97, 0.18, 0.83},
+                                   {64, 128, 2 * kCus, 4.5, 0.07, 0.52},
+                                   {64, 64, 2 * kCus, 1.6, 0.06, 0.38}};
+
+enum Kind : int { kTiles = 0, kSmall = 1, kGemv = 2 };
+
 struct Plan {
-  int tile;  // 64 tile rows and lines; 0: the few rows' kernel
-  int splits;
-  int waves;  // of the few rows' kernel
+  Kind kind;
+  int shape, splits;  // of the tiles
+  int waves;          // of the small kernel: a workgroup's; of the gemv: those that share a line
+  int lines;          // of the gemv: a wavefront's
 };
 
-constexpr int kCus = 256;
-
+// The figures above are fitted to 80 sizes (70 to 4096 rows, k 512 to 14336, n 128 to 14336),
+// each on all tiles and up to 16 splits; the choice by them is 4% slower than the best of each
+// on average, 35% at worst (70 rows of 4096 x 288: 11.1 us for 8.2).
 Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated) {
   const int64_t lines = gated ? 2 * n : n;
-  if (rows <= 64) {
+  if (rows <= kGemvRows) {
+    // a line a wavefront, and as many wavefronts a line as fill the card with four each SIMD
+    const int64_t steps = parts_of(k, kGemvStep);
+    Plan p{kGemv, 0, 1, 1, lines >= 8192 || gated ? 2 : 1};
+    while (p.waves < kGemvWaves && p.waves < steps && parts_of(lines, p.lines) * p.waves < 16 * kCus) p.waves *= 2;
+    return p;
+  }
+  if (rows <= kSmallRows) {
     const int64_t steps = parts_of(k, kChunk * kStepChunks);
-    // (up to 64 KB of sums)
-    return {0, 1, steps >= 16 && !(gated && rows > 32) ? 16 : steps >= 8 ? 8 : 4};
+    return {kSmall, 0, 1, steps >= 16 ? 16 : steps >= 8 ? 8 : 4, 0};
   }
   const int64_t stages = parts_of(k, kChunk * kStageChunks);
-  Plan best{4, 1, 0};
+  Plan best{kTiles, 0, 1, 0, 0};
   double least = 0;
-  for (int tile : {4, 2, 1}) {
-    if (gated && tile == 1) continue;
-    const int64_t tiles = parts_of(rows, 64 * tile) * parts_of(lines, 64 * tile);
-    const int64_t places = kCus * (tile == 4 ? 1 : 2);
+  for (int i = 0; i < kShapes; ++i) {
+    const Shape& t = kShape[i];
+    const int64_t tiles = parts_of(rows, t.rows) * parts_of(n, gated ? t.lines / 2 : t.lines);
     for (int64_t splits = 1; splits <= 16 && splits <= std::max<int64_t>(1, stages / 4); ++splits) {
-      const double rounds = double(parts_of(tiles * splits, places));
-      const double stage = tile == 4 ? 1.0 : tile == 2 ? 0.7 : 0.4;
-      double cost = rounds * (4 + double(parts_of(stages, splits)) * stage);
-      if (splits > 1) cost += 4 + double(splits) * double(rows) * double(lines) * 8 / 4e6;
+      if (splits > 1 && tiles * splits > 8 * kCus) break;
+      const int64_t each = parts_of(stages, splits), all = tiles * parts_of(stages, each);
+      const int64_t rest = all % t.places;
+      double cost = double(all / t.places) * (t.start + double(each) * t.full);
+      if (rest) cost += t.start + double(each) * (t.alone + (t.full - t.alone) * double(rest) / t.places);
+      if (splits > 1) cost += 3 + double(splits) * double(rows) * double(lines) * 4 / 6.5e6;  // written and added up
       if (least == 0 || cost < least) {
         least = cost;
-        best = {tile, int(splits), 0};
+        best = {kTiles, i, int(splits), 0, 0};
       }
     }
   }
@@ -407,59 +527,67 @@ bool direct(const Operand& o, int64_t k) { return aligned(o.p, 16) && o.stride %
 
 int64_t sums_bytes(const Plan& p, int64_t rows, int64_t lines) { return p.splits > 1 ? p.splits * rows * lines * 4 : 0; }
 
-template <int kTiles>
-void launch_small(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, bool bf16, int waves, hipStream_t s) {
-  const bool gated = e.activation == kSwiglu;
+template <bool kBf16>
+void launch_small(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, int waves, hipStream_t s) {
   const dim3 grid(unsigned(parts_of(e.n, 16))), block(unsigned(64 * waves));
-  const size_t lds = size_t(waves) * (gated ? 2 : 1) * kTiles * 64 * 16;
-  if (gated) {
-    if (bf16) hipLaunchKernelGGL((small_kernel<kTiles, true, true>), grid, block, lds, s, x, w, k, e);
-    else hipLaunchKernelGGL((small_kernel<kTiles, true, false>), grid, block, lds, s, x, w, k, e);
-  } else {
-    if (bf16) hipLaunchKernelGGL((small_kernel<kTiles, false, true>), grid, block, lds, s, x, w, k, e);
-    else hipLaunchKernelGGL((small_kernel<kTiles, false, false>), grid, block, lds, s, x, w, k, e);
-  }
+  if (e.activation == kSwiglu) hipLaunchKernelGGL((small_kernel<true, kBf16>), grid, block, 0, s, x, w, k, e);
+  else hipLaunchKernelGGL((small_kernel<false, kBf16>), grid, block, 0, s, x, w, k, e);
 }
 
-template <typename T>
-void launch_tile(TileArgs& t, bool bf16, int64_t splits, hipStream_t s) {
-  const bool gated = t.e.activation == kSwiglu;
-  const int64_t total = int64_t(t.tiles_n) * t.tiles_m;
-  const dim3 grid(unsigned(up_to(total, 8)), unsigned(splits)), block(T::kThreads);
-  if constexpr (T::kN >= 2) {
-    if (gated) {
-      if (bf16) hipLaunchKernelGGL((tile_kernel<T, true, true>), grid, block, 0, s, t);
-      else hipLaunchKernelGGL((tile_kernel<T, true, false>), grid, block, 0, s, t);
-      return;
-    }
-  }
-  if (bf16) hipLaunchKernelGGL((tile_kernel<T, false, true>), grid, block, 0, s, t);
-  else hipLaunchKernelGGL((tile_kernel<T, false, false>), grid, block, 0, s, t);
+template <int kRows, bool kBf16>
+void launch_gemv(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, const Plan& p, hipStream_t s) {
+  const bool gated = e.activation == kSwiglu;
+  const int64_t each = kGemvWaves / p.waves * (gated ? 1 : p.lines);
+  const dim3 grid(unsigned(parts_of(e.n, each))), block(64 * kGemvWaves);
+  if (gated) hipLaunchKernelGGL((gemv_kernel<kRows, 2, true, kBf16>), grid, block, 0, s, x, w, k, p.waves, e);
+  else if (p.lines == 2) hipLaunchKernelGGL((gemv_kernel<kRows, 2, false, kBf16>), grid, block, 0, s, x, w, k, p.waves, e);
+  else hipLaunchKernelGGL((gemv_kernel<kRows, 1, false, kBf16>), grid, block, 0, s, x, w, k, p.waves, e);
+}
+
+// Plain: without a gated activation.
+template <typename Plain, typename Gated, bool kBf16>
+void launch_tile(const TileArgs& t, int64_t splits, hipStream_t s) {
+  const dim3 grid(unsigned(up_to(int64_t(t.tiles_n) * t.tiles_m, 8)), unsigned(splits));
+  if (t.e.activation == kSwiglu) hipLaunchKernelGGL((tile_kernel<Gated, true, kBf16>), grid, dim3(Gated::kThreads), 0, s, t);
+  else hipLaunchKernelGGL((tile_kernel<Plain, false, kBf16>), grid, dim3(Plain::kThreads), 0, s, t);
 }
 
 // x [rows][k] times W's transpose, finished by e; sums: the plan's K splits' room.
-int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, bool bf16, float* sums, const Plan& p, hipStream_t s) {
-  if (p.tile == 0) {
-    if (x.rows <= 16) launch_small<1>(x, w, k, e, bf16, p.waves, s);
-    else if (x.rows <= 32) launch_small<2>(x, w, k, e, bf16, p.waves, s);
-    else launch_small<4>(x, w, k, e, bf16, p.waves, s);
+template <bool kBf16>
+int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, float* sums, const Plan& p, hipStream_t s) {
+  if (p.kind == kGemv) {
+    if (x.rows == 1) launch_gemv<1, kBf16>(x, w, k, e, p, s);
+    else if (x.rows == 2) launch_gemv<2, kBf16>(x, w, k, e, p, s);
+    else if (x.rows <= 4) launch_gemv<4, kBf16>(x, w, k, e, p, s);
+    else launch_gemv<8, kBf16>(x, w, k, e, p, s);
+    return vq::check_launch("dense_linear");
+  }
+  if (p.kind == kSmall) {
+    launch_small<kBf16>(x, w, k, e, p.waves, s);
     return vq::check_launch("dense_linear");
   }
   const bool gated = e.activation == kSwiglu;
-  const int64_t side = 64 * p.tile, stages = parts_of(k, kChunk * kStageChunks);
-  const int64_t tiles_n = parts_of(e.n, gated ? side / 2 : side), tiles_m = parts_of(x.rows, side);
+  const Shape& shape = kShape[p.shape];
+  const int64_t stages = parts_of(k, kChunk * kStageChunks);
+  const int64_t tiles_n = parts_of(e.n, gated ? shape.lines / 2 : shape.lines), tiles_m = parts_of(x.rows, shape.rows);
   if (tiles_n * tiles_m > INT_MAX / 2) return vq::fail("dense_linear: too many rows and columns");
   const int64_t split = parts_of(stages, p.splits);
-  TileArgs t{x, w, int(parts_of(k, kChunk)), int(tiles_n), int(tiles_m), int(split), sums, e};
+  const TileArgs t{x, w, int(parts_of(k, kChunk)), int(tiles_n), int(tiles_m), int(split), sums, e};
   const int64_t splits = parts_of(stages, split);  // (none without a stage)
-  if (p.tile == 4) launch_tile<Tile<2, 4, 4, 2, 2>>(t, bf16, splits, s);
-  else if (p.tile == 2) launch_tile<Tile<2, 2, 2, 2, 2>>(t, bf16, splits, s);
-  else launch_tile<Tile<2, 2, 1, 1, 4>>(t, bf16, splits, s);
+  switch (p.shape) {
+    case 0: launch_tile<Tile<4, 2, 2, 4, 5>, Tile<4, 2, 2, 4, 5>, kBf16>(t, splits, s); break;
+    case 1: launch_tile<Tile<4, 2, 2, 2, 6>, Tile<4, 2, 2, 2, 6>, kBf16>(t, splits, s); break;
+    case 2: launch_tile<Tile<2, 2, 1, 2, 6>, Tile<1, 4, 2, 1, 6>, kBf16>(t, splits, s); break;
+    default: launch_tile<Tile<2, 2, 1, 1, 8>, Tile<1, 2, 2, 1, 8>, kBf16>(t, splits, s); break;
+  }
   if (int rc = vq::check_launch("dense_linear")) return rc;
   if (splits == 1) return vq::kOk;
   const int64_t groups = parts_of(x.rows * parts_of(e.n, 8), 256);
   hipLaunchKernelGGL(finish_kernel, dim3(unsigned(std::min<int64_t>(groups, 8192))), dim3(256), 0, s, sums, int(splits), x.rows, e);
   return vq::check_launch("dense_linear");
+}
+int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, bool bf16, float* sums, const Plan& p, hipStream_t s) {
+  return bf16 ? product<true>(x, w, k, e, sums, p, s) : product<false>(x, w, k, e, sums, p, s);
 }
 
 int pack(Operand& o, int64_t k, uint16_t* to, hipStream_t s) {
@@ -562,7 +690,7 @@ extern "C" int64_t dense_linear_workspace_size(const void* x, int64_t rows, int6
   const bool gated = activation == kSwiglu;
   const int64_t lines = gated ? 2 * n : n;
   const Plan p = plan_of(rows, k, n, gated);
-  const bool tiles = p.tile != 0;
+  const bool tiles = p.kind == kTiles;
   const Operand xo{static_cast<const uint16_t*>(x), rows, x_stride}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
   return Room(rows, k, lines, p, tiles && !direct(xo, k), tiles && !direct(wo, k)).bytes;
 }
@@ -572,9 +700,10 @@ extern "C" int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activat
   if (int rc = check_sizes(rows, k, n, activation)) return rc;
   if (!plan) return vq::fail("dense_linear: null pointer");
   const Plan p = plan_of(rows, k, n, activation == kSwiglu);
-  plan[0] = 64 * p.tile;
-  plan[1] = p.splits;
-  plan[2] = p.waves;
+  plan[0] = p.kind;
+  plan[1] = p.kind == kTiles ? kShape[p.shape].rows : 0;
+  plan[2] = p.kind == kTiles ? kShape[p.shape].lines : p.lines;
+  plan[3] = p.kind == kTiles ? p.splits : p.waves;
   return vq::kOk;
 }
 
@@ -595,7 +724,7 @@ extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, i
   const int64_t lines = gated ? 2 * n : n;
   Operand xo{static_cast<const uint16_t*>(x), rows, rows > 1 ? x_stride : k}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
   const Plan p = plan_of(rows, k, n, gated);
-  const bool pack_x = p.tile && !direct(xo, k), pack_w = p.tile && !direct(wo, k);
+  const bool pack_x = p.kind == kTiles && !direct(xo, k), pack_w = p.kind == kTiles && !direct(wo, k);
   const Room room(rows, k, lines, p, pack_x, pack_w);
   if (room.bytes && (!workspace || workspace_bytes < room.bytes || !aligned(workspace, 16))) {
     return vq::fail("dense_linear: workspace too small or misaligned");

@@ -2,9 +2,10 @@
 //
 // A workgroup of four or eight wavefronts computes kCols lines of W by kRows rows of x, each
 // wavefront 32 kN x 32 kM of v_mfma_f32_32x32x16 tiles.  A stage is 64 k: 128
-// bytes of every row and line, in one of kBufs buffers, one barrier a stage.
-//  * Rows come to LDS by DMA, one 128-byte line in eight lanes, up to kBufs - 1 stages
-//    ahead.  A line's eight 16-byte chunks lie in LDS in the order chunk ^ (line / 2 &
+// bytes of every row and line, one barrier a stage.
+//  * Rows come to LDS by DMA, one 128-byte line in eight lanes, into a ring of kParts
+//    buffers, each a stage's lines of W or its rows of x: odd numbers of them keep LDS
+//    full, and some loads are on their way whenever a stage is waited for.  A line's eight 16-byte chunks lie in LDS in the order chunk ^ (line / 2 &
 //    7), so that the 16 lines that a ds_read_b128 reads at once, all at one chunk, lie
 //    on 16 different 16-byte columns of the 64 banks.
 //  * A lane of the MFMA holds one chunk: line lane & 31, chunk 2 sub + (lane >> 5) of
@@ -51,38 +52,41 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base, uint3
 // An offset past any buffer: such loads give zeros.
 constexpr uint32_t kPastEnd = 0x80000000u;
 
-// A workgroup's kWn x kWm wavefronts, each of 32 kN lines by 32 kM rows, and its stage buffers.
-template <int kWn_, int kWm_, int kN_, int kM_, int kBufs_>
+// A workgroup's kWn x kWm wavefronts, each of 32 kN lines by 32 kM rows, and its ring's parts.
+template <int kWn_, int kWm_, int kN_, int kM_, int kParts_>
 struct Tile {
-  static constexpr int kWn = kWn_, kWm = kWm_, kN = kN_, kM = kM_, kBufs = kBufs_;
+  static constexpr int kWn = kWn_, kWm = kWm_, kN = kN_, kM = kM_, kParts = kParts_;
   static constexpr int kWaves = kWn * kWm, kThreads = 64 * kWaves;
-  static constexpr int kCols = 32 * kN * kWn, kRows = 32 * kM * kWm, kLines = kCols + kRows;
+  static constexpr int kCols = 32 * kN * kWn, kRows = 32 * kM * kWm;
+  // part i's bytes: even ones hold lines of W and odd ones rows of x, where there is an odd
+  // number of them each both in turn
+  static constexpr int part_bytes(int i) {
+    return kStageBytes * (kParts % 2 ? (kCols > kRows ? kCols : kRows) : i % 2 ? kRows : kCols);
+  }
+  static constexpr int kBytes = part_bytes(0) * ((kParts + 1) / 2) + part_bytes(1) * (kParts / 2);
   // workgroups that a CU's LDS holds, two at most
-  static constexpr int kGroups = kLines * kStageBytes * kBufs > 80 * 1024 ? 1 : 2;
+  static constexpr int kGroups = kBytes > 80 * 1024 ? 1 : 2;
 };
+
+// Part i of the ring.  (Buffers by name: the compiler then sees that a stage's reads are
+// not of the buffer that the DMA is filling, and does not wait for it.)
+template <typename T, int i>
+__device__ __forceinline__ uint8_t* ring_part() {
+  static __shared__ __attribute__((aligned(1024))) uint8_t part[T::part_bytes(i)];
+  return part;
+}
 
 template <typename T, bool kGated, bool kBf16>
 __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_kernel(TileArgs g) {
-  constexpr int kN = T::kN, kM = T::kM, kBufs = T::kBufs, kWaves = T::kWaves;
-  constexpr int kCols = T::kCols, kRows = T::kRows, kLines = T::kLines;
+  constexpr int kN = T::kN, kM = T::kM, kParts = T::kParts, kWaves = T::kWaves;
+  constexpr int kCols = T::kCols, kRows = T::kRows;
   constexpr int kLoadRows = 8;  // lines of a 1 KB DMA load
   constexpr int kLoadsW = kCols / (kWaves * kLoadRows), kLoadsX = kRows / (kWaves * kLoadRows);  // loads a wavefront and stage
   constexpr int kLoads = kLoadsW + kLoadsX;
-  static_assert(kBufs >= 2 && kBufs <= 4, "stage buffers");
+  static_assert(kParts >= 4, "two stages");
   static_assert(kLoadsW * kWaves * kLoadRows == kCols && kLoadsX * kWaves * kLoadRows == kRows, "whole loads");
   static_assert(!kGated || (kN >= 2 && kLoadRows * kLoadsW <= 16 * kN), "a wavefront loads gate or up lines alone");
-  // (buffers by name: the compiler then sees that a stage's reads are not of the
-  // buffer that the DMA is filling, and does not wait for it)
-  constexpr int kBufBytes = kLines * kStageBytes;
-  __shared__ __attribute__((aligned(1024))) uint8_t buf0[kBufBytes], buf1[kBufBytes], buf2[kBufs > 2 ? kBufBytes : 16],
-      buf3[kBufs > 3 ? kBufBytes : 16];
-  const auto buf = [&](auto i_c) -> uint8_t* {
-    constexpr int i = decltype(i_c)::value % kBufs;
-    if constexpr (i == 0) return buf0;
-    else if constexpr (i == 1) return buf1;
-    else if constexpr (i == 2) return buf2;
-    else return buf3;
-  };
+  const auto part_of = [](auto i_c) { return ring_part<T, decltype(i_c)::value % kParts>(); };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = vq::uniform(tid >> 6);
@@ -109,44 +113,53 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
   const __amdgpu_buffer_rsrc_t wbuf = buffer(g.w.p + (c0 + (up ? g.e.n : 0)) * g.w.stride, uint32_t(ncols - 1) * wline + line_bytes);
   const __amdgpu_buffer_rsrc_t xbuf = buffer(g.x.p + m0 * g.x.stride, uint32_t(nrows - 1) * xline + line_bytes);
   const int sub_row = lane >> 3;
-  const auto first_line = [&](int i) {
-    return i < kLoadsW ? w_first + kLoadRows * i : kCols + kLoadRows * (kLoadsX * wave + i - kLoadsW);
-  };
+  const int x_first = kLoadRows * kLoadsX * wave;
   const auto swizzle_of = [](int l) { return (l >> 1) & 7; };
   const int kb[2] = {(lane & 7) ^ swizzle_of(sub_row), (lane & 7) ^ swizzle_of(kLoadRows + sub_row)};
-  // the scalar first row of load i (a row of the buffer also where the load's lie past
+  // the scalar first row of load i of W (x) (a row of the buffer also where the load's lie past
   // its end: their sums are not stored; the rest of a load that begins inside it is zeros)
-  const auto first_row = [&](int i) -> int {
-    int l;
-    if (i >= kLoadsW) {
-      l = first_line(i) - kCols;
-      return l < nrows ? l : 0;
-    }
-    l = first_line(i);
+  const auto w_row = [&](int i) -> int {
+    int l = w_first + kLoadRows * i;
     if constexpr (kGated) l = l / (32 * kN) * (16 * kN) + l % (16 * kN);
     return l < ncols ? l : 0;
+  };
+  const auto x_row = [&](int i) -> int {
+    const int l = x_first + kLoadRows * i;
+    return l < nrows ? l : 0;
   };
   const uint32_t wlane[2] = {sub_row * wline + kb[0] * kChunkBytes, sub_row * wline + kb[1] * kChunkBytes};
   const uint32_t xlane[2] = {sub_row * xline + kb[0] * kChunkBytes, sub_row * xline + kb[1] * kChunkBytes};
   const int all_stages = (g.chunks + kStageChunks - 1) / kStageChunks;
   const int first = int(blockIdx.y) * g.split_stages;
   const int stages = min(first + g.split_stages, all_stages);
-  // DMA load i of stage s (zeros past the last stage)
-  const auto fetch = [&](auto i_c, int s, uint8_t* into) __attribute__((always_inline)) {
-    constexpr int i = decltype(i_c)::value;
+  // DMA load i of stage s's lines of W or rows of x (zeros past the last stage)
+  const auto fetch = [&](auto x_c, int i, int s, uint8_t* into) __attribute__((always_inline)) {
+    constexpr bool kX = decltype(x_c)::value;
     const int left = s < stages ? g.chunks - s * kStageChunks : 0;
-    const int parity = (i < kLoadsW ? kLoadsW * wave + i : kLoadsX * wave + i - kLoadsW) & 1;
-    const uint32_t lane_part = i < kLoadsW ? wlane[parity] : xlane[parity];
-    const uint32_t o = left >= kStageChunks || kb[parity] < left ? lane_part : kPastEnd;
-    const int row_part = first_row(i) * int(i < kLoadsW ? wline : xline);
+    const int parity = ((kX ? kLoadsX : kLoadsW) * wave + i) & 1;
+    const uint32_t o = left >= kStageChunks || kb[parity] < left ? (kX ? xlane[parity] : wlane[parity]) : kPastEnd;
+    const int row_part = kX ? x_row(i) * int(xline) : w_row(i) * int(wline);
     // (the scalar offset stays below the buffer's size, or its bounds check would wrap)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(i < kLoadsW ? wbuf : xbuf, (lds_ptr_t)(into + first_line(i) * kStageBytes), 16, int(o),
-                                             row_part + (left > 0 ? s * kStageBytes : 0), 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kX ? xbuf : wbuf, (lds_ptr_t)(into + ((kX ? x_first : w_first) + kLoadRows * i) * kStageBytes),
+                                             16, int(o), row_part + (left > 0 ? s * kStageBytes : 0), 0, 0);
   };
-  // a stage has landed (its loads of this wavefront, behind which kBufs - 2 stages'
+  // Part kFrom + 2 s (an odd one is of x) and the next one are loaded together, load i of
+  // kLoads; both take the places of stage s - kParts / 2's.
+  const auto fetch_pair = [&](auto from_c, auto place_c, int i, int s) __attribute__((always_inline)) {
+    constexpr int kFrom = decltype(from_c)::value, kPlace = decltype(place_c)::value;
+    constexpr int kFirst = kFrom % 2 ? kLoadsX : kLoadsW;
+    using std::integral_constant;
+    if (i < kFirst) {
+      fetch(integral_constant<bool, kFrom % 2 != 0>{}, i, s + kFrom / 2, part_of(integral_constant<int, kPlace>{}));
+    } else {
+      fetch(integral_constant<bool, kFrom % 2 == 0>{}, i - kFirst, s + (kFrom + 1) / 2, part_of(integral_constant<int, kPlace + 1>{}));
+    }
+  };
+  // a stage has landed (this wavefront's loads of it, behind which those of kBehind more parts
   // stay on their way, then everyone's), and no wavefront reads the one before any more
-  const auto land = [&]() __attribute__((always_inline)) {
-    vq::wait_vmcnt<(kBufs - 2) * kLoads>();
+  const auto land = [&](auto behind_c) __attribute__((always_inline)) {
+    constexpr int kBehind = decltype(behind_c)::value;  // (the first of them a part of W)
+    vq::wait_vmcnt<(kBehind + 1) / 2 * kLoadsW + kBehind / 2 * kLoadsX>();
     // (a barrier that leaves the loads on their way: __syncthreads() waits for them)
     vq::wait_lgkmcnt0();
     __builtin_amdgcn_s_barrier();
@@ -162,65 +175,74 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
 #pragma unroll
       for (int k = 0; k < 16; ++k) acc[i][j][k] = 0;
 
-  const int wl = 32 * kN * wn + r, xl = kCols + 32 * kM * wm + r;
+  const int wl = 32 * kN * wn + r, xl = 32 * kM * wm + r;
   const int swizzle = swizzle_of(r);
   u32x4_t fw[2][kN], fx[2][kM];  // this sub-step's operands and the next one's
   // operand i of a sub-step: kN of W, then kM of x
-  const auto read = [&](auto i_c, const uint8_t* from, int sub, int set) __attribute__((always_inline)) {
+  const auto read = [&](auto i_c, const uint8_t* w, const uint8_t* x, int sub, int set) __attribute__((always_inline)) {
     constexpr int i = decltype(i_c)::value;
     const int at = ((2 * sub + h) ^ swizzle) * kChunkBytes;
-    if constexpr (i < kN) fw[set][i] = *reinterpret_cast<const u32x4_t*>(from + (wl + 32 * i) * kStageBytes + at);
-    else fx[set][i - kN] = *reinterpret_cast<const u32x4_t*>(from + (xl + 32 * (i - kN)) * kStageBytes + at);
+    if constexpr (i < kN) fw[set][i] = *reinterpret_cast<const u32x4_t*>(w + (wl + 32 * i) * kStageBytes + at);
+    else fx[set][i - kN] = *reinterpret_cast<const u32x4_t*>(x + (xl + 32 * (i - kN)) * kStageBytes + at);
   };
-  // Sub-step `sub` of a stage: between its kN kM MFMAs, one or two at a time, the
-  // next sub-step's operands are read (of `next`, at sub-step next_sub) and loads
-  // kFirst .. kLast - 1 of stage s issued into `into`.
-  const auto step = [&](auto sub_c, auto first_c, auto last_c, const uint8_t* next, int next_sub, int s,
-                        uint8_t* into) __attribute__((always_inline)) {
-    constexpr int sub = decltype(sub_c)::value, kFirst = decltype(first_c)::value, kLast = decltype(last_c)::value;
+  // Sub-step `sub` of stage s, in place `i` of the ring's turn: between its kN kM MFMAs, one or
+  // two at a time, the next sub-step's operands are read and a quarter of the loads issued
+  // that take the places of the stage before (after the barrier: of this one).
+  const auto step = [&](auto i_c, auto sub_c, int s) __attribute__((always_inline)) {
+    constexpr int i = decltype(i_c)::value, sub = decltype(sub_c)::value;
+    using std::integral_constant;
     constexpr int kReads = kN + kM, kSlots = kN * kM;
+    constexpr int kAt = sub == 3 ? 2 * i : 2 * i + 2 * kParts - 2;  // the freed places
+    constexpr int kNext = 2 * i + (sub == 3 ? 2 : 0);
+    const uint8_t* const w = part_of(integral_constant<int, kNext>{});
+    const uint8_t* const x = part_of(integral_constant<int, kNext + 1>{});
     for_range<0, kSlots>([&](auto slot_c) __attribute__((always_inline)) {
-      constexpr int slot = decltype(slot_c)::value, i = slot / kM, j = slot % kM;
+      constexpr int slot = decltype(slot_c)::value, a = slot / kM, b = slot % kM;
       for_range<slot * kReads / kSlots, (slot + 1) * kReads / kSlots>([&](auto k) __attribute__((always_inline)) {
-        read(k, next, next_sub, (sub + 1) & 1);
+        read(k, w, x, (sub + 1) & 3, (sub + 1) & 1);
       });
-      constexpr int kFetch = kLast - kFirst, kTurn = (slot + kSlots / 2) % kSlots;  // in other slots than the reads
-      for_range<kFirst + kTurn * kFetch / kSlots, kFirst + (kTurn + 1) * kFetch / kSlots>(
-          [&](auto k) __attribute__((always_inline)) { fetch(k, s, into); });
+      constexpr int kTurn = (slot + kSlots / 2) % kSlots;  // in other slots than the reads
+      constexpr int kQuarter = (sub + 1) & 3;  // of the loads
+      constexpr int kFirst = kQuarter * kLoads / 4, kFetch = (kQuarter + 1) * kLoads / 4 - kFirst;
+      for_range<kFirst + kTurn * kFetch / kSlots, kFirst + (kTurn + 1) * kFetch / kSlots>([&](auto k) __attribute__((always_inline)) {
+        fetch_pair(integral_constant<int, kParts>{}, integral_constant<int, kAt>{}, decltype(k)::value, sub == 3 ? s : s - 1);
+      });
       __builtin_amdgcn_sched_barrier(0);
-      mfma32<kBf16>(acc[i][j], fw[sub & 1][i], fx[sub & 1][j]);
+      mfma32<kBf16>(acc[a][b], fw[sub & 1][a], fx[sub & 1][b]);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  // Stage s, the i-th of a round of kBufs.  The barrier comes before the last sub-step,
-  // whose operands are in registers by then: its MFMAs run while the next stage's first
-  // operands are read, and its buffer takes stage s + kBufs: half of those loads here,
-  // the others in the next stage's first sub-steps.
-  constexpr int kHalf = kLoads / 2, kMore = kHalf + kLoads / 4;
+  // Stage s, in place i.  The barrier comes before the last sub-step, whose operands are in
+  // registers by then: its MFMAs run while the next stage's first operands are read.
   const auto stage = [&](auto i_c, int s) __attribute__((always_inline)) {
-    constexpr int i = decltype(i_c)::value;
     using std::integral_constant;
-    constexpr integral_constant<int, 0> none{};
-    uint8_t* const cur = buf(i_c);
-    uint8_t* const next = buf(integral_constant<int, i + 1>{});
-    uint8_t* const prev = buf(integral_constant<int, i + kBufs - 1>{});
-    step(none, integral_constant<int, kHalf>{}, integral_constant<int, kMore>{}, cur, 1, s + kBufs - 1, prev);
-    step(integral_constant<int, 1>{}, integral_constant<int, kMore>{}, integral_constant<int, kLoads>{}, cur, 2, s + kBufs - 1, prev);
-    step(integral_constant<int, 2>{}, none, none, cur, 3, 0, cur);
-    land();
-    step(integral_constant<int, 3>{}, none, integral_constant<int, kHalf>{}, next, 0, s + kBufs, cur);
+    step(i_c, integral_constant<int, 0>{}, s);
+    step(i_c, integral_constant<int, 1>{}, s);
+    step(i_c, integral_constant<int, 2>{}, s);
+    land(integral_constant<int, kParts - 4>{});
+    step(i_c, integral_constant<int, 3>{}, s);
   };
-  for_range<0, kBufs - 1>([&](auto b_c) {
-    for_range<0, kLoads>([&](auto k) { fetch(k, first + decltype(b_c)::value, buf(b_c)); });
+  // The ring's first turn of loads: its last two parts come in the place of a stage before
+  // the first one's, so that the first sub-steps load most of them.
+  for_range<0, kParts - 2>([&](auto p_c) {
+    constexpr int p = decltype(p_c)::value;
+    for_range<0, p % 2 ? kLoadsX : kLoadsW>([&](auto k) {
+      fetch(std::integral_constant<bool, p % 2 != 0>{}, decltype(k)::value, first + p / 2, part_of(p_c));
+    });
   });
-  land();
-  for_range<0, kHalf>([&](auto k) { fetch(k, first + kBufs - 1, buf(std::integral_constant<int, kBufs - 1>{})); });
-  for_range<0, kN + kM>([&](auto k) { read(k, buf0, 0, 0); });
+  land(std::integral_constant<int, kParts - 4>{});
+  for_range<0, kLoads / 4>([&](auto k) {
+    fetch_pair(std::integral_constant<int, kParts>{}, std::integral_constant<int, 2 * kParts - 2>{}, decltype(k)::value, first - 1);
+  });
+  for_range<0, kN + kM>([&](auto k) {
+    read(k, part_of(std::integral_constant<int, 0>{}), part_of(std::integral_constant<int, 1>{}), 0, 0);
+  });
+  constexpr int kTurn = kParts % 2 ? kParts : kParts / 2;  // stages
   int s = first;
-  for (; s + kBufs <= stages; s += kBufs) {
-    for_range<0, kBufs>([&](auto i) __attribute__((always_inline)) { stage(i, s + decltype(i)::value); });
+  for (; s + kTurn <= stages; s += kTurn) {
+    for_range<0, kTurn>([&](auto i) __attribute__((always_inline)) { stage(i, s + decltype(i)::value); });
   }
-  for_range<0, kBufs - 1>([&](auto i) __attribute__((always_inline)) {
+  for_range<0, kTurn - 1>([&](auto i) __attribute__((always_inline)) {
     if (s + decltype(i)::value < stages) stage(i, s + decltype(i)::value);
   });
   vq::wait_vmcnt<0>();  // the last loads (zeros) are in before their buffers are used again
@@ -229,10 +251,13 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
   // chunks in an order by the row), then four columns of a row a lane.
   constexpr int kStride = 32 * kN;
   const auto exchange_at = [](int row, int chunk) { return row * kStride + 4 * (chunk ^ (kN > 1 ? row & 15 : (row >> 1) & 7)); };
-  constexpr int kEach = (kWaves + kBufs - 1) / kBufs;  // exchanges in one buffer
-  static_assert(kEach * 32 * kStride * 4 <= kBufBytes, "the wavefronts' exchanges fit the stage buffers");
-  const int in = wave / kEach;
-  float* part = reinterpret_cast<float*>(in == 0 ? buf0 : in == 1 ? buf1 : in == 2 ? buf2 : buf3) + wave % kEach * 32 * kStride;
+  // exchanges in one part of the ring (the smaller ones' share)
+  constexpr int kEach = (T::part_bytes(0) < T::part_bytes(1) ? T::part_bytes(0) : T::part_bytes(1)) / (32 * kStride * 4);
+  static_assert(kEach * kParts >= kWaves, "the wavefronts' exchanges fit the ring");
+  float* part = nullptr;
+  for_range<0, (kWaves + kEach - 1) / kEach>([&](auto p_c) {
+    if (wave / kEach == decltype(p_c)::value) part = reinterpret_cast<float*>(part_of(p_c)) + wave % kEach * 32 * kStride;
+  });
   __syncthreads();
   const bool split = gridDim.y > 1;
   constexpr int kWave = kGated ? 16 * kN : 32 * kN;  // a wavefront's output columns
