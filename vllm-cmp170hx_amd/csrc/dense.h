@@ -43,7 +43,7 @@ struct Epilogue {
   // much to gradients as that of dz: of 4096 rows through 4096 x 28672 gated, in BF16, 1.7
   // times the result's own rounding for 1.4.)
   float* z;
-  const float* factor;  // multiplies the sums, or null
+  const uint32_t* top;  // the sums are over scale_of(*top), or null
 };
 
 inline bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -119,28 +119,46 @@ __device__ __forceinline__ float silu_slope(float z) {
 __device__ __forceinline__ float clamp_above(float v, float limit) { return v > limit ? limit : v; }
 __device__ __forceinline__ float clamp_both(float v, float limit) { return v > limit ? limit : (v < -limit ? -limit : v); }
 
+// FP16 holds gradients over a power of two that brings the largest magnitude to 2^13 .. 2^14:
+// those of a mean are often below what FP16 holds, and products with up lines may be above.
+// top: the FP32 bits of that magnitude.
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  const int e = int(top >> 23);
+  if (e == 0 || e == 255) return 1.0f;  // nothing, or no number
+  return __builtin_amdgcn_ldexpf(1.0f, min(13 - (e - 127), 126));
+}
+
+// What all rows have at columns c .. c + kC - 1.
+template <int kC, bool kGated>
+struct Columns {
+  float bias[kC], up_bias[kC], factor;
+  __device__ __forceinline__ Columns(const Epilogue& e, int64_t c) {
+    factor = e.top ? 1 / scale_of(*e.top) : 1.0f;
+#pragma unroll
+    for (int q = 0; q < kC; ++q) bias[q] = up_bias[q] = 0;
+    if (!e.bias || c >= e.n) return;
+    load_columns<kC>(e.bias, e.bias_dtype, c, e.n - c, bias);
+    if constexpr (kGated) load_columns<kC>(e.bias, e.bias_dtype, e.n + c, e.n - c, up_bias);
+  }
+};
+
+// A row's residual there.
+template <int kC>
+__device__ __forceinline__ void load_residual(const Epilogue& e, int64_t row, int64_t c, float (&r)[kC]) {
+  if (e.residual && c < e.n) load_columns<kC>(e.residual, e.residual_dtype, row * e.residual_stride + c, e.n - c, r);
+}
+
 // Columns c .. c + kC - 1 of a row from its sums (u: of a gated activation's up lines).
 template <int kC, bool kGated>
-__device__ __forceinline__ void finish_columns(const Epilogue& e, int64_t row, int64_t c, float (&v)[kC], float (&u)[kC]) {
+__device__ __forceinline__ void finish_columns(const Epilogue& e, int64_t row, int64_t c, float (&v)[kC], float (&u)[kC],
+                                               const Columns<kC, kGated>& columns, const float (&residual)[kC]) {
   const int64_t valid = e.n - c;
   if (valid <= 0) return;
-  if (e.factor) {
-    const float f = *e.factor;
 #pragma unroll
-    for (int q = 0; q < kC; ++q) v[q] *= f;
-  }
-  if (e.bias) {
-    float b[kC];
-    load_columns<kC>(e.bias, e.bias_dtype, c, valid, b);
-#pragma unroll
-    for (int q = 0; q < kC; ++q) v[q] += b[q];
-    if constexpr (kGated) {
-      load_columns<kC>(e.bias, e.bias_dtype, e.n + c, valid, b);
-#pragma unroll
-      for (int q = 0; q < kC; ++q) u[q] += b[q];
-    }
-  }
+  for (int q = 0; q < kC; ++q) v[q] = v[q] * columns.factor + columns.bias[q];
   if constexpr (kGated) {
+#pragma unroll
+    for (int q = 0; q < kC; ++q) u[q] += columns.up_bias[q];
     if (e.z) {
       store_columns<kC>(e.z, vq::kFP32, row * 2 * e.n + c, valid, v);
       store_columns<kC>(e.z, vq::kFP32, row * 2 * e.n + e.n + c, valid, u);
@@ -164,12 +182,16 @@ __device__ __forceinline__ void finish_columns(const Epilogue& e, int64_t row, i
     }
   }
   if (e.residual) {
-    float r[kC];
-    load_columns<kC>(e.residual, e.residual_dtype, row * e.residual_stride + c, valid, r);
 #pragma unroll
-    for (int q = 0; q < kC; ++q) v[q] += r[q];
+    for (int q = 0; q < kC; ++q) v[q] += residual[q];
   }
   store_columns<kC>(e.out, e.out_dtype, row * e.n + c, valid, v);
+}
+template <int kC, bool kGated>
+__device__ __forceinline__ void finish_columns(const Epilogue& e, int64_t row, int64_t c, float (&v)[kC], float (&u)[kC]) {
+  float r[kC];
+  load_residual<kC>(e, row, c, r);
+  finish_columns<kC, kGated>(e, row, c, v, u, Columns<kC, kGated>(e, c), r);
 }
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));

@@ -334,21 +334,21 @@ __device__ __forceinline__ void slopes8(const Slopes& g, int64_t m, int64_t c, f
   }
 }
 
-// FP16 holds dz over a power of two that brings its largest magnitude to 2^13 .. 2^14:
-// gradients of a mean are often below what FP16 holds, and products with up lines may be
-// above.  top: the FP32 bits of that magnitude.
-__device__ __forceinline__ float scale_of(uint32_t top) {
-  const int e = int(top >> 23);
-  if (e == 0 || e == 255) return 1.0f;  // nothing, or no number
-  return __builtin_amdgcn_ldexpf(1.0f, min(13 - (e - 127), 126));
-}
+// The largest magnitude of dz: each workgroup's, and of these all's (in whole numbers, as
+// FP32's magnitudes order).
+constexpr int kTops = 256;
 
-__global__ void clear_kernel(uint32_t* top) {
-  if (threadIdx.x == 0) *top = 0;
+__device__ __forceinline__ uint32_t block_top(uint32_t mine, uint32_t (&lds)[4]) {
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) mine = max(mine, uint32_t(__shfl_xor(int(mine), d)));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  return max(max(lds[0], lds[1]), max(lds[2], lds[3]));
 }
 
 template <bool kGated>
-__global__ __launch_bounds__(256) void top_kernel(Slopes g, uint32_t* top) {
+__global__ __launch_bounds__(256) void top_kernel(Slopes g, uint32_t* tops) {
+  __shared__ uint32_t lds[4];
   const int64_t eighths = (g.n + 7) / 8;
   uint32_t most = 0;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < g.rows * eighths; i += int64_t(gridDim.x) * 256) {
@@ -361,20 +361,16 @@ __global__ __launch_bounds__(256) void top_kernel(Slopes g, uint32_t* top) {
       for (int q = 0; q < 8; ++q) most = max(most, __builtin_bit_cast(uint32_t, u[q]) & 0x7fffffffu);
     }
   }
-#pragma unroll
-  for (int d = 32; d > 0; d /= 2) most = max(most, uint32_t(__shfl_xor(int(most), d)));
-  if ((threadIdx.x & 63) == 0 && most) atomicMax(top, most);  // (the largest, in any order)
+  most = block_top(most, lds);
+  if (threadIdx.x == 0) tops[blockIdx.x] = most;
 }
 
-__global__ void factor_kernel(const uint32_t* top, float* factor) {
-  if (threadIdx.x == 0) *factor = 1 / scale_of(*top);
-}
-
-// dz of 64 rows and 64 columns (gated: of the gate and of the up lines): by rows (stride
+// dz of 64 rows and 64 columns (gated: of the gate and of the up lines; FP16 over scale_of the
+// largest of `tops`): by rows (stride
 // `ld`, zeros up to whole chunks of lines), by lines (stride `ldt`, zeros up to whole
 // chunks of rows), and the lines' sums over these rows.
 template <bool kGated>
-__global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* top, uint16_t* dz, int64_t ld, uint16_t* dzt, int64_t ldt,
+__global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* tops, int parts, uint32_t* top, uint16_t* dz, int64_t ld, uint16_t* dzt, int64_t ldt,
                                                      float* partial) {
   constexpr int kHalves = kGated ? 2 : 1;
   __shared__ uint16_t part[kHalves][kPart * kPartStride];
@@ -382,7 +378,13 @@ __global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* t
   const int64_t m0 = int64_t(blockIdx.y) * kPart, c0 = int64_t(blockIdx.x) * kPart;
   const int ch = threadIdx.x & 7, row = threadIdx.x >> 3;
   const int64_t c = c0 + kChunk * ch;
-  const float scale = top ? scale_of(*top) : 1.0f;
+  float scale = 1.0f;
+  if (tops) {
+    __shared__ uint32_t lds[4];
+    const uint32_t all = block_top(int(threadIdx.x) < parts ? tops[threadIdx.x] : 0, lds);
+    scale = scale_of(all);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *top = all;  // for the products
+  }
   float mine[kHalves][8];
 #pragma unroll
   for (int o = 0; o < kHalves; ++o)
@@ -455,6 +457,7 @@ __global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t
   const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (c >= lines) return;
   float all = 0;
+#pragma unroll 8
   for (int64_t p = 0; p < parts; ++p) all += partial[p * lines + c];
   vq::store_act(out, dtype, c, all);
 }
@@ -471,10 +474,10 @@ struct Shape {
   double start, alone, full;
 };
 constexpr int kCus = 256, kShapes = 4;
-constexpr Shape kShape[kShapes] = {{256, 256, kCus, 10.95, 0.38, 1.6},
-                                   {256, 128, kCus, 8.97, 0.18, 0.83},
-                                   {64, 128, 2 * kCus, 4.5, 0.07, 0.52},
-                                   {64, 64, 2 * kCus, 1.6, 0.06, 0.38}};
+constexpr Shape kShape[kShapes] = {{256, 256, kCus, 10.8, 0.77, 1.56},
+                                   {256, 128, kCus, 8.3, 0.34, 0.84},
+                                   {64, 128, 2 * kCus, 4.3, 0.18, 0.59},
+                                   {64, 64, 2 * kCus, 3.9, 0.12, 0.35}};
 
 enum Kind : int { kTiles = 0, kSmall = 1, kGemv = 2 };
 
@@ -485,7 +488,7 @@ struct Plan {
   int lines;          // of the gemv: a wavefront's
 };
 
-// The figures above are fitted to 80 sizes (70 to 4096 rows, k 512 to 14336, n 128 to 14336),
+// The figures above are fitted to 119 sizes (17 to 4096 rows, k 512 to 14336, n 128 to 14336),
 // each on all tiles and up to 16 splits; the choice by them is 4% slower than the best of each
 // on average, 35% at worst (70 rows of 4096 x 288: 11.1 us for 8.2).
 Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated) {
@@ -674,7 +677,7 @@ struct GradRoom {
     dz = need_x ? up_to(rows * ld, 256) : 0;
     dzt = need_w ? up_to(lines * ldt, 256) : 0;
     partial = need_bias ? up_to(parts_of(rows, kPart) * lines * 4, 256) : 0;
-    top = 256;
+    top = up_to((1 + kTops) * 4, 256);  // all's, then the workgroups'
     bytes = sums + wt + xt + dz + dzt + partial + top;
   }
 };
@@ -803,22 +806,20 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
   uint16_t* dzt = reinterpret_cast<uint16_t*>(take(room.dzt));
   float* partial = reinterpret_cast<float*>(take(room.partial));
   uint32_t* top = reinterpret_cast<uint32_t*>(take(room.top));
-  float* factor = reinterpret_cast<float*>(top) + 1;
   const int64_t ld = up_to(lines, kChunk), ldt = up_to(rows, kChunk);
   const Slopes g{dy, dy_dtype, rows > 1 ? dy_stride : n, activation == kNone ? nullptr : z, dtype, activation, limit,
                  rows, n, lines};
   const bool scaled = dtype == vq::kFP16 && (dx || dw);
+  int tops = 0;
   if (scaled) {
-    hipLaunchKernelGGL(clear_kernel, dim3(1), dim3(64), 0, s, top);
-    const dim3 grid(unsigned(std::min<int64_t>(parts_of(rows * parts_of(n, 8), 256), 2048)));
-    if (gated) hipLaunchKernelGGL(top_kernel<true>, grid, dim3(256), 0, s, g, top);
-    else hipLaunchKernelGGL(top_kernel<false>, grid, dim3(256), 0, s, g, top);
-    hipLaunchKernelGGL(factor_kernel, dim3(1), dim3(64), 0, s, top, factor);
+    tops = int(std::min<int64_t>(parts_of(rows * parts_of(n, 8), 256), kTops));
+    if (gated) hipLaunchKernelGGL(top_kernel<true>, dim3(unsigned(tops)), dim3(256), 0, s, g, top + 1);
+    else hipLaunchKernelGGL(top_kernel<false>, dim3(unsigned(tops)), dim3(256), 0, s, g, top + 1);
     if (int rc = vq::check_launch("dense_linear gradient")) return rc;
   }
   const dim3 parts(unsigned(parts_of(n, kPart)), unsigned(parts_of(rows, kPart)));
-  if (gated) hipLaunchKernelGGL(slopes_kernel<true>, parts, dim3(256), 0, s, g, scaled ? top : nullptr, dz, ld, dzt, ldt, partial);
-  else hipLaunchKernelGGL(slopes_kernel<false>, parts, dim3(256), 0, s, g, scaled ? top : nullptr, dz, ld, dzt, ldt, partial);
+  if (gated) hipLaunchKernelGGL(slopes_kernel<true>, parts, dim3(256), 0, s, g, scaled ? top + 1 : nullptr, tops, top, dz, ld, dzt, ldt, partial);
+  else hipLaunchKernelGGL(slopes_kernel<false>, parts, dim3(256), 0, s, g, scaled ? top + 1 : nullptr, tops, top, dz, ld, dzt, ldt, partial);
   if (int rc = vq::check_launch("dense_linear gradient")) return rc;
   if (dbias) {
     hipLaunchKernelGGL(bias_kernel, dim3(unsigned(parts_of(lines, 256))), dim3(256), 0, s, partial, parts_of(rows, kPart), lines, dbias,
@@ -827,7 +828,7 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
   }
   const bool bf16 = dtype == vq::kBF16;
   const auto plain = [&](void* out) {
-    return Epilogue{nullptr, 0, kNone, __builtin_inff(), nullptr, 0, 0, out, dtype, k, nullptr, scaled ? factor : nullptr};
+    return Epilogue{nullptr, 0, kNone, __builtin_inff(), nullptr, 0, 0, out, dtype, k, nullptr, scaled ? top : nullptr};
   };
   if (dx) {
     if (int rc = transpose(wo, k, wt, ld, s)) return rc;

@@ -261,7 +261,19 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
   __syncthreads();
   const bool split = gridDim.y > 1;
   constexpr int kWave = kGated ? 16 * kN : 32 * kN;  // a wavefront's output columns
-  // (a loop, so that there is one copy of what follows the sums)
+  // (Loops, so that there is one copy of what follows the sums.)  A lane's columns are the same in
+  // all its rows; a row's residual is on its way while the row before is finished.
+  constexpr int kChunksRow = kWave / 4;  // of four columns
+  const int chunk = lane % kChunksRow, r0 = lane / kChunksRow;
+  const int64_t c = c0 + kWave * wn + 4 * chunk;
+  const Columns<4, kGated> columns(g.e, split ? g.e.n : c);
+  const auto row_at = [&](int i, int k) { return 32 * (kM * wm + i) + r0 + k * (64 / kChunksRow); };
+  float next[4];
+  const auto ask = [&](int i, int k) {
+    const int m = row_at(i, k);
+    if (!split && m < nrows) load_residual<4>(g.e, m0 + m, c, next);
+  };
+  ask(0, 0);
 #pragma unroll 1
   for (int i = 0; i < kM; ++i) {
     for_range<0, kM>([&](auto i_c) __attribute__((always_inline)) {
@@ -278,16 +290,14 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
         }
       }
     });
-    const int mt = 32 * (kM * wm + i);
-    const int64_t ct = c0 + kWave * wn;
-    constexpr int kChunksRow = kWave / 4;  // of four columns
-    const int chunk = lane % kChunksRow, r0 = lane / kChunksRow;
 #pragma unroll 1
     for (int k = 0; k < kChunksRow / 2; ++k) {
-      const int mr = r0 + k * (64 / kChunksRow), m = mt + mr;
+      const int m = row_at(i, k), mr = m & 31;
+      const float residual[4] = {next[0], next[1], next[2], next[3]};
+      if (k + 1 < kChunksRow / 2) ask(i, k + 1);
+      else if (i + 1 < kM) ask(i + 1, 0);
       const f32x4_t a = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk));
       const f32x4_t b = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk + (kGated ? 4 * kN : 0)));
-      const int64_t c = ct + 4 * chunk;
       if (m >= nrows || c >= g.e.n) continue;
       float v[4] = {a[0], a[1], a[2], a[3]}, u[4] = {b[0], b[1], b[2], b[3]};
       if (split) {
@@ -296,7 +306,7 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
         store_columns<4>(to, vq::kFP32, 0, g.e.n - c, v);
         if constexpr (kGated) store_columns<4>(to + g.e.n, vq::kFP32, 0, g.e.n - c, u);
       } else {
-        finish_columns<4, kGated>(g.e, m0 + m, c, v, u);
+        finish_columns<4, kGated>(g.e, m0 + m, c, v, u, columns, residual);
       }
     }
   }

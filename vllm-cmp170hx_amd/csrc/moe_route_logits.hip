@@ -116,19 +116,31 @@ struct Top2 {
   }
 };
 
-// What lies in LDS for groups that do not fill whole lanes of a step: the
-// wavefront's rows of keys, and the groups of four neighbouring experts, a byte each.
+// What lies in LDS: the wavefront's rows of keys, and for groups that do not fill whole
+// lanes of a step the groups of four neighbouring experts, a byte each.
 template <typename S>
-struct GroupSpace {
+struct KeySpace {
   static constexpr int kPadded = 4 * S::kLanes * S::kSteps;
   double* keys;            // [kRows][kPadded], FP32 ones in its first half
   const uint32_t* group4;  // [kPadded / 4]
+  uint16_t* list;          // [64]: a place a lane
+
+  template <typename Key>
+  __device__ __forceinline__ Key* row(int lane) const {
+    return reinterpret_cast<Key*>(keys) + (lane / S::kLanes) * kPadded;
+  }
 };
+
+// LDS of one wavefront's own: what its lanes have written, its lanes may read.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 
 // Keys of closed groups become -inf.  error: what an FP32 key may be off by at most,
 // apart from its own rounding; doubt: set where it may decide (64-bit keys: never).
 template <typename S, bool kTwo, typename Key>
-__device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Choice& c, const GroupSpace<S>& space, int l, int lane,
+__device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
                                              float error, bool& doubt) {
   const Key none = minus_inf();
   const bool in_lanes = c.group_lanes > 0;
@@ -163,15 +175,13 @@ __device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Cho
     }
   } else {
     // lane g takes group g, its keys from LDS (each lane from a place of its own on)
-    Key* rows = reinterpret_cast<Key*>(space.keys);
-    Key* row = rows + (lane / S::kLanes) * GroupSpace<S>::kPadded;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    Key* row = space.template row<Key>(lane);
+    wave_lds_fence();
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) row[4 * (S::kLanes * i + l) + j] = key[i][j];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave_lds_fence();
     Top2<Key> t{none, none};
     if (l < c.groups) {
       int at = l % c.group_experts;
@@ -180,8 +190,7 @@ __device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Cho
         at = at + 1 == c.group_experts ? 0 : at + 1;
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    wave_lds_fence();
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i) score[i] = none;
     score[0] = finish(t);
@@ -225,14 +234,104 @@ __device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Cho
   }
 }
 
+// v from the lane kTurn places on in the row of 16 lanes.
+template <int kTurn>
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_mov_dpp(int(v), 0x120 | kTurn, 0xF, 0xF, false));  // row_ror
+}
+template <int kTurn = 1, typename F>
+__device__ __forceinline__ void each_turn(const F& f) {
+  if constexpr (kTurn < 16) {
+    f(std::integral_constant<int, kTurn>{});
+    each_turn<kTurn + 1>(f);
+  }
+}
+
+// The same as choose (below) for rows of 16 lanes and up to 15 slots, where few enough keys
+// come into question, else false: those not below the least of the lanes' `need` largest
+// maxima, which `need` keys at least are not.  They go to a lane each, 16 at most, which counts
+// the better ones.  (65536 rows of 256 with groups and a bias: 70 us with a search
+// for each slot among all keys.)
+template <typename S, bool kBias>
+__device__ __forceinline__ bool choose_ranked(const float (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
+                                              float error, bool& doubt, int& mine) {
+  static_assert(S::kLanes == 16 && S::kSteps <= 4, "rows of 16 lanes");
+  const int need = c.top_k + (kBias ? 1 : 0);
+  float* row = space.template row<float>(lane);
+  wave_lds_fence();
+  float m = key[0][0];
+#pragma unroll
+  for (int i = 0; i < S::kSteps; ++i) {
+    typedef float f4_t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<f4_t*>(row + 4 * (16 * i + l)) = f4_t{key[i][0], key[i][1], key[i][2], key[i][3]};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, key[i][j]);
+  }
+  int above = 0;
+  each_turn([&](auto turn) { above += __builtin_bit_cast(float, turned<decltype(turn)::value>(__builtin_bit_cast(uint32_t, m))) > m; });
+  const float least = -lanes_max<16>(above < need ? -m : minus_inf(), lane);
+  uint32_t marks = 0;  // bit 4 i + j: key[i][j] comes into question
+#pragma unroll
+  for (int i = S::kSteps - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = 3; j >= 0; --j) marks = 2 * marks + (key[i][j] >= least ? 1 : 0);
+  const int count = __builtin_popcount(marks);
+  // (lanes before this one's, and all)
+  int total = 0, before = 0;
+  each_turn([&](auto turn) {
+    constexpr int n = decltype(turn)::value;
+    const int other = int(turned<n>(uint32_t(count)));
+    total += other;
+    before += l >= n ? other : 0;  // row_ror brings lane l - n's
+  });
+  total += count;
+  if (__any(total > 16)) return false;
+  uint16_t* list = space.list + (lane & 48);
+  for (int at = before; __any(marks != 0); ++at) {
+    if (marks) {
+      const int bit = __builtin_ctz(marks);
+      list[at] = uint16_t(4 * (16 * (bit >> 2) + l) + (bit & 3));
+      marks &= marks - 1;
+    }
+  }
+  wave_lds_fence();
+  const int e = l < total ? list[l] : 0;
+  const float k = l < total ? row[e] : minus_inf();
+  // larger keys are larger whole numbers (both zeros one), of equals the lower expert's
+  const uint32_t bits = __builtin_bit_cast(uint32_t, k + 0.0f), high = bits ^ (uint32_t(int(bits) >> 31) | 0x80000000u), low = ~uint32_t(e);
+  const uint64_t place = l < total ? uint64_t(high) << 32 | low : 0;
+  int rank = 0;
+  each_turn([&](auto turn) {
+    constexpr int n = decltype(turn)::value;
+    const uint64_t other = uint64_t(turned<n>(uint32_t(place >> 32))) << 32 | turned<n>(uint32_t(place));
+    rank += other > place;
+  });
+  const int to = 4 * ((lane & 48) | (l < total ? rank : 15));
+  // (of lanes without a key the last lane may hear, where there is none better)
+  int sorted = __builtin_amdgcn_ds_permute(to, l < total ? e : -1);
+  float best = __builtin_bit_cast(float, __builtin_amdgcn_ds_permute(to, __builtin_bit_cast(int, k)));
+  if (l >= total) best = minus_inf();
+  if constexpr (kBias) {
+    const float next = __builtin_bit_cast(float, turned<15>(__builtin_bit_cast(uint32_t, best)));
+    const bool close = l < c.top_k && best - next <= 2 * error + fabsf(best) * 0x1p-22f;
+    const uint64_t any = __ballot(close);
+    doubt = doubt || ((any >> (lane & 48)) & 0xffff) != 0;
+  }
+  mine = l < c.top_k && best > minus_inf() ? sorted : -1;
+  return true;
+}
+
 // Slot l's expert, or -1, in lane l of the row's lanes; the keys are used up.
 template <typename S, bool kBias, typename Key>
-__device__ __forceinline__ int choose(Key (&key)[S::kSteps][4], const Choice& c, const GroupSpace<S>& space, int l, int lane, float error,
+__device__ __forceinline__ int choose(Key (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane, float error,
                                       bool& doubt) {
   const Key none = minus_inf();
   constexpr bool kDoubt = kBias && std::is_same<Key, float>::value;
   if (c.groups > 1) close_groups<S, kBias>(key, c, space, l, lane, error, doubt);
   int mine = -1;
+  if constexpr (S::kLanes == 16 && std::is_same<Key, float>::value) {
+    if (c.top_k < 16 && choose_ranked<S, kBias>(key, c, space, l, lane, error, doubt, mine)) return mine;
+  }
   Key last = none;
   for (int k = 0;; ++k) {
     if (!kDoubt && k == c.top_k) break;
@@ -264,7 +363,10 @@ __device__ __forceinline__ int choose(Key (&key)[S::kSteps][4], const Choice& c,
   return mine;
 }
 
-// 1 / (1 + e^-x), off by 2^-21 of it.
+// 1 / (1 + e^-x), off by 2^-21 (whatever e^-x is off by times |x|, its part is small there).
+__device__ __forceinline__ float sigmoid_key(float x) { return __builtin_amdgcn_rcpf(1 + __builtin_amdgcn_exp2f(x * -kLog2e)); }
+
+// The same, off by 2^-21 of it.
 __device__ __forceinline__ float sigmoid_of(float x) {
   const float u = exp_nonpositive(-fabsf(x)), large = __builtin_amdgcn_rcpf(1 + u);
   return x >= 0 ? large : u * large;
@@ -272,10 +374,11 @@ __device__ __forceinline__ float sigmoid_of(float x) {
 
 template <typename S, int kDtype, bool kSigmoid, bool kBias>
 __global__ __launch_bounds__(kThreads) void choose_kernel(Rows g, Choice c) {
-  constexpr int kPadded = GroupSpace<S>::kPadded;
+  constexpr int kPadded = KeySpace<S>::kPadded;
   __shared__ __attribute__((aligned(16))) float bias[kBias ? kPadded : 4];
   __shared__ uint32_t group4[kPadded / 4];
-  __shared__ double rows[kWaves][S::kRows * kPadded];
+  __shared__ __attribute__((aligned(16))) double rows[kWaves][S::kRows * kPadded];
+  __shared__ uint16_t lists[kWaves][64];
   typedef float f4_t __attribute__((ext_vector_type(4)));
   const int tid = threadIdx.x, lane = tid & 63, wave = vq::uniform(tid >> 6);
   const int l = lane % S::kLanes, sub = lane / S::kLanes;
@@ -290,7 +393,7 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Rows g, Choice c) {
     }
   }
   __syncthreads();
-  const GroupSpace<S> space{rows[wave], group4};
+  const KeySpace<S> space{rows[wave], group4, lists[wave]};
   const int64_t step = int64_t(gridDim.x) * kWaves * S::kRows;
   const int64_t first = (int64_t(blockIdx.x) * kWaves + wave) * S::kRows;
   if (first >= g.rows) return;
@@ -354,7 +457,7 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Rows g, Choice c) {
         for (int j = 0; j < 4; ++j) {
           const float v = x.v[i][j];
           float k = v;
-          if constexpr (kBias) k = (kSigmoid ? sigmoid_of(v) : exp_nonpositive(v - largest) * inv) + b[j];
+          if constexpr (kBias) k = (kSigmoid ? sigmoid_key(v) : exp_nonpositive(v - largest) * inv) + b[j];
           key[i][j] = masked(v) || !(k > minus_inf()) ? minus_inf() : k;
         }
       }
