@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <initializer_list>
 
 #include "../../include/vllm_mi355x.h"
@@ -212,28 +213,29 @@ __global__ __launch_bounds__(1024) void small_kernel(Operand x, Operand w, int64
 
 // ---- the sum of K splits --------------------------------------------------------------
 
+// Four columns a thread, the splits' sums of four splits on their way at a time.
+template <bool kGated>
 __global__ __launch_bounds__(256) void finish_kernel(const float* sums, int splits, int64_t rows, Epilogue e) {
-  const bool gated = e.activation == kSwiglu;
-  const int64_t lines = gated ? 2 * e.n : e.n, eighths = (e.n + 7) / 8;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * eighths; i += int64_t(gridDim.x) * 256) {
-    const int64_t m = i / eighths, c = i % eighths * 8;
-    float v[8], u[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = u[q] = 0;
+  const int64_t lines = kGated ? 2 * e.n : e.n, quarters = (e.n + 3) / 4;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * quarters; i += int64_t(gridDim.x) * 256) {
+    const int64_t m = i / quarters, c = i % quarters * 4;
+    float v[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0}, residual[4];
+    const Columns<4, kGated> columns(e, c);
+    load_residual<4>(e, m, c, residual);
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-      float a[8];
+      float a[4];
       const float* from = sums + (s * rows + m) * lines + c;
-      load_columns<8>(from, vq::kFP32, 0, e.n - c, a);
+      load_columns<4>(from, vq::kFP32, 0, e.n - c, a);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] += a[q];
-      if (gated) {
-        load_columns<8>(from + e.n, vq::kFP32, 0, e.n - c, a);
+      for (int q = 0; q < 4; ++q) v[q] += a[q];
+      if constexpr (kGated) {
+        load_columns<4>(from + e.n, vq::kFP32, 0, e.n - c, a);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) u[q] += a[q];
+        for (int q = 0; q < 4; ++q) u[q] += a[q];
       }
     }
-    if (gated) finish_columns<8, true>(e, m, c, v, u);
-    else finish_columns<8, false>(e, m, c, v, u);
+    finish_columns<4, kGated>(e, m, c, v, u, columns, residual);
   }
 }
 
@@ -575,8 +577,10 @@ int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, fl
   const int64_t tiles_n = parts_of(e.n, gated ? shape.lines / 2 : shape.lines), tiles_m = parts_of(x.rows, shape.rows);
   if (tiles_n * tiles_m > INT_MAX / 2) return vq::fail("dense_linear: too many rows and columns");
   const int64_t split = parts_of(stages, p.splits);
-  const TileArgs t{x, w, int(parts_of(k, kChunk)), int(tiles_n), int(tiles_m), int(split), sums, e};
   const int64_t splits = parts_of(stages, split);  // (none without a stage)
+  const double at_work = std::min(double(tiles_n * tiles_m), double(shape.places)) / 8;  // on an XCD
+  const int64_t band = std::max<int64_t>(1, std::min<int64_t>(tiles_m, int64_t(std::sqrt(at_work * shape.lines / shape.rows) + 0.5)));
+  const TileArgs t{x, w, int(parts_of(k, kChunk)), int(tiles_n), int(tiles_m), int(band), int(split), sums, e};
   switch (p.shape) {
     case 0: launch_tile<Tile<4, 2, 2, 4, 5>, Tile<4, 2, 2, 4, 5>, kBf16>(t, splits, s); break;
     case 1: launch_tile<Tile<4, 2, 2, 2, 6>, Tile<4, 2, 2, 2, 6>, kBf16>(t, splits, s); break;
@@ -585,8 +589,9 @@ int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, fl
   }
   if (int rc = vq::check_launch("dense_linear")) return rc;
   if (splits == 1) return vq::kOk;
-  const int64_t groups = parts_of(x.rows * parts_of(e.n, 8), 256);
-  hipLaunchKernelGGL(finish_kernel, dim3(unsigned(std::min<int64_t>(groups, 8192))), dim3(256), 0, s, sums, int(splits), x.rows, e);
+  const dim3 groups(unsigned(std::min<int64_t>(parts_of(x.rows * parts_of(e.n, 4), 256), 8192)));
+  if (gated) hipLaunchKernelGGL(finish_kernel<true>, groups, dim3(256), 0, s, sums, int(splits), x.rows, e);
+  else hipLaunchKernelGGL(finish_kernel<false>, groups, dim3(256), 0, s, sums, int(splits), x.rows, e);
   return vq::check_launch("dense_linear");
 }
 int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, bool bf16, float* sums, const Plan& p, hipStream_t s) {

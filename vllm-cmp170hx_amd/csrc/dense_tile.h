@@ -40,6 +40,7 @@ struct TileArgs {
   Operand x, w;      // rows on 16 bytes, k whole chunks
   int chunks;        // of a row
   int tiles_n, tiles_m;
+  int band;          // rows of tiles that are gone through together, column by column
   int split_stages;  // stages of one split of K (gridDim.y splits)
   float* sums;       // more than one split: FP32 [split][rows][lines] for finish_kernel
   Epilogue e;
@@ -93,14 +94,15 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
   const int r = lane & 31, h = lane >> 5;
   const int wn = wave % T::kWn, wm = wave / T::kWn;
 
-  // XCD x (workgroups x, x + 8, ...) takes a run of tiles, rows first: it fetches few
-  // lines of W and its L2 keeps them for all the rows
+  // XCD x (workgroups x, x + 8, ...) takes a run of tiles, in bands of rows about as high as
+  // the tiles at work at a time are wide, so that its L2 fetches few rows and lines for them
   const int total = g.tiles_n * g.tiles_m, per = (total + 7) / 8;
   const int t = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
   if (int(blockIdx.x >> 3) >= per || t >= total) return;
   constexpr int kOut = kGated ? kCols / 2 : kCols;  // output columns
-  const int64_t c0 = int64_t(t / g.tiles_m) * kOut;
-  const int64_t m0 = int64_t(t % g.tiles_m) * kRows;
+  const int top = t / (g.band * g.tiles_n) * g.band, height = min(g.band, g.tiles_m - top), in_band = t - top * g.tiles_n;
+  const int64_t c0 = int64_t(in_band / height) * kOut;
+  const int64_t m0 = int64_t(top + in_band % height) * kRows;
   const int nrows = int(min(int64_t(kRows), g.x.rows - m0));
   const int ncols = int(min(int64_t(kOut), g.e.n - c0));
   const uint32_t wline = uint32_t(g.w.stride) * 2, xline = uint32_t(g.x.stride) * 2;

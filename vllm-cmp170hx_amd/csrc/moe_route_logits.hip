@@ -72,11 +72,6 @@ template <int d>
 __device__ __forceinline__ int xor_int(int v, int lane) {
   return __builtin_bit_cast(int, vq::xor_lanes<d>(__builtin_bit_cast(float, v), lane));
 }
-template <int d>
-__device__ __forceinline__ float xor_key(float v, int lane) { return vq::xor_lanes<d>(v, lane); }
-template <int d>
-__device__ __forceinline__ double xor_key(double v, int lane) { return __shfl_xor(v, d); }
-
 template <int kLanes>
 __device__ __forceinline__ int lanes_min(int v, int lane) {
   if constexpr (kLanes > 32) v = min(v, xor_int<32>(v, lane));
@@ -86,19 +81,16 @@ __device__ __forceinline__ int lanes_min(int v, int lane) {
   v = min(v, xor_int<2>(v, lane));
   return min(v, xor_int<1>(v, lane));
 }
+template <int kLanes>
+__device__ __forceinline__ double lanes_max(double v) {
+#pragma unroll
+  for (int d = kLanes / 2; d > 0; d /= 2) v = fmax(v, __shfl_xor(v, d));
+  return v;
+}
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
 __device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
 __device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
-template <int kLanes, typename Key>
-__device__ __forceinline__ Key keys_max(Key v, int lane) {
-  if constexpr (kLanes > 32) v = larger(v, xor_key<32>(v, lane));
-  if constexpr (kLanes > 16) v = larger(v, xor_key<16>(v, lane));
-  v = larger(v, xor_key<8>(v, lane));
-  v = larger(v, xor_key<4>(v, lane));
-  v = larger(v, xor_key<2>(v, lane));
-  return larger(v, xor_key<1>(v, lane));
-}
 
 // The two largest of a run of keys.
 template <typename Key>
@@ -110,7 +102,7 @@ struct Top2 {
   }
   template <int d>
   __device__ __forceinline__ void join(int lane) {
-    const Key a = xor_key<d>(first, lane), b = xor_key<d>(second, lane);
+    const Key a = vq::xor_lanes<d>(first, lane), b = vq::xor_lanes<d>(second, lane);
     second = larger(smaller(first, a), larger(second, b));
     first = larger(first, a);
   }
@@ -137,17 +129,17 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Keys of closed groups become -inf.  error: what an FP32 key may be off by at most,
-// apart from its own rounding; doubt: set where it may decide (64-bit keys: never).
-template <typename S, bool kTwo, typename Key>
-__device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
+// Keys of closed groups become -inf.  error: what a key may be off by at most, apart from its
+// own rounding; doubt: set where it may decide.
+template <typename S, bool kTwo>
+__device__ __forceinline__ void close_groups(float (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
                                              float error, bool& doubt) {
-  const Key none = minus_inf();
+  const float none = minus_inf();
   const bool in_lanes = c.group_lanes > 0;
-  Key score[S::kSteps];
+  float score[S::kSteps];
   float size = 0;  // of the keys that scores are made of
-  const auto finish = [&](const Top2<Key>& t) {
-    if constexpr (std::is_same<Key, float>::value && kTwo) {
+  const auto finish = [&](const Top2<float>& t) {
+    if constexpr (kTwo) {
       const float a = fabsf(t.first), b = fabsf(t.second);
       size = fmaxf(size, fmaxf(a < __builtin_inff() ? a : 0.0f, b < __builtin_inff() ? b : 0.0f));
     }
@@ -158,7 +150,7 @@ __device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Cho
   if (in_lanes) {
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i) {
-      Top2<Key> t{key[i][0], none};
+      Top2<float> t{key[i][0], none};
 #pragma unroll
       for (int j = 1; j < 4; ++j) t.add(key[i][j]);
       if (c.group_lanes > 1) t.template join<1>(lane);
@@ -175,14 +167,14 @@ __device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Cho
     }
   } else {
     // lane g takes group g, its keys from LDS (each lane from a place of its own on)
-    Key* row = space.template row<Key>(lane);
+    float* row = space.template row<float>(lane);
     wave_lds_fence();
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) row[4 * (S::kLanes * i + l) + j] = key[i][j];
     wave_lds_fence();
-    Top2<Key> t{none, none};
+    Top2<float> t{none, none};
     if (l < c.groups) {
       int at = l % c.group_experts;
       for (int n = 0; n < c.group_experts; ++n) {
@@ -196,19 +188,19 @@ __device__ __forceinline__ void close_groups(Key (&key)[S::kSteps][4], const Cho
     score[0] = finish(t);
   }
   float tolerance = 0;
-  if constexpr (std::is_same<Key, float>::value && kTwo) {
+  if constexpr (kTwo) {
     // four keys decide between two scores, each off by its error and half a step
     tolerance = 4 * error + lanes_max<S::kLanes>(size, lane) * 0x1p-21f;
   }
   uint64_t open = 0;
-  Key last = none;
+  float last = none;
   for (int q = 0;; ++q) {
-    Key m = score[0];
+    float m = score[0];
 #pragma unroll
-    for (int i = 1; i < S::kSteps; ++i) m = larger(m, score[i]);
-    m = keys_max<S::kLanes>(m, lane);
+    for (int i = 1; i < S::kSteps; ++i) m = fmaxf(m, score[i]);
+    m = lanes_max<S::kLanes>(m, lane);
     if (q == c.topk_groups) {
-      if constexpr (std::is_same<Key, float>::value && kTwo) doubt = doubt || last - m <= tolerance;
+      if constexpr (kTwo) doubt = doubt || last - m <= tolerance;
       break;
     }
     int g = INT_MAX;
@@ -322,26 +314,25 @@ __device__ __forceinline__ bool choose_ranked(const float (&key)[S::kSteps][4], 
 }
 
 // Slot l's expert, or -1, in lane l of the row's lanes; the keys are used up.
-template <typename S, bool kBias, typename Key>
-__device__ __forceinline__ int choose(Key (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane, float error,
+template <typename S, bool kBias>
+__device__ __forceinline__ int choose(float (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane, float error,
                                       bool& doubt) {
-  const Key none = minus_inf();
-  constexpr bool kDoubt = kBias && std::is_same<Key, float>::value;
+  const float none = minus_inf();
   if (c.groups > 1) close_groups<S, kBias>(key, c, space, l, lane, error, doubt);
   int mine = -1;
-  if constexpr (S::kLanes == 16 && std::is_same<Key, float>::value) {
+  if constexpr (S::kLanes == 16) {
     if (c.top_k < 16 && choose_ranked<S, kBias>(key, c, space, l, lane, error, doubt, mine)) return mine;
   }
-  Key last = none;
+  float last = none;
   for (int k = 0;; ++k) {
-    if (!kDoubt && k == c.top_k) break;
-    Key m = key[0][0];
+    if (!kBias && k == c.top_k) break;
+    float m = key[0][0];
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m = larger(m, key[i][j]);
-    m = keys_max<S::kLanes>(m, lane);
-    if constexpr (kDoubt) {
+      for (int j = 0; j < 4; ++j) m = fmaxf(m, key[i][j]);
+    m = lanes_max<S::kLanes>(m, lane);
+    if constexpr (kBias) {
       // (both off by their errors and half a step)
       doubt = doubt || (k > 0 && last - m <= 2 * error + fabsf(last) * 0x1p-22f);
       if (k == c.top_k) break;
@@ -363,6 +354,53 @@ __device__ __forceinline__ int choose(Key (&key)[S::kSteps][4], const Choice& c,
   return mine;
 }
 
+// The same from 64-bit keys in LDS (-inf: not to be chosen), which are used up.  Rare: in
+// loops, so that it costs the others no registers.
+template <typename S>
+__device__ __forceinline__ int choose_exact(double* row, const Choice& c, int experts, int l) {
+  const double none = -__builtin_inf();
+  wave_lds_fence();
+  if (c.groups > 1) {
+    Top2<double> t{none, none};
+    if (l < c.groups) {
+#pragma unroll 1
+      for (int n = 0; n < c.group_experts; ++n) t.add(row[l * c.group_experts + n]);
+    }
+    double score = t.second > none ? t.first + t.second : t.first;
+    uint64_t open = 0;
+#pragma unroll 1
+    for (int q = 0; q < c.topk_groups; ++q) {
+      const double m = lanes_max<S::kLanes>(score);
+      const int g = lanes_min<S::kLanes>(score == m ? l : INT_MAX, threadIdx.x & 63);
+      if (m > none) open |= uint64_t(1) << (g & 63);
+      score = l == g ? none : score;
+    }
+#pragma unroll 1
+    for (int e = l; e < experts; e += S::kLanes) {
+      if (!((open >> (e / c.group_experts)) & 1)) row[e] = none;
+    }
+    wave_lds_fence();
+  }
+  int mine = -1;
+#pragma unroll 1
+  for (int k = 0; k < c.top_k; ++k) {
+    double best = none;
+    int at = INT_MAX;
+#pragma unroll 1
+    for (int e = l; e < experts; e += S::kLanes) {  // (its lowest of equals)
+      const double v = row[e];
+      at = v > best ? e : at;
+      best = fmax(best, v);
+    }
+    const double m = lanes_max<S::kLanes>(best);
+    const int e = lanes_min<S::kLanes>(best == m ? at : INT_MAX, threadIdx.x & 63);
+    if (l == k && m > none) mine = e;
+    if (m > none && at == e) row[e] = none;
+    wave_lds_fence();
+  }
+  return mine;
+}
+
 // 1 / (1 + e^-x), off by 2^-21 (whatever e^-x is off by times |x|, its part is small there).
 __device__ __forceinline__ float sigmoid_key(float x) { return __builtin_amdgcn_rcpf(1 + __builtin_amdgcn_exp2f(x * -kLog2e)); }
 
@@ -373,7 +411,7 @@ __device__ __forceinline__ float sigmoid_of(float x) {
 }
 
 template <typename S, int kDtype, bool kSigmoid, bool kBias>
-__global__ __launch_bounds__(kThreads) void choose_kernel(Rows g, Choice c) {
+__global__ __launch_bounds__(kThreads, 4) void choose_kernel(Rows g, Choice c) {
   constexpr int kPadded = KeySpace<S>::kPadded;
   __shared__ __attribute__((aligned(16))) float bias[kBias ? kPadded : 4];
   __shared__ uint32_t group4[kPadded / 4];
@@ -466,33 +504,33 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Rows g, Choice c) {
     if constexpr (kBias) {
       doubt = doubt && !padding;
       if (__builtin_expect(__any(doubt), 0)) {
-        double key[S::kSteps][4], total = 0;
-        const Values<S> again = row(t);  // (kept in registers it would cost all rows)
-#pragma unroll
-        for (int i = 0; i < S::kSteps; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float v = again.v[i][j];
-            const bool b = kSigmoid ? v != v : !(v < __builtin_inff());
-            const double d = b ? -__builtin_inf() : double(v);
-            key[i][j] = kSigmoid ? 1 / (1 + exp(-d)) : exp(d - double(largest));
-            total += key[i][j];
-          }
+        double* keys = space.template row<double>(lane);
+        double total = 0;
+        const int64_t base = min(t, g.rows - 1) * g.stride;
+        const auto exponential = [&](int e, float& v) {
+          v = vq::load_act(g.logits, kDtype, base + e);
+          const bool bad = kSigmoid ? v != v : !(v < __builtin_inff());
+          if (bad) v = minus_inf();
+          return exp(double(kSigmoid ? -v : v) - (kSigmoid ? 0.0 : double(largest)));
+        };
         if constexpr (!kSigmoid) {
+#pragma unroll 1
+          for (int e = l; e < g.experts; e += S::kLanes) {
+            float v;
+            total += exponential(e, v);
+          }
 #pragma unroll
           for (int d = S::kLanes / 2; d > 0; d /= 2) total += __shfl_xor(total, d);
         }
-#pragma unroll
-        for (int i = 0; i < S::kSteps; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float v = again.v[i][j], b = bias[4 * (S::kLanes * i + l) + j];
-            const double k = (kSigmoid ? key[i][j] : key[i][j] / total) + double(b);
-            const bool out = v != v || (!kSigmoid && v == __builtin_inff()) || masked(v) || !(k > -__builtin_inf());
-            key[i][j] = out ? -__builtin_inf() : k;
-          }
-        bool none = false;
-        const int exact = choose<S, true>(key, c, space, l, lane, 0.0f, none);
+        wave_lds_fence();
+#pragma unroll 1
+        for (int e = l; e < g.experts; e += S::kLanes) {
+          float v;
+          const double u = exponential(e, v);
+          const double k = (kSigmoid ? 1 / (1 + u) : u / total) + double(bias[e]);
+          keys[e] = masked(v) || !(k > -__builtin_inf()) ? -__builtin_inf() : k;
+        }
+        const int exact = choose_exact<S>(keys, c, g.experts, l);
         if (doubt) mine = exact;
       }
     }
