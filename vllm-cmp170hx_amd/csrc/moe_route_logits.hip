@@ -53,7 +53,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 64;   // a lane a slot
 constexpr int kMaxGroups = 64;  // a bit a group
-constexpr unsigned kMaxGrid = 2048;
+constexpr unsigned kMaxGrid = 1024;  // four workgroups a CU, as many as are at work
 
 struct Choice {
   const float* bias;
@@ -68,28 +68,55 @@ struct Choice {
 
 __device__ __forceinline__ float minus_inf() { return -__builtin_inff(); }
 
+// Keys are compared as whole numbers of FP32's order (whose maxima take one instruction
+// across lanes; a float's are quieted first).  Both zeros are one.
+__device__ __forceinline__ int ordered(float v) {
+  const int b = __builtin_bit_cast(int, v + 0.0f);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float value_of(int v) { return __builtin_bit_cast(float, v ^ ((v >> 31) & 0x7fffffff)); }
+constexpr int kNone = int(0x807fffffu);  // -inf
+
+// v from the lane kTurn places before in the row of 16 lanes, from its first ones on the last.
+template <int kTurn>
+__device__ __forceinline__ int turned(int v) {
+  return __builtin_amdgcn_mov_dpp(v, 0x120 | kTurn, 0xF, 0xF, false);  // row_ror
+}
+template <int kTurn = 1, typename F>
+__device__ __forceinline__ void each_turn(const F& f) {
+  if constexpr (kTurn < 16) {
+    f(std::integral_constant<int, kTurn>{});
+    each_turn<kTurn + 1>(f);
+  }
+}
 template <int d>
 __device__ __forceinline__ int xor_int(int v, int lane) {
-  return __builtin_bit_cast(int, vq::xor_lanes<d>(__builtin_bit_cast(float, v), lane));
+  if constexpr (d == 4) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, false);  // row_half_mirror: lane ^ 7
+  else return __builtin_bit_cast(int, vq::xor_lanes<d>(__builtin_bit_cast(float, v), lane));
+}
+// f over a row's lanes.
+template <int kLanes, typename F>
+__device__ __forceinline__ int over_lanes(int v, int lane, const F& f) {
+  if constexpr (kLanes > 32) v = f(v, xor_int<32>(v, lane));
+  if constexpr (kLanes > 16) v = f(v, xor_int<16>(v, lane));
+  v = f(v, turned<8>(v));
+  v = f(v, turned<4>(v));
+  v = f(v, turned<2>(v));
+  return f(v, turned<1>(v));
 }
 template <int kLanes>
-__device__ __forceinline__ int lanes_min(int v, int lane) {
-  if constexpr (kLanes > 32) v = min(v, xor_int<32>(v, lane));
-  if constexpr (kLanes > 16) v = min(v, xor_int<16>(v, lane));
-  v = min(v, xor_int<8>(v, lane));
-  v = min(v, xor_int<4>(v, lane));
-  v = min(v, xor_int<2>(v, lane));
-  return min(v, xor_int<1>(v, lane));
-}
+__device__ __forceinline__ int most(int v, int lane) { return over_lanes<kLanes>(v, lane, [](int a, int b) { return max(a, b); }); }
+template <int kLanes>
+__device__ __forceinline__ int least(int v, int lane) { return over_lanes<kLanes>(v, lane, [](int a, int b) { return min(a, b); }); }
 template <int kLanes>
 __device__ __forceinline__ double lanes_max(double v) {
 #pragma unroll
   for (int d = kLanes / 2; d > 0; d /= 2) v = fmax(v, __shfl_xor(v, d));
   return v;
 }
-__device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ int larger(int a, int b) { return max(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
-__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ int smaller(int a, int b) { return min(a, b); }
 __device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
 
 // The two largest of a run of keys.
@@ -100,9 +127,10 @@ struct Top2 {
     second = larger(second, smaller(first, k));
     first = larger(first, k);
   }
+  // with the lanes' d places on, where those between have joined (whichever of these)
   template <int d>
   __device__ __forceinline__ void join(int lane) {
-    const Key a = vq::xor_lanes<d>(first, lane), b = vq::xor_lanes<d>(second, lane);
+    const Key a = xor_int<d>(first, lane), b = xor_int<d>(second, lane);
     second = larger(smaller(first, a), larger(second, b));
     first = larger(first, a);
   }
@@ -113,7 +141,7 @@ struct Top2 {
 template <typename S>
 struct KeySpace {
   static constexpr int kPadded = 4 * S::kLanes * S::kSteps;
-  double* keys;            // [kRows][kPadded], FP32 ones in its first half
+  double* keys;            // [kRows][kPadded], those of 32 bits in its first half
   const uint32_t* group4;  // [kPadded / 4]
   uint16_t* list;          // [64]: a place a lane
 
@@ -132,49 +160,53 @@ __device__ __forceinline__ void wave_lds_fence() {
 // Keys of closed groups become -inf.  error: what a key may be off by at most, apart from its
 // own rounding; doubt: set where it may decide.
 template <typename S, bool kTwo>
-__device__ __forceinline__ void close_groups(float (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
+__device__ __forceinline__ void close_groups(int (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
                                              float error, bool& doubt) {
-  const float none = minus_inf();
   const bool in_lanes = c.group_lanes > 0;
-  float score[S::kSteps];
+  int score[S::kSteps];
   float size = 0;  // of the keys that scores are made of
-  const auto finish = [&](const Top2<float>& t) {
-    if constexpr (kTwo) {
-      const float a = fabsf(t.first), b = fabsf(t.second);
-      size = fmaxf(size, fmaxf(a < __builtin_inff() ? a : 0.0f, b < __builtin_inff() ? b : 0.0f));
-    }
-    return kTwo && t.second > none ? t.first + t.second : t.first;
+  const auto finish = [&](const Top2<int>& t) {
+    if constexpr (!kTwo) return t.first;
+    const float a = value_of(t.first), b = value_of(t.second), m = fmaxf(fabsf(a), b > minus_inf() ? fabsf(b) : 0.0f);
+    size = fmaxf(size, m < __builtin_inff() ? m : 0.0f);
+    return ordered(b > minus_inf() ? a + b : a);
   };
   const int shift = in_lanes ? __builtin_ctz(c.group_lanes) : 0;
   const auto group_at = [&](int i) { return in_lanes ? (S::kLanes * i + l) >> shift : l; };
   if (in_lanes) {
+    Top2<int> t[S::kSteps];
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i) {
-      Top2<float> t{key[i][0], none};
+      t[i] = {key[i][0], kNone};
 #pragma unroll
-      for (int j = 1; j < 4; ++j) t.add(key[i][j]);
-      if (c.group_lanes > 1) t.template join<1>(lane);
-      if (c.group_lanes > 2) t.template join<2>(lane);
-      if (c.group_lanes > 4) t.template join<4>(lane);
-      if (c.group_lanes > 8) t.template join<8>(lane);
-      if constexpr (S::kLanes > 16) {
-        if (c.group_lanes > 16) t.template join<16>(lane);
-      }
-      if constexpr (S::kLanes > 32) {
-        if (c.group_lanes > 32) t.template join<32>(lane);
-      }
-      score[i] = finish(t);
+      for (int j = 1; j < 4; ++j) t[i].add(key[i][j]);
     }
+    const auto join = [&](auto d) {
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i) t[i].template join<decltype(d)::value>(lane);
+    };
+    if (c.group_lanes > 1) join(std::integral_constant<int, 1>{});
+    if (c.group_lanes > 2) join(std::integral_constant<int, 2>{});
+    if (c.group_lanes > 4) join(std::integral_constant<int, 4>{});
+    if (c.group_lanes > 8) join(std::integral_constant<int, 8>{});
+    if constexpr (S::kLanes > 16) {
+      if (c.group_lanes > 16) join(std::integral_constant<int, 16>{});
+    }
+    if constexpr (S::kLanes > 32) {
+      if (c.group_lanes > 32) join(std::integral_constant<int, 32>{});
+    }
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) score[i] = finish(t[i]);
   } else {
     // lane g takes group g, its keys from LDS (each lane from a place of its own on)
-    float* row = space.template row<float>(lane);
+    int* row = space.template row<int>(lane);
     wave_lds_fence();
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) row[4 * (S::kLanes * i + l) + j] = key[i][j];
     wave_lds_fence();
-    Top2<float> t{none, none};
+    Top2<int> t{kNone, kNone};
     if (l < c.groups) {
       int at = l % c.group_experts;
       for (int n = 0; n < c.group_experts; ++n) {
@@ -184,32 +216,33 @@ __device__ __forceinline__ void close_groups(float (&key)[S::kSteps][4], const C
     }
     wave_lds_fence();
 #pragma unroll
-    for (int i = 0; i < S::kSteps; ++i) score[i] = none;
+    for (int i = 0; i < S::kSteps; ++i) score[i] = kNone;
     score[0] = finish(t);
   }
   float tolerance = 0;
   if constexpr (kTwo) {
     // four keys decide between two scores, each off by its error and half a step
-    tolerance = 4 * error + lanes_max<S::kLanes>(size, lane) * 0x1p-21f;
+    // (sizes are not negative: they order as their bits)
+    tolerance = 4 * error + value_of(most<S::kLanes>(ordered(size), lane)) * 0x1p-21f;
   }
   uint64_t open = 0;
-  float last = none;
+  int last = kNone;
   for (int q = 0;; ++q) {
-    float m = score[0];
+    int m = score[0];
 #pragma unroll
-    for (int i = 1; i < S::kSteps; ++i) m = fmaxf(m, score[i]);
-    m = lanes_max<S::kLanes>(m, lane);
+    for (int i = 1; i < S::kSteps; ++i) m = max(m, score[i]);
+    m = most<S::kLanes>(m, lane);
     if (q == c.topk_groups) {
-      if constexpr (kTwo) doubt = doubt || last - m <= tolerance;
+      if constexpr (kTwo) doubt = doubt || value_of(last) - value_of(m) <= tolerance;
       break;
     }
     int g = INT_MAX;
 #pragma unroll
     for (int i = S::kSteps - 1; i >= 0; --i) g = score[i] == m ? group_at(i) : g;
-    g = lanes_min<S::kLanes>(g, lane);
-    if (m > none) open |= uint64_t(1) << (g & 63);
+    g = least<S::kLanes>(g, lane);
+    if (m > kNone) open |= uint64_t(1) << (g & 63);
 #pragma unroll
-    for (int i = 0; i < S::kSteps; ++i) score[i] = group_at(i) == g ? none : score[i];
+    for (int i = 0; i < S::kSteps; ++i) score[i] = group_at(i) == g ? kNone : score[i];
     last = m;
   }
 #pragma unroll
@@ -217,69 +250,59 @@ __device__ __forceinline__ void close_groups(float (&key)[S::kSteps][4], const C
     if (in_lanes) {
       const bool kept = (open >> (group_at(i) & 63)) & 1;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) key[i][j] = kept ? key[i][j] : none;
+      for (int j = 0; j < 4; ++j) key[i][j] = kept ? key[i][j] : kNone;
     } else {
       const uint32_t four = space.group4[S::kLanes * i + l];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) key[i][j] = (open >> (four >> (8 * j) & 63)) & 1 ? key[i][j] : none;
+      for (int j = 0; j < 4; ++j) key[i][j] = (open >> (four >> (8 * j) & 63)) & 1 ? key[i][j] : kNone;
     }
   }
 }
 
-// v from the lane kTurn places on in the row of 16 lanes.
-template <int kTurn>
-__device__ __forceinline__ uint32_t turned(uint32_t v) {
-  return uint32_t(__builtin_amdgcn_mov_dpp(int(v), 0x120 | kTurn, 0xF, 0xF, false));  // row_ror
-}
-template <int kTurn = 1, typename F>
-__device__ __forceinline__ void each_turn(const F& f) {
-  if constexpr (kTurn < 16) {
-    f(std::integral_constant<int, kTurn>{});
-    each_turn<kTurn + 1>(f);
-  }
-}
-
 // The same as choose (below) for rows of 16 lanes and up to 15 slots, where few enough keys
-// come into question, else false: those not below the least of the lanes' `need` largest
-// maxima, which `need` keys at least are not.  They go to a lane each, 16 at most, which counts
-// the better ones.  (65536 rows of 256 with groups and a bias: 70 us with a search
-// for each slot among all keys.)
+// come into question, else false: those not below the `need`th of the lanes' two largest each,
+// which `need` keys at least are not.  They go to a lane each, 16 at most, which counts
+// the better ones.  (By the largest of each lane alone one row in eight had more than 16.)
 template <typename S, bool kBias>
-__device__ __forceinline__ bool choose_ranked(const float (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
+__device__ __forceinline__ bool choose_ranked(const int (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane,
                                               float error, bool& doubt, int& mine) {
   static_assert(S::kLanes == 16 && S::kSteps <= 4, "rows of 16 lanes");
   const int need = c.top_k + (kBias ? 1 : 0);
-  float* row = space.template row<float>(lane);
+  int* row = space.template row<int>(lane);
   wave_lds_fence();
-  float m = key[0][0];
+  Top2<int> t{key[0][0], kNone};
 #pragma unroll
   for (int i = 0; i < S::kSteps; ++i) {
-    typedef float f4_t __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<f4_t*>(row + 4 * (16 * i + l)) = f4_t{key[i][0], key[i][1], key[i][2], key[i][3]};
+    typedef int i4_t __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<i4_t*>(row + 4 * (16 * i + l)) = i4_t{key[i][0], key[i][1], key[i][2], key[i][3]};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = fmaxf(m, key[i][j]);
+    for (int j = i == 0; j < 4; ++j) t.add(key[i][j]);
   }
-  int above = 0;
-  each_turn([&](auto turn) { above += __builtin_bit_cast(float, turned<decltype(turn)::value>(__builtin_bit_cast(uint32_t, m))) > m; });
-  const float least = -lanes_max<16>(above < need ? -m : minus_inf(), lane);
+  // (lanes with equal ones go on together: the border is no higher for it)
+  int border = kNone;
+#pragma unroll 1
+  for (int k = 0; k < need; ++k) {
+    border = most<16>(t.first, lane);
+    const bool gone = t.first == border;
+    t.first = gone ? t.second : t.first;
+    t.second = gone ? kNone : t.second;
+  }
   uint32_t marks = 0;  // bit 4 i + j: key[i][j] comes into question
 #pragma unroll
   for (int i = S::kSteps - 1; i >= 0; --i)
 #pragma unroll
-    for (int j = 3; j >= 0; --j) marks = 2 * marks + (key[i][j] >= least ? 1 : 0);
+    for (int j = 3; j >= 0; --j) marks = 2 * marks + (key[i][j] >= border ? 1 : 0);
+  // (the lanes' before this one's and its own, and all)
   const int count = __builtin_popcount(marks);
-  // (lanes before this one's, and all)
-  int total = 0, before = 0;
-  each_turn([&](auto turn) {
-    constexpr int n = decltype(turn)::value;
-    const int other = int(turned<n>(uint32_t(count)));
-    total += other;
-    before += l >= n ? other : 0;  // row_ror brings lane l - n's
-  });
-  total += count;
+  int sum = count;
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x111, 0xF, 0xF, true);  // row_shr
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x112, 0xF, 0xF, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x114, 0xF, 0xF, true);
+  sum += __builtin_amdgcn_update_dpp(0, sum, 0x118, 0xF, 0xF, true);
+  const int total = most<16>(sum, lane);
   if (__any(total > 16)) return false;
   uint16_t* list = space.list + (lane & 48);
-  for (int at = before; __any(marks != 0); ++at) {
+  for (int at = sum - count; __any(marks != 0); ++at) {
     if (marks) {
       const int bit = __builtin_ctz(marks);
       list[at] = uint16_t(4 * (16 * (bit >> 2) + l) + (bit & 3));
@@ -288,68 +311,66 @@ __device__ __forceinline__ bool choose_ranked(const float (&key)[S::kSteps][4], 
   }
   wave_lds_fence();
   const int e = l < total ? list[l] : 0;
-  const float k = l < total ? row[e] : minus_inf();
-  // larger keys are larger whole numbers (both zeros one), of equals the lower expert's
-  const uint32_t bits = __builtin_bit_cast(uint32_t, k + 0.0f), high = bits ^ (uint32_t(int(bits) >> 31) | 0x80000000u), low = ~uint32_t(e);
-  const uint64_t place = l < total ? uint64_t(high) << 32 | low : 0;
+  const int k = l < total ? row[e] : kNone;
+  // of equals the lower expert's
+  const uint64_t place = l < total ? uint64_t(uint32_t(k) ^ 0x80000000u) << 32 | ~uint32_t(e) : 0;
   int rank = 0;
   each_turn([&](auto turn) {
     constexpr int n = decltype(turn)::value;
-    const uint64_t other = uint64_t(turned<n>(uint32_t(place >> 32))) << 32 | turned<n>(uint32_t(place));
+    const uint64_t other = uint64_t(uint32_t(turned<n>(int(place >> 32)))) << 32 | uint32_t(turned<n>(int(place)));
     rank += other > place;
   });
   const int to = 4 * ((lane & 48) | (l < total ? rank : 15));
   // (of lanes without a key the last lane may hear, where there is none better)
-  int sorted = __builtin_amdgcn_ds_permute(to, l < total ? e : -1);
-  float best = __builtin_bit_cast(float, __builtin_amdgcn_ds_permute(to, __builtin_bit_cast(int, k)));
-  if (l >= total) best = minus_inf();
+  const int sorted = __builtin_amdgcn_ds_permute(to, l < total ? e : -1);
+  int best = __builtin_amdgcn_ds_permute(to, k);
+  if (l >= total) best = kNone;
   if constexpr (kBias) {
-    const float next = __builtin_bit_cast(float, turned<15>(__builtin_bit_cast(uint32_t, best)));
-    const bool close = l < c.top_k && best - next <= 2 * error + fabsf(best) * 0x1p-22f;
+    const float own = value_of(best), next = value_of(turned<15>(best));
+    const bool close = l < c.top_k && own - next <= 2 * error + fabsf(own) * 0x1p-22f;
     const uint64_t any = __ballot(close);
     doubt = doubt || ((any >> (lane & 48)) & 0xffff) != 0;
   }
-  mine = l < c.top_k && best > minus_inf() ? sorted : -1;
+  mine = l < c.top_k && best > kNone ? sorted : -1;
   return true;
 }
 
 // Slot l's expert, or -1, in lane l of the row's lanes; the keys are used up.
 template <typename S, bool kBias>
-__device__ __forceinline__ int choose(float (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane, float error,
+__device__ __forceinline__ int choose(int (&key)[S::kSteps][4], const Choice& c, const KeySpace<S>& space, int l, int lane, float error,
                                       bool& doubt) {
-  const float none = minus_inf();
   if (c.groups > 1) close_groups<S, kBias>(key, c, space, l, lane, error, doubt);
   int mine = -1;
   if constexpr (S::kLanes == 16) {
     if (c.top_k < 16 && choose_ranked<S, kBias>(key, c, space, l, lane, error, doubt, mine)) return mine;
   }
-  float last = none;
+  float last = 0;
   for (int k = 0;; ++k) {
     if (!kBias && k == c.top_k) break;
-    float m = key[0][0];
+    int m = key[0][0];
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m = fmaxf(m, key[i][j]);
-    m = lanes_max<S::kLanes>(m, lane);
+      for (int j = 0; j < 4; ++j) m = max(m, key[i][j]);
+    m = most<S::kLanes>(m, lane);
     if constexpr (kBias) {
       // (both off by their errors and half a step)
-      doubt = doubt || (k > 0 && last - m <= 2 * error + fabsf(last) * 0x1p-22f);
+      doubt = doubt || (k > 0 && last - value_of(m) <= 2 * error + fabsf(last) * 0x1p-22f);
       if (k == c.top_k) break;
-      last = m;
+      last = value_of(m);
     }
     int e = INT_MAX;
 #pragma unroll
     for (int i = S::kSteps - 1; i >= 0; --i)
 #pragma unroll
       for (int j = 3; j >= 0; --j) e = key[i][j] == m ? 4 * S::kLanes * i + j : e;
-    e = lanes_min<S::kLanes>(e == INT_MAX ? e : e + 4 * l, lane);
-    if (l == k && m > none) mine = e;
+    e = least<S::kLanes>(e == INT_MAX ? e : e + 4 * l, lane);
+    if (l == k && m > kNone) mine = e;
     const int here = e - 4 * l;
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) key[i][j] = here == 4 * S::kLanes * i + j ? none : key[i][j];
+      for (int j = 0; j < 4; ++j) key[i][j] = here == 4 * S::kLanes * i + j ? kNone : key[i][j];
   }
   return mine;
 }
@@ -371,7 +392,7 @@ __device__ __forceinline__ int choose_exact(double* row, const Choice& c, int ex
 #pragma unroll 1
     for (int q = 0; q < c.topk_groups; ++q) {
       const double m = lanes_max<S::kLanes>(score);
-      const int g = lanes_min<S::kLanes>(score == m ? l : INT_MAX, threadIdx.x & 63);
+      const int g = least<S::kLanes>(score == m ? l : INT_MAX, threadIdx.x & 63);
       if (m > none) open |= uint64_t(1) << (g & 63);
       score = l == g ? none : score;
     }
@@ -393,7 +414,7 @@ __device__ __forceinline__ int choose_exact(double* row, const Choice& c, int ex
       best = fmax(best, v);
     }
     const double m = lanes_max<S::kLanes>(best);
-    const int e = lanes_min<S::kLanes>(best == m ? at : INT_MAX, threadIdx.x & 63);
+    const int e = least<S::kLanes>(best == m ? at : INT_MAX, threadIdx.x & 63);
     if (l == k && m > none) mine = e;
     if (m > none && at == e) row[e] = none;
     wave_lds_fence();
@@ -456,7 +477,7 @@ __global__ __launch_bounds__(kThreads, 4) void choose_kernel(Rows g, Choice c) {
       for (int j = 0; j < 4; ++j) {
         float& v = x.v[i][j];
         const bool b = kSigmoid ? v != v : !(v < __builtin_inff());
-        bad = bad || b;
+        bad |= b;
         v = b ? minus_inf() : v;
         if (!kSigmoid) largest = fmaxf(largest, v);
       }
@@ -486,7 +507,7 @@ __global__ __launch_bounds__(kThreads, 4) void choose_kernel(Rows g, Choice c) {
     bool doubt = false;
     int mine;
     {
-      float key[S::kSteps][4];
+      int key[S::kSteps][4];
 #pragma unroll
       for (int i = 0; i < S::kSteps; ++i) {
         f4_t b{0, 0, 0, 0};
@@ -495,8 +516,12 @@ __global__ __launch_bounds__(kThreads, 4) void choose_kernel(Rows g, Choice c) {
         for (int j = 0; j < 4; ++j) {
           const float v = x.v[i][j];
           float k = v;
-          if constexpr (kBias) k = (kSigmoid ? sigmoid_key(v) : exp_nonpositive(v - largest) * inv) + b[j];
-          key[i][j] = masked(v) || !(k > minus_inf()) ? minus_inf() : k;
+          bool out = masked(v);
+          if constexpr (kBias) {
+            k = (kSigmoid ? sigmoid_key(v) : exp_nonpositive(v - largest) * inv) + b[j];
+            out |= !(k > minus_inf());  // (no short cut: a branch an expert would cost more)
+          }
+          key[i][j] = out ? kNone : ordered(k);
         }
       }
       mine = choose<S, kBias>(key, c, space, l, lane, error, doubt);
