@@ -213,6 +213,26 @@ def test_gradient_by_differences(moe, device, scoring, renormalize):
             assert abs(grad[t, e].item() - diff) <= 1e-8 + 2.0 ** -18 * 2.5 * np.abs(up[t]).sum()
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_one_slot_has_no_gradient(moe, device, scoring):
+    """A single renormalized weight is the scale whatever the logits: its gradient is 0, not a
+    rounding; rows with one expert left likewise."""
+    g = torch.Generator(device=device).manual_seed(2)
+    logits = torch.randn(300, 40, device=device, generator=g)
+    up = torch.randn(300, 1, device=device, generator=g)
+    leaf = logits.clone().requires_grad_()
+    w, _ = moe.moe_route_logits(leaf, 1, routed_scaling_factor=2.3, scoring=scoring)
+    grad, = torch.autograd.grad(w, leaf, up)
+    assert (w == torch.tensor(2.3, device=device)).all() and not grad.any()
+    logits[:, 3:] = -float("inf")
+    logits[:, :2] = -float("inf")
+    leaf = logits.requires_grad_()
+    w, ids = moe.moe_route_logits(leaf, 4, routed_scaling_factor=2.3, scoring=scoring)
+    assert (ids == torch.tensor([2, -1, -1, -1], device=device)).all()
+    grad, = torch.autograd.grad(w, leaf, torch.randn(300, 4, device=device, generator=g))
+    assert not grad.any()
+
+
 def test_deterministic_and_backward_twice(moe, device):
     rng = np.random.default_rng(4)
     logits = torch.from_numpy(rng.standard_normal((3000, 128))).float().to(device).requires_grad_()

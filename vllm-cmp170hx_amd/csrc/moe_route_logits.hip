@@ -11,8 +11,8 @@
 //
 // and with g the weights' gradient, the choice constant, d_e = dL/dl_e:
 //
-//   softmax, renormalized:  w_e (g_e - sum_j w_j g_j / c)            of chosen experts
-//   sigmoid, renormalized:  w_e (1 - s_e) (g_e - sum_j w_j g_j / c)
+//   softmax, renormalized:  w_e (g_e - sum_j w_j g_j / sum_j w_j)            of chosen experts
+//   sigmoid, renormalized:  w_e (1 - s_e) (g_e - sum_j w_j g_j / sum_j w_j)
 //   sigmoid:                w_e (1 - s_e) g_e
 //   softmax:                [chosen] w_e g_e - s_e sum_j w_j g_j     of all experts.
 //
@@ -600,7 +600,6 @@ struct Slots {
   const float* upstream;
   int top_k;
   bool renormalize;
-  float scale;
 };
 
 template <typename S, int kDtype, bool kSigmoid>
@@ -616,7 +615,6 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Rows g, Slots c, void* g
   for (int i = 0; i < S::kSteps; ++i) *reinterpret_cast<f4_t*>(part + 4 * (S::kLanes * i + l)) = f4_t{0, 0, 0, 0};
   const bool wide = g.experts % 4 == 0;  // (rows of the gradient lie close)
   const bool dense = !kSigmoid && !c.renormalize;
-  const float over = c.scale != 0 ? 1 / c.scale : 0.0f;
   const int64_t step = int64_t(gridDim.x) * kWaves * S::kRows;
   for (int64_t t0 = (int64_t(blockIdx.x) * kWaves + wave) * S::kRows; t0 < g.rows; t0 += step) {
     const int64_t t = t0 + sub, at = min(t, g.rows - 1);
@@ -629,9 +627,14 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(Rows g, Slots c, void* g
     }
     const bool chosen = e >= 0 && e < g.experts;
     if (!chosen) w = up = 0;
-    float d = w * up;
-    const float all = lanes_sum<S::kLanes>(d, lane);
-    if (c.renormalize) d = w * (up - all * over);
+    float d = w * up, all = 0;
+    if (c.renormalize) {
+      // (shares of the weights' own sum: a single one's gradient is 0 as it stands)
+      const float sum = lanes_sum<S::kLanes>(w, lane), share = sum != 0 ? w / sum : 0.0f;
+      d = w * (up - lanes_sum<S::kLanes>(share * up, lane));
+    } else if (!kSigmoid) {
+      all = lanes_sum<S::kLanes>(d, lane);
+    }
     if constexpr (kSigmoid) {
       // 1 - sigmoid of the logit is the sigmoid of its opposite
       const float v = chosen ? vq::load_act(g.logits, kDtype, at * g.stride + e) : 0.0f;
@@ -819,7 +822,7 @@ extern "C" int moe_route_grad(const void* logits, int dtype, int64_t rows, int64
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Rows g = rows_of(logits, dtype, rows, experts, stride, nullptr);
-  const Slots c{topk_weights, topk_ids, upstream, int(top_k), renormalize != 0, scale};
+  const Slots c{topk_weights, topk_ids, upstream, int(top_k), renormalize != 0};
   return dispatch(experts, top_k, dtype, scoring == 1, [&](auto shape, auto type, auto sigmoid) {
     using S = decltype(shape);
     hipLaunchKernelGGL((grad_kernel<S, decltype(type)::value, decltype(sigmoid)::value>), dim3(grid_of<S>(rows)), dim3(kThreads), 0, s, g, c,
