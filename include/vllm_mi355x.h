@@ -648,7 +648,7 @@ int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, co
  * residual [rows][n] (or null) of any of the three types; out contiguous, of any of them;
  * it may be a contiguous residual of its type.  z (or null): contiguous FP32 [rows][lines],
  * x W^T + bias for dense_linear_grad.  The order of the sums, and so the last bits, depend on the sizes alone.  k
- * up to 2^21.  workspace: dense_linear_workspace_size bytes of the same x, w and strides,
+ * up to 2^21, lines up to 2^24, rows up to 2^26.  workspace: dense_linear_workspace_size bytes of the same x, w and strides,
  * 16-byte aligned (null where that is 0), used by one call at a time.
  */
 int64_t dense_linear_workspace_size(const void* x, int64_t rows, int64_t k, int64_t x_stride,
@@ -668,7 +668,7 @@ int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int32_
  * From dy, the gradient of out ([rows][n] of any of the three types): dx [rows][k] and dw
  * [lines][k] (contiguous, of dtype) and dbias [lines]; each may be null.  z as dense_linear
  * left it (with VQ_ACT_NONE null).  The gradient of z is rounded to dtype, in FP16 over a
- * power of two of the whole, before its products.  At least one row.
+ * power of two of the whole, before its products.  At least one row; rows and lines up to 2^21.
  */
 int64_t dense_linear_grad_workspace_size(int64_t rows, int64_t k, int64_t n, int activation,
                                          int need_x, int need_w, int need_bias);

@@ -121,10 +121,10 @@ __device__ __forceinline__ float clamp_both(float v, float limit) { return v > l
 
 // FP16 holds gradients over a power of two that brings the largest magnitude to 2^13 .. 2^14:
 // those of a mean are often below what FP16 holds, and products with up lines may be above.
-// top: the FP32 bits of that magnitude.
+// top: the FP32 bits of that (finite) magnitude.
 __device__ __forceinline__ float scale_of(uint32_t top) {
   const int e = int(top >> 23);
-  if (e == 0 || e == 255) return 1.0f;  // nothing, or no number
+  if (e == 0) return 1.0f;  // nothing
   return __builtin_amdgcn_ldexpf(1.0f, min(13 - (e - 127), 126));
 }
 

@@ -25,9 +25,9 @@
 namespace dense {
 namespace {
 
-constexpr int64_t kMaxK = 1 << 21;       // 256 rows of a tile stay below 2^31 bytes
-constexpr int64_t kMaxStride = 1 << 22;
-constexpr int64_t kMaxSize = int64_t(1) << 30;  // rows, lines
+constexpr int64_t kMaxK = 1 << 21;  // 256 rows of a tile stay below 2^31 bytes
+constexpr int64_t kMaxRows = 1 << 26, kMaxLines = 1 << 24;
+constexpr int64_t kMaxGroups = 1 << 22;  // tiles, of up to 512 threads: below 2^32
 
 // ---- eight rows at most -------------------------------------------------------------
 //
@@ -252,11 +252,12 @@ __global__ __launch_bounds__(256) void pack_kernel(Operand in, int64_t k, uint16
 
 // A 64 x 64 part of a transposition through LDS: rows of 64 elements and one dword more.
 constexpr int kPart = 64, kPartStride = kPart + 2;
+constexpr int64_t kMaxParts = 1 << 23;  // workgroups of 256 threads: below 2^32
 
 // out [k][out_stride] = the transpose of in [rows][k], zeros up to whole chunks of rows.
 __global__ __launch_bounds__(256) void transpose_kernel(Operand in, int64_t k, uint16_t* out, int64_t out_stride) {
   __shared__ uint16_t part[kPart * kPartStride];
-  const int64_t m0 = int64_t(blockIdx.y) * kPart, k0 = int64_t(blockIdx.x) * kPart;
+  const int64_t across = (k + kPart - 1) / kPart, m0 = blockIdx.x / across * kPart, k0 = blockIdx.x % across * kPart;
   const int ch = threadIdx.x & 7, row = threadIdx.x >> 3;
 #pragma unroll
   for (int i = 0; i < kPart; i += 32) {
@@ -336,9 +337,14 @@ __device__ __forceinline__ void slopes8(const Slopes& g, int64_t m, int64_t c, f
   }
 }
 
-// The largest magnitude of dz: each workgroup's, and of these all's (in whole numbers, as
-// FP32's magnitudes order).
+// The largest finite magnitude of dz: each workgroup's, and of these all's (in whole numbers,
+// as FP32's magnitudes order; a row without numbers leaves the others' scale).
 constexpr int kTops = 256;
+
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+  return bits < 0x7f800000u ? bits : 0;
+}
 
 __device__ __forceinline__ uint32_t block_top(uint32_t mine, uint32_t (&lds)[4]) {
 #pragma unroll
@@ -357,10 +363,10 @@ __global__ __launch_bounds__(256) void top_kernel(Slopes g, uint32_t* tops) {
     float v[8], u[8];
     slopes8<kGated>(g, i / eighths, i % eighths * 8, v, u);
 #pragma unroll
-    for (int q = 0; q < 8; ++q) most = max(most, __builtin_bit_cast(uint32_t, v[q]) & 0x7fffffffu);
+    for (int q = 0; q < 8; ++q) most = max(most, finite_bits(v[q]));
     if constexpr (kGated) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) most = max(most, __builtin_bit_cast(uint32_t, u[q]) & 0x7fffffffu);
+      for (int q = 0; q < 8; ++q) most = max(most, finite_bits(u[q]));
     }
   }
   most = block_top(most, lds);
@@ -377,7 +383,7 @@ __global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* t
   constexpr int kHalves = kGated ? 2 : 1;
   __shared__ uint16_t part[kHalves][kPart * kPartStride];
   __shared__ float sum[kHalves][32][kPart + 1];
-  const int64_t m0 = int64_t(blockIdx.y) * kPart, c0 = int64_t(blockIdx.x) * kPart;
+  const int64_t across = (g.n + kPart - 1) / kPart, down = blockIdx.x / across, m0 = down * kPart, c0 = blockIdx.x % across * kPart;
   const int ch = threadIdx.x & 7, row = threadIdx.x >> 3;
   const int64_t c = c0 + kChunk * ch;
   float scale = 1.0f;
@@ -385,7 +391,7 @@ __global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* t
     __shared__ uint32_t lds[4];
     const uint32_t all = block_top(int(threadIdx.x) < parts ? tops[threadIdx.x] : 0, lds);
     scale = scale_of(all);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *top = all;  // for the products
+    if (blockIdx.x == 0 && threadIdx.x == 0) *top = all;  // for the products
   }
   float mine[kHalves][8];
 #pragma unroll
@@ -449,7 +455,7 @@ __global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* t
     if (c0 + col < g.n) {
       float all = 0;
       for (int i = 0; i < 32; ++i) all += sum[o][i][col];
-      partial[int64_t(blockIdx.y) * g.lines + o * g.n + c0 + col] = all;
+      partial[down * g.lines + o * g.n + c0 + col] = all;
     }
   }
 }
@@ -528,7 +534,7 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated) {
   return best;
 }
 
-bool direct(const Operand& o, int64_t k) { return aligned(o.p, 16) && o.stride % kChunk == 0 && k % kChunk == 0 && o.stride <= kMaxStride; }
+bool direct(const Operand& o, int64_t k) { return aligned(o.p, 16) && o.stride % kChunk == 0 && k % kChunk == 0 && o.stride <= kMaxK; }
 
 int64_t sums_bytes(const Plan& p, int64_t rows, int64_t lines) { return p.splits > 1 ? p.splits * rows * lines * 4 : 0; }
 
@@ -575,7 +581,7 @@ int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, fl
   const Shape& shape = kShape[p.shape];
   const int64_t stages = parts_of(k, kChunk * kStageChunks);
   const int64_t tiles_n = parts_of(e.n, gated ? shape.lines / 2 : shape.lines), tiles_m = parts_of(x.rows, shape.rows);
-  if (tiles_n * tiles_m > INT_MAX / 2) return vq::fail("dense_linear: too many rows and columns");
+  if (tiles_n * tiles_m > kMaxGroups) return vq::fail("dense_linear: too many rows and columns");
   const int64_t split = parts_of(stages, p.splits);
   const int64_t splits = parts_of(stages, split);  // (none without a stage)
   const double at_work = std::min(double(tiles_n * tiles_m), double(shape.places)) / 8;  // on an XCD
@@ -607,15 +613,28 @@ int pack(Operand& o, int64_t k, uint16_t* to, hipStream_t s) {
 }
 
 int transpose(const Operand& o, int64_t k, uint16_t* to, int64_t stride, hipStream_t s) {
-  hipLaunchKernelGGL(transpose_kernel, dim3(unsigned(parts_of(k, kPart)), unsigned(parts_of(o.rows, kPart))), dim3(256), 0, s, o, k, to, stride);
+  const int64_t groups = parts_of(k, kPart) * parts_of(o.rows, kPart);  // (check_grad_sizes)
+  hipLaunchKernelGGL(transpose_kernel, dim3(unsigned(groups)), dim3(256), 0, s, o, k, to, stride);
   return vq::check_launch("dense_linear");
 }
 
 int check_sizes(int64_t rows, int64_t k, int64_t n, int activation) {
-  if (rows < 0 || rows > kMaxSize) return vq::fail("dense_linear: rows out of range");
+  if (rows < 0 || rows > kMaxRows) return vq::fail("dense_linear: rows out of range");
   if (k <= 0 || k > kMaxK) return vq::fail("dense_linear: k must be between 1 and 2^21");
-  if (n <= 0 || n > kMaxSize) return vq::fail("dense_linear: columns out of range");
+  if (n <= 0 || (activation == kSwiglu ? 2 * n : n) > kMaxLines) return vq::fail("dense_linear: columns out of range");
   if (activation < kNone || activation > kSwiglu) return vq::fail("dense_linear: unknown activation");
+  return vq::kOk;
+}
+
+int check_grad_sizes(int64_t rows, int64_t k, int64_t n, int activation) {
+  if (int rc = check_sizes(rows, k, n, activation)) return rc;
+  const int64_t lines = activation == kSwiglu ? 2 * n : n;
+  // (the products' sums run over the lines and the rows)
+  if (rows > kMaxK || lines > kMaxK) return vq::fail("dense_linear: a gradient takes up to 2^21 rows and weight rows");
+  const int64_t across = parts_of(std::max(lines, k), kPart);
+  if (across * parts_of(rows, kPart) > kMaxParts || parts_of(k, kPart) * parts_of(lines, kPart) > kMaxParts) {
+    return vq::fail("dense_linear: too many rows and columns");
+  }
   return vq::kOk;
 }
 
@@ -766,7 +785,7 @@ extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, i
 
 extern "C" int64_t dense_linear_grad_workspace_size(int64_t rows, int64_t k, int64_t n, int activation, int need_x, int need_w, int need_bias) {
   using namespace dense;
-  if (check_sizes(rows, k, n, activation)) return -1;
+  if (check_grad_sizes(rows, k, n, activation)) return -1;
   if (rows == 0) return 0;
   return GradRoom(rows, k, activation == kSwiglu ? 2 * n : n, need_x, need_w, need_bias).bytes;
 }
@@ -776,7 +795,7 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
                                  int64_t dy_stride, void* dx, void* dw, void* dbias, int bias_dtype, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
   using namespace dense;
-  if (int rc = check_sizes(rows, k, n, activation)) return rc;
+  if (int rc = check_grad_sizes(rows, k, n, activation)) return rc;
   if (!is_float(dy_dtype) || (dbias && !is_float(bias_dtype))) return vq::fail("dense_linear: bias and output must be BF16, FP16 or FP32");
   if (rows == 0) return vq::fail("dense_linear: no rows have no gradient to compute");
   if (int rc = check_inputs(x, dtype, rows, k, x_stride, w, w_stride, limit)) return rc;
@@ -822,7 +841,7 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
     else hipLaunchKernelGGL(top_kernel<false>, dim3(unsigned(tops)), dim3(256), 0, s, g, top + 1);
     if (int rc = vq::check_launch("dense_linear gradient")) return rc;
   }
-  const dim3 parts(unsigned(parts_of(n, kPart)), unsigned(parts_of(rows, kPart)));
+  const dim3 parts(unsigned(parts_of(n, kPart) * parts_of(rows, kPart)));
   if (gated) hipLaunchKernelGGL(slopes_kernel<true>, parts, dim3(256), 0, s, g, scaled ? top + 1 : nullptr, tops, top, dz, ld, dzt, ldt, partial);
   else hipLaunchKernelGGL(slopes_kernel<false>, parts, dim3(256), 0, s, g, scaled ? top + 1 : nullptr, tops, top, dz, ld, dzt, ldt, partial);
   if (int rc = vq::check_launch("dense_linear gradient")) return rc;

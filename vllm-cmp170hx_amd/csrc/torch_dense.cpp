@@ -141,6 +141,7 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor
   const c10::DeviceGuard guard(x.device());
   const int64_t n = columns_of(w, activation), k = x.size(-1);
   TORCH_CHECK(k > 0, kWhat, ": the weights must be [n, k] of x's k = 0");
+  TORCH_CHECK(x.numel() / k <= (1 << 21) && w.size(0) <= (1 << 21), kWhat, ": a gradient takes up to 2^21 rows and weight rows");
   at::Tensor out = at::empty(with_last(x.sizes(), n), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
   at::Tensor z = at::empty({activation ? x.numel() / k : 0, w.size(0)}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
   run(x, w, bias, activation, residual, limit, out, activation ? z : at::Tensor());
@@ -242,6 +243,20 @@ at::Tensor linear_autograd(const at::Tensor& x, const at::Tensor& w, const std::
   return DenseLinear::apply(x, w, bias, activation, residual, out_dtype, limit);
 }
 
+void linear_out_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                         const std::optional<at::Tensor>& residual, double limit, const at::Tensor& out) {
+  for (const at::Tensor* t : {&x, &w, bias ? &*bias : nullptr, residual ? &*residual : nullptr, &out}) {
+    if (!t) continue;
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), kWhat, ": no forward-mode derivative");
+    TORCH_CHECK(!t->requires_grad() || !c10::GradMode::is_enabled(), kWhat, ": out carries no gradient");
+  }
+  static const auto op = handle<decltype(linear_out)>("_vllm_mi355x::dense_linear_out");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  op.call(x, w, bias, activation, residual, limit, out);
+  // (a gradient that was to use what out held finds it changed)
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 // Shapes alone, for tracing.
 at::Tensor linear_meta(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
                        const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
@@ -304,5 +319,5 @@ TORCH_LIBRARY_IMPL(_vllm_mi355x, Meta, m) {
 }
 TORCH_LIBRARY_IMPL(_vllm_mi355x, Autograd, m) {
   m.impl("dense_linear", &linear_autograd);
-  m.impl("dense_linear_out", torch::CppFunction::makeFallthrough());
+  m.impl("dense_linear_out", &linear_out_autograd);
 }

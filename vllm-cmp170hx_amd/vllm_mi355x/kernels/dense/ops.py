@@ -35,7 +35,8 @@ def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     given).
 
     x [..., k] and weight [n, k] bf16 or fp16, of one type; x's leading axes one run of
-    rows, unit inner strides, any k up to 2^21 and any n.  bias [n] (contiguous) and residual
+    rows, unit inner strides; k up to 2^21, weight rows up to 2^24 and rows up to 2^26 (for
+    gradients both up to 2^21).  bias [n] (contiguous) and residual
     [..., n] (rows as x's) bf16, fp16 or fp32.  activation: None, "relu", "gelu" (of the
     error function), "gelu_tanh", "silu", or "swiglu": weight [2 n, k] and bias [2 n] hold the
     gate rows and then the up rows, and the result is SiLU(min(g, L)) clamp(u, -L, L), L the
@@ -58,8 +59,5 @@ def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         return ops.dense_linear(x, weight, bias, code, residual, out_dtype or x.dtype, limit)
     if out_dtype is not None and out.dtype != out_dtype:
         raise RuntimeError("dense_linear: out must be of out_dtype")
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias, residual, out)):
-        raise RuntimeError("dense_linear: out carries no gradient")
     ops.dense_linear_out(x, weight, bias, code, residual, limit, out)
     return out
