@@ -298,3 +298,29 @@ def test_graph_and_streams(linear, device, rows, activation):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
         assert all(torch.equal(a, b) for a, b in zip(again, want[i]))
+
+
+@pytest.mark.parametrize("rows", [1, 5, 12, 40, 300])
+def test_subnormal_operands(linear, device, rows):
+    """FP16 values below its normal ones count in full, as rows and as weights."""
+    rng = np.random.default_rng(rows)
+    small = lambda *s: torch.from_numpy(rng.integers(-1000, 1000, s) * 2.0 ** -24).half().to(device)
+    large = lambda *s: torch.from_numpy(rng.integers(-8, 8, s) * 2.0 ** 11).half().to(device)
+    check(linear, small(rows, 130), large(48, 130), out_dtype=torch.float32)
+    check(linear, large(rows, 130), small(48, 130), out_dtype=torch.float32)
+
+
+def test_a_row_without_numbers_leaves_the_others_scale(linear, device):
+    """FP16 gradients of 1e-6 keep their digits beside a row of infinities or NaN."""
+    rng = np.random.default_rng(11)
+    x, w = normal(rng, (70, 64), "fp16", device), normal(rng, (96, 64), "fp16", device)
+    dy = normal(rng, (70, 96), "fp32", device, 1e-6)
+    for bad in (float("inf"), float("nan")):
+        worse = dy.clone()
+        worse[33, 5] = bad
+        got = []
+        for up in (dy, worse):
+            leaf = x.detach().requires_grad_()
+            got.append(torch.autograd.grad(linear(leaf, w, out_dtype=torch.float32), leaf, up)[0])
+        keep = torch.arange(70, device=device) != 33
+        assert got[0].any() and torch.equal(got[0][keep], got[1][keep]) and not torch.isfinite(got[1][33]).any()
