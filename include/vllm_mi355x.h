@@ -647,9 +647,10 @@ int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, co
  * > 0 (infinity: no clamp).  FP32 sums of exact products; bias [lines] (or null) and
  * residual [rows][n] (or null) of any of the three types; out contiguous, of any of them;
  * it may be a contiguous residual of its type.  z (or null): contiguous FP32 [rows][lines],
- * x W^T + bias for dense_linear_grad.  The order of the sums, and so the last bits, depend on the sizes alone.  k
- * up to 2^21, lines up to 2^24, rows up to 2^26.  workspace: dense_linear_workspace_size bytes of the same x, w and strides,
- * 16-byte aligned (null where that is 0), used by one call at a time.
+ * x W^T + bias for dense_linear_grad.  The order of the sums, and so the last bits, depend
+ * on the sizes alone.  k up to 2^21, lines up to 2^24, rows up to 2^26.  workspace:
+ * dense_linear_workspace_size bytes of the same x, w and strides, 16-byte aligned (null
+ * where that is 0), used by one call at a time.
  */
 int64_t dense_linear_workspace_size(const void* x, int64_t rows, int64_t k, int64_t x_stride,
                                     const void* w, int64_t n, int64_t w_stride, int activation);
@@ -707,7 +708,7 @@ int moe_route_logits(const void* logits, int dtype, int64_t rows, int64_t expert
  * choice constant; weights and ids as moe_route_logits gave them. */
 int moe_route_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride,
                    const float* topk_weights, const int32_t* topk_ids, int64_t top_k, int scoring,
-                   int renormalize, float scale, const float* upstream, void* grad, void* stream);
+                   int renormalize, const float* upstream, void* grad, void* stream);
 
 /* ---- a router's load -----------------------------------------------------------
  * Up to 1024 experts; rows with is_padding[t] != 0 (optional uint8 [rows]) are

@@ -732,13 +732,12 @@ Rows rows_of(const void* logits, int dtype, int64_t rows, int64_t experts, int64
   return {logits, stride, padding, rows, int(experts), wide};
 }
 
-int check_call(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, int64_t top_k, int scoring, float scale) {
+int check_call(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, int64_t top_k, int scoring) {
   if (dtype != vq::kBF16 && dtype != vq::kFP16 && dtype != vq::kFP32) return vq::fail("moe_route_logits: logits must be BF16, FP16 or FP32");
   if (rows < 0 || rows > INT_MAX) return vq::fail("moe_route_logits: rows out of range");
   if (experts <= 0 || experts > kMaxExperts) return vq::fail("moe_route_logits: between 1 and 1024 experts");
   if (top_k <= 0 || top_k > kMaxSlots || top_k > experts) return vq::fail("moe_route_logits: topk must be between 1 and 64, and at most the experts");
   if (scoring != 0 && scoring != 1) return vq::fail("moe_route_logits: scoring must be softmax (0) or sigmoid (1)");
-  if (!(scale > -__builtin_inff() && scale < __builtin_inff())) return vq::fail("moe_route_logits: the scale must be finite");
   if (stride < 0 || (rows > 1 && stride < experts) || stride > (int64_t(1) << 31)) return vq::fail("moe_route_logits: row stride out of range");
   if (rows > 0 && !logits) return vq::fail("moe_route_logits: null pointer");
   return vq::kOk;
@@ -777,7 +776,8 @@ extern "C" int moe_route_logits(const void* logits, int dtype, int64_t rows, int
                                 int64_t top_k, int64_t groups, int64_t topk_groups, int scoring, int renormalize, float scale,
                                 const uint8_t* is_padding, float* topk_weights, int32_t* topk_ids, void* stream) {
   using namespace route;
-  if (int rc = check_call(logits, dtype, rows, experts, stride, top_k, scoring, scale)) return rc;
+  if (int rc = check_call(logits, dtype, rows, experts, stride, top_k, scoring)) return rc;
+  if (!(scale > -__builtin_inff() && scale < __builtin_inff())) return vq::fail("moe_route_logits: the scale must be finite");
   if (groups <= 0 || groups > kMaxGroups || experts % groups) return vq::fail("moe_route_logits: up to 64 groups of equal size");
   if (topk_groups <= 0 || topk_groups > groups) return vq::fail("moe_route_logits: topk_groups must be between 1 and the groups");
   if (top_k > topk_groups * (experts / groups)) return vq::fail("moe_route_logits: topk experts do not fit topk_groups groups");
@@ -808,10 +808,10 @@ extern "C" int moe_route_logits(const void* logits, int dtype, int64_t rows, int
 }
 
 extern "C" int moe_route_grad(const void* logits, int dtype, int64_t rows, int64_t experts, int64_t stride, const float* topk_weights,
-                              const int32_t* topk_ids, int64_t top_k, int scoring, int renormalize, float scale, const float* upstream,
+                              const int32_t* topk_ids, int64_t top_k, int scoring, int renormalize, const float* upstream,
                               void* grad, void* stream) {
   using namespace route;
-  if (int rc = check_call(logits, dtype, rows, experts, stride, top_k, scoring, scale)) return rc;
+  if (int rc = check_call(logits, dtype, rows, experts, stride, top_k, scoring)) return rc;
   if (rows == 0) return vq::kOk;
   if (!topk_weights || !topk_ids || !upstream || !grad) return vq::fail("moe_route_logits: null pointer");
   const int64_t slots = rows * top_k, bytes = vq::dtype_bytes(dtype);

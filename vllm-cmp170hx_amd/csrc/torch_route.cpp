@@ -74,7 +74,7 @@ std::tuple<at::Tensor, at::Tensor> route(const at::Tensor& logits, const std::op
 }
 
 at::Tensor gradient(const at::Tensor& logits, const at::Tensor& weights, const at::Tensor& ids, const at::Tensor& upstream,
-                    int64_t scoring, bool renormalize, double scale) {
+                    int64_t scoring, bool renormalize) {
   check_logits(logits);
   TORCH_CHECK(weights.dim() == 2 && weights.size(0) == logits.size(0) && ids.sizes() == weights.sizes() && upstream.sizes() == weights.sizes(),
               kWhat, ": the gradient's weights, ids and upstream must be [rows, topk]");
@@ -87,7 +87,7 @@ at::Tensor gradient(const at::Tensor& logits, const at::Tensor& weights, const a
   at::Tensor grad = at::empty({rows, experts}, logits.options());
   check_status(native_grad(logits.const_data_ptr(), dtype_code(logits.scalar_type()), rows, experts, stride_of(logits),
                            weights.const_data_ptr<float>(), ids.const_data_ptr<int32_t>(), weights.size(1), int(scoring), renormalize,
-                           static_cast<float>(scale), upstream.const_data_ptr<float>(), grad.mutable_data_ptr(), stream_of(logits)));
+                           upstream.const_data_ptr<float>(), grad.mutable_data_ptr(), stream_of(logits)));
   return grad;
 }
 
@@ -112,7 +112,6 @@ struct RouteWeights : torch::autograd::Function<RouteWeights> {
     ctx->save_for_backward({logits, weights, ids});
     ctx->saved_data["scoring"] = scoring;
     ctx->saved_data["renormalize"] = renormalize;
-    ctx->saved_data["scale"] = scale;
     ctx->mark_non_differentiable({ids});
     return {weights, ids};
   }
@@ -125,8 +124,7 @@ struct RouteWeights : torch::autograd::Function<RouteWeights> {
     const torch::autograd::variable_list saved = ctx->get_saved_variables();
     const at::Tensor upstream = grads[0].to(at::kFloat).contiguous();
     const at::AutoDispatchBelowADInplaceOrView below;
-    none[0] = op.call(saved[0], saved[1], saved[2], upstream, ctx->saved_data["scoring"].toInt(), ctx->saved_data["renormalize"].toBool(),
-                      ctx->saved_data["scale"].toDouble());
+    none[0] = op.call(saved[0], saved[1], saved[2], upstream, ctx->saved_data["scoring"].toInt(), ctx->saved_data["renormalize"].toBool());
     return none;
   }
 };
@@ -149,7 +147,7 @@ std::tuple<at::Tensor, at::Tensor> route_meta(const at::Tensor& logits, const st
   const c10::SymInt rows = logits.sym_size(0);
   return {at::empty_symint({rows, topk}, logits.options().dtype(at::kFloat)), at::empty_symint({rows, topk}, logits.options().dtype(at::kInt))};
 }
-at::Tensor gradient_meta(const at::Tensor& logits, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool, double) {
+at::Tensor gradient_meta(const at::Tensor& logits, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, bool) {
   return at::empty_symint(logits.sym_sizes(), logits.options());
 }
 
@@ -170,8 +168,8 @@ TORCH_LIBRARY_FRAGMENT(_vllm_mi355x, m) {
       "moe_route_logits(Tensor logits, Tensor? bias, int topk, int num_groups, int topk_groups, int scoring, bool renormalize, "
       "float scale, Tensor? is_padding) -> (Tensor, Tensor)");
   m.def(
-      "moe_route_grad(Tensor logits, Tensor topk_weights, Tensor topk_ids, Tensor upstream, int scoring, bool renormalize, "
-      "float scale) -> Tensor");
+      "moe_route_grad(Tensor logits, Tensor topk_weights, Tensor topk_ids, Tensor upstream, int scoring, bool renormalize) "
+      "-> Tensor");
 }
 TORCH_LIBRARY_IMPL(_vllm_mi355x, CUDA, m) {
   m.impl("moe_route_logits", &route);

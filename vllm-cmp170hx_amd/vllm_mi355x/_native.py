@@ -186,7 +186,7 @@ SIGNATURES = {
     "moe_route_grad": (c_int, [
         c_vp, c_int, c_i64, c_i64, c_i64,        # logits, dtype, rows, experts, stride
         c_vp, c_vp, c_i64, c_int, c_int,         # topk_weights, topk_ids, top_k, scoring, renormalize
-        ctypes.c_float, c_vp, c_vp, c_vp,        # scale, upstream, grad, stream
+        c_vp, c_vp, c_vp,                        # upstream, grad, stream
     ]),
     "dense_linear_workspace_size": (c_i64, [
         c_vp, c_i64, c_i64, c_i64,               # x, rows, k, x_stride
