@@ -661,9 +661,10 @@ int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_st
                  int64_t workspace_bytes, void* stream);
 
 /* How it runs at a size, for tests: plan[0] 0 on tiles of plan[1] rows and plan[2] lines, K in
- * plan[3] splits; 1 (16 rows at most) with K over plan[3] wavefronts; 2 (eight at most)
+ * plan[3] splits, plan[4] parts in LDS's ring; 1 (16 rows at most) with K over plan[3] wavefronts; 2 (eight at most)
  * with plan[2] lines a wavefront, K over plan[3]. */
-int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int32_t* plan);
+int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int has_residual,
+                      int32_t* plan);
 
 /*
  * From dy, the gradient of out ([rows][n] of any of the three types): dx [rows][k] and dw

@@ -73,7 +73,7 @@ def test_no_rows_and_sizes(lib):
 
 
 def plan(lib, *size):
-    out = (ctypes.c_int32 * 4)()
+    out = (ctypes.c_int32 * 5)()
     assert lib.dense_linear_plan(*size, out) == 0
     return list(out)
 
@@ -81,13 +81,16 @@ def plan(lib, *size):
 def test_every_plan_has_a_size(lib):
     """The sizes at which test_gpu_dense_plans.py runs reach every kernel and split."""
     from tests.test_gpu_dense_plans import SIZES
-    seen = {tuple(plan(lib, rows, k, n, 5 if gated else 0)[:3]) + (plan(lib, rows, k, n, 5 if gated else 0)[3] > 1, gated)
-            for rows, k, n, gated in SIZES}
+    seen = set()
+    for rows, k, n, gated in SIZES:
+        kind, tile_rows, lines, parts, ring = plan(lib, rows, k, n, 5 if gated else 0, 1)
+        seen.add((kind, tile_rows, lines, ring, parts > 1, gated))
     for gated in (False, True):
-        for shape in ((256, 256), (128, 256), (128, 64), (64, 64)):
+        for shape in ((256, 256, 5), (128, 256, 6), (128, 64, 6), (64, 64, 8)):
             assert (0, *shape, False, gated) in seen and (0, *shape, True, gated) in seen, (shape, gated)
+        assert (0, 128, 64, 4, False, gated) in seen and (0, 64, 64, 4, False, gated) in seen
         assert {s[0] for s in seen if s[-1] == gated} == {0, 1, 2}
-    assert (2, 0, 1, False, False) in seen and (2, 0, 1, True, False) in seen and (2, 0, 2, False, False) in seen and (2, 0, 2, True, True) in seen
+    assert {(2, 0, 1, 0, False, False), (2, 0, 1, 0, True, False), (2, 0, 2, 0, False, False), (2, 0, 2, 0, True, True)} <= seen
 
 
 def test_shapes_and_gradient_of_meta_tensors(linear):

@@ -17,7 +17,8 @@ SIZES = [(1, 4096, 300, False), (2, 8200, 65, False), (3, 520, 8200, False), (7,
          (2040, 256, 2050, True), (2048, 512, 6000, False), (2048, 512, 3000, True), (700, 4096, 4096, False), (700, 4096, 2048, True),
          (4096, 192, 4100, False), (4096, 192, 2049, True), (300, 8192, 8192, False), (300, 8192, 4096, True), (100, 4096, 14336, False),
          (100, 4096, 7168, True), (600, 14336, 4096, False), (600, 14336, 2048, True), (1500, 8192, 3000, False), (1500, 8192, 1500, True), (500, 4096, 1500, False),
-         (500, 4096, 750, True), (700, 8192, 750, True)]
+         (500, 4096, 750, True), (700, 8192, 750, True), (500, 8192, 1500, False), (2500, 192, 1250, True), (3000, 4096, 3000, False),
+         (3000, 4096, 1500, True), (40, 64, 100, False)]
 
 
 @pytest.mark.parametrize("rows,k,n,gated", SIZES)

@@ -476,16 +476,18 @@ int64_t up_to(int64_t v, int64_t step) { return (v + step - 1) / step * step; }
 int64_t parts_of(int64_t v, int64_t step) { return (v + step - 1) / step; }
 
 // The tiles, and for the choice between them what they take in us: a round of workgroups
-// `start`, and a stage `alone` on a card hardly filled or `full` on a full one.
+// `start` (and `residual` with one), a stage `alone` on a card hardly filled or `full` on a
+// full one.  The last two have four parts in their ring in the place of six and eight: of
+// few stages more workgroups a CU, which store while others load, are worth more than loads
+// far ahead (8179 rows of 192 x 1152: 16 us for 20; of 4096 x 1152, on 64 x 64: 129 for 111).
 struct Shape {
-  int lines, rows, places;  // places: workgroups that the card holds
-  double start, alone, full;
+  int lines, rows, parts, places;  // places: workgroups that the card holds
+  double start, alone, full, residual;
 };
-constexpr int kCus = 256, kShapes = 4;
-constexpr Shape kShape[kShapes] = {{256, 256, kCus, 10.8, 0.77, 1.56},
-                                   {256, 128, kCus, 8.3, 0.34, 0.84},
-                                   {64, 128, 2 * kCus, 4.3, 0.18, 0.59},
-                                   {64, 64, 2 * kCus, 3.9, 0.12, 0.35}};
+constexpr int kCus = 256, kShapes = 6;
+constexpr Shape kShape[kShapes] = {{256, 256, 5, kCus, 17.1, 0.32, 1.70, 13.6}, {256, 128, 6, kCus, 9.1, 0.31, 0.90, 2.4},
+                                   {64, 128, 6, 2 * kCus, 5.5, 0.17, 0.55, 1.8},  {64, 64, 8, 2 * kCus, 4.0, 0.11, 0.33, 0.9},
+                                   {64, 128, 4, 3 * kCus, 4.6, 0.38, 0.88, 1.7},  {64, 64, 4, 5 * kCus, 3.5, 0.28, 1.02, 1.2}};
 
 enum Kind : int { kTiles = 0, kSmall = 1, kGemv = 2 };
 
@@ -496,10 +498,11 @@ struct Plan {
   int lines;          // of the gemv: a wavefront's
 };
 
-// The figures above are fitted to 119 sizes (17 to 4096 rows, k 512 to 14336, n 128 to 14336),
-// each on all tiles and up to 16 splits; the choice by them is 4% slower than the best of each
-// on average, 35% at worst (70 rows of 4096 x 288: 11.1 us for 8.2).
-Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated) {
+// The figures above are fitted to 245 sizes (17 to 8179 rows, k 64 to 14336, n 128 to 20434; of
+// small k with an FP32 residual and without), each on all tiles and up to 16 splits; the choice
+// by them is 1% slower than the best of each on average, 30% at worst (300 rows of 360 x
+// 20434 with a residual: 28 us for 22).
+Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated, bool residual) {
   const int64_t lines = gated ? 2 * n : n;
   if (rows <= kGemvRows) {
     // a line a wavefront, and as many wavefronts a line as fill the card with four each SIMD
@@ -522,9 +525,10 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated) {
       if (splits > 1 && tiles * splits > 8 * kCus) break;
       const int64_t each = parts_of(stages, splits), all = tiles * parts_of(stages, each);
       const int64_t rest = all % t.places;
-      double cost = double(all / t.places) * (t.start + double(each) * t.full);
-      if (rest) cost += t.start + double(each) * (t.alone + (t.full - t.alone) * double(rest) / t.places);
-      if (splits > 1) cost += 3 + double(splits) * double(rows) * double(lines) * 4 / 6.5e6;  // written and added up
+      const double start = t.start + (residual && splits == 1 ? t.residual : 0);
+      double cost = double(all / t.places) * (start + double(each) * t.full);
+      if (rest) cost += start + double(each) * (t.alone + (t.full - t.alone) * double(rest) / t.places);
+      if (splits > 1) cost += 4 + double(splits) * (0.25 + double(rows) * double(lines) * 4 / 8e6);  // written and added up
       if (least == 0 || cost < least) {
         least = cost;
         best = {kTiles, i, int(splits), 0, 0};
@@ -591,7 +595,9 @@ int product(const Operand& x, const Operand& w, int64_t k, const Epilogue& e, fl
     case 0: launch_tile<Tile<4, 2, 2, 4, 5>, Tile<4, 2, 2, 4, 5>, kBf16>(t, splits, s); break;
     case 1: launch_tile<Tile<4, 2, 2, 2, 6>, Tile<4, 2, 2, 2, 6>, kBf16>(t, splits, s); break;
     case 2: launch_tile<Tile<2, 2, 1, 2, 6>, Tile<1, 4, 2, 1, 6>, kBf16>(t, splits, s); break;
-    default: launch_tile<Tile<2, 2, 1, 1, 8>, Tile<1, 2, 2, 1, 8>, kBf16>(t, splits, s); break;
+    case 3: launch_tile<Tile<2, 2, 1, 1, 8>, Tile<1, 2, 2, 1, 8>, kBf16>(t, splits, s); break;
+    case 4: launch_tile<Tile<2, 2, 1, 2, 4>, Tile<1, 4, 2, 1, 4>, kBf16>(t, splits, s); break;
+    default: launch_tile<Tile<2, 2, 1, 1, 4>, Tile<1, 2, 2, 1, 4>, kBf16>(t, splits, s); break;
   }
   if (int rc = vq::check_launch("dense_linear")) return rc;
   if (splits == 1) return vq::kOk;
@@ -692,8 +698,8 @@ struct GradRoom {
   Plan px, pw;
   int64_t sums, wt, xt, dz, dzt, partial, top, bytes;
   GradRoom(int64_t rows, int64_t k, int64_t lines, bool need_x, bool need_w, bool need_bias) {
-    px = plan_of(rows, lines, k, false);
-    pw = plan_of(lines, rows, k, false);
+    px = plan_of(rows, lines, k, false, false);
+    pw = plan_of(lines, rows, k, false, false);
     const int64_t ld = up_to(lines, kChunk) * 2, ldt = up_to(rows, kChunk) * 2;
     sums = up_to(std::max(need_x ? sums_bytes(px, rows, k) : 0, need_w ? sums_bytes(pw, lines, k) : 0), 256);
     wt = need_x ? up_to(k * ld, 256) : 0;
@@ -716,21 +722,26 @@ extern "C" int64_t dense_linear_workspace_size(const void* x, int64_t rows, int6
   if (rows == 0) return 0;
   const bool gated = activation == kSwiglu;
   const int64_t lines = gated ? 2 * n : n;
-  const Plan p = plan_of(rows, k, n, gated);
-  const bool tiles = p.kind == kTiles;
   const Operand xo{static_cast<const uint16_t*>(x), rows, x_stride}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
-  return Room(rows, k, lines, p, tiles && !direct(xo, k), tiles && !direct(wo, k)).bytes;
+  int64_t most = 0;
+  for (const bool residual : {false, true}) {
+    const Plan p = plan_of(rows, k, n, gated, residual);
+    const bool tiles = p.kind == kTiles;
+    most = std::max(most, Room(rows, k, lines, p, tiles && !direct(xo, k), tiles && !direct(wo, k)).bytes);
+  }
+  return most;
 }
 
-extern "C" int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int32_t* plan) {
+extern "C" int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int has_residual, int32_t* plan) {
   using namespace dense;
   if (int rc = check_sizes(rows, k, n, activation)) return rc;
   if (!plan) return vq::fail("dense_linear: null pointer");
-  const Plan p = plan_of(rows, k, n, activation == kSwiglu);
+  const Plan p = plan_of(rows, k, n, activation == kSwiglu, has_residual);
   plan[0] = p.kind;
   plan[1] = p.kind == kTiles ? kShape[p.shape].rows : 0;
   plan[2] = p.kind == kTiles ? kShape[p.shape].lines : p.lines;
   plan[3] = p.kind == kTiles ? p.splits : p.waves;
+  plan[4] = p.kind == kTiles ? kShape[p.shape].parts : 0;
   return vq::kOk;
 }
 
@@ -750,7 +761,7 @@ extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, i
   const bool gated = activation == kSwiglu;
   const int64_t lines = gated ? 2 * n : n;
   Operand xo{static_cast<const uint16_t*>(x), rows, rows > 1 ? x_stride : k}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
-  const Plan p = plan_of(rows, k, n, gated);
+  const Plan p = plan_of(rows, k, n, gated, residual);
   const bool pack_x = p.kind == kTiles && !direct(xo, k), pack_w = p.kind == kTiles && !direct(wo, k);
   const Room room(rows, k, lines, p, pack_x, pack_w);
   if (room.bytes && (!workspace || workspace_bytes < room.bytes || !aligned(workspace, 16))) {

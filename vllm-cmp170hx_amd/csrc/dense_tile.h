@@ -65,8 +65,8 @@ struct Tile {
     return kStageBytes * (kParts % 2 ? (kCols > kRows ? kCols : kRows) : i % 2 ? kRows : kCols);
   }
   static constexpr int kBytes = part_bytes(0) * ((kParts + 1) / 2) + part_bytes(1) * (kParts / 2);
-  // workgroups that a CU's LDS holds, two at most
-  static constexpr int kGroups = kBytes > 80 * 1024 ? 1 : 2;
+  // workgroups that a CU's LDS holds, and whose registers (128 a lane) it does
+  static constexpr int kGroups = 160 * 1024 / kBytes < 4 ? 160 * 1024 / kBytes : 4;
 };
 
 // Part i of the ring.  (Buffers by name: the compiler then sees that a stage's reads are
@@ -263,17 +263,23 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
   __syncthreads();
   const bool split = gridDim.y > 1;
   constexpr int kWave = kGated ? 16 * kN : 32 * kN;  // a wavefront's output columns
-  // (Loops, so that there is one copy of what follows the sums.)  A lane's columns are the same in
-  // all its rows; a row's residual is on its way while the row before is finished.
+  // (Loops, so that there are few copies of what follows the sums.)  A lane's columns are the same
+  // in all its rows; the residuals of two or four rows are on their way while those before are
+  // finished (asked for before their stores, which a wait would count otherwise).
   constexpr int kChunksRow = kWave / 4;  // of four columns
+  static_assert(kChunksRow % 8 == 0, "whole groups of rows");
   const int chunk = lane % kChunksRow, r0 = lane / kChunksRow;
   const int64_t c = c0 + kWave * wn + 4 * chunk;
   const Columns<4, kGated> columns(g.e, split ? g.e.n : c);
   const auto row_at = [&](int i, int k) { return 32 * (kM * wm + i) + r0 + k * (64 / kChunksRow); };
-  float next[4];
-  const auto ask = [&](int i, int k) {
-    const int m = row_at(i, k);
-    if (!split && m < nrows) load_residual<4>(g.e, m0 + m, c, next);
+  constexpr int kTogether = kM == 4 ? 2 : 4;  // (registers)
+  float next[kTogether][4];
+  const auto ask = [&](int i, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int y = 0; y < kTogether; ++y) {
+      const int m = row_at(i, k + y);
+      if (!split && m < nrows) load_residual<4>(g.e, m0 + m, c, next[y]);
+    }
   };
   ask(0, 0);
 #pragma unroll 1
@@ -293,22 +299,29 @@ __global__ __launch_bounds__(T::kThreads, T::kGroups * T::kWaves / 4) void tile_
       }
     });
 #pragma unroll 1
-    for (int k = 0; k < kChunksRow / 2; ++k) {
-      const int m = row_at(i, k), mr = m & 31;
-      const float residual[4] = {next[0], next[1], next[2], next[3]};
-      if (k + 1 < kChunksRow / 2) ask(i, k + 1);
+    for (int k = 0; k < kChunksRow / 2; k += kTogether) {
+      float residual[kTogether][4];
+#pragma unroll
+      for (int y = 0; y < kTogether; ++y)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) residual[y][q] = next[y][q];
+      if (k + kTogether < kChunksRow / 2) ask(i, k + kTogether);
       else if (i + 1 < kM) ask(i + 1, 0);
-      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk));
-      const f32x4_t b = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk + (kGated ? 4 * kN : 0)));
-      if (m >= nrows || c >= g.e.n) continue;
-      float v[4] = {a[0], a[1], a[2], a[3]}, u[4] = {b[0], b[1], b[2], b[3]};
-      if (split) {
-        const int64_t lines = kGated ? 2 * g.e.n : g.e.n;
-        float* to = g.sums + (int64_t(blockIdx.y) * g.x.rows + m0 + m) * lines + c;
-        store_columns<4>(to, vq::kFP32, 0, g.e.n - c, v);
-        if constexpr (kGated) store_columns<4>(to + g.e.n, vq::kFP32, 0, g.e.n - c, u);
-      } else {
-        finish_columns<4, kGated>(g.e, m0 + m, c, v, u, columns, residual);
+#pragma unroll
+      for (int y = 0; y < kTogether; ++y) {
+        const int m = row_at(i, k + y), mr = m & 31;
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk));
+        const f32x4_t b = *reinterpret_cast<const f32x4_t*>(part + exchange_at(mr, chunk + (kGated ? 4 * kN : 0)));
+        if (m >= nrows || c >= g.e.n) continue;
+        float v[4] = {a[0], a[1], a[2], a[3]}, u[4] = {b[0], b[1], b[2], b[3]};
+        if (split) {
+          const int64_t lines = kGated ? 2 * g.e.n : g.e.n;
+          float* to = g.sums + (int64_t(blockIdx.y) * g.x.rows + m0 + m) * lines + c;
+          store_columns<4>(to, vq::kFP32, 0, g.e.n - c, v);
+          if constexpr (kGated) store_columns<4>(to + g.e.n, vq::kFP32, 0, g.e.n - c, u);
+        } else {
+          finish_columns<4, kGated>(g.e, m0 + m, c, v, u, columns, residual[y]);
+        }
       }
     }
   }

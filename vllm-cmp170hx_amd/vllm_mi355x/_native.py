@@ -199,7 +199,7 @@ SIGNATURES = {
         c_vp, c_int, c_i64, c_vp, c_int,         # residual, dtype, stride, out, out_dtype
         c_vp, c_vp, c_i64, c_vp,                 # z, workspace, bytes, stream
     ]),
-    "dense_linear_plan": (c_int, [c_i64, c_i64, c_i64, c_int, c_vp]),
+    "dense_linear_plan": (c_int, [c_i64, c_i64, c_i64, c_int, c_int, c_vp]),
     "dense_linear_grad_workspace_size": (c_i64, [
         c_i64, c_i64, c_i64, c_int, c_int, c_int, c_int,  # rows, k, n, activation, need x, w, bias
     ]),
