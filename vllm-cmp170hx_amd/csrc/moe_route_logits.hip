@@ -24,6 +24,11 @@
 // Keys with a bias are FP32 sums, off by up to 2^-20; where two that decide the
 // choice or its order lie closer than their errors, the wavefront's rows are keyed and
 // chosen again in 64 bits, so that the choice is always that of 64-bit keys.
+//
+// What bounds it: few rows, the launch (1 row of 256, eight groups: 5.2 us on the GPU, 7.4 a
+// call); many, vector instructions: 65536 rows of 256 FP32 logits, sigmoid, bias, four of eight
+// groups open, take 57 us forward (67 MB at 1.2 TB/s: the sigmoids and the selection) and 15
+// back (the gradient's stores, 67 MB at 4.5 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
