@@ -18,7 +18,8 @@ SIZES = [(1, 4096, 300, False), (2, 8200, 65, False), (3, 520, 8200, False), (7,
          (4096, 192, 4100, False), (4096, 192, 2049, True), (300, 8192, 8192, False), (300, 8192, 4096, True), (100, 4096, 14336, False),
          (100, 4096, 7168, True), (600, 14336, 4096, False), (600, 14336, 2048, True), (1500, 8192, 3000, False), (1500, 8192, 1500, True), (500, 4096, 1500, False),
          (500, 4096, 750, True), (700, 8192, 750, True), (500, 8192, 1500, False), (2500, 192, 1250, True), (3000, 4096, 3000, False),
-         (3000, 4096, 1500, True), (40, 64, 100, False)]
+         (3000, 4096, 1500, True), (40, 64, 100, False), (6, 4096, 9000, False), (12, 8192, 2100, True), (16, 5000, 300, False),
+         (3, 8192, 4200, False), (9, 8192, 5000, False)]
 
 
 @pytest.mark.parametrize("rows,k,n,gated", SIZES)
@@ -53,6 +54,10 @@ def test_weights_and_outputs_past_32_bits(linear, device):
         y = linear(x, w, out_dtype=torch.float32)
         want, tol = D.forward(exact(x), exact(w[some]), None, None, None)
         close(y[:, some], want, tol, f"{rows} rows")
+        if rows == 12:  # off 16 bytes
+            y = linear(x[:, 1:], w[:, 1:], out_dtype=torch.float32)
+            want, tol = D.forward(exact(x[:, 1:]), exact(w[some, 1:]), None, None, None)
+            close(y[:, some], want, tol, f"{rows} rows off 16 bytes")
     del w
     x = torch.randn(66000, 8, device=device, generator=torch.Generator(device=device).manual_seed(5)).half()
     w = torch.randn(66000, 8, device=device, generator=torch.Generator(device=device).manual_seed(6)).half()

@@ -156,15 +156,15 @@ __global__ __launch_bounds__(64 * kGemvWaves) void gemv_kernel(Operand x, Operan
   finish_columns<kCols, kGated>(e, lane, c, v, u);
 }
 
-// ---- nine to 16 rows ------------------------------------------------------------------
+// ---- 16 rows at most ------------------------------------------------------------------
 //
 // W is read once, from memory to the registers of the wavefront that multiplies it: a
 // wavefront holds 16 lines (a gated activation: 16 gate and the 16 up lines of the same
 // columns), per step 128 k, in which lane (r = lane & 15, q = lane >> 4) loads the
 // chunks 4 j + q (j < 4) of line r and of x's row r and multiplies them in four
 // v_mfma_16x16x32.  K is split over the wavefronts of a workgroup, whose sums meet in
-// LDS and are added in order.  From 17 rows on tiles are the faster ones (20 rows of 2592 x
-// 5003: 15 us for 20 with two of these products a lane), at eight rows and fewer the above.
+// LDS and are added in order.  Bound by the loads' latency: 8 rows of 4096 x 4096 take 9.2 us
+// (3.6 TB/s; tiles with K splits and their sum 12.3).
 
 constexpr int kSmallRows = 16;  // of one B operand
 constexpr int kStepChunks = 16;
@@ -508,17 +508,28 @@ struct Plan {
 // small k with an FP32 residual and without), each on all tiles and up to 16 splits; the choice
 // by them is 1% slower than the best of each on average, 30% at worst (300 rows of 360 x
 // 20434 with a residual: 28 us for 22).
-Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated, bool residual) {
+//
+// Up to 16 rows (us, a wavefront a line / the small kernel / tiles; k x lines): 4096 x 28672
+// 4 rows 48 / 59 / 46, 8 rows 73 / 60 / 45, 16 rows - / 70 / 45; 14336 x 4096 2 rows 25 / 26 /
+// 26, 4 rows 35 / 28 / 26; 4096 x 4096 4 rows 9.4 / 9.0 / 12, 8 rows 15 / 9.2 / 12, 16 rows
+// - / 10.4 / 12.3; 7168 x 256 8 rows 5.9 / 12 / 8.7, 16 rows - / 14.6 / 9.0.  So W of more than 2^25 elements goes to the tiles
+// from three rows on (if it lies as they want it: a packed copy costs more than it gains),
+// few and long lines from nine.
+constexpr int64_t kLargeW = int64_t(1) << 25, kFewLines = 512;
+
+// direct: x and W lie as the tiles want them.
+Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated, bool residual, bool direct) {
   const int64_t lines = gated ? 2 * n : n;
-  if (rows <= kGemvRows) {
+  const bool large = direct && lines * k > kLargeW;
+  if (rows <= kGemvRows && !(large && rows > 2) && !(rows > 4 && lines > kFewLines)) {
     // a line a wavefront, and as many wavefronts a line as fill the card with four each SIMD
     const int64_t steps = parts_of(k, kGemvStep);
     Plan p{kGemv, 0, 1, 1, lines >= 8192 || gated ? 2 : 1};
     while (p.waves < kGemvWaves && p.waves < steps && parts_of(lines, p.lines) * p.waves < 16 * kCus) p.waves *= 2;
     return p;
   }
-  if (rows <= kSmallRows) {
-    const int64_t steps = parts_of(k, kChunk * kStepChunks);
+  const int64_t steps = parts_of(k, kChunk * kStepChunks);
+  if (rows <= kSmallRows && !large && !(direct && rows > kGemvRows && lines <= kFewLines && steps > 32)) {
     return {kSmall, 0, 1, steps >= 16 ? 16 : steps >= 8 ? 8 : 4, 0};
   }
   const int64_t stages = parts_of(k, kChunk * kStageChunks);
@@ -704,8 +715,8 @@ struct GradRoom {
   Plan px, pw;
   int64_t sums, wt, xt, dz, dzt, partial, top, bytes;
   GradRoom(int64_t rows, int64_t k, int64_t lines, bool need_x, bool need_w, bool need_bias) {
-    px = plan_of(rows, lines, k, false, false);
-    pw = plan_of(lines, rows, k, false, false);
+    px = plan_of(rows, lines, k, false, false, true);
+    pw = plan_of(lines, rows, k, false, false, true);
     const int64_t ld = up_to(lines, kChunk) * 2, ldt = up_to(rows, kChunk) * 2;
     sums = up_to(std::max(need_x ? sums_bytes(px, rows, k) : 0, need_w ? sums_bytes(pw, lines, k) : 0), 256);
     wt = need_x ? up_to(k * ld, 256) : 0;
@@ -728,10 +739,10 @@ extern "C" int64_t dense_linear_workspace_size(const void* x, int64_t rows, int6
   if (rows == 0) return 0;
   const bool gated = activation == kSwiglu;
   const int64_t lines = gated ? 2 * n : n;
-  const Operand xo{static_cast<const uint16_t*>(x), rows, x_stride}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
+  const Operand xo{static_cast<const uint16_t*>(x), rows, rows > 1 ? x_stride : k}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
   int64_t most = 0;
   for (const bool residual : {false, true}) {
-    const Plan p = plan_of(rows, k, n, gated, residual);
+    const Plan p = plan_of(rows, k, n, gated, residual, direct(xo, k) && direct(wo, k));
     const bool tiles = p.kind == kTiles;
     most = std::max(most, Room(rows, k, lines, p, tiles && !direct(xo, k), tiles && !direct(wo, k)).bytes);
   }
@@ -742,7 +753,7 @@ extern "C" int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activat
   using namespace dense;
   if (int rc = check_sizes(rows, k, n, activation)) return rc;
   if (!plan) return vq::fail("dense_linear: null pointer");
-  const Plan p = plan_of(rows, k, n, activation == kSwiglu, has_residual);
+  const Plan p = plan_of(rows, k, n, activation == kSwiglu, has_residual, k % kChunk == 0);
   plan[0] = p.kind;
   plan[1] = p.kind == kTiles ? kShape[p.shape].rows : 0;
   plan[2] = p.kind == kTiles ? kShape[p.shape].lines : p.lines;
@@ -767,7 +778,7 @@ extern "C" int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, i
   const bool gated = activation == kSwiglu;
   const int64_t lines = gated ? 2 * n : n;
   Operand xo{static_cast<const uint16_t*>(x), rows, rows > 1 ? x_stride : k}, wo{static_cast<const uint16_t*>(w), lines, w_stride};
-  const Plan p = plan_of(rows, k, n, gated, residual);
+  const Plan p = plan_of(rows, k, n, gated, residual, direct(xo, k) && direct(wo, k));
   const bool pack_x = p.kind == kTiles && !direct(xo, k), pack_w = p.kind == kTiles && !direct(wo, k);
   const Room room(rows, k, lines, p, pack_x, pack_w);
   if (room.bytes && (!workspace || workspace_bytes < room.bytes || !aligned(workspace, 16))) {
