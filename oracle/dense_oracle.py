@@ -34,7 +34,7 @@ def activate(name, z):
 
 def slope(name, z):
     if name == "relu":
-        return (z > 0).astype(np.float64)
+        return (~(z <= 0)).astype(np.float64)  # (1 at a NaN, which relu keeps)
     if name == "gelu":
         return special.ndtr(z) + z * np.exp(-z * z / 2) / np.sqrt(2 * np.pi)
     if name == "gelu_tanh":

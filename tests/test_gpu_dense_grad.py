@@ -1,0 +1,41 @@
+"""The dense layer's gradients where the sizes and values of test_gpu_dense.py do not reach.
+Tolerances as there."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import dense_oracle as D
+from tests.test_gpu_dense import TYPES, close, exact, linear, normal  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [1, 5, 40, 300])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_relu_passes_gradients_where_it_keeps_nan(linear, device, rows, dtype):
+    """relu(NaN) is NaN, and dy passes there as it passes torch's relu: dz = dy in the row with a NaN,
+    which the type of x holds in full, and the other rows are as they are without it."""
+    rng = np.random.default_rng(rows)
+    x, w = normal(rng, (rows, 64), dtype, device), normal(rng, (48, 64), dtype, device, 0.1)
+    bias = normal(rng, 48, "fp32", device)
+    dy = normal(rng, (rows, 48), dtype, device)
+    at = rows // 2
+    keep = torch.arange(rows, device=device) != at
+    bad = x.clone()
+    bad[at, 3] = float("nan")
+    got = []
+    for a in (x, bad):
+        leaves = [t.detach().requires_grad_() for t in (a, w, bias)]
+        got.append(torch.autograd.grad(linear(*leaves, "relu"), leaves, dy))
+    dx, dw, db = got[1]
+    assert torch.equal(dx[keep], got[0][0][keep])
+    z = torch.from_numpy(exact(bad) @ exact(w).T + exact(bias)).requires_grad_()
+    dz, = torch.autograd.grad(torch.relu(z), z, dy.double().cpu())
+    assert torch.equal(dz[at], dy[at].double().cpu())
+    dz = dz.numpy()
+    close(dx[at], dz[at] @ exact(w), D.sum_error(dz[at:at + 1], exact(w).T), "dx of the row with a NaN")
+    others, _ = D.backward(exact(x[keep]), exact(w), exact(bias), "relu", exact(dy[keep]), torch.finfo(x.dtype).eps)
+    close(db, dz.sum(0), others["bias"][1] + 2.0 ** -23 * np.abs(dz).sum(0), "db")
+    # (the NaN is in column 3 of x, and so of dw, alone)
+    assert torch.isnan(dw[:, 3]).all() and torch.isfinite(dw[:, :3]).all() and torch.isfinite(dw[:, 4:]).all()

@@ -41,3 +41,14 @@ def test_gradient_by_differences(activation):
             diff = (up - loss()) / 2e-6
             a[at] = old
             assert abs(grads[name][0][at] - diff) <= 1e-7
+
+
+@pytest.mark.parametrize("name", [None, "relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_at_nan(name):
+    """As torch's: an activation that keeps a NaN does not drop its gradient."""
+    f = torch.nn.functional
+    z = torch.tensor([float("nan")], dtype=torch.float64, requires_grad=True)
+    y = {None: z * 1, "relu": f.relu(z), "gelu": f.gelu(z), "gelu_tanh": f.gelu(z, approximate="tanh"), "silu": f.silu(z)}[name]
+    want, = torch.autograd.grad(y, z)
+    assert torch.isnan(y) and np.isnan(D.activate(name, z.detach().numpy())).all()
+    assert np.array_equal(D.slope(name, z.detach().numpy()), want.numpy(), equal_nan=True)

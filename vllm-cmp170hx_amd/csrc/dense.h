@@ -104,7 +104,8 @@ __device__ __forceinline__ float gelu(float z) { return 0.5f * z * erfcf(z * -0.
 __device__ __forceinline__ float gelu_tanh(float z) { return z * sigmoid(2 * kTanhA * (z + kTanhB * z * z * z)); }
 __device__ __forceinline__ float silu(float z) { return z * sigmoid(z); }
 
-__device__ __forceinline__ float relu_slope(float z) { return z > 0 ? 1.0f : 0.0f; }
+// (a NaN passes gradients as it passes relu)
+__device__ __forceinline__ float relu_slope(float z) { return z > 0 || z != z ? 1.0f : 0.0f; }
 __device__ __forceinline__ float gelu_slope(float z) { return 0.5f * erfcf(z * -0.707106781f) + z * 0.398942280f * __expf(-0.5f * z * z); }
 __device__ __forceinline__ float gelu_tanh_slope(float z) {
   const float s = sigmoid(2 * kTanhA * (z + kTanhB * z * z * z));
