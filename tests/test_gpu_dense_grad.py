@@ -39,3 +39,19 @@ def test_relu_passes_gradients_where_it_keeps_nan(linear, device, rows, dtype):
     close(db, dz.sum(0), others["bias"][1] + 2.0 ** -23 * np.abs(dz).sum(0), "db")
     # (the NaN is in column 3 of x, and so of dw, alone)
     assert torch.isnan(dw[:, 3]).all() and torch.isfinite(dw[:, :3]).all() and torch.isfinite(dw[:, 4:]).all()
+
+
+@pytest.mark.parametrize("rows,lines", [(1 << 21, 24), ((1 << 21) - 37, 33), (65536, 256), (100_001, 7)])
+def test_bias_gradient_over_many_rows(linear, device, rows, lines):
+    """Of gradients of one sign, whose sums go on growing, against 64-bit sums: a workgroup's 64
+    rows are 34 additions in FP32, each off by half a step of the sum so far; what is added
+    of those must not add to it, but for the result's rounding."""
+    g = torch.Generator(device=device).manual_seed(rows)
+    x = torch.randn(rows, 8, device=device, generator=g).bfloat16()
+    w = torch.randn(lines, 8, device=device, generator=g).bfloat16()
+    dy = 0.1 + 0.001 * torch.rand(rows, lines, device=device, generator=g)
+    for dtype in ("fp32", "bf16"):
+        bias = torch.zeros(lines, device=device, dtype=TYPES[dtype], requires_grad=True)
+        db, = torch.autograd.grad(linear(x, w, bias, out_dtype=torch.float32), bias, dy)
+        want = dy.double().sum(0).cpu().numpy()
+        close(db, want, 34 * 2.0 ** -24 * want, f"db in {dtype}")

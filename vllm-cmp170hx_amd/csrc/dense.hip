@@ -466,14 +466,26 @@ __global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* t
   }
 }
 
-// db = the parts' sums, in order.
-__global__ __launch_bounds__(256) void bias_kernel(const float* partial, int64_t parts, int64_t lines, void* out, int dtype) {
-  const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (c >= lines) return;
-  float all = 0;
+// db = the parts' sums, in 64 bits: 2^21 rows have 32768 of them, whose sum in FP32 one after
+// another was off by 2^-12.6 of itself where gradients have one sign.  32 threads a line take every
+// 32nd part, and one adds theirs up in order.  Bound by the loads' latency: 65536 rows of 256 take
+// 3.9 us (a thread a line 37), 2^21 of 24 51 (1080), 1000 of 768 2.6 (2.1).
+constexpr int kSumLines = 32, kSumRuns = 32;
+
+__global__ __launch_bounds__(kSumLines * kSumRuns) void bias_kernel(const float* partial, int64_t parts, int64_t lines, void* out, int dtype) {
+  __shared__ double sums[kSumRuns][kSumLines];
+  const int col = threadIdx.x % kSumLines, run = threadIdx.x / kSumLines;
+  const int64_t c = int64_t(blockIdx.x) * kSumLines + col;
+  double all = 0;
+  if (c < lines) {
 #pragma unroll 8
-  for (int64_t p = 0; p < parts; ++p) all += partial[p * lines + c];
-  vq::store_act(out, dtype, c, all);
+    for (int64_t p = run; p < parts; p += kSumRuns) all += partial[p * lines + c];
+  }
+  sums[run][col] = all;
+  __syncthreads();
+  if (run || c >= lines) return;
+  for (int r = 1; r < kSumRuns; ++r) all += sums[r][col];
+  vq::store_act(out, dtype, c, float(all));
 }
 
 // ---- how a product runs -----------------------------------------------------------------
@@ -874,8 +886,8 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
   else hipLaunchKernelGGL(slopes_kernel<false>, parts, dim3(256), 0, s, g, scaled ? top + 1 : nullptr, tops, top, dz, ld, dzt, ldt, partial);
   if (int rc = vq::check_launch("dense_linear gradient")) return rc;
   if (dbias) {
-    hipLaunchKernelGGL(bias_kernel, dim3(unsigned(parts_of(lines, 256))), dim3(256), 0, s, partial, parts_of(rows, kPart), lines, dbias,
-                       bias_dtype);
+    hipLaunchKernelGGL(bias_kernel, dim3(unsigned(parts_of(lines, kSumLines))), dim3(kSumLines * kSumRuns), 0, s, partial, parts_of(rows, kPart),
+                       lines, dbias, bias_dtype);
     if (int rc = vq::check_launch("dense_linear gradient")) return rc;
   }
   const bool bf16 = dtype == vq::kBF16;
