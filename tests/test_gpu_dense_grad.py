@@ -55,3 +55,20 @@ def test_bias_gradient_over_many_rows(linear, device, rows, lines):
         db, = torch.autograd.grad(linear(x, w, bias, out_dtype=torch.float32), bias, dy)
         want = dy.double().sum(0).cpu().numpy()
         close(db, want, 34 * 2.0 ** -24 * want, f"db in {dtype}")
+
+
+@pytest.mark.parametrize("activation", [None, "silu", "swiglu"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_some_gradients_of_trainable_leaves(linear, device, activation, dtype):
+    """Asked for by themselves, gradients have the bits that they have beside the others."""
+    rng = np.random.default_rng(21)
+    lines = 2 * 60 if activation == "swiglu" else 60
+    t = {"x": normal(rng, (100, 72), dtype, device), "w": normal(rng, (lines, 72), dtype, device, 0.1),
+         "bias": normal(rng, lines, "fp32", device), "residual": normal(rng, (100, 60), "fp32", device)}
+    leaves = {k: v.requires_grad_() for k, v in t.items()}
+    dy = normal(rng, (100, 60), dtype, device)
+    y = linear(leaves["x"], leaves["w"], leaves["bias"], activation, leaves["residual"], TYPES[dtype])
+    every = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy, retain_graph=True)))
+    for names in (["x"], ["w"], ["bias"], ["residual"], ["w", "x"], ["residual", "bias"], ["bias", "x"]):
+        for name, g in zip(names, torch.autograd.grad(y, [leaves[k] for k in names], dy, retain_graph=True)):
+            assert torch.equal(g, every[name]), (names, name)

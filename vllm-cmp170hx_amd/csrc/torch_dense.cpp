@@ -201,6 +201,7 @@ struct DenseLinear : torch::autograd::Function<DenseLinear> {
     ctx->saved_data["limit"] = limit;
     ctx->saved_data["x"] = x.requires_grad();
     ctx->saved_data["w"] = w.requires_grad();
+    ctx->saved_data["has_bias"] = bias.has_value();
     ctx->saved_data["bias"] = bias && bias->requires_grad() ? int64_t(bias->scalar_type()) : int64_t(-1);
     ctx->saved_data["residual"] = residual && residual->requires_grad() ? int64_t(residual->scalar_type()) : int64_t(-1);
     return y;
@@ -212,8 +213,15 @@ struct DenseLinear : torch::autograd::Function<DenseLinear> {
     TORCH_CHECK(!c10::GradMode::is_enabled(), kWhat, ": its gradient has no gradient (create_graph)");
     static const auto op = handle<decltype(::gradient)>("_vllm_mi355x::dense_linear_grad");
     const torch::autograd::variable_list saved = ctx->get_saved_variables();
-    const int64_t bias = ctx->saved_data["bias"].toInt(), residual = ctx->saved_data["residual"].toInt();
-    const bool need_x = ctx->saved_data["x"].toBool(), need_w = ctx->saved_data["w"].toBool();
+    // what this pass asks for (an edge an input that is there: x, w, bias, residual)
+    const bool has_bias = ctx->saved_data["has_bias"].toBool();
+    const auto asked = [&](const char* name, size_t edge) {
+      const int64_t type = ctx->saved_data[name].toInt();
+      return type >= 0 && ctx->needs_input_grad(edge) ? type : int64_t(-1);
+    };
+    const int64_t bias = asked("bias", 2), residual = asked("residual", has_bias ? 3 : 2);
+    const bool need_x = ctx->saved_data["x"].toBool() && ctx->needs_input_grad(0);
+    const bool need_w = ctx->saved_data["w"].toBool() && ctx->needs_input_grad(1);
     if (residual >= 0) out[4] = grads[0].to(at::ScalarType(residual));
     if (need_x || need_w || bias >= 0) {
       const at::AutoDispatchBelowADInplaceOrView below;
