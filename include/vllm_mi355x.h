@@ -668,7 +668,8 @@ int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int ha
 
 /*
  * From dy, the gradient of out ([rows][n] of any of the three types): dx [rows][k] and dw
- * [lines][k] (contiguous, of dtype) and dbias [lines]; each may be null.  z as dense_linear
+ * [lines][k] (contiguous, of dtype) and dbias [lines]; each may be null.  x is read for dw
+ * alone and w for dx alone, and may be null where they are.  z as dense_linear
  * left it (with VQ_ACT_NONE null).  The gradient of z is rounded to dtype, in FP16 over a
  * power of two of the whole, before its products.  At least one row; rows and lines up to 2^21.
  */

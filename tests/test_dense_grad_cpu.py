@@ -12,6 +12,12 @@ def linear():
     return dense_linear
 
 
+@pytest.fixture(scope="module")
+def lib():
+    from vllm_mi355x import _native
+    return _native.load()
+
+
 class Calls(TorchDispatchMode):
     """The dense layer's operators that run, with their arguments by name."""
 
@@ -60,3 +66,46 @@ def test_a_single_trainable_input(linear, which):
     y = linear(t["x"], t["w"], t["bias"], "gelu", t["residual"])
     y.backward(torch.empty_like(y))
     assert [k for k, v in t.items() if v.grad is not None] == [which] and t[which].grad.dtype == t[which].dtype
+
+
+def test_a_residual_alone_keeps_nothing(linear):
+    t = leaves()
+    t["residual"].requires_grad_()
+    with Calls() as calls:
+        y = linear(t["x"], t["w"], t["bias"], "silu", t["residual"])
+    assert [name for name, _ in calls.seen] == ["dense_linear"] and y.requires_grad
+
+
+@pytest.mark.parametrize("activation", [None, "gelu"])
+@pytest.mark.parametrize("trained", [["x"], ["w"], ["bias"], ["x", "bias"], ["w", "bias"], ["residual"], ["x", "w"]])
+def test_what_is_not_kept_may_change(linear, activation, trained):
+    """The gradient of x is computed from the weights, theirs from x: a frozen one's counterpart is
+    neither kept nor found to have changed; the one that is used is."""
+    t = {k: v.requires_grad_(k in trained) for k, v in leaves().items()}
+    made = {k: (v * 1 if v.requires_grad else v) for k, v in t.items()}  # (leaves cannot be written to)
+    y = linear(made["x"], made["w"], made["bias"], activation, made["residual"])
+    used = {"x": "w" in trained, "w": "x" in trained, "bias": False, "residual": False}
+    with torch.no_grad():
+        for k, v in made.items():
+            if not used[k]:
+                v.add_(1)
+    with Calls() as calls:
+        grads = torch.autograd.grad(y, [t[k] for k in trained], torch.empty_like(y), retain_graph=True)
+    assert [(g.shape, g.dtype) for g in grads] == [(t[k].shape, t[k].dtype) for k in trained]
+    for _, args in calls.seen:
+        assert (args["x"] is not None) == used["x"] and (args["w"] is not None) == used["w"]
+    for k in ("x", "w"):
+        if used[k]:
+            with torch.no_grad():
+                made[k].add_(1)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(y, [t[k] for k in trained], torch.empty_like(y), retain_graph=True)
+
+
+def test_null_operands(lib):
+    """The entry point takes null for what it does not read: the next check is the workspace's."""
+    from tests.test_dense_cpu import grad
+    for args, word in ((grad(x=0, dw=0, work=0), "workspace"), (grad(w=0, dx=0, work=0), "workspace"),
+                       (grad(x=0, w=0, dx=0, dw=0, work=0), "workspace"), (grad(x=0, work=0), "null"), (grad(w=0, work=0), "null")):
+        assert lib.dense_linear_grad(*args) == 1
+        assert word in lib.vllm_mi355x_last_error().decode(), lib.vllm_mi355x_last_error()

@@ -72,3 +72,39 @@ def test_some_gradients_of_trainable_leaves(linear, device, activation, dtype):
     for names in (["x"], ["w"], ["bias"], ["residual"], ["w", "x"], ["residual", "bias"], ["bias", "x"]):
         for name, g in zip(names, torch.autograd.grad(y, [leaves[k] for k in names], dy, retain_graph=True)):
             assert torch.equal(g, every[name]), (names, name)
+
+
+@pytest.mark.parametrize("activation", [None, "silu", "swiglu"])
+def test_frozen_inputs_are_not_kept(linear, device, activation):
+    """x written over where only its own and the bias's gradients are asked for, the weights where only
+    theirs are: the bits that they have without it."""
+    rng = np.random.default_rng(22)
+    lines = 2 * 64 if activation == "swiglu" else 64
+    for rows in (3, 130):
+        x, w, bias = normal(rng, (rows, 72), "fp16", device), normal(rng, (lines, 72), "fp16", device, 0.1), normal(rng, lines, "fp32", device)
+        dy = normal(rng, (rows, 64), "fp16", device)
+        for names in (["x", "bias"], ["w", "bias"], ["bias"], ["x"], ["w"]):
+            got = []
+            for change in (False, True):
+                t = {k: v.clone().requires_grad_(k in names) for k, v in (("x", x), ("w", w), ("bias", bias))}
+                made = {k: (v * 1 if v.requires_grad else v) for k, v in t.items()}
+                y = linear(made["x"], made["w"], made["bias"], activation)
+                with torch.no_grad():
+                    if change:
+                        for k, other in (("x", "w"), ("w", "x")):
+                            if other not in names:
+                                made[k].fill_(float("nan"))
+                got.append(torch.autograd.grad(y, [t[k] for k in names], dy))
+            assert all(torch.equal(a, b) for a, b in zip(*got)), names
+
+
+def test_a_residual_alone_keeps_no_memory(linear, device):
+    x, w = (torch.zeros(256, k, device=device).half() for k in (64, 64))
+    residual = torch.zeros(256, 256, device=device).half().requires_grad_()
+    linear(x, w, None, "silu", residual)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(device)
+    y = linear(x, w, None, "silu", residual)
+    assert torch.cuda.memory_allocated(device) - before == y.numel() * 2
+    dy = torch.ones_like(y)
+    assert torch.equal(torch.autograd.grad(y, residual, dy)[0], dy)

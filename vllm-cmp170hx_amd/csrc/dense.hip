@@ -676,9 +676,10 @@ int check_grad_sizes(int64_t rows, int64_t k, int64_t n, int activation) {
 bool is_half(int dtype) { return dtype == vq::kBF16 || dtype == vq::kFP16; }
 bool is_float(int dtype) { return is_half(dtype) || dtype == vq::kFP32; }
 
-int check_inputs(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t w_stride, float limit) {
+int check_inputs(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_stride, const void* w, int64_t w_stride, float limit,
+                 bool read_x = true, bool read_w = true) {
   if (!is_half(dtype)) return vq::fail("dense_linear: x and the weights must be BF16 or FP16");
-  if (!x || !w) return vq::fail("dense_linear: null pointer");
+  if ((read_x && !x) || (read_w && !w)) return vq::fail("dense_linear: null pointer");
   if (x_stride < 0 || (rows > 1 && x_stride < k) || x_stride > (int64_t(1) << 40) || w_stride < k || w_stride > (int64_t(1) << 40)) {
     return vq::fail("dense_linear: row stride out of range");
   }
@@ -838,7 +839,7 @@ extern "C" int dense_linear_grad(const void* x, int dtype, int64_t rows, int64_t
   if (int rc = check_grad_sizes(rows, k, n, activation)) return rc;
   if (!is_float(dy_dtype) || (dbias && !is_float(bias_dtype))) return vq::fail("dense_linear: bias and output must be BF16, FP16 or FP32");
   if (rows == 0) return vq::fail("dense_linear: no rows have no gradient to compute");
-  if (int rc = check_inputs(x, dtype, rows, k, x_stride, w, w_stride, limit)) return rc;
+  if (int rc = check_inputs(x, dtype, rows, k, x_stride, w, w_stride, limit, dw, dx)) return rc;
   if (!dy || (activation != kNone && !z)) return vq::fail("dense_linear: null pointer");
   if (dy_stride < 0 || (rows > 1 && dy_stride < n)) return vq::fail("dense_linear: gradient stride out of range");
   const bool gated = activation == kSwiglu;

@@ -148,38 +148,40 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor
   return {out, z};
 }
 
-// (dx, dw, dbias) from dy; those not asked for are empty.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient(const at::Tensor& x, const at::Tensor& w, const at::Tensor& z, int64_t activation,
-                                                        double limit, const at::Tensor& given, bool need_x, bool need_w,
-                                                        std::optional<at::ScalarType> bias_dtype) {
-  check_kinds(x, w, std::nullopt, activation, std::nullopt, given.scalar_type(), limit);
-  TORCH_CHECK(x.is_cuda() && given.device() == x.device() && z.device() == x.device(), kWhat, ": the gradient's tensors must be on x's GPU");
-  const int64_t n = columns_of(w, activation);
-  const Rows r = rows_of(x);
-  TORCH_CHECK(r.stride >= 0 && w.size(1) == r.k && given.numel() == r.rows * n &&
-                  (!activation || (z.is_contiguous() && z.numel() == r.rows * w.size(0) && z.scalar_type() == at::kFloat)),
+// (dx, dw, dbias) from dy; those not asked for are empty.  x is read for dw alone, w for dx alone.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient(const std::optional<at::Tensor>& x, const std::optional<at::Tensor>& w,
+                                                        const at::Tensor& z, int64_t activation, double limit, const at::Tensor& given,
+                                                        bool need_x, bool need_w, std::optional<at::ScalarType> bias_dtype) {
+  TORCH_CHECK((x || !need_w) && (w || !need_x) && given.is_cuda() && z.device() == given.device() && given.dim() >= 1 && given.size(-1) > 0, kWhat,
+              ": the gradient's tensors must be there, on a GPU");
+  if (x && w) check_kinds(*x, *w, std::nullopt, activation, std::nullopt, given.scalar_type(), limit);
+  const int64_t n = given.size(-1), rows = given.numel() / n, lines = activation == kSwiglu ? 2 * n : n;
+  const Rows r = x ? rows_of(*x) : Rows{rows, w ? w->size(1) : 1, w ? w->size(1) : 1};
+  TORCH_CHECK((!x || (x->device() == given.device() && x->dim() == given.dim() && r.stride >= 0 && r.rows == rows)) &&
+                  (!w || (w->device() == given.device() && w->dim() == 2 && w->size(0) == lines && w->size(1) == r.k)) &&
+                  (!activation || (z.is_contiguous() && z.numel() == rows * lines && z.scalar_type() == at::kFloat)),
               kWhat, ": the gradient's tensors must be the forward's");
-  const c10::DeviceGuard guard(x.device());
-  const auto nothing = [&] { return at::empty({0}, x.options()); };
-  const auto like = [&](const at::Tensor& t) {
-    return r.rows ? at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)) : at::zeros(t.sizes(), t.options());
+  const at::ScalarType type = x ? x->scalar_type() : w ? w->scalar_type() : at::kBFloat16;
+  const c10::DeviceGuard guard(given.device());
+  const auto make = [&](at::IntArrayRef sizes, at::ScalarType t) {
+    const auto options = given.options().dtype(t).memory_format(at::MemoryFormat::Contiguous);
+    return rows ? at::empty(sizes, options) : at::zeros(sizes, given.options().dtype(t));
   };
-  at::Tensor dx = need_x ? like(x) : nothing(), dw = need_w ? like(w) : nothing();
-  at::Tensor db = !bias_dtype ? nothing()
-                  : r.rows    ? at::empty({w.size(0)}, x.options().dtype(*bias_dtype))
-                              : at::zeros({w.size(0)}, x.options().dtype(*bias_dtype));
-  if (r.rows == 0) return {dx, dw, db};
+  at::Tensor dx = need_x ? make(with_last(given.sizes(), r.k), type) : make({0}, type);
+  at::Tensor dw = need_w ? make({lines, r.k}, type) : make({0}, type);
+  at::Tensor db = bias_dtype ? make({lines}, *bias_dtype) : make({0}, type);
+  if (rows == 0) return {dx, dw, db};
   // (autograd gives broadcast and transposed gradients too)
   const at::Tensor dy = rows_of(given).stride >= 0 ? given : given.contiguous();
-  const int64_t bytes = native_grad_workspace(r.rows, r.k, n, int(activation), need_x, need_w, bias_dtype.has_value());
+  const int64_t bytes = native_grad_workspace(rows, r.k, n, int(activation), need_x, need_w, bias_dtype.has_value());
   if (bytes < 0) TORCH_CHECK(false, native_error());
-  const at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
-  check_status(native_grad(x.const_data_ptr(), dtype_code(x.scalar_type()), r.rows, r.k, r.stride, w.const_data_ptr(), n,
-                           w.size(0) > 1 ? w.stride(0) : r.k, activation ? z.const_data_ptr<float>() : nullptr, int(activation),
+  const at::Tensor ws = at::empty({bytes}, given.options().dtype(at::kByte));
+  check_status(native_grad(x ? x->const_data_ptr() : nullptr, dtype_code(type), rows, r.k, r.stride, w ? w->const_data_ptr() : nullptr, n,
+                           w && lines > 1 ? w->stride(0) : r.k, activation ? z.const_data_ptr<float>() : nullptr, int(activation),
                            static_cast<float>(limit), dy.const_data_ptr(), dtype_code(dy.scalar_type()), rows_of(dy).stride,
                            need_x ? dx.mutable_data_ptr() : nullptr, need_w ? dw.mutable_data_ptr() : nullptr,
                            bias_dtype ? db.mutable_data_ptr() : nullptr, bias_dtype ? dtype_code(*bias_dtype) : 0, ws.mutable_data_ptr(), bytes,
-                           stream_of(x)));
+                           stream_of(given)));
   return {dx, dw, db};
 }
 
@@ -192,17 +194,24 @@ struct DenseLinear : torch::autograd::Function<DenseLinear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const std::optional<at::Tensor>& bias, int64_t activation, const std::optional<at::Tensor>& residual,
                             at::ScalarType out_dtype, double limit) {
-    static const auto op = handle<decltype(::forward)>("_vllm_mi355x::dense_linear_forward");
+    const bool need_x = x.requires_grad(), need_w = w.requires_grad(), need_bias = bias && bias->requires_grad();
     const at::AutoDispatchBelowADInplaceOrView below;
-    auto [y, z] = op.call(x, w, bias, activation, residual, out_dtype, limit);
-    // (x and w both: their types and sizes are those of the gradients)
-    ctx->save_for_backward({x, w, z});
+    at::Tensor y, z;
+    if (need_x || need_w || need_bias) {
+      static const auto op = handle<decltype(::forward)>("_vllm_mi355x::dense_linear_forward");
+      std::tie(y, z) = op.call(x, w, bias, activation, residual, out_dtype, limit);
+    } else {  // (the residual's gradient is dy)
+      static const auto op = handle<decltype(linear)>("_vllm_mi355x::dense_linear");
+      y = op.call(x, w, bias, activation, residual, out_dtype, limit);
+    }
+    // (what no gradient is computed from is not kept, and may be written to)
+    ctx->save_for_backward({need_w ? x : at::Tensor(), need_x ? w : at::Tensor(), z});
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["limit"] = limit;
-    ctx->saved_data["x"] = x.requires_grad();
-    ctx->saved_data["w"] = w.requires_grad();
+    ctx->saved_data["x"] = need_x;
+    ctx->saved_data["w"] = need_w;
     ctx->saved_data["has_bias"] = bias.has_value();
-    ctx->saved_data["bias"] = bias && bias->requires_grad() ? int64_t(bias->scalar_type()) : int64_t(-1);
+    ctx->saved_data["bias"] = need_bias ? int64_t(bias->scalar_type()) : int64_t(-1);
     ctx->saved_data["residual"] = residual && residual->requires_grad() ? int64_t(residual->scalar_type()) : int64_t(-1);
     return y;
   }
@@ -225,7 +234,8 @@ struct DenseLinear : torch::autograd::Function<DenseLinear> {
     if (residual >= 0) out[4] = grads[0].to(at::ScalarType(residual));
     if (need_x || need_w || bias >= 0) {
       const at::AutoDispatchBelowADInplaceOrView below;
-      auto [dx, dw, db] = op.call(saved[0], saved[1], saved[2], ctx->saved_data["activation"].toInt(), ctx->saved_data["limit"].toDouble(),
+      const auto kept = [&](size_t i) { return saved[i].defined() ? std::optional<at::Tensor>(saved[i]) : std::nullopt; };
+      auto [dx, dw, db] = op.call(kept(0), kept(1), saved[2], ctx->saved_data["activation"].toInt(), ctx->saved_data["limit"].toDouble(),
                                   grads[0], need_x, need_w, bias >= 0 ? std::optional<at::ScalarType>(at::ScalarType(bias)) : std::nullopt);
       if (need_x) out[0] = dx;
       if (need_w) out[1] = dw;
@@ -281,12 +291,16 @@ std::tuple<at::Tensor, at::Tensor> forward_meta(const at::Tensor& x, const at::T
   const c10::SymInt rows = activation ? x.sym_numel() / x.sym_size(-1) : c10::SymInt(0);
   return {y, at::empty_symint({rows, w.sym_size(0)}, x.options().dtype(at::kFloat))};
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient_meta(const at::Tensor& x, const at::Tensor& w, const at::Tensor&, int64_t, double,
-                                                             const at::Tensor&, bool need_x, bool need_w,
-                                                             std::optional<at::ScalarType> bias_dtype) {
-  const auto nothing = [&] { return at::empty({0}, x.options()); };
-  return {need_x ? at::empty_symint(x.sym_sizes(), x.options()) : nothing(), need_w ? at::empty_symint(w.sym_sizes(), w.options()) : nothing(),
-          bias_dtype ? at::empty_symint({w.sym_size(0)}, x.options().dtype(*bias_dtype)) : nothing()};
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient_meta(const std::optional<at::Tensor>& x, const std::optional<at::Tensor>& w,
+                                                             const at::Tensor&, int64_t activation, double, const at::Tensor& given,
+                                                             bool need_x, bool need_w, std::optional<at::ScalarType> bias_dtype) {
+  TORCH_CHECK((x || !need_w) && (w || !need_x), kWhat, ": the gradient's tensors must be there");
+  const at::ScalarType type = x ? x->scalar_type() : w ? w->scalar_type() : at::kBFloat16;
+  const auto make = [&](c10::SymIntArrayRef sizes, at::ScalarType t) { return at::empty_symint(sizes, given.options().dtype(t)); };
+  const c10::SymInt n = given.sym_size(-1), lines = activation == kSwiglu ? n * 2 : n;
+  return {need_x ? make(with_last(given.sym_sizes(), w->sym_size(1)), type) : make({c10::SymInt(0)}, type),
+          need_w ? make({lines, x->sym_size(-1)}, type) : make({c10::SymInt(0)}, type),
+          bias_dtype ? make({lines}, *bias_dtype) : make({c10::SymInt(0)}, type)};
 }
 
 template <typename F>
@@ -310,7 +324,7 @@ TORCH_LIBRARY_FRAGMENT(_vllm_mi355x, m) {
       "dense_linear_forward(Tensor x, Tensor w, Tensor? bias, int activation, Tensor? residual, ScalarType out_dtype, float limit) "
       "-> (Tensor, Tensor)");
   m.def(
-      "dense_linear_grad(Tensor x, Tensor w, Tensor z, int activation, float limit, Tensor dy, bool need_x, bool need_w, "
+      "dense_linear_grad(Tensor? x, Tensor? w, Tensor z, int activation, float limit, Tensor dy, bool need_x, bool need_w, "
       "ScalarType? bias_dtype) -> (Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(_vllm_mi355x, CUDA, m) {
