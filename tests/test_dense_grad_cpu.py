@@ -109,3 +109,14 @@ def test_null_operands(lib):
                        (grad(x=0, w=0, dx=0, dw=0, work=0), "workspace"), (grad(x=0, work=0), "null"), (grad(w=0, work=0), "null")):
         assert lib.dense_linear_grad(*args) == 1
         assert word in lib.vllm_mi355x_last_error().decode(), lib.vllm_mi355x_last_error()
+
+
+@pytest.mark.parametrize("rows,k,n", [(1 << 21, 64, 16384), ((1 << 21) + 1, 64, 8200), (1 << 26, 8, 300), (400, 128, 1 << 23), (1 << 21, 192, 16384),
+                                      (1 << 22, 64, 20000)])
+@pytest.mark.parametrize("residual", [0, 1])
+def test_large_results_have_a_plan(lib, rows, k, n, residual):
+    """Of few stages the smallest tiles are the fastest, but not more of them than a launch takes
+    (2^22): within the sizes that are taken, a result that fits a card is not refused."""
+    from tests.test_dense_cpu import plan
+    kind, tile_rows, lines, splits, _ = plan(lib, rows, k, n, 0, residual)
+    assert kind == 0 and -(-rows // tile_rows) * -(-n // lines) * splits <= 1 << 22

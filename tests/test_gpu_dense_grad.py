@@ -108,3 +108,25 @@ def test_a_residual_alone_keeps_no_memory(linear, device):
     assert torch.cuda.memory_allocated(device) - before == y.numel() * 2
     dy = torch.ones_like(y)
     assert torch.equal(torch.autograd.grad(y, residual, dy)[0], dy)
+
+
+@pytest.mark.parametrize("which", ["y", "dx"])
+def test_more_results_than_a_launch_has_smallest_tiles(linear, device, which):
+    """2^21 and one rows of 8200 columns from 64: the forward's result, and the gradient of as many rows
+    as it takes."""
+    rows, n, k = (1 << 21) + (which == "y"), 8200, 64
+    rng = np.random.default_rng(23)
+    g = torch.Generator(device=device).manual_seed(23)
+    small = torch.randn(rows, k, device=device, generator=g).bfloat16()
+    if which == "y":
+        w = normal(rng, (n, k), "bf16", device)
+        got, want = linear(small, w), exact(w)
+    else:
+        w = normal(rng, (k, n), "bf16", device)
+        x = torch.zeros(rows, n, device=device, dtype=torch.bfloat16, requires_grad=True)
+        got, want = torch.autograd.grad(linear(x, w), x, small)[0], exact(w).T
+    some = torch.tensor([0, 1, 127, 128, 65535, 1 << 20, rows - 130, rows - 2, rows - 1], device=device)
+    a = exact(small[some])
+    close(got[some], a @ want.T, D.sum_error(a, want), which)
+    del got
+    torch.cuda.empty_cache()

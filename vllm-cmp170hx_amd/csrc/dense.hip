@@ -550,6 +550,7 @@ Plan plan_of(int64_t rows, int64_t k, int64_t n, bool gated, bool residual, bool
   for (int i = 0; i < kShapes; ++i) {
     const Shape& t = kShape[i];
     const int64_t tiles = parts_of(rows, t.rows) * parts_of(n, gated ? t.lines / 2 : t.lines);
+    if (i && tiles > kMaxGroups) continue;  // (a result that fits a card has no more of the largest)
     for (int64_t splits = 1; splits <= 16 && splits <= std::max<int64_t>(1, stages / 4); ++splits) {
       if (splits > 1 && tiles * splits > 8 * kCus) break;
       const int64_t each = parts_of(stages, splits), all = tiles * parts_of(stages, each);
