@@ -671,7 +671,8 @@ int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int ha
  * [lines][k] (contiguous, of dtype) and dbias [lines]; each may be null.  x is read for dw
  * alone and w for dx alone, and may be null where they are.  z as dense_linear
  * left it (with VQ_ACT_NONE null).  The gradient of z is rounded to dtype, in FP16 over a
- * power of two of the whole, before its products.  At least one row; rows and lines up to 2^21.
+ * power of two of the whole, before its products.  At least one row; rows and lines up to 2^21, and no
+ * more than 2^23 parts of 64 x 64 in x, in w and in rows x lines (the size is -1 otherwise).
  */
 int64_t dense_linear_grad_workspace_size(int64_t rows, int64_t k, int64_t n, int activation,
                                          int need_x, int need_w, int need_bias);

@@ -120,3 +120,20 @@ def test_large_results_have_a_plan(lib, rows, k, n, residual):
     from tests.test_dense_cpu import plan
     kind, tile_rows, lines, splits, _ = plan(lib, rows, k, n, 0, residual)
     assert kind == 0 and -(-rows // tile_rows) * -(-n // lines) * splits <= 1 << 22
+
+
+@pytest.mark.parametrize("x,w", [(((1 << 21), 1), (16448, 1)), ((1 << 20, 2, 1), (16448, 1)), ((1 << 21, 16448), (1, 16448)), ((4, 1 << 21), ((1 << 14) + 64, 1 << 21)),
+                                 (((1 << 21) + 1, 8), (5, 8)), ((4, 8), ((1 << 21) + 1, 8))])
+def test_a_gradient_that_would_be_refused_is_at_the_call(linear, lib, x, w):
+    """Not after the forward pass has run; without a gradient the call is taken."""
+    rows = torch.empty(*x, device="meta", dtype=torch.half)
+    weights = torch.empty(*w, device="meta", dtype=torch.half)
+    assert lib.dense_linear_grad_workspace_size(rows.numel() // x[-1], x[-1], w[0], 0, 0, 1, 0) == -1
+    assert linear(rows, weights).shape == (*x[:-1], w[0])
+    with pytest.raises(RuntimeError, match="too many rows and columns|a gradient takes up to"):
+        linear(rows, weights.requires_grad_())
+    with pytest.raises(RuntimeError, match="too many rows and columns|a gradient takes up to"):
+        linear(rows, weights.detach(), torch.empty(w[0], device="meta", requires_grad=True), "silu")
+    # (a residual's gradient needs no product)
+    residual = torch.empty(*x[:-1], w[0], device="meta", requires_grad=True)
+    assert linear(rows, weights.detach(), None, "silu", residual).requires_grad

@@ -130,3 +130,12 @@ def test_more_results_than_a_launch_has_smallest_tiles(linear, device, which):
     close(got[some], a @ want.T, D.sum_error(a, want), which)
     del got
     torch.cuda.empty_cache()
+
+
+def test_refused_gradients_take_no_memory(linear, device):
+    x, w = torch.zeros(1 << 21, 1, device=device).half(), torch.zeros(16448, 1, device=device).half().requires_grad_()
+    before = torch.cuda.memory_allocated(device)
+    torch.cuda.reset_peak_memory_stats(device)
+    with pytest.raises(RuntimeError, match="too many rows and columns"):
+        linear(x, w, None, "silu")
+    assert torch.cuda.max_memory_allocated(device) == before

@@ -133,6 +133,11 @@ void linear_out(const at::Tensor& x, const at::Tensor& w, const std::optional<at
   run(x, w, bias, activation, residual, limit, out, at::Tensor());
 }
 
+// Sizes that the gradient takes (so that it is not refused after the forward has run).
+void check_trains(int64_t rows, int64_t k, int64_t n, int64_t activation) {
+  if (rows > 0 && native_grad_workspace(rows, k, n, int(activation), 1, 1, 1) < 0) TORCH_CHECK(false, native_error());
+}
+
 // (y, z): z is what the gradient needs beside x and w, x w^T + bias in FP32 (nothing
 // without an activation).
 std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
@@ -141,7 +146,7 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor
   const c10::DeviceGuard guard(x.device());
   const int64_t n = columns_of(w, activation), k = x.size(-1);
   TORCH_CHECK(k > 0, kWhat, ": the weights must be [n, k] of x's k = 0");
-  TORCH_CHECK(x.numel() / k <= (1 << 21) && w.size(0) <= (1 << 21), kWhat, ": a gradient takes up to 2^21 rows and weight rows");
+  check_trains(x.numel() / k, k, n, activation);
   at::Tensor out = at::empty(with_last(x.sizes(), n), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
   at::Tensor z = at::empty({activation ? x.numel() / k : 0, w.size(0)}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
   run(x, w, bias, activation, residual, limit, out, activation ? z : at::Tensor());
@@ -289,6 +294,8 @@ std::tuple<at::Tensor, at::Tensor> forward_meta(const at::Tensor& x, const at::T
                                                 double limit) {
   at::Tensor y = linear_meta(x, w, bias, activation, residual, out_dtype, limit);
   const c10::SymInt rows = activation ? x.sym_numel() / x.sym_size(-1) : c10::SymInt(0);
+  const auto all = x.sym_numel().maybe_as_int(), k = x.sym_size(-1).maybe_as_int(), n = y.sym_size(-1).maybe_as_int();
+  if (all && k && n && *k > 0) check_trains(*all / *k, *k, *n, activation);
   return {y, at::empty_symint({rows, w.sym_size(0)}, x.options().dtype(at::kFloat))};
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient_meta(const std::optional<at::Tensor>& x, const std::optional<at::Tensor>& w,

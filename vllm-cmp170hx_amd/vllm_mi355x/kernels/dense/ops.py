@@ -36,7 +36,8 @@ def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
 
     x [..., k] and weight [n, k] bf16 or fp16, of one type; x's leading axes one run of
     rows, unit inner strides; k up to 2^21, weight rows up to 2^24 and rows up to 2^26 (for
-    gradients both up to 2^21).  bias [n] (contiguous) and residual
+    gradients of x, weight or bias both up to 2^21, and 2^23 parts of 64 x 64 of x, of weight and
+    of x W^T).  bias [n] (contiguous) and residual
     [..., n] (rows as x's) bf16, fp16 or fp32.  activation: None, "relu", "gelu" (of the
     error function), "gelu_tanh", "silu", or "swiglu": weight [2 n, k] and bias [2 n] hold the
     gate rows and then the up rows, and the result is SiLU(min(g, L)) clamp(u, -L, L), L the
