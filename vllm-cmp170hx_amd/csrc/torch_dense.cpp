@@ -65,7 +65,7 @@ Rows rows_of(const at::Tensor& t) {
   return {rows, k, rows > 1 && stride < k ? -1 : stride};
 }
 
-// What needs no data; sizes may be symbolic.
+// Shapes and types (not how tensors lie); sizes may be symbolic.
 void check_kinds(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
                  const std::optional<at::Tensor>& residual, at::ScalarType out_dtype, double limit) {
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, kWhat, ": x must be BF16 or FP16");
@@ -80,26 +80,35 @@ void check_kinds(const at::Tensor& x, const at::Tensor& w, const std::optional<a
   for (const at::Tensor* t : {&w, bias ? &*bias : nullptr, residual ? &*residual : nullptr}) {
     TORCH_CHECK(!t || t->device() == x.device(), kWhat, ": tensors must be on x's device");
   }
+  const c10::SymInt k = x.sym_size(-1), lines = w.sym_size(0);
+  TORCH_SYM_CHECK(k.sym_gt(0), kWhat, ": the weights must be [n, k] of x's k = ", k);
+  TORCH_SYM_CHECK(w.sym_size(1).sym_eq(k), kWhat, ": the weights must be [n, k] of x's k = ", k);
+  TORCH_SYM_CHECK(lines.sym_gt(0), kWhat, ": the weights must be [n, k], not without rows");
+  if (activation == kSwiglu) {
+    TORCH_SYM_CHECK((lines % 2).sym_eq(0), kWhat, ": a gated activation needs gate and up rows in equal number");
+  }
+  if (bias) TORCH_SYM_CHECK(bias->sym_size(0).sym_eq(lines), kWhat, ": bias must be a value a weight row");
+  if (residual) {
+    for (int64_t d = 0; d < x.dim(); ++d) {
+      TORCH_SYM_CHECK(residual->sym_size(d).sym_eq(d + 1 < x.dim() ? x.sym_size(d) : activation == kSwiglu ? lines / 2 : lines), kWhat,
+                      ": residual must have the output's shape");
+    }
+  }
 }
 
-int64_t columns_of(const at::Tensor& w, int64_t activation) {
-  TORCH_CHECK(activation != kSwiglu || w.size(0) % 2 == 0, kWhat, ": a gated activation needs gate and up rows in equal number");
-  return activation == kSwiglu ? w.size(0) / 2 : w.size(0);
-}
+int64_t columns_of(const at::Tensor& w, int64_t activation) { return activation == kSwiglu ? w.size(0) / 2 : w.size(0); }
 
 void run(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
          const std::optional<at::Tensor>& residual, double limit, const at::Tensor& out, const at::Tensor& z) {
   TORCH_CHECK(x.is_cuda(), kWhat, ": x must be on a GPU");
   const Rows r = rows_of(x);
-  TORCH_CHECK(r.k > 0 && w.size(1) == r.k && w.size(0) > 0, kWhat, ": the weights must be [n, k] of x's k = ", r.k);
   TORCH_CHECK(r.stride >= 0, kWhat, ": x needs unit stride along its last axis and leading axes that are one run of rows, not overlapping");
   TORCH_CHECK((r.k == 1 || w.stride(1) == 1) && (w.size(0) == 1 || w.stride(0) >= r.k), kWhat,
               ": the weights need unit inner stride and rows that do not overlap");
   const int64_t n = columns_of(w, activation);
-  TORCH_CHECK(!bias || (bias->size(0) == w.size(0) && bias->is_contiguous()), kWhat, ": bias must be contiguous, a value a weight row");
+  TORCH_CHECK(!bias || bias->is_contiguous(), kWhat, ": bias must be contiguous");
   Rows res{0, 0, 0};
   if (residual) {
-    TORCH_CHECK(residual->sizes() == out.sizes(), kWhat, ": residual must have the output's shape");
     res = rows_of(*residual);
     TORCH_CHECK(res.stride >= 0, kWhat, ": residual needs unit stride along its last axis and leading axes that are one run of rows, not overlapping");
   }
@@ -125,11 +134,20 @@ at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const std::optional<
   return out;
 }
 
+void check_out(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+               const std::optional<at::Tensor>& residual, double limit, const at::Tensor& out) {
+  check_kinds(x, w, bias, activation, residual, out.scalar_type(), limit);
+  TORCH_CHECK(out.is_contiguous() && out.device() == x.device() && out.dim() == x.dim(), kWhat, ": out must be a contiguous [..., n] on x's GPU");
+  for (int64_t d = 0; d < x.dim(); ++d) {
+    const c10::SymInt lines = w.sym_size(0);
+    TORCH_SYM_CHECK(out.sym_size(d).sym_eq(d + 1 < x.dim() ? x.sym_size(d) : activation == kSwiglu ? lines / 2 : lines), kWhat,
+                    ": out must be a contiguous [..., n] on x's GPU");
+  }
+}
+
 void linear_out(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
                 const std::optional<at::Tensor>& residual, double limit, const at::Tensor& out) {
-  check_kinds(x, w, bias, activation, residual, out.scalar_type(), limit);
-  TORCH_CHECK(out.is_contiguous() && out.device() == x.device() && out.sizes().vec() == with_last(x.sizes(), columns_of(w, activation)), kWhat,
-              ": out must be a contiguous [..., n] on x's GPU");
+  check_out(x, w, bias, activation, residual, limit, out);
   run(x, w, bias, activation, residual, limit, out, at::Tensor());
 }
 
@@ -145,7 +163,6 @@ std::tuple<at::Tensor, at::Tensor> forward(const at::Tensor& x, const at::Tensor
   check_kinds(x, w, bias, activation, residual, out_dtype, limit);
   const c10::DeviceGuard guard(x.device());
   const int64_t n = columns_of(w, activation), k = x.size(-1);
-  TORCH_CHECK(k > 0, kWhat, ": the weights must be [n, k] of x's k = 0");
   check_trains(x.numel() / k, k, n, activation);
   at::Tensor out = at::empty(with_last(x.sizes(), n), x.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
   at::Tensor z = at::empty({activation ? x.numel() / k : 0, w.size(0)}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
@@ -287,15 +304,17 @@ at::Tensor linear_meta(const at::Tensor& x, const at::Tensor& w, const std::opti
   const c10::SymInt lines = w.sym_size(0);
   return at::empty_symint(with_last(x.sym_sizes(), activation == kSwiglu ? lines / 2 : lines), x.options().dtype(out_dtype));
 }
-void linear_out_meta(const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&, int64_t, const std::optional<at::Tensor>&, double,
-                     const at::Tensor&) {}
+void linear_out_meta(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias, int64_t activation,
+                     const std::optional<at::Tensor>& residual, double limit, const at::Tensor& out) {
+  check_out(x, w, bias, activation, residual, limit, out);
+}
 std::tuple<at::Tensor, at::Tensor> forward_meta(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
                                                 int64_t activation, const std::optional<at::Tensor>& residual, at::ScalarType out_dtype,
                                                 double limit) {
   at::Tensor y = linear_meta(x, w, bias, activation, residual, out_dtype, limit);
   const c10::SymInt rows = activation ? x.sym_numel() / x.sym_size(-1) : c10::SymInt(0);
   const auto all = x.sym_numel().maybe_as_int(), k = x.sym_size(-1).maybe_as_int(), n = y.sym_size(-1).maybe_as_int();
-  if (all && k && n && *k > 0) check_trains(*all / *k, *k, *n, activation);
+  if (all && k && n) check_trains(*all / *k, *k, *n, activation);
   return {y, at::empty_symint({rows, w.sym_size(0)}, x.options().dtype(at::kFloat))};
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> gradient_meta(const std::optional<at::Tensor>& x, const std::optional<at::Tensor>& w,
