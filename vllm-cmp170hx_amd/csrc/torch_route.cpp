@@ -29,13 +29,34 @@ decltype(&moe_route_grad) native_grad = nullptr;
 
 constexpr const char* kWhat = "moe_route_logits";
 
-// (symbolic sizes pass: the shape alone)
-void check_shapes(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t topk,
-                  const std::optional<at::Tensor>& padding) {
+// Shapes, types and options; sizes may be symbolic.
+void check_call(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t topk, int64_t groups, int64_t topk_groups,
+                int64_t scoring, double scale, const std::optional<at::Tensor>& padding) {
   TORCH_CHECK(logits.dim() == 2, kWhat, ": logits must be [rows, experts]");
-  TORCH_CHECK(topk > 0, kWhat, ": topk must be positive");
-  TORCH_CHECK(!bias || bias->dim() == 1, kWhat, ": bias must be FP32 [experts]");
-  TORCH_CHECK(!padding || padding->dim() == 1, kWhat, ": is_padding must be [rows]");
+  TORCH_CHECK(logits.scalar_type() == at::kBFloat16 || logits.scalar_type() == at::kHalf || logits.scalar_type() == at::kFloat, kWhat,
+              ": logits must be BF16, FP16 or FP32");
+  const c10::SymInt rows = logits.sym_size(0), experts = logits.sym_size(1);
+  TORCH_SYM_CHECK(experts.sym_gt(0), kWhat, ": between 1 and 1024 experts");
+  TORCH_SYM_CHECK(experts.sym_le(1024), kWhat, ": between 1 and 1024 experts");
+  TORCH_CHECK(topk > 0 && topk <= 64, kWhat, ": topk must be between 1 and 64, and at most the experts");
+  TORCH_SYM_CHECK(experts.sym_ge(topk), kWhat, ": topk must be between 1 and 64, and at most the experts");
+  TORCH_CHECK(groups > 0 && groups <= 64, kWhat, ": up to 64 groups of equal size");
+  TORCH_SYM_CHECK((experts % groups).sym_eq(0), kWhat, ": up to 64 groups of equal size");
+  TORCH_CHECK(topk_groups > 0 && topk_groups <= groups, kWhat, ": topk_groups must be between 1 and the groups");
+  TORCH_SYM_CHECK((experts / groups * topk_groups).sym_ge(topk), kWhat, ": topk experts do not fit topk_groups groups");
+  TORCH_CHECK(scoring == 0 || scoring == 1, kWhat, ": scoring must be softmax (0) or sigmoid (1)");
+  TORCH_CHECK(std::isfinite(static_cast<float>(scale)), kWhat, ": the scale must be finite");
+  if (bias) {
+    TORCH_CHECK(bias->dim() == 1 && bias->device() == logits.device() && bias->scalar_type() == at::kFloat, kWhat,
+                ": bias must be FP32 [experts] on the logits' GPU");
+    TORCH_SYM_CHECK(bias->sym_size(0).sym_eq(experts), kWhat, ": bias must be FP32 [experts] on the logits' GPU");
+  }
+  if (padding) {
+    TORCH_CHECK(padding->dim() == 1 && padding->device() == logits.device() &&
+                    (padding->scalar_type() == at::kBool || padding->scalar_type() == at::kByte),
+                kWhat, ": is_padding must be a contiguous bool or uint8 [rows] on the logits' GPU");
+    TORCH_SYM_CHECK(padding->sym_size(0).sym_eq(rows), kWhat, ": is_padding must be a contiguous bool or uint8 [rows] on the logits' GPU");
+  }
 }
 
 void check_logits(const at::Tensor& logits) {
@@ -52,18 +73,12 @@ int64_t stride_of(const at::Tensor& logits) { return logits.size(0) > 1 ? logits
 std::tuple<at::Tensor, at::Tensor> route(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t topk, int64_t groups,
                                          int64_t topk_groups, int64_t scoring, bool renormalize, double scale,
                                          const std::optional<at::Tensor>& padding) {
-  check_shapes(logits, bias, topk, padding);
+  check_call(logits, bias, topk, groups, topk_groups, scoring, scale, padding);
   check_logits(logits);
   const int64_t rows = logits.size(0), experts = logits.size(1);
-  TORCH_CHECK(!bias || (bias->device() == logits.device() && bias->scalar_type() == at::kFloat && bias->size(0) == experts), kWhat,
-              ": bias must be FP32 [experts] on the logits' GPU");
-  TORCH_CHECK(!padding || (padding->device() == logits.device() &&
-                           (padding->scalar_type() == at::kBool || padding->scalar_type() == at::kByte) && padding->size(0) == rows &&
-                           padding->is_contiguous()),
-              kWhat, ": is_padding must be a contiguous bool or uint8 [rows] on the logits' GPU");
+  TORCH_CHECK(!padding || padding->is_contiguous(), kWhat, ": is_padding must be a contiguous bool or uint8 [rows] on the logits' GPU");
   const c10::DeviceGuard guard(logits.device());
   const at::Tensor close = bias ? bias->contiguous() : at::Tensor();
-  TORCH_CHECK(topk <= experts, kWhat, ": topk must be between 1 and 64, and at most the experts");
   at::Tensor weights = at::empty({rows, topk}, logits.options().dtype(at::kFloat));
   at::Tensor ids = at::empty({rows, topk}, logits.options().dtype(at::kInt));
   check_status(native_route(logits.const_data_ptr(), dtype_code(logits.scalar_type()), rows, experts, stride_of(logits),
@@ -141,9 +156,10 @@ std::tuple<at::Tensor, at::Tensor> route_autograd(const at::Tensor& logits, cons
 }
 
 // Shapes alone, for tracing.
-std::tuple<at::Tensor, at::Tensor> route_meta(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t topk, int64_t, int64_t,
-                                              int64_t, bool, double, const std::optional<at::Tensor>& padding) {
-  check_shapes(logits, bias, topk, padding);
+std::tuple<at::Tensor, at::Tensor> route_meta(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t topk, int64_t groups,
+                                              int64_t topk_groups, int64_t scoring, bool, double scale,
+                                              const std::optional<at::Tensor>& padding) {
+  check_call(logits, bias, topk, groups, topk_groups, scoring, scale, padding);
   const c10::SymInt rows = logits.sym_size(0);
   return {at::empty_symint({rows, topk}, logits.options().dtype(at::kFloat)), at::empty_symint({rows, topk}, logits.options().dtype(at::kInt))};
 }
