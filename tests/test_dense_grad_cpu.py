@@ -137,3 +137,20 @@ def test_a_gradient_that_would_be_refused_is_at_the_call(linear, lib, x, w):
     # (a residual's gradient needs no product)
     residual = torch.empty(*x[:-1], w[0], device="meta", requires_grad=True)
     assert linear(rows, weights.detach(), None, "silu", residual).requires_grad
+
+
+def test_every_plan_of_the_gradients_has_a_size(lib):
+    """The sizes of test_gpu_dense_grad_plans.py: both products on every kernel, every tile with and
+    without K splits (the smallest short ring is for products of few stages, which are not split)."""
+    from tests.test_dense_cpu import plan
+    from tests.test_gpu_dense_grad_plans import SIZES
+    seen = {"x": set(), "w": set()}
+    for rows, k, lines, _ in SIZES:
+        for name, size in (("x", (rows, lines, k)), ("w", (lines, rows, k))):
+            kind, tile_rows, tile_lines, parts, ring = plan(lib, *size, 0, 0)
+            seen[name].add((kind, tile_rows, tile_lines, ring, parts > 1) if kind == 0 else (kind,))
+    tiles = ((256, 256, 5), (128, 256, 6), (128, 64, 6), (64, 64, 8), (128, 64, 4))
+    for name, got in seen.items():
+        for shape in tiles:
+            assert {(0, *shape, False), (0, *shape, True)} <= got, (name, shape)
+        assert (0, 64, 64, 4, False) in got and got & {(1,), (2,)}, name
