@@ -139,3 +139,45 @@ def test_refused_gradients_take_no_memory(linear, device):
     with pytest.raises(RuntimeError, match="too many rows and columns"):
         linear(x, w, None, "silu")
     assert torch.cuda.max_memory_allocated(device) == before
+
+
+def grads_of(linear, x, w, bias, activation, dy):
+    leaves = [t.detach().requires_grad_() for t in (x, w, bias)]
+    y = linear(*leaves, activation, out_dtype=torch.float32)
+    return torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.parametrize("rows,n,k", [(200, 96, 64), (4000, 40, 72), (30, 3000, 72), (8, 33, 200)])
+@pytest.mark.parametrize("activation", [None, "silu", "swiglu"])
+def test_fp16_gradients_above_its_range(linear, device, rows, n, k, activation):
+    """dz of about 2^20, which FP16 does not hold, and results that it does: dy of 2^20 before x and
+    weights of 2^-14.  (Biases keep z, and with it the slopes and up lines, near 1.)"""
+    rng = np.random.default_rng(rows + n)
+    lines = 2 * n if activation == "swiglu" else n
+    x, w = normal(rng, (rows, k), "fp16", device, 2.0 ** -14), normal(rng, (lines, k), "fp16", device, 2.0 ** -14)
+    bias, dy = normal(rng, lines, "fp32", device), normal(rng, (rows, n), "fp32", device, 2.0 ** 20)
+    wants, dz = D.backward(exact(x), exact(w), exact(bias), activation, exact(dy), torch.finfo(torch.float16).eps)
+    assert np.abs(dz).max() > 2 * 65504
+    for got, name in zip(grads_of(linear, x, w, bias, activation, dy), ("x", "w", "bias")):
+        assert torch.isfinite(got).all() and np.abs(wants[name][0]).max() > 100
+        close(got, *wants[name], name)
+
+
+@pytest.mark.parametrize("rows,n,k", [(200, 96, 64), (4000, 40, 72), (30, 3000, 72), (8, 33, 200)])
+@pytest.mark.parametrize("activation", [None, "silu", "swiglu"])
+@pytest.mark.parametrize("which", ["x", "w"])
+def test_fp16_gradients_below_its_range(linear, device, rows, n, k, activation, which):
+    """dz of about 2^-26, which FP16 rounds to zero or its least numbers, and results among its normal ones:
+    what dz is multiplied with is 2^13, the other operand as much smaller."""
+    rng = np.random.default_rng(rows + n + 1)
+    lines = 2 * n if activation == "swiglu" else n
+    large, small = (13, -16) if which == "w" else (-16, 13)
+    x, w = normal(rng, (rows, k), "fp16", device, 2.0 ** large), normal(rng, (lines, k), "fp16", device, 2.0 ** small)
+    bias, dy = normal(rng, lines, "fp32", device), normal(rng, (rows, n), "fp32", device, 2.0 ** -26)
+    wants, dz = D.backward(exact(x), exact(w), exact(bias), activation, exact(dy), torch.finfo(torch.float16).eps)
+    # (as FP16 by itself would hold it, most of dz is lost)
+    assert np.abs(dz.astype(np.float16) - dz).max() > np.abs(dz).max() / 100
+    want = wants[which][0]
+    assert np.median(np.abs(want)) > 2.0 ** -14
+    for got, name in zip(grads_of(linear, x, w, bias, activation, dy), ("x", "w", "bias")):
+        close(got, *wants[name], name)
