@@ -154,3 +154,27 @@ def test_every_plan_of_the_gradients_has_a_size(lib):
         for shape in tiles:
             assert {(0, *shape, False), (0, *shape, True)} <= got, (name, shape)
         assert (0, 64, 64, 4, False) in got and got & {(1,), (2,)}, name
+
+
+@pytest.mark.parametrize("trained", [["x"], ["w"], ["bias"], ["residual"], ["x", "residual"]])
+@pytest.mark.parametrize("mode", ["real", "symbolic"])
+def test_traces_of_some_trainable_inputs(linear, trained, mode):
+    """A trace holds the gradient without the operands that it does not read, for other sizes too."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(x, w, bias, residual, dy):
+        t = {k: v.detach().requires_grad_(k in trained) for k, v in (("x", x), ("w", w), ("bias", bias), ("residual", residual))}
+        y = linear(t["x"], t["w"], t["bias"], "swiglu", t["residual"])
+        return torch.autograd.grad(y, [t[k] for k in trained], dy)
+
+    def args(rows, k, n):
+        return [torch.empty(*s, device="meta", dtype=torch.half) for s in ((rows, k), (2 * n, k), (2 * n,), (rows, n), (rows, n))]
+
+    shapes = lambda a: [tuple(a[("x", "w", "bias", "residual").index(k)].shape) for k in trained]
+    traced = make_fx(step, tracing_mode=mode)(*args(6, 8, 5))
+    for size in ((6, 8, 5), (9, 24, 7))[:2 if mode == "symbolic" else 1]:
+        assert [tuple(g.shape) for g in traced(*args(*size))] == shapes(args(*size))
+    calls = [n for n in traced.graph.nodes if "dense_linear_grad" in str(n.target)]
+    assert len(calls) == (trained != ["residual"])
+    for call in calls:
+        assert (call.args[0] is None) == ("w" not in trained) and (call.args[1] is None) == ("x" not in trained)
