@@ -648,9 +648,10 @@ int mxfp4_moe(const void* x, int act_dtype, int64_t tokens, int64_t x_stride, co
  * residual [rows][n] (or null) of any of the three types; out contiguous, of any of them;
  * it may be a contiguous residual of its type.  z (or null): contiguous FP32 [rows][lines],
  * x W^T + bias for dense_linear_grad.  The order of the sums, and so the last bits, depend
- * on the sizes, on whether there is a residual and on whether x and w lie on 16 bytes.  k up to 2^21, lines up to 2^24, rows up to 2^26.  workspace:
- * dense_linear_workspace_size bytes of the same x, w and strides, 16-byte aligned (null
- * where that is 0), used by one call at a time.
+ * on the sizes, on whether there is a residual and on whether x and w lie on 16 bytes.  k up
+ * to 2^21, lines up to 2^24, rows up to 2^26.  workspace: dense_linear_workspace_size bytes
+ * of the same x, w and strides, 16-byte aligned (null where that is 0), used by one call at a
+ * time.
  */
 int64_t dense_linear_workspace_size(const void* x, int64_t rows, int64_t k, int64_t x_stride,
                                     const void* w, int64_t n, int64_t w_stride, int activation);
@@ -660,9 +661,10 @@ int dense_linear(const void* x, int dtype, int64_t rows, int64_t k, int64_t x_st
                  int64_t residual_stride, void* out, int out_dtype, float* z, void* workspace,
                  int64_t workspace_bytes, void* stream);
 
-/* How it runs at a size, x and w on 16 bytes, for tests: plan[0] 0 on tiles of plan[1] rows and plan[2] lines, K in
- * plan[3] splits, plan[4] parts in LDS's ring; 1 (16 rows at most) with K over plan[3] wavefronts; 2 (eight at most)
- * with plan[2] lines a wavefront, K over plan[3]. */
+/* How it runs at a size, x and w on 16 bytes, for tests: plan[0] 0 on tiles of plan[1] rows
+ * and plan[2] lines, K in plan[3] splits, plan[4] parts in LDS's ring; 1 (16 rows at most)
+ * with K over plan[3] wavefronts; 2 (eight at most) with plan[2] lines a wavefront, K over
+ * plan[3]. */
 int dense_linear_plan(int64_t rows, int64_t k, int64_t n, int activation, int has_residual,
                       int32_t* plan);
 

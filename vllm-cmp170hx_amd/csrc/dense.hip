@@ -164,7 +164,8 @@ __global__ __launch_bounds__(64 * kGemvWaves) void gemv_kernel(Operand x, Operan
 // chunks 4 j + q (j < 4) of line r and of x's row r and multiplies them in four
 // v_mfma_16x16x32.  K is split over the wavefronts of a workgroup, whose sums meet in
 // LDS and are added in order.  Bound by the loads' latency: 8 rows of 4096 x 4096 take 9.2 us
-// (3.6 TB/s; tiles with K splits and their sum 12.3).
+// (3.6 TB/s; tiles with K splits and their sum 12.3).  From 17 rows on tiles are the faster ones
+// (20 rows of 2592 x 5003: 15 us for 20 with two of these products a lane).
 
 constexpr int kSmallRows = 16;  // of one B operand
 constexpr int kStepChunks = 16;
@@ -383,9 +384,15 @@ __global__ __launch_bounds__(256) void top_kernel(Slopes g, uint32_t* tops) {
 // dz of 64 rows and 64 columns (gated: of the gate and of the up lines; FP16 over scale_of
 // the largest of `tops`): by rows (stride `ld`, zeros up to whole chunks of lines), by lines
 // (stride `ldt`, zeros up to whole chunks of rows), and the lines' sums over these rows.
+//
+// dz is rounded to x's type: the matrix cores multiply 16-bit operands of one type, and a second
+// product for what the rounding takes off would double the time of both gradients.  It is all that dx
+// and dW lose beside their own rounding: against 64 bits they are off by 0.00235 in BF16 and 0.00029
+// in FP16 (norms; rounded once 0.00166 and 0.00021), against 64 bits from the rounded dz by
+// 0.00166 and 0.00021 (4096 x 4096 x 288, 1000 x 2048 x 768, 4096 x 4096 x 28672).
 template <bool kGated>
-__global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* tops, int parts, uint32_t* top, uint16_t* dz, int64_t ld, uint16_t* dzt, int64_t ldt,
-                                                     float* partial) {
+__global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* tops, int parts, uint32_t* top, uint16_t* dz, int64_t ld,
+                                                     uint16_t* dzt, int64_t ldt, float* partial) {
   constexpr int kHalves = kGated ? 2 : 1;
   __shared__ uint16_t part[kHalves][kPart * kPartStride];
   __shared__ float sum[kHalves][32][kPart + 1];
@@ -472,7 +479,8 @@ __global__ __launch_bounds__(256) void slopes_kernel(Slopes g, const uint32_t* t
 // 3.9 us (a thread a line 37), 2^21 of 24 51 (1080), 1000 of 768 2.6 (2.1).
 constexpr int kSumLines = 32, kSumRuns = 32;
 
-__global__ __launch_bounds__(kSumLines * kSumRuns) void bias_kernel(const float* partial, int64_t parts, int64_t lines, void* out, int dtype) {
+__global__ __launch_bounds__(kSumLines * kSumRuns) void bias_kernel(const float* partial, int64_t parts, int64_t lines, void* out,
+                                                                    int dtype) {
   __shared__ double sums[kSumRuns][kSumLines];
   const int col = threadIdx.x % kSumLines, run = threadIdx.x / kSumLines;
   const int64_t c = int64_t(blockIdx.x) * kSumLines + col;
@@ -524,9 +532,9 @@ struct Plan {
 // Up to 16 rows (us, a wavefront a line / the small kernel / tiles; k x lines): 4096 x 28672
 // 4 rows 48 / 59 / 46, 8 rows 73 / 60 / 45, 16 rows - / 70 / 45; 14336 x 4096 2 rows 25 / 26 /
 // 26, 4 rows 35 / 28 / 26; 4096 x 4096 4 rows 9.4 / 9.0 / 12, 8 rows 15 / 9.2 / 12, 16 rows
-// - / 10.4 / 12.3; 7168 x 256 8 rows 5.9 / 12 / 8.7, 16 rows - / 14.6 / 9.0.  So W of more than 2^25 elements goes to the tiles
-// from three rows on (if it lies as they want it: a packed copy costs more than it gains),
-// few and long lines from nine.
+// - / 10.4 / 12.3; 7168 x 256 8 rows 5.9 / 12 / 8.7, 16 rows - / 14.6 / 9.0.  So W of more than
+// 2^25 elements goes to the tiles from three rows on (if it lies as they want it: a packed copy
+// costs more than it gains), few and long lines from nine.
 constexpr int64_t kLargeW = int64_t(1) << 25, kFewLines = 512;
 
 // direct: x and W lie as the tiles want them.

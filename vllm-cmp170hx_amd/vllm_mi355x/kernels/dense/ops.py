@@ -45,10 +45,11 @@ def dense_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     itself; it carries no gradient.
 
     Differentiable once in x, weight, bias and residual, in reverse mode (a forward-mode tangent
-    raises): x W^T + bias is kept in fp32, its gradient rounded to x's type (in fp16 over a
-    power of two of the whole tensor) before the two products that follow.  To capture a
-    backward pass into a graph, let go of eager results of the same leaves first, as for any
-    operator of torch."""
+    and torch.func's grad and vjp raise): x W^T + bias is kept in fp32, its gradient rounded to x's
+    type (in fp16 over a power of two of the whole tensor) before the two products that follow.
+    A backward pass computes the gradients that it is asked for; x is kept for the weight's alone,
+    the weight for x's.  To capture a backward pass into a graph, let go of eager results of the
+    same leaves first, as for any operator of torch."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
     if clamp_limit is not None and activation != "swiglu":

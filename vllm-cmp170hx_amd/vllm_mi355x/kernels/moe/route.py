@@ -108,7 +108,7 @@ def moe_route_logits(logits: torch.Tensor, topk: int, bias: torch.Tensor | None 
     weights NaN.
 
     The weights are differentiable once in the logits, in reverse mode (a forward-mode
-    tangent raises), the choice and the bias constants.  Failed checks raise RuntimeError.
+    tangent and torch.func's grad and vjp raise), the choice and the bias constants.  Failed checks raise RuntimeError.
     To capture a backward pass into a graph, let go of eager results of the same leaves
     first, as for any operator of torch."""
     if scoring not in _SCORING:
